@@ -757,6 +757,132 @@ int loom_decode_epilogue(int dtype, const void* stage_k, const void* stage_v, vo
                          uint8_t* pending, int64_t* pos_dev, int64_t B, int64_t N,
                          int64_t max_keys, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Paged key-value cache and beam search.  No counterparts in the reference
+ * (its decode is greedy over one dense cache); they extend the decode step's
+ * attention (loomformer.py:3300-3329) and token choice (:5306).
+ *
+ * A pool holds n_pages pages of page_size tokens (a power of two, 16 to 1024)
+ * for keys and one for values, element (page, kv head, token, d) at
+ * page*page_stride + head*head_stride + token*token_stride + d; pools and
+ * strides are multiples of 16 bytes.  Row r's token t lies in page
+ * table[r*table_ld + t / page_size] at place t % page_size; lens[r] is its
+ * number of tokens, -1 for a row that holds no sequence; table entries outside
+ * [0, n_pages) are no page.  refs[p] counts the table entries that hold page p
+ * (0: the page is free).  table, lens, refs, parent: int32 on the device, read
+ * there, so that every call can be captured into a graph.  Pages may be shared
+ * by rows; tokens behind lens[r] in them are never read.  At most 1024 rows and
+ * 2^24 tokens per row (max_pages * page_size).
+ * ------------------------------------------------------------------------ */
+
+/* Bytes of workspace of the two calls below on the current device, for rows of
+ * up to `capacity` = max_pages * page_size tokens.  Scratch: no initial contents;
+ * calls that share a workspace must not overlap. */
+int64_t loom_paged_decode_workspace_bytes(int64_t B, int64_t capacity, int64_t QH, int64_t KVH, int64_t HD);
+
+/* loom_gqa_decode_step over a paged cache with a length per row: row b's new
+ * token stands at position lens[b]; q and k of the projection row qkv
+ * [B, (QH + 2 KVH) HD] (row stride qkv_ld) are roped with row lens[b] of the
+ * tables [n_pos, HD] and rounded to dtype, (k, v) are written to the row's page
+ * (which no other row may hold: see loom_paged_update), and the row attends to
+ * its positions 0..lens[b].  c_out, kctx_out (or NULL): A.V and A.K_roped, rows
+ * out_ld elements apart; q_out (or NULL): the roped q [B, QH, HD].  lens is not
+ * advanced.  A row with lens[b] = -1 writes nothing to the pools and its outputs
+ * are zeros.  A row whose position lies past its table or the rotary tables, or
+ * one of whose pages is missing, gives NaN (and writes nothing where it has no
+ * page).  head_dim 8, 16, 32, 64, 96, 128 or 256. */
+int loom_paged_decode_step(int dtype, const void* qkv, int64_t qkv_ld, void* k_pages, void* v_pages,
+                           int64_t page_stride, int64_t token_stride, int64_t head_stride, int64_t n_pages,
+                           int64_t page_size, const int32_t* table, int64_t table_ld, int64_t max_pages,
+                           const int32_t* lens, const float* cos_table, const float* sin_table, int64_t n_pos,
+                           void* q_out, void* c_out, void* kctx_out, int64_t out_ld, float* workspace,
+                           int64_t workspace_bytes, int64_t B, int64_t QH, int64_t KVH, int64_t HD,
+                           void* stream);
+
+/* Its attention alone: q [B, QH, HD] (row stride q_ld, roped already) over the
+ * row's positions 0..lens[b]-1; a row of no token (lens[b] <= 0) gives zeros. */
+int loom_paged_decode_attention(int dtype, const void* q, int64_t q_ld, const void* k_pages, const void* v_pages,
+                                int64_t page_stride, int64_t token_stride, int64_t head_stride, int64_t n_pages,
+                                int64_t page_size, const int32_t* table, int64_t table_ld, int64_t max_pages,
+                                const int32_t* lens, void* c_out, void* kctx_out, int64_t out_ld,
+                                float* workspace, int64_t workspace_bytes, int64_t B, int64_t QH, int64_t KVH,
+                                int64_t HD, void* stream);
+
+/* The cache side of a step, over the pools of all layers (layer_stride between
+ * them; one table for all).  In this order, in place:
+ *   parent != NULL: row r takes the pages and the length of row parent[r] (a
+ *     parent outside [0, rows): row r becomes empty, lens[r] = -1), and lets go of
+ *     its own; pages that no row holds any more are free.  Pages reserved ahead
+ *     (behind the parent's lens + advance tokens) are not passed on.
+ *   lens[r] += advance, for rows that hold a sequence (the tokens written since).
+ *   tokens lens[r] .. lens[r] + n_new - 1 are made writable: missing pages are
+ *     taken from the free ones, and a partly filled last page that is held more
+ *     than once is copied (its tokens below lens[r], all layers) to a free page,
+ *     by each of its rows in row order for as long as others hold it.  Free pages
+ *     go lowest id first, in row order, a row's copy before its new pages.
+ * status[0] is raised by the number of pages that could not be had (a row whose
+ * copy failed loses its last page: its outputs are NaN, never another row's
+ * data) and by 1 for every row whose table ends before lens + n_new.  workspace:
+ * loom_paged_update_workspace_bytes(rows), scratch. */
+int64_t loom_paged_update_workspace_bytes(int64_t rows);
+int loom_paged_update(int dtype, void* k_pages, void* v_pages, int64_t layers, int64_t layer_stride,
+                      int64_t page_stride, int64_t token_stride, int64_t head_stride, int64_t n_pages,
+                      int64_t page_size, int64_t KVH, int64_t HD, int32_t* table, int64_t table_ld,
+                      int64_t max_pages, int32_t* lens, int32_t* refs, int32_t* status, const int32_t* parent,
+                      int64_t n_new, int64_t advance, void* workspace, int64_t workspace_bytes, int64_t rows,
+                      void* stream);
+
+/* Copies tokens first[r] .. last[r] - 1 of every row r of a dense cache
+ * (src_tokens positions, element (layer, r, kv head, t, d) at the four source
+ * strides + d; the decode engine's cache after a prefill) into the row's pages.
+ * Positions outside the source or the table, or without a page, are left out. */
+int loom_paged_write(int dtype, void* k_pages, void* v_pages, int64_t layers, int64_t layer_stride,
+                     int64_t page_stride, int64_t token_stride, int64_t head_stride, int64_t n_pages,
+                     int64_t page_size, int64_t KVH, int64_t HD, const int32_t* table, int64_t table_ld,
+                     int64_t max_pages, const void* k_rows, const void* v_rows, int64_t src_layer_stride,
+                     int64_t src_row_stride, int64_t src_head_stride, int64_t src_token_stride,
+                     int64_t src_tokens, const int32_t* first, const int32_t* last, int64_t rows, void* stream);
+
+/* Moves the pages in use to the lowest ids: with U of them in use, the k-th one
+ * with id >= U goes to the k-th free id below U (pools of all layers, tables and
+ * refs follow), and *used = U.  Pages U.. are free afterwards.  workspace:
+ * loom_paged_compact_workspace_bytes(n_pages), scratch. */
+int64_t loom_paged_compact_workspace_bytes(int64_t n_pages);
+int loom_paged_compact(int dtype, void* k_pages, void* v_pages, int64_t layers, int64_t layer_stride,
+                       int64_t page_stride, int64_t token_stride, int64_t head_stride, int64_t n_pages,
+                       int64_t page_size, int64_t KVH, int64_t HD, int32_t* table, int64_t table_ld,
+                       int64_t max_pages, int32_t* refs, int32_t* used, void* workspace,
+                       int64_t workspace_bytes, int64_t rows, void* stream);
+
+/* Beam search's choice.  Row g*beams + w is beam w of group g (one prompt).
+ * Candidate (w, v) of a group has the value scores[row] + logits[row, v] -
+ * logsumexp(logits[row]); a finished row (finished[row] != 0; finished may be
+ * NULL) has one candidate, pad_id at scores[row].  The n_out (1 to 64, at most
+ * beams * V) largest values of each group come out in order, ties by the lowest
+ * (w, v): out_scores [groups, n_out] float, out_parent = the candidate's row
+ * (g*beams + w), out_token, out_finished (or NULL) = the parent's flag or token
+ * == eos_id (eos_id < 0: never).  Values that are not finite are no candidates (a
+ * row with a NaN or +inf logit or a score that is not finite has none; a -inf
+ * logit is a token ruled out); places without a candidate come out as score
+ * -inf, token pad_id, parent g*beams, not finished.  Logits [groups*beams, V]
+ * dtype, row stride logits_ld, any alignment; at most 32 beams, V <= 2^24.
+ * Values are ranked in fp64.  out_scores / out_finished may be scores / finished
+ * where n_out == beams.  workspace: loom_beam_select_workspace_bytes. */
+int64_t loom_beam_select_workspace_bytes(int64_t groups, int64_t beams, int64_t V, int64_t n_out);
+int loom_beam_select(int dtype, const void* logits, int64_t logits_ld, const float* scores,
+                     const uint8_t* finished, float* out_scores, int32_t* out_parent, int64_t* out_token,
+                     uint8_t* out_finished, int64_t groups, int64_t beams, int64_t V, int64_t n_out,
+                     int64_t eos_id, int64_t pad_id, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* In place, row r of every tensor becomes the former row parent[r] (rows whose
+ * parent is outside [0, rows) stay as they are).  n <= 16 tensors; tensor i has
+ * outer[i] slices, outer_stride[i] bytes apart, of `rows` rows of row_bytes[i]
+ * bytes, row_stride[i] bytes apart.  The arrays are host arrays, read before the
+ * call returns; rows of different tensors, slices or places must not overlap. */
+int loom_reorder_rows(int64_t n, void* const* tensors, const int64_t* outer, const int64_t* outer_stride,
+                      const int64_t* row_stride, const int64_t* row_bytes, const int32_t* parent, int64_t rows,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif

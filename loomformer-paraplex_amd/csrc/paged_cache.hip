@@ -1,0 +1,475 @@
+// Bookkeeping of a paged key-value cache, on the device: forking and freeing
+// rows, making the next tokens writable (copy on write), loading dense rows,
+// compacting the pool.
+//
+// A pool has n_pages pages; refs[p] counts the table entries that hold page p
+// (0: free).  Row r holds lens[r] tokens (-1: no sequence); its table entries
+// below ceil(lens[r] / PS) are its pages, entries behind them are -1 or pages
+// reserved ahead, which only this row holds.
+#include "loom_common.h"
+
+namespace loom {
+
+constexpr int kPcMaxRows = 1024;
+constexpr int kForkCols = 16;       // table columns of a fork block
+
+struct PageCopy {                   // one copy on write: the first `tokens` tokens of a page
+    int32_t src, dst, tokens, pad;
+};
+
+struct PoolArgs {
+    char* k;
+    char* v;
+    int64_t layer, page, tok, head;     // strides in bytes
+    int layers, KVH, row_bytes;         // row_bytes: HD elements
+};
+
+__device__ __forceinline__ bool in_range(int v, int n) { return (unsigned)v < (unsigned)n; }
+
+// ------------------------------------------------------------------ fork
+
+// Row r takes the pages of row parent[r] (none where parent[r] is no row).  A
+// block owns kForkCols columns of the whole table: it reads them for all rows,
+// then writes, so the gather is in place.  refs change by atomic additions of
+// integers: their order does not matter.
+__global__ void __launch_bounds__(256)
+paged_fork_kernel(int32_t* __restrict__ table, int64_t ld, int MP, const int32_t* __restrict__ lens,
+                  int32_t* __restrict__ refs, int NP, int log_ps, const int32_t* __restrict__ parent, int R,
+                  int advance) {
+    extern __shared__ int32_t old[];                 // [R][kForkCols]
+    const int c0 = blockIdx.x * kForkCols;
+    for (int i = threadIdx.x; i < R * kForkCols; i += blockDim.x) {
+        const int c = c0 + i % kForkCols;
+        old[i] = c < MP ? table[(int64_t)(i / kForkCols) * ld + c] : -1;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < R * kForkCols; i += blockDim.x) {
+        const int r = i / kForkCols, cc = i % kForkCols, c = c0 + cc;
+        const int p = parent[r];
+        if (c >= MP || p == r) continue;
+        int now = -1;
+        if (in_range(p, R)) {
+            const int len = lens[p];                 // with the tokens written since: len + advance
+            const int held = len >= 0 ? (len + advance + (1 << log_ps) - 1) >> log_ps : 0;
+            if (c < held) now = old[p * kForkCols + cc];
+        }
+        const int was = old[i];
+        if (was == now) continue;
+        if (in_range(was, NP)) atomicSub(refs + was, 1);
+        if (in_range(now, NP)) atomicAdd(refs + now, 1);
+        table[(int64_t)r * ld + c] = now;
+    }
+}
+
+// ------------------------------------------------------------------ reserve
+
+// Exclusive scan over the 1024 threads of a block; *total: the sum.
+template <typename V>
+__device__ __forceinline__ V block_scan(V v, V* waves, V* total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    V incl = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const V o = __shfl_up(incl, d, 64);
+        if (lane >= d) incl += o;
+    }
+    __syncthreads();                                 // the previous use of `waves` is over
+    if (lane == 63) waves[wave] = incl;
+    __syncthreads();
+    V before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+        const V x = waves[w];
+        if (w < wave) before += x;
+        all += x;
+    }
+    *total = all;
+    return before + incl - v;
+}
+
+constexpr int kScanIds = 4;         // groups of four page ids per thread and round
+
+// One block.  lens[r] = lens[parent[r]] + advance, then the tokens lens[r] ..
+// lens[r] + n_new - 1 get pages of their own: where the row's last page is
+// partly filled and held more than once, row order decides who copies it (each
+// row in turn copies while others hold it), and pages that are missing are
+// appended.  The free pages are taken lowest id first, in row order, by one
+// scan over refs: a free page's rank among the free ones names its row.
+__global__ void __launch_bounds__(1024)
+paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* __restrict__ lens,
+                     int32_t* refs, int NP, int log_ps, const int32_t* __restrict__ parent, int R,
+                     int n_new, int advance, PageCopy* __restrict__ copies, int32_t* __restrict__ status) {
+    __shared__ int32_t tail[kPcMaxRows], base[kPcMaxRows], slot0[kPcMaxRows];
+    __shared__ int64_t waves[16];
+    const int r = threadIdx.x, PS = 1 << log_ps;
+    int len = -1;
+    if (r < R) {
+        const int p = parent != nullptr ? parent[r] : r;
+        if (in_range(p, R)) len = lens[p];
+        if (len >= 0) len += advance;
+        else len = -1;
+    }
+    __syncthreads();                                 // every parent's length is read
+    int page = -1, want = 0, ntail = 0, short_of = 0;
+    bool copy = false;
+    if (r < R) lens[r] = len;
+    const int cap = MP * PS;
+    int n = len >= 0 ? min(n_new, cap - len) : 0;
+    if (len >= 0 && n_new > 0 && n < n_new) short_of = 1;
+    n = max(n, 0);
+    int miss0 = 0, nmiss = 0;
+    int32_t* row = table + (int64_t)r * ld;
+    if (n > 0) {
+        ntail = len & (PS - 1);
+        if (ntail) {
+            page = row[len >> log_ps];
+            if (!in_range(page, NP)) page = -1;
+        }
+        const int last = (len + n - 1) >> log_ps;
+        miss0 = (len + PS - 1) >> log_ps;
+        while (miss0 <= last && in_range(row[miss0], NP)) ++miss0;
+        nmiss = last + 1 - miss0;
+    }
+    tail[r] = page;
+    __syncthreads();
+    if (page >= 0) {
+        const int held = refs[page];
+        if (held > 1) {
+            int before = 0;
+            for (int i = 0; i < r; ++i) before += tail[i] == page;
+            copy = held - before > 1;
+        }
+    }
+    want = nmiss + (copy ? 1 : 0);
+    int64_t total64;
+    const int first = (int)block_scan<int64_t>(want, waves, &total64);
+    base[r] = first;
+    slot0[r] = copy ? ~miss0 : miss0;                // (the sign says whether the first page is a copy's)
+    if (r < R) copies[r] = PageCopy{-1, -1, 0, 0};
+    const int64_t need = total64;
+    int64_t given = 0;                               // free pages handed out so far
+    __syncthreads();
+    for (int64_t seg = 0; seg < NP && given < need; seg += 1024 * 4 * kScanIds) {
+        uint32_t mask = 0;                           // bit 4 j + e: page seg + 4096 j + 4 r + e is free
+        int64_t count = 0;                           // 16 bits per j
+#pragma unroll
+        for (int j = 0; j < kScanIds; ++j) {
+            const int64_t id = seg + 4096 * j + 4 * r;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (id + e < NP && refs[id + e] <= 0) mask |= 1u << (4 * j + e);
+            count |= (int64_t)__popc((mask >> (4 * j)) & 15u) << (16 * j);
+        }
+        int64_t all;
+        const int64_t before = block_scan<int64_t>(count, waves, &all);
+        int64_t at = given;
+#pragma unroll
+        for (int j = 0; j < kScanIds; ++j) {
+            int64_t rank = at + ((before >> (16 * j)) & 0xffff);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (!((mask >> (4 * j + e)) & 1u)) continue;
+                if (rank < need) {
+                    const int id = (int)(seg + 4096 * j + 4 * r + e);
+                    int lo = 0, hi = R - 1;          // the last row whose base is at most `rank`
+                    while (lo < hi) {
+                        const int mid = (lo + hi + 1) >> 1;
+                        if (base[mid] <= rank) lo = mid; else hi = mid - 1;
+                    }
+                    const bool cp = slot0[lo] < 0;
+                    const int k = (int)rank - base[lo], m0 = cp ? ~slot0[lo] : slot0[lo];
+                    refs[id] = 1;
+                    if (cp && k == 0) {
+                        const int l = lens[lo], sl = l >> log_ps;
+                        copies[lo] = PageCopy{tail[lo], id, l & (PS - 1), 0};
+                        table[(int64_t)lo * ld + sl] = id;
+                        atomicSub(refs + tail[lo], 1);
+                    } else {
+                        table[(int64_t)lo * ld + m0 + k - (cp ? 1 : 0)] = id;
+                    }
+                }
+                ++rank;
+            }
+            at += (all >> (16 * j)) & 0xffff;
+        }
+        given = at;
+    }
+    // a row whose copy found no page must not write into the shared one
+    if (copy && first >= given) {
+        row[len >> log_ps] = -1;
+        atomicSub(refs + page, 1);
+    }
+    if (short_of) atomicAdd(status, 1);
+    if (r == 0 && given < need) atomicAdd(status, (int)(need - given));
+}
+
+// Copies of `copies[r]`, both pools of all layers: grid (rows, 2 * layers).
+__global__ void __launch_bounds__(256)
+paged_cow_kernel(PoolArgs a, const PageCopy* __restrict__ copies) {
+    const PageCopy c = copies[blockIdx.x];
+    if (c.src < 0) return;
+    char* pool = (blockIdx.y & 1 ? a.v : a.k) + (int64_t)(blockIdx.y >> 1) * a.layer;
+    const char* src = pool + c.src * a.page;
+    char* dst = pool + c.dst * a.page;
+    const int pieces = a.row_bytes / 16, per_head = c.tokens * pieces;
+    for (int i = threadIdx.x; i < a.KVH * per_head; i += 256) {
+        const int h = i / per_head, k = i - h * per_head, t = k / pieces;
+        const int64_t off = h * a.head + t * a.tok + (int64_t)(k - t * pieces) * 16;
+        *reinterpret_cast<u32x4*>(dst + off) = *reinterpret_cast<const u32x4*>(src + off);
+    }
+}
+
+// ------------------------------------------------------------------ dense rows into pages
+
+// Tokens first[r] .. last[r] - 1 of row r of a dense cache (element (layer, r,
+// head, t) at the strides given) into the row's pages: grid (token tiles of
+// kWriteTile, rows, layers * KVH * 2).  Tokens without a page are left out.
+constexpr int kWriteTile = 64;
+
+__global__ void __launch_bounds__(256)
+paged_write_kernel(PoolArgs a, const char* __restrict__ kd, const char* __restrict__ vd, int64_t s_layer,
+                   int64_t s_row, int64_t s_head, int64_t s_tok, int T, const int32_t* __restrict__ table,
+                   int64_t ld, int MP, int NP, int log_ps, const int32_t* __restrict__ first,
+                   const int32_t* __restrict__ last) {
+    const int r = blockIdx.y, t0 = blockIdx.x * kWriteTile;
+    const int lo = max(max(first[r], 0), t0);
+    const int hi = min(min(min(last[r], T), MP << log_ps), t0 + kWriteTile);
+    if (lo >= hi) return;
+    const int z = blockIdx.z, which = z & 1, h = (z >> 1) % a.KVH;
+    const int64_t l = (z >> 1) / a.KVH;
+    char* pool = (which ? a.v : a.k) + l * a.layer + h * a.head;
+    const char* src = (which ? vd : kd) + l * s_layer + r * s_row + h * s_head;
+    const int pieces = a.row_bytes / 16, mask = (1 << log_ps) - 1;
+    for (int i = threadIdx.x; i < (hi - lo) * pieces; i += 256) {
+        const int t = lo + i / pieces, c = i % pieces;
+        const int page = table[(int64_t)r * ld + (t >> log_ps)];
+        if (!in_range(page, NP)) continue;
+        *reinterpret_cast<u32x4*>(pool + page * a.page + (int64_t)(t & mask) * a.tok + 16 * c) =
+            *reinterpret_cast<const u32x4*>(src + (int64_t)t * s_tok + 16 * c);
+    }
+}
+
+// ------------------------------------------------------------------ compact
+
+// One block: U = pages in use; the k-th used page with id >= U (movers) goes to
+// the k-th free id below U (holes); map[p] = the new id of page p.  ws: [0] the
+// number of moves, then movers [NP], holes [NP], map [NP].
+__global__ void __launch_bounds__(1024)
+paged_compact_plan_kernel(int32_t* refs, int NP, int32_t* __restrict__ used, int32_t* ws) {
+    __shared__ int64_t waves[16];
+    int32_t *movers = ws + 4, *holes = movers + NP, *map = holes + NP;
+    const int r = threadIdx.x;
+    int mine = 0;
+    for (int64_t i = r; i < NP; i += 1024) mine += refs[i] > 0;
+    int64_t total;
+    block_scan<int64_t>(mine, waves, &total);
+    const int U = (int)total;
+    int nm = 0, nh = 0;
+    for (int64_t seg = 0; seg < NP; seg += 4096) {
+        int64_t count = 0;                           // movers low, holes high
+        uint32_t bits = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int64_t id = seg + 4 * r + e;
+            if (id >= NP) continue;
+            const bool inuse = refs[id] > 0;
+            map[id] = (int)id;
+            if (inuse && id >= U) { count += 1; bits |= 1u << e; }
+            if (!inuse && id < U) { count += (int64_t)1 << 32; bits |= 16u << e; }
+        }
+        int64_t all;
+        const int64_t before = block_scan<int64_t>(count, waves, &all);
+        int m = nm + (int)(before & 0xffffffff), h = nh + (int)(before >> 32);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int id = (int)(seg + 4 * r + e);
+            if (bits >> e & 1u) movers[m++] = id;
+            if (bits >> (4 + e) & 1u) holes[h++] = id;
+        }
+        nm += (int)(all & 0xffffffff);
+        nh += (int)(all >> 32);
+    }
+    __syncthreads();                                 // the lists and the map are written
+    for (int i = r; i < nm; i += 1024) {             // (as many holes as movers)
+        const int from = movers[i], to = holes[i];
+        map[from] = to;
+        refs[to] = refs[from];
+        refs[from] = 0;
+    }
+    if (r == 0) {
+        ws[0] = nm;
+        *used = U;
+    }
+}
+
+// The moves (a page of one layer's K or V pool each) and, in the blocks of
+// y = 1, the tables' new ids.
+__global__ void __launch_bounds__(256)
+paged_compact_move_kernel(PoolArgs a, int PS, const int32_t* __restrict__ ws, int NP, int32_t* __restrict__ table,
+                          int64_t ld, int MP, int R) {
+    const int32_t *movers = ws + 4, *holes = movers + NP, *map = holes + NP;
+    if (blockIdx.y == 1) {
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)R * MP; i += (int64_t)gridDim.x * 256) {
+            int32_t* e = table + (i / MP) * ld + i % MP;
+            const int p = *e;
+            if (in_range(p, NP)) *e = map[p];
+        }
+        return;
+    }
+    const int64_t units = (int64_t)ws[0] * 2 * a.layers;
+    const int pieces = a.row_bytes / 16, per_head = PS * pieces;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int i = (int)(u / (2 * a.layers)), lp = (int)(u % (2 * a.layers));
+        char* pool = (lp & 1 ? a.v : a.k) + (int64_t)(lp >> 1) * a.layer;
+        const char* src = pool + movers[i] * a.page;
+        char* dst = pool + holes[i] * a.page;
+        for (int k0 = threadIdx.x; k0 < a.KVH * per_head; k0 += 256) {
+            const int h = k0 / per_head, k = k0 - h * per_head, t = k / pieces;
+            const int64_t off = h * a.head + t * a.tok + (int64_t)(k - t * pieces) * 16;
+            *reinterpret_cast<u32x4*>(dst + off) = *reinterpret_cast<const u32x4*>(src + off);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ host side
+
+static int pool_checks(const char* who, int dtype, const void* k, const void* v, int64_t L, int64_t layer,
+                       int64_t page, int64_t tok, int64_t head, int64_t NP, int64_t PS, int64_t KVH, int64_t HD,
+                       PoolArgs* out) {
+    LOOM_CHECK(dtype == LOOM_F32 || dtype == LOOM_BF16 || dtype == LOOM_F16, "%s: unsupported dtype %d", who, dtype);
+    const int64_t es = dtype == LOOM_F32 ? 4 : 2;
+    LOOM_CHECK(PS >= 16 && PS <= 1024 && (PS & (PS - 1)) == 0,
+               "%s: page_size must be a power of two from 16 to 1024, got %lld", who, (long long)PS);
+    LOOM_CHECK(NP >= 1 && NP < ((int64_t)1 << 30), "%s: bad n_pages %lld", who, (long long)NP);
+    LOOM_CHECK(L >= 1 && L <= 4096 && KVH >= 1 && KVH <= 4096 && HD >= 8 && HD <= 1024 && HD % 8 == 0,
+               "%s: bad pool shape layers=%lld heads=%lld head_dim=%lld", who, (long long)L, (long long)KVH, (long long)HD);
+    LOOM_CHECK(tok >= HD && page >= 0 && head >= 0 && layer >= 0, "%s: bad pool strides", who);
+    LOOM_CHECK((tok * es) % 16 == 0 && (page * es) % 16 == 0 && (head * es) % 16 == 0 && (layer * es) % 16 == 0 &&
+                   k != nullptr && v != nullptr && (((uintptr_t)k | (uintptr_t)v) % 16) == 0,
+               "%s: the pools must be given, they and their strides multiples of 16 bytes", who);
+    *out = PoolArgs{(char*)k, (char*)v, layer * es, page * es, tok * es, head * es, (int)L, (int)KVH, (int)(HD * es)};
+    return LOOM_OK;
+}
+
+static int table_checks(const char* who, const int32_t* table, int64_t ld, int64_t MP, int64_t PS, int64_t R) {
+    LOOM_CHECK(R >= 0 && R <= kPcMaxRows, "%s: 0 to %d rows, got %lld", who, kPcMaxRows, (long long)R);
+    LOOM_CHECK(MP >= 1 && MP * PS <= ((int64_t)1 << 24) && ld >= MP,
+               "%s: the table must hold 1 page to 2^24 tokens per row (max_pages=%lld, row stride %lld)", who,
+               (long long)MP, (long long)ld);
+    LOOM_CHECK(table != nullptr, "%s: a required pointer is NULL", who);
+    return LOOM_OK;
+}
+
+}  // namespace loom
+
+using namespace loom;
+
+extern "C" int64_t loom_paged_update_workspace_bytes(int64_t rows) {
+    return rows > 0 ? rows * (int64_t)sizeof(PageCopy) : 0;
+}
+
+extern "C" int loom_paged_update(int dtype, void* k_pages, void* v_pages, int64_t layers, int64_t layer_stride,
+                                 int64_t page_stride, int64_t token_stride, int64_t head_stride, int64_t n_pages,
+                                 int64_t page_size, int64_t KVH, int64_t HD, int32_t* table, int64_t table_ld,
+                                 int64_t max_pages, int32_t* lens, int32_t* refs, int32_t* status,
+                                 const int32_t* parent, int64_t n_new, int64_t advance, void* workspace,
+                                 int64_t workspace_bytes, int64_t rows, void* stream) {
+    clear_error();
+    const char* who = "paged_update";
+    PoolArgs a;
+    if (int rc = pool_checks(who, dtype, k_pages, v_pages, layers, layer_stride, page_stride, token_stride,
+                             head_stride, n_pages, page_size, KVH, HD, &a))
+        return rc;
+    if (int rc = table_checks(who, table, table_ld, max_pages, page_size, rows)) return rc;
+    LOOM_CHECK(lens && refs && status, "%s: a required pointer is NULL", who);
+    LOOM_CHECK(n_new >= 0 && n_new <= max_pages * page_size && advance >= 0 && advance <= max_pages * page_size,
+               "%s: n_new=%lld and advance=%lld must lie in 0..%lld", who, (long long)n_new, (long long)advance,
+               (long long)(max_pages * page_size));
+    LOOM_CHECK(workspace_bytes >= loom_paged_update_workspace_bytes(rows) && (workspace != nullptr || rows == 0) &&
+                   ((uintptr_t)workspace % 16) == 0,
+               "%s: a 16-byte aligned workspace of %lld bytes is needed, got %lld", who,
+               (long long)loom_paged_update_workspace_bytes(rows), (long long)workspace_bytes);
+    if (rows == 0) return LOOM_OK;
+    hipStream_t st = (hipStream_t)stream;
+    const int log_ps = __builtin_ctzll((unsigned long long)page_size);
+    if (parent != nullptr) {
+        hipLaunchKernelGGL(paged_fork_kernel, dim3((unsigned)ceil_div(max_pages, kForkCols)), dim3(256),
+                           (unsigned)(rows * kForkCols * sizeof(int32_t)), st, table, table_ld, (int)max_pages, lens,
+                           refs, (int)n_pages, log_ps, parent, (int)rows, (int)advance);
+        if (int rc = launch_status("loom_paged_update(fork)")) return rc;
+    }
+    if (parent == nullptr && n_new == 0 && advance == 0) return LOOM_OK;
+    hipLaunchKernelGGL(paged_reserve_kernel, dim3(1), dim3(1024), 0, st, table, table_ld, (int)max_pages, lens, refs,
+                       (int)n_pages, log_ps, parent, (int)rows, (int)n_new, (int)advance, (PageCopy*)workspace,
+                       status);
+    if (int rc = launch_status("loom_paged_update(reserve)")) return rc;
+    if (n_new == 0) return LOOM_OK;
+    hipLaunchKernelGGL(paged_cow_kernel, dim3((unsigned)rows, (unsigned)(2 * layers)), dim3(256), 0, st, a,
+                       (const PageCopy*)workspace);
+    return launch_status("loom_paged_update(copy)");
+}
+
+extern "C" int loom_paged_write(int dtype, void* k_pages, void* v_pages, int64_t layers, int64_t layer_stride,
+                                int64_t page_stride, int64_t token_stride, int64_t head_stride, int64_t n_pages,
+                                int64_t page_size, int64_t KVH, int64_t HD, const int32_t* table, int64_t table_ld,
+                                int64_t max_pages, const void* k_rows, const void* v_rows, int64_t src_layer_stride,
+                                int64_t src_row_stride, int64_t src_head_stride, int64_t src_token_stride,
+                                int64_t src_tokens, const int32_t* first, const int32_t* last, int64_t rows,
+                                void* stream) {
+    clear_error();
+    const char* who = "paged_write";
+    PoolArgs a;
+    if (int rc = pool_checks(who, dtype, k_pages, v_pages, layers, layer_stride, page_stride, token_stride,
+                             head_stride, n_pages, page_size, KVH, HD, &a))
+        return rc;
+    if (int rc = table_checks(who, table, table_ld, max_pages, page_size, rows)) return rc;
+    const int64_t es = dtype == LOOM_F32 ? 4 : 2;
+    LOOM_CHECK(k_rows && v_rows && first && last, "%s: a required pointer is NULL", who);
+    LOOM_CHECK(src_tokens >= 0 && src_tokens <= ((int64_t)1 << 24) && src_token_stride >= HD &&
+                   src_layer_stride >= 0 && src_row_stride >= 0 && src_head_stride >= 0,
+               "%s: bad source shape", who);
+    LOOM_CHECK((src_layer_stride * es) % 16 == 0 && (src_row_stride * es) % 16 == 0 &&
+                   (src_head_stride * es) % 16 == 0 && (src_token_stride * es) % 16 == 0 &&
+                   (((uintptr_t)k_rows | (uintptr_t)v_rows) % 16) == 0,
+               "%s: the source rows and their strides must be multiples of 16 bytes", who);
+    LOOM_CHECK(2 * layers * KVH <= 65535, "%s: too many layers x heads", who);
+    if (rows == 0 || src_tokens == 0) return LOOM_OK;
+    const int64_t tiles = ceil_div(src_tokens, kWriteTile);
+    hipLaunchKernelGGL(paged_write_kernel, dim3((unsigned)tiles, (unsigned)rows, (unsigned)(2 * layers * KVH)),
+                       dim3(256), 0, (hipStream_t)stream, a, (const char*)k_rows, (const char*)v_rows,
+                       src_layer_stride * es, src_row_stride * es, src_head_stride * es, src_token_stride * es,
+                       (int)src_tokens, table, table_ld, (int)max_pages, (int)n_pages,
+                       __builtin_ctzll((unsigned long long)page_size), first, last);
+    return launch_status("loom_paged_write");
+}
+
+extern "C" int64_t loom_paged_compact_workspace_bytes(int64_t n_pages) {
+    return n_pages > 0 ? (4 + 3 * n_pages) * (int64_t)sizeof(int32_t) : 0;
+}
+
+extern "C" int loom_paged_compact(int dtype, void* k_pages, void* v_pages, int64_t layers, int64_t layer_stride,
+                                  int64_t page_stride, int64_t token_stride, int64_t head_stride, int64_t n_pages,
+                                  int64_t page_size, int64_t KVH, int64_t HD, int32_t* table, int64_t table_ld,
+                                  int64_t max_pages, int32_t* refs, int32_t* used, void* workspace,
+                                  int64_t workspace_bytes, int64_t rows, void* stream) {
+    clear_error();
+    const char* who = "paged_compact";
+    PoolArgs a;
+    if (int rc = pool_checks(who, dtype, k_pages, v_pages, layers, layer_stride, page_stride, token_stride,
+                             head_stride, n_pages, page_size, KVH, HD, &a))
+        return rc;
+    if (int rc = table_checks(who, table, table_ld, max_pages, page_size, rows)) return rc;
+    LOOM_CHECK(refs && used, "%s: a required pointer is NULL", who);
+    LOOM_CHECK(workspace_bytes >= loom_paged_compact_workspace_bytes(n_pages) && workspace != nullptr &&
+                   ((uintptr_t)workspace % 16) == 0,
+               "%s: a 16-byte aligned workspace of %lld bytes is needed, got %lld", who,
+               (long long)loom_paged_compact_workspace_bytes(n_pages), (long long)workspace_bytes);
+    hipStream_t st = (hipStream_t)stream;
+    hipLaunchKernelGGL(paged_compact_plan_kernel, dim3(1), dim3(1024), 0, st, refs, (int)n_pages, used,
+                       (int32_t*)workspace);
+    if (int rc = launch_status("loom_paged_compact(plan)")) return rc;
+    hipLaunchKernelGGL(paged_compact_move_kernel, dim3((unsigned)(8 * device_cus()), 2), dim3(256), 0, st, a,
+                       (int)page_size, (const int32_t*)workspace, (int)n_pages, table, table_ld, (int)max_pages,
+                       (int)rows);
+    return launch_status("loom_paged_compact(move)");
+}

@@ -33,6 +33,10 @@ class LinearMultiDesc(ctypes.Structure):
                 ("seg", LinearSegment * 4), ("only_if", c_void_p), ("only_if_n", c_int64),
                 ("x_frag", c_void_p), ("x2_frag", c_void_p)]
 
+# the pools of a paged cache: dtype, k, v, layers, strides (layer, page, token, head), n_pages,
+# page_size, kv heads, head_dim
+_POOL = [c_int, _P, _P] + [c_int64] * 9
+
 # name -> argument types (all return c_int status)
 SIGNATURES = {
     "loom_paraplex_forward": [c_int, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
@@ -117,6 +121,20 @@ SIGNATURES = {
                                   _P],
     "loom_decode_tria_readout": [c_int, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64,
                                  c_int64, c_int64, c_int64, c_float, c_float, _P],
+    "loom_paged_decode_step": [c_int, _P, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64,
+                               _P, c_int64, c_int64, _P, _P, _P, c_int64, _P, _P, _P, c_int64, _P,
+                               c_int64, c_int64, c_int64, c_int64, c_int64, _P],
+    "loom_paged_decode_attention": [c_int, _P, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int64,
+                                    c_int64, _P, c_int64, c_int64, _P, _P, _P, c_int64, _P, c_int64,
+                                    c_int64, c_int64, c_int64, c_int64, _P],
+    "loom_paged_update": [*_POOL, _P, c_int64, c_int64, _P, _P, _P, _P, c_int64, c_int64, _P, c_int64,
+                          c_int64, _P],
+    "loom_paged_write": [*_POOL, _P, c_int64, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int64,
+                         c_int64, _P, _P, c_int64, _P],
+    "loom_paged_compact": [*_POOL, _P, c_int64, c_int64, _P, _P, _P, c_int64, c_int64, _P],
+    "loom_beam_select": [c_int, _P, c_int64, _P, _P, _P, _P, _P, _P, c_int64, c_int64, c_int64, c_int64,
+                         c_int64, c_int64, _P, c_int64, _P],
+    "loom_reorder_rows": [c_int64, _P, _P, _P, _P, _P, _P, c_int64, _P],
 }
 # entry points that return a value instead of a status
 QUERIES = {"loom_gqa_workspace_bytes": ([c_int64] * 5, c_int64),
@@ -126,6 +144,10 @@ QUERIES = {"loom_gqa_workspace_bytes": ([c_int64] * 5, c_int64),
            "loom_ffn_decode_desc_bytes": ([], c_int64),
            "loom_linear_ln_workspace_bytes": ([c_int64, c_int64], c_int64),
            "loom_tria_chunked_workspace_bytes": ([c_int64] * 4, c_int64),
+           "loom_paged_decode_workspace_bytes": ([c_int64] * 5, c_int64),
+           "loom_paged_update_workspace_bytes": ([c_int64], c_int64),
+           "loom_paged_compact_workspace_bytes": ([c_int64], c_int64),
+           "loom_beam_select_workspace_bytes": ([c_int64] * 4, c_int64),
            "loom_tria_chunked_fires_workspace_bytes": ([c_int64, c_int64, c_int64, _P, c_int64],
                                                        c_int64)}
 
