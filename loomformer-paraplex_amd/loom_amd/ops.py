@@ -559,102 +559,21 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 # ---------------------------------------------------------------- paged cache, beam search
 # (no counterparts in the reference: its decode is greedy over one dense cache)
 
-def _on(dev: torch.device, name: str, *args) -> None:
-    """The call on the current stream of `dev`, which need not be the current device."""
-    if torch.cuda.current_device() == dev.index:
-        call(name, *args, raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            call(name, *args, raw_stream(dev))
+_host_module = None
 
 
-def _query(dev: torch.device, name: str, *args) -> int:
-    """A workspace query, which goes by the device it is for."""
-    lib = _lib.load()
-    if torch.cuda.current_device() == dev.index:
-        return getattr(lib, name)(*args)
-    with torch.cuda.device(dev):
-        return getattr(lib, name)(*args)
-
-
-def _i32(name: str, what: str, t: torch.Tensor, shape, dev) -> torch.Tensor:
-    _check(t.is_cuda and t.device == dev and t.dtype is torch.int32 and t.shape == shape and t.is_contiguous(),
-           f"{name}: {what} must be a contiguous int32 tensor of shape {list(shape)} on {dev}")
-    return t
-
-
-def _table(name: str, table: torch.Tensor, rows: Optional[int], dev) -> torch.Tensor:
-    _check(table.is_cuda and table.device == dev and table.dtype is torch.int32 and table.dim() == 2
-           and (rows is None or table.shape[0] == rows) and (table.stride(1) == 1 or table.shape[1] == 1),
-           f"{name}: table must be an int32 [rows, max_pages] tensor of dense rows on {dev}")
-    return table
-
-
-def _table_ld(table: torch.Tensor) -> int:
-    """Row stride of a table (of one row: its width)."""
-    return table.stride(0) if table.shape[0] > 1 else max(table.shape[1], table.stride(0))
-
-
-def _pools(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor, dim: int) -> None:
-    _check(k_pages.is_cuda and v_pages.is_cuda, f"{name}: all inputs must be CUDA tensors")
-    _check(k_pages.dim() == dim and k_pages.shape == v_pages.shape and k_pages.stride() == v_pages.stride()
-           and k_pages.stride(-1) == 1,
-           f"{name}: k_pages and v_pages must be [{'layers, ' if dim == 5 else ''}pages, kv_heads, page_size, head_dim] "
-           "tensors of the same layout with dense heads")
-    _check(k_pages.dtype == v_pages.dtype and k_pages.dtype in _FLOATS and k_pages.device == v_pages.device,
-           f"{name}: k_pages and v_pages must have one dtype and one device")
-
-
-def _pool_args(k: torch.Tensor, v: torch.Tensor):
-    L, NP, KVH, PS, HD = k.shape
-    s = k.stride()
-    return (dtype_code(k), addr(k), addr(v), L, s[0], s[1], s[3], s[2], NP, PS, KVH, HD)
-
-
-def _paged_attention(name: str, step: bool, q, k_pages, v_pages, table, lens, cos, sin, want_kctx: bool):
-    _pools(name, k_pages, v_pages, 4)
-    dev, dt = k_pages.device, k_pages.dtype
-    NP, KVH, PS, HD = k_pages.shape
-    _check(q.is_cuda and q.device == dev and q.dtype is dt, f"{name}: {'qkv' if step else 'q'} must have the pools' dtype and device")
-    B = q.shape[0]
-    if step:
-        _check(q.dim() == 2 and HD > 0 and q.shape[1] % HD == 0 and q.shape[1] // HD > 2 * KVH,
-               f"{name}: qkv must be [rows, (q_heads + 2 kv_heads) * head_dim]")
-        QH = q.shape[1] // HD - 2 * KVH
-        for t in (cos, sin):
-            _check(t.is_cuda and t.device == dev and t.dtype is torch.float32 and t.dim() == 2 and t.shape[1] == HD
-                   and t.shape == cos.shape and t.is_contiguous(),
-                   f"{name}: cos and sin must be contiguous float32 [positions, head_dim] tables")
-        if q.stride(1) != 1:
-            q = q.contiguous()
-    else:
-        _check(q.dim() == 3 and q.shape[2] == HD, f"{name}: q must be [rows, q_heads, head_dim]")
-        QH = q.shape[1]
-        if q.stride(2) != 1 or q.stride(1) != HD:
-            q = q.contiguous()
-    _check(QH % KVH == 0, f"{name}: {QH} query heads over {KVH} kv heads")
-    _table(name, table, B, dev)
-    _i32(name, "lens", lens, (B,), dev)
-    width = (QH + 2 * KVH) * HD if step else QH * HD
-    ld = q.stride(0) if B > 1 else width
-    if q.data_ptr() % 16 or (ld * q.element_size()) % 16 or ld < width:     # rows the kernels can load
-        q = q.clone(memory_format=torch.contiguous_format)
-        ld = width
-    MP = table.shape[1]
-    c = torch.empty((B, QH, HD), dtype=dt, device=dev)
-    kctx = torch.empty_like(c) if want_kctx else None
-    nws = _query(dev, "loom_paged_decode_workspace_bytes", B, MP * PS, QH, KVH, HD)
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
-    s = k_pages.stride()
-    args = (dtype_code(k_pages), addr(q), ld, addr(k_pages), addr(v_pages), s[0], s[2], s[1], NP, PS, addr(table),
-            _table_ld(table), MP, addr(lens))
-    tail = (QH * HD, addr(ws), nws, B, QH, KVH, HD)
-    if step:
-        qo = torch.empty_like(c)
-        _on(dev, "loom_paged_decode_step", *args, addr(cos), addr(sin), cos.shape[0], addr(qo), addr(c), addr(kctx), *tail)
-        return [c, kctx, qo]
-    _on(dev, "loom_paged_decode_attention", *args, addr(c), addr(kctx), *tail)
-    return [c, kctx]
+def _host():
+    """The compiled host module of these operators (csrc/host_ops.cpp); there is no fallback."""
+    global _host_module
+    if _host_module is None:
+        _lib.load()
+        try:
+            from . import _host as m
+        except ImportError as e:
+            raise RuntimeError(f"loom_amd._host cannot be loaded ({e}); build it with "
+                               "`python loomformer-paraplex_amd/build_lib.py` (or __graft_entry__.build())") from e
+        _host_module = m
+    return _host_module
 
 
 def paged_decode_step(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
@@ -670,14 +589,14 @@ def paged_decode_step(qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     page and returns [c, kctx or None, q]: A.V, A.K_roped and the roped q, each
     [rows, q_heads, head_dim].  lens is not advanced (paged_update does).  Idle
     rows give zeros; rows without room or with a missing page give NaN."""
-    return _paged_attention("paged_decode_step", True, qkv, k_pages, v_pages, table, lens, cos, sin, want_kctx)
+    return (_host_module or _host()).paged_decode_step(qkv, k_pages, v_pages, table, lens, cos, sin, want_kctx)
 
 
 def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
                            lens: torch.Tensor, want_kctx: bool = True) -> List[Optional[torch.Tensor]]:
     """The attention of paged_decode_step alone: q [rows, q_heads, head_dim], roped
     already, over the row's lens[r] tokens (none: zeros).  Returns [c, kctx or None]."""
-    return _paged_attention("paged_decode_attention", False, q, k_pages, v_pages, table, lens, None, None, want_kctx)
+    return (_host_module or _host()).paged_decode_attention(q, k_pages, v_pages, table, lens, want_kctx)
 
 
 def paged_update(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
@@ -690,19 +609,7 @@ def paged_update(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tens
     taken from the free ones, a shared last page copied).  refs [pages] counts
     the holders of each page; status [1] is raised where pages ran out.  All
     bookkeeping is on the device."""
-    name = "paged_update"
-    _pools(name, k_pages, v_pages, 5)
-    dev = k_pages.device
-    _table(name, table, None, dev)
-    R = table.shape[0]
-    _i32(name, "lens", lens, (R,), dev)
-    _i32(name, "refs", refs, (k_pages.shape[1],), dev)
-    _i32(name, "status", status, (1,), dev)
-    if parent is not None:
-        _i32(name, "parent", parent, (R,), dev)
-    ws = torch.empty(16 * R, dtype=torch.uint8, device=dev)
-    _on(dev, "loom_paged_update", *_pool_args(k_pages, v_pages), addr(table), _table_ld(table), table.shape[1],
-        addr(lens), addr(refs), addr(status), addr(parent), int(n_new), int(advance), addr(ws), 16 * R, R)
+    (_host_module or _host()).paged_update(k_pages, v_pages, table, lens, refs, status, parent, n_new, advance)
 
 
 def paged_write(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, k_rows: torch.Tensor,
@@ -710,39 +617,14 @@ def paged_write(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tenso
     """Copies positions first[r] .. last[r] - 1 of row r of a dense cache
     [layers, rows, kv_heads, positions, head_dim] into the row's pages (which
     paged_update made writable).  first, last: int32 [rows]."""
-    name = "paged_write"
-    _pools(name, k_pages, v_pages, 5)
-    dev = k_pages.device
-    _table(name, table, None, dev)
-    R = table.shape[0]
-    L, _, KVH, _, HD = k_pages.shape
-    _check(k_rows.is_cuda and k_rows.device == dev and v_rows.device == dev and k_rows.dtype == v_rows.dtype == k_pages.dtype
-           and k_rows.dim() == 5 and k_rows.shape == v_rows.shape and k_rows.stride() == v_rows.stride()
-           and k_rows.shape[:3] == (L, R, KVH) and k_rows.shape[4] == HD and k_rows.stride(4) == 1,
-           f"{name}: k_rows and v_rows must be [layers, rows, kv_heads, positions, head_dim] tensors of the pools' dtype "
-           "and one layout")
-    _i32(name, "first", first, (R,), dev)
-    _i32(name, "last", last, (R,), dev)
-    s = k_rows.stride()
-    _on(dev, "loom_paged_write", *_pool_args(k_pages, v_pages), addr(table), _table_ld(table), table.shape[1],
-        addr(k_rows), addr(v_rows), s[0], s[1], s[2], s[3], k_rows.shape[3], addr(first), addr(last), R)
+    (_host_module or _host()).paged_write(k_pages, v_pages, table, k_rows, v_rows, first, last)
 
 
 def paged_compact(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, refs: torch.Tensor,
                   used: torch.Tensor) -> None:
     """Moves the pages in use to the lowest ids of the pools, in place (tables and
     refs follow); used [1] int32 = their number."""
-    name = "paged_compact"
-    _pools(name, k_pages, v_pages, 5)
-    dev = k_pages.device
-    _table(name, table, None, dev)
-    NP = k_pages.shape[1]
-    _i32(name, "refs", refs, (NP,), dev)
-    _i32(name, "used", used, (1,), dev)
-    nws = 4 * (4 + 3 * NP)
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev)
-    _on(dev, "loom_paged_compact", *_pool_args(k_pages, v_pages), addr(table), _table_ld(table), table.shape[1],
-        addr(refs), addr(used), addr(ws), nws, table.shape[0])
+    (_host_module or _host()).paged_compact(k_pages, v_pages, table, refs, used)
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_out: Optional[int] = None,
@@ -753,36 +635,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_out: Optional[int]
     score).  Returns [scores [groups, n_out], parent int32 (the row of logits),
     token int64, finished bool], in order, ties by the lowest (beam, token);
     places without a candidate hold -inf, the group's first row, pad_id, False."""
-    name = "beam_select"
-    _check(logits.is_cuda and scores.is_cuda, f"{name}: all inputs must be CUDA tensors")
-    dev = logits.device
-    _check(logits.dim() == 2 and logits.dtype in _FLOATS, f"{name}: logits must be a float32, bfloat16 or float16 [rows, V] tensor")
-    _check(scores.device == dev and scores.dtype is torch.float32 and scores.dim() == 2
-           and scores.numel() == logits.shape[0], f"{name}: scores must be a float32 [groups, beams] tensor, a value for each row of logits")
-    S, W = scores.shape
-    V = logits.shape[1]
-    K = W if n_out is None else int(n_out)
-    x = logits if V == 1 or logits.stride(1) == 1 else logits.contiguous()
-    ld = x.stride(0) if S * W > 1 else V
-    if ld < V:
-        x = x.contiguous()
-        ld = V
-    sc = scores.contiguous()
-    fin = None
-    if finished is not None:
-        _check(finished.is_cuda and finished.device == dev and finished.dtype is torch.bool and finished.numel() == S * W,
-               f"{name}: finished must be a bool tensor with a value for each row of logits")
-        fin = finished.contiguous()
-    _check(K >= 1, f"{name}: n_out must be at least 1")
-    out = torch.empty((S, K), dtype=torch.float32, device=dev)
-    parent = torch.empty((S, K), dtype=torch.int32, device=dev)
-    token = torch.empty((S, K), dtype=torch.int64, device=dev)
-    fo = torch.empty((S, K), dtype=torch.bool, device=dev)
-    nws = _query(dev, "loom_beam_select_workspace_bytes", S, W, V, K)
-    ws = torch.empty(nws, dtype=torch.uint8, device=dev) if nws else None
-    _on(dev, "loom_beam_select", dtype_code(x), addr(x), ld, addr(sc), addr(fin), addr(out), addr(parent),
-        addr(token), addr(fo), S, W, V, K, int(eos_id), int(pad_id), addr(ws), nws)
-    return [out, parent, token, fo]
+    return (_host_module or _host()).beam_select(logits, scores, n_out, finished, eos_id, pad_id)
 
 
 def reorder_rows(tensors: Sequence[torch.Tensor], parent: torch.Tensor, dims: Optional[Sequence[int]] = None) -> None:
@@ -790,38 +643,4 @@ def reorder_rows(tensors: Sequence[torch.Tensor], parent: torch.Tensor, dims: Op
     [rows]; a parent outside [0, rows): the row stays).  dims: each tensor's row
     dimension (default 0); what follows it must be dense, what precedes it one
     run of equal steps.  One launch for up to 16 tensors, which must not overlap."""
-    name = "reorder_rows"
-    _check(parent.is_cuda and parent.dtype is torch.int32 and parent.dim() == 1 and parent.is_contiguous(),
-           f"{name}: parent must be a contiguous CUDA int32 tensor")
-    dev, R = parent.device, parent.shape[0]
-    dims = [0] * len(tensors) if dims is None else list(dims)
-    _check(len(dims) == len(tensors), f"{name}: one dimension per tensor")
-    segs = []
-    for t, d in zip(tensors, dims):
-        _check(t.is_cuda and t.device == dev and 0 <= d < t.dim() and t.shape[d] == R,
-               f"{name}: every tensor must be on {dev} and have {R} rows in its row dimension")
-        es, shape, st = t.element_size(), t.shape, t.stride()
-        inner = 1
-        for k in range(t.dim() - 1, d, -1):
-            _check(shape[k] == 1 or st[k] == inner, f"{name}: the rows of a tensor must be dense")
-            inner *= shape[k]
-        outer, step = 1, 0
-        for k in range(d - 1, -1, -1):
-            if shape[k] == 1:
-                continue
-            _check(outer == 1 or st[k] == step * outer, f"{name}: the dimensions before the row dimension must be one run of equal steps")
-            step = st[k] if outer == 1 else step
-            outer *= shape[k]
-        row = st[d] if R > 1 else inner
-        # rows, and the slices that hold them, lie apart from each other
-        _check(row >= inner and (outer == 1 or step >= row * (R - 1) + inner or (row >= step * (outer - 1) + inner and step >= inner)),
-               f"{name}: the rows of a tensor must not overlap")
-        segs.append((t.data_ptr(), outer, step * es, row * es, inner * es))
-    if not segs or R == 0:
-        return
-    for i in range(0, len(segs), 16):
-        part = segs[i:i + 16]
-        n = len(part)
-        cols = list(zip(*part))
-        a = [(ctypes.c_void_p * n)(*cols[0])] + [(ctypes.c_int64 * n)(*c) for c in cols[1:]]
-        _on(dev, "loom_reorder_rows", n, *a, addr(parent), R)
+    (_host_module or _host()).reorder_rows(tensors, parent, dims)
