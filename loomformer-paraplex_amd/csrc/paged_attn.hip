@@ -7,8 +7,9 @@
 // its own maximum m and sum l, and the join weighs them by e^(m - max m).
 //
 // The rows have lengths of their own that only the device knows, so the host
-// launches a fixed number of blocks and every block works out its share
-// (plan_item): chunks of equal size over all rows, as many as fill the device.
+// launches a fixed number of blocks and every block works out its share from
+// lens (make_plan): either chunks of equal size, at most one per block, or, where
+// a block has many tiles to do, equal stretches of all rows laid end to end.
 #include "attn_tile.h"
 
 namespace loom {
@@ -18,7 +19,10 @@ typedef __bf16 pg_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 pg_f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kPgTile = 32;       // tokens of one wave step of the matrix-core form
-constexpr int kPgMinTiles = 4;    // tokens of a chunk: at least one tile per wave
+constexpr int kPgMinTiles = 4;    // tiles of a chunk at least: one per wave
+constexpr int kPgStream = 16;     // tiles per block from which the rows are laid end to end
+constexpr int kPgRowCost = 2;     // what starting on a row costs a block, in tiles
+constexpr int kPgWhole = 512;     // rows of up to so many tokens are not split
 constexpr int kPgMaxRows = 1024;
 
 template <typename T>
@@ -40,7 +44,8 @@ struct PagedArgs {
     float* rec;            // chunk records: [item, QH, 2 HD] then [item, QH, 2]
     int64_t rec_ml;        // float offset of the second part
     int n_pages, log_ps, cap, n_pos;
-    int B, QH, KVH, G, target;
+    int B, QH, KVH, G;
+    int slots;             // blocks per kv head to share the work among; 0: a block per row
     float qscale;
 };
 
@@ -53,69 +58,155 @@ __device__ __forceinline__ int row_tokens(const int32_t* lens, int b, int step, 
     return n < 0 || *bad ? 0 : n + step;
 }
 
-// The share of a block: which row and which of its chunks.  Every wave works
-// it out by itself (64 rows per lane step), so no barrier is needed.
-struct PlanItem {
-    int row, chunk, nchunk, item0, tokens;   // item0: the record of the row's chunk 0
-    bool bad;
-};
-
 __device__ __forceinline__ int wave_sum_int(int v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
+    v += __builtin_amdgcn_update_dpp(0, v, kDppQuad1032, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, kDppQuad2301, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, kDppHalfMirror, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, kDppMirror, 0xF, 0xF, false);
+    return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) +
+           __builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48);
+}
+
+// inclusive scan over the wave
+__device__ __forceinline__ int wave_scan_int(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);      // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);      // lane 15 to row 1, 47 to row 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);      // lane 31 to rows 2, 3
     return v;
 }
 
-// Tiles per chunk: the rows' tiles over `target` chunks, at least kPgMinTiles.
-__device__ __forceinline__ int plan_chunk_tiles(const int32_t* lens, int B, int step, int cap,
-                                                int n_pos, int target) {
-    const int lane = threadIdx.x & 63;
-    int total = 0;
-    for (int b0 = 0; b0 < B; b0 += 64) {
-        bool bad;
-        const int b = b0 + lane;
-        const int n = b < B ? row_tokens(lens, b, step, cap, n_pos, &bad) : 0;
-        total += wave_sum_int((n + kPgTile - 1) / kPgTile);
-    }
-    return max(kPgMinTiles, (total + target - 1) / target);
+// Lanes 16 and 32 apart: the two values of each pair in every lane of it
+__device__ __forceinline__ float2 pair16(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float2 pair32(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_16_32(float v) {
+    float2 p = pair16(v, v);
+    v = fmaxf(p.x, p.y);
+    p = pair32(v, v);
+    return fmaxf(p.x, p.y);
+}
+__device__ __forceinline__ float sum_16_32(float v) {
+    float2 p = pair16(v, v);
+    v = p.x + p.y;
+    p = pair32(v, v);
+    return p.x + p.y;
 }
 
-// by_row: the plan of row `want`; else of item `want` (row = -1: none).
-template <bool BY_ROW>
-__device__ __forceinline__ PlanItem plan_item(const int32_t* lens, int B, int step, int cap,
-                                              int n_pos, int target, int want) {
+// Tiles of a row of n tokens; a row of none counts as one, which writes its outputs.
+__device__ __forceinline__ int row_tiles(int n) { return n > 0 ? (n + kPgTile - 1) / kPgTile : 1; }
+
+// How the rows' tiles are shared out.  q > 0: block j takes units j q .. (j+1) q - 1
+// of the rows laid end to end, a row being kPgRowCost units and its tiles.  Else a
+// row of t tiles is cut into slots * t / total equal chunks (at least one, each of
+// kPgMinTiles or more), one block each: no more chunks than slots, but for rows
+// of less than a chunk (a block more than the device holds at once would run
+// after all others).
+struct Plan {
+    int q, slots, total;
+};
+
+template <bool STEP>
+__device__ __forceinline__ Plan make_plan(const int32_t* lens, int B, int cap, int n_pos, int slots) {
+    if (slots == 0) return Plan{0, 0, 1};
+    int total = 0;
+    bool bad;
+    for (int b = threadIdx.x & 63; b < B; b += 64) total += row_tiles(row_tokens(lens, b, STEP, cap, n_pos, &bad));
+    total = wave_sum_int(total);
+    const bool stream = total >= kPgStream * slots;
+    return Plan{stream ? (total + B * kPgRowCost + slots - 1) / slots : 0, slots, total};
+}
+
+__device__ __forceinline__ int plan_units(const Plan& p, int tiles) {
+    if (p.q > 0) return tiles + kPgRowCost;
+    const uint32_t n = (uint32_t)tiles * (uint32_t)p.slots / (uint32_t)p.total;      // (< 2^19 * 2^9)
+    return max(1, (int)min(n, (uint32_t)(tiles + kPgMinTiles - 1) / kPgMinTiles));
+}
+
+// A row's place in the plan: the units before it, its tokens
+struct PlanRow {
+    int row, before, tokens;
+    bool bad;
+};
+
+// The row that unit x lies in (BY_ROW: row x); row = -1: behind the last.
+template <bool STEP, bool BY_ROW>
+__device__ __forceinline__ PlanRow plan_find(const Plan& p, const int32_t* lens, int B, int cap, int n_pos, int x) {
     const int lane = threadIdx.x & 63;
-    const int ct = plan_chunk_tiles(lens, B, step, cap, n_pos, target);
-    PlanItem it;
-    it.row = -1;
     int base = 0;
     for (int b0 = 0; b0 < B; b0 += 64) {
         const int b = b0 + lane;
         bool bad = false;
-        const int n = b < B ? row_tokens(lens, b, step, cap, n_pos, &bad) : 0;
-        const int nch = b < B ? max(1, ((n + kPgTile - 1) / kPgTile + ct - 1) / ct) : 0;
-        int incl = nch;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int o = __shfl_up(incl, d, 64);
-            if (lane >= d) incl += o;
-        }
-        const int first = base + incl - nch;
-        const bool mine = BY_ROW ? b == want : (b < B && want >= first && want < first + nch);
+        const int n = b < B ? row_tokens(lens, b, STEP, cap, n_pos, &bad) : 0;
+        const int u = b < B ? plan_units(p, row_tiles(n)) : 0;
+        const int incl = wave_scan_int(u);
+        const int first = base + incl - u;
+        const bool mine = b < B && (BY_ROW ? b == x : x >= first && x < first + u);
         const unsigned long long who = __ballot(mine);
         if (who) {
-            const int src = __ffsll(who) - 1;
-            it.row = b0 + src;
-            it.nchunk = __builtin_amdgcn_readlane(nch, src);
-            it.item0 = __builtin_amdgcn_readlane(first, src);
-            it.tokens = __builtin_amdgcn_readlane(n, src);
-            it.bad = __builtin_amdgcn_readlane((int)bad, src) != 0;
-            it.chunk = want - it.item0;
-            return it;
+            const int src = __builtin_amdgcn_readfirstlane(__ffsll(who) - 1);
+            return PlanRow{b0 + src, __builtin_amdgcn_readlane(first, src), __builtin_amdgcn_readlane(n, src),
+                           __builtin_amdgcn_readlane((int)bad, src) != 0};
         }
         base += __builtin_amdgcn_readlane(incl, 63);
     }
+    return PlanRow{-1, 0, 0, false};
+}
+
+// What block j does of a row: tiles tile0 .. tile1 - 1 (none: tile0 >= tile1),
+// as chunk `chunk` of nchunk, whose records start at item0 (block + row along the
+// staircase of blocks and rows: a number of its own for each pair).
+struct PlanItem {
+    int row, tokens, tile0, tile1, chunk, nchunk, item0;
+    bool bad;
+};
+
+__device__ __forceinline__ PlanItem plan_item(const Plan& p, const PlanRow& r, int j) {
+    PlanItem it;
+    it.row = r.row;
+    it.tokens = r.tokens;
+    it.bad = r.bad;
+    const int t = row_tiles(r.tokens);
+    if (p.q > 0) {
+        const int p0 = r.before + kPgRowCost;        // the row's first tile
+        const int first = (int)((uint32_t)p0 / (uint32_t)p.q);
+        it.nchunk = (int)((uint32_t)(p0 + t - 1) / (uint32_t)p.q) - first + 1;
+        it.chunk = j - first;
+        it.tile0 = max(j * p.q - p0, 0);
+        it.tile1 = min((j + 1) * p.q - p0, t);
+        it.item0 = first + r.row;
+    } else {
+        it.nchunk = plan_units(p, t);
+        it.chunk = j - r.before;
+        it.tile0 = (int)((uint32_t)it.chunk * (uint32_t)t / (uint32_t)it.nchunk);
+        it.tile1 = (int)((uint32_t)(it.chunk + 1) * (uint32_t)t / (uint32_t)it.nchunk);
+        it.item0 = r.before;
+    }
     return it;
+}
+
+// The rows of block j, one after the other: f(PlanItem).
+template <bool STEP, typename F>
+__device__ __forceinline__ void plan_walk(const int32_t* lens, int B, int cap, int n_pos, int slots, int j, F f) {
+    const Plan p = make_plan<STEP>(lens, B, cap, n_pos, slots);
+    PlanRow r = plan_find<STEP, false>(p, lens, B, cap, n_pos, p.q > 0 ? j * p.q : j);
+    if (r.row < 0) return;
+    while (true) {
+        const PlanItem it = plan_item(p, r, j);
+        if (it.tile0 < it.tile1) f(it);
+        if (p.q == 0) return;
+        r.before += plan_units(p, row_tiles(r.tokens));
+        if (++r.row >= B || r.before >= (j + 1) * p.q) return;
+        r.tokens = __builtin_amdgcn_readfirstlane(row_tokens(lens, r.row, STEP, cap, n_pos, &r.bad));
+        r.bad = __builtin_amdgcn_readfirstlane((int)r.bad) != 0;
+    }
 }
 
 // Element pair helpers by type
@@ -140,35 +231,44 @@ template <> struct Mfma16<f16_t> {
     }
 };
 
-// One element d of a head, roped: x cos + rotate_half(x) sin
+// Eight elements of a head from d0 on (a multiple of 8, as HD / 2 is) as they are
+// loaded for the rotation x cos + rotate_half(x) sin: all loads first, so that a
+// row's are one wait.
 template <typename T>
-__device__ __forceinline__ float paged_rope(const T* head, const float* cr, const float* sr, int d,
-                                            int HD) {
-    const int half = HD / 2;
-    const float x = ld(head + d), y = ld(head + (d < half ? d + half : d - half));
-    return fmaf(x, cr[d], (d < half ? -y : y) * sr[d]);
-}
-
-// Eight of them from d0 on (a multiple of 8, as HD / 2 is)
-template <typename T>
-__device__ __forceinline__ void paged_rope8(const T* head, const float* cr, const float* sr, int d0,
-                                            int HD, float out[8]) {
-    const int half = HD / 2;
-    float x[8], y[8], c[8], s[8];
-    Vec8<T>::load(head + d0, x);
-    Vec8<T>::load(head + (d0 < half ? d0 + half : d0 - half), y);
-    Vec8<float>::load(cr + d0, c);
-    Vec8<float>::load(sr + d0, s);
-    const float sg = d0 < half ? -1.0f : 1.0f;
+struct Rope8 {
+    uint4 x, y;
+    float c[8], s[8];
+    bool low;                                        // of the first half: x cos - y sin
+    __device__ __forceinline__ void load(const T* head, const float* cr, const float* sr, int d0, int HD) {
+        const int half = HD / 2;
+        low = d0 < half;
+        x = *reinterpret_cast<const uint4*>(head + d0);
+        y = *reinterpret_cast<const uint4*>(head + (low ? d0 + half : d0 - half));
+        Vec8<float>::load(cr + d0, c);
+        Vec8<float>::load(sr + d0, s);
+    }
+    __device__ __forceinline__ uint4 packed() const {
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+        uint32_t o[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) out[e] = fmaf(x[e], c[e], sg * y[e] * s[e]);
-}
+        for (int k = 0; k < 4; ++k) {
+            float v[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const T xe{(uint16_t)(xs[k] >> (16 * h))}, ye{(uint16_t)(ys[k] >> (16 * h))};
+                v[h] = fmaf(ld(&xe), c[2 * k + h], (low ? -ld(&ye) : ld(&ye)) * s[2 * k + h]);
+            }
+            o[k] = Mfma16<T>::pack(v[0], v[1]);
+        }
+        return make_uint4(o[0], o[1], o[2], o[3]);
+    }
+};
 
-// The end of a chunk: the four waves' (m, l, C, Kctx) of `g1 - g0` heads from
-// LDS (wave w, head j: wm[w][j], wl[w][j], and wacc + ((w * NH + j) * 2 + which) * HD)
+// The end of a chunk: the NW waves' (m, l, C, Kctx) of nh heads from LDS (wave w,
+// head j: wm[j][w], wl[j][w], and wacc + ((w * NH + j) * 2 + which) * HD)
 // joined into the chunk's record, or into the outputs when it is the row's only
 // chunk.  A sum of 0 (no token) gives zeros; NaN weights stay NaN.
-template <typename T>
+template <int NW, typename T>
 __device__ __forceinline__ void paged_finish(const PagedArgs<T>& a, const PlanItem& it, int h0, int nh,
                                              int NH, int HD, bool kctx, bool broken, const float* wm,
                                              const float* wl, const float* wacc) {
@@ -176,13 +276,13 @@ __device__ __forceinline__ void paged_finish(const PagedArgs<T>& a, const PlanIt
         const int j = k / HD, d = k - j * HD, h = h0 + j;
         float m = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) m = fmaxf(m, wm[w * NH + j]);
+        for (int w = 0; w < NW; ++w) m = fmaxf(m, wm[j * NW + w]);
         float l = 0.0f, c = 0.0f, kx = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(wm[w * NH + j] - m);
+        for (int w = 0; w < NW; ++w) {
+            const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(wm[j * NW + w] - m);
             const float* acc = wacc + (size_t)((w * NH + j) * 2) * HD + d;
-            l = fmaf(wl[w * NH + j], f, l);
+            l = fmaf(wl[j * NW + w], f, l);
             c = fmaf(acc[0], f, c);
             if (kctx) kx = fmaf(acc[HD], f, kx);
         }
@@ -205,14 +305,14 @@ __device__ __forceinline__ void paged_finish(const PagedArgs<T>& a, const PlanIt
 }
 
 // ------------------------------------------------------------------ matrix-core form
-// 16-bit types, HD 32 / 64 / 96 / 128, up to 16 query heads per kv head.  Four
+// 16-bit types, HD 32 / 64 / 96 / 128, up to 16 query heads per kv head.  NW
 // waves, each 32 tokens at a time through LDS tiles of its own (no barrier in the
 // loop): S^T = K Q^T, P from the score registers, C = P V and Kctx = P K through
 // the transposing LDS read.  A 16-token half of a tile lies in one page (pages
 // hold a multiple of 16 tokens), so its base address and its bound are scalar:
 // rows past the chunk's end and pages that are missing load zeros.
-template <typename T, int HD, bool STEP, bool KCTX>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+template <typename T, int HD, int NW, bool STEP, bool KCTX>
+__global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 paged_mfma_kernel(PagedArgs<T> a) {
     constexpr int KK = HD / 32, DT = HD / 16, CPR = HD / 8;
     constexpr int NH2 = CPR / 4;              // load instructions per 16-row half
@@ -221,30 +321,17 @@ paged_mfma_kernel(PagedArgs<T> a) {
         gqa_u4 k[kPgTile * CPR];
         gqa_u4 v[kPgTile * CPR];
     };
-    constexpr int kTileBytes = 4 * (int)sizeof(Tiles);
-    constexpr int kRedBytes = 4 * NH * (2 + 2 * HD) * (int)sizeof(float);
+    constexpr int kTileBytes = NW * (int)sizeof(Tiles);
+    constexpr int kRedBytes = NW * NH * (2 + 2 * HD) * (int)sizeof(float);
     __shared__ __align__(16) unsigned char lds[kTileBytes > kRedBytes ? kTileBytes : kRedBytes];
-    __shared__ uint4 knew[HD / 8], vnew[HD / 8];
+    __shared__ uint4 heads[STEP ? 18 * CPR : 1];      // q of up to 16 heads, k, v of the new token
     using M = Mfma16<T>;
-    const int kvh = blockIdx.y;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int kvh = blockIdx.y, G = a.G;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int lr = lane & 15, lq = lane >> 4;
-    const PlanItem it = plan_item<false>(a.lens, a.B, STEP, a.cap, a.n_pos, a.target, blockIdx.x);
-    if (it.row < 0) return;
-    const int G = a.G;
-    const int64_t b = it.row;
-    const int pos = it.tokens - 1;
-    const int tiles = (it.tokens + kPgTile - 1) / kPgTile;
-    const int tile0 = (int)((int64_t)it.chunk * tiles / it.nchunk);
-    const int tile1 = (int)((int64_t)(it.chunk + 1) * tiles / it.nchunk);
-    const int t1 = min(tile1 * kPgTile, it.tokens);
-    const int nstep = (tile1 - tile0 + 3) / 4;
-    const int32_t* trow = a.table + b * a.table_ld;
     const int ps_mask = (1 << a.log_ps) - 1;
     Tiles& tl = reinterpret_cast<Tiles*>(lds)[wave];
     const TileLane<CPR> tln(lq, lr);
-    bool broken = it.bad;
-
     // byte offset of this lane's piece of load i inside a 16-row half
     uint32_t loff[NH2];
 #pragma unroll
@@ -252,199 +339,218 @@ paged_mfma_kernel(PagedArgs<T> a) {
         const int j = i * 64 + lane, row = j / CPR, c = j - row * CPR;
         loff[i] = (uint32_t)(row * a.ps_tok * (int)sizeof(T)) + 16 * c;
     }
-    gqa_u4 kr[2 * NH2], vr[2 * NH2];
-    auto load_kv = [&](int ts) {
+    plan_walk<STEP>(a.lens, a.B, a.cap, a.n_pos, a.slots, blockIdx.x, [&](const PlanItem& it) {
+        const int64_t b = it.row;
+        const int pos = it.tokens - 1;
+        const int t1 = min(it.tile1 * kPgTile, it.tokens);
+        const int ts0 = (it.tile0 + wave) * kPgTile;
+        const int32_t* trow = a.table + b * a.table_ld;
+        bool broken = it.bad;
+        // page of each half of the tile at ts (past the chunk's end: of no use)
+        auto pages_of = [&](int ts, int (&pg)[2]) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int t = ts + 16 * h;
-            const int rows = min(16, t1 - t);             // tokens of this half (<= 0: none)
-            int bytes = 0;
-            int64_t off = 0;
-            if (rows > 0) {
-                const int page = __builtin_amdgcn_readfirstlane(trow[t >> a.log_ps]);
-                if ((unsigned)page < (unsigned)a.n_pages) {
-                    bytes = ((rows - 1) * (int)a.ps_tok + HD) * (int)sizeof(T);
-                    off = (int64_t)page * a.ps_page + (int64_t)(t & ps_mask) * a.ps_tok + kvh * a.ps_head;
-                } else {
-                    broken = true;
+            for (int h = 0; h < 2; ++h) pg[h] = trow[min(ts + 16 * h, a.cap - 1) >> a.log_ps];
+        };
+        int pg[2];
+        pages_of(ts0, pg);
+
+        // the new token's heads, roped and rounded by one thread per eight elements
+        // (q of the block's heads, then k, then v); all waves take q from LDS, and in
+        // the block of the row's last chunk the tile that holds the new token takes
+        // (k, v) from there: nothing in this launch depends on the row in the pool
+        const T* qrow = a.q + b * a.q_ld;
+        const bool holds_new = STEP && it.tokens > 0 && it.chunk == it.nchunk - 1;
+        constexpr int kNew = 18 * CPR / (NW * 64) + 1;       // rounds for 16 + 2 heads
+        Rope8<T> rq[STEP ? kNew : 1];
+        int pgn = -1;
+        if constexpr (STEP) {
+            if (holds_new) pgn = trow[pos >> a.log_ps];
+            if (it.tokens > 0) {
+                const float* cr = a.cosv + (int64_t)pos * HD;
+                const float* sr = a.sinv + (int64_t)pos * HD;
+#pragma unroll
+                for (int n = 0; n < kNew; ++n) {
+                    const int i = tid + n * NW * 64, hh = i / CPR;
+                    if (hh >= G + 2) continue;
+                    const int h = hh < G ? kvh * G + hh : a.QH + kvh + (hh - G) * a.KVH;
+                    rq[n].load(qrow + h * HD, cr, sr, 8 * (i - hh * CPR), HD);
                 }
             }
-            const auto rk = __builtin_amdgcn_make_buffer_rsrc((void*)(a.kp + off), (short)0, bytes, kBufferDword3);
-            const auto rv = __builtin_amdgcn_make_buffer_rsrc((void*)(a.vp + off), (short)0, bytes, kBufferDword3);
-#pragma unroll
-            for (int i = 0; i < NH2; ++i) {
-                kr[h * NH2 + i] = __builtin_amdgcn_raw_buffer_load_b128(rk, loff[i], 0, 2);
-                vr[h * NH2 + i] = __builtin_amdgcn_raw_buffer_load_b128(rv, loff[i], 0, 2);
-            }
         }
-    };
-    const int ts0 = __builtin_amdgcn_readfirstlane((tile0 + wave) * kPgTile);
-    load_kv(ts0);
+        gqa_u4 kr[2 * NH2], vr[2 * NH2];
+        auto load_kv = [&](int ts) {                 // the tile at ts, whose pages are in pg
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int t = ts + 16 * h;
+                const int rows = min(16, t1 - t);    // tokens of this half (<= 0: none)
+                const int page = __builtin_amdgcn_readfirstlane(pg[h]);
+                int bytes = 0;
+                int64_t off = 0;
+                if (rows > 0) {
+                    if ((unsigned)page < (unsigned)a.n_pages) {
+                        bytes = ((rows - 1) * (int)a.ps_tok + HD) * (int)sizeof(T);
+                        off = (int64_t)page * a.ps_page + (int64_t)(t & ps_mask) * a.ps_tok + kvh * a.ps_head;
+                    } else {
+                        broken = true;
+                    }
+                }
+                const auto rk_ = __builtin_amdgcn_make_buffer_rsrc((void*)(a.kp + off), (short)0, bytes, kBufferDword3);
+                const auto rv_ = __builtin_amdgcn_make_buffer_rsrc((void*)(a.vp + off), (short)0, bytes, kBufferDword3);
+#pragma unroll
+                for (int i = 0; i < NH2; ++i) {
+                    kr[h * NH2 + i] = __builtin_amdgcn_raw_buffer_load_b128(rk_, loff[i], 0, 2);
+                    vr[h * NH2 + i] = __builtin_amdgcn_raw_buffer_load_b128(rv_, loff[i], 0, 2);
+                }
+            }
+        };
+        load_kv(ts0);
+        pages_of(ts0 + NW * kPgTile, pg);
 
-    const T* qrow = a.q + b * a.q_ld;
-    const bool holds_new = STEP && it.tokens > 0 && it.chunk == it.nchunk - 1;
-    if constexpr (STEP) {
-        // the block of the row's last chunk appends this token's (k roped, v) and
-        // keeps it in LDS: its own scores take the row from there
-        if (holds_new) {
-            const int page = __builtin_amdgcn_readfirstlane(trow[pos >> a.log_ps]);
+        uint4 qf[KK];                                        // B operand of S^T: head lr, dims 32 kk + 8 lq ..
+        if constexpr (STEP) {
+            const int page = __builtin_amdgcn_readfirstlane(pgn);
             const bool have = (unsigned)page < (unsigned)a.n_pages;
-            if (tid < HD / 8) {
-                const T* kh = qrow + (a.QH + kvh) * HD;
-                float x[8];
-                paged_rope8(kh, a.cosv + (int64_t)pos * HD, a.sinv + (int64_t)pos * HD, 8 * tid, HD, x);
-                const uint4 kw = make_uint4(M::pack(x[0], x[1]), M::pack(x[2], x[3]), M::pack(x[4], x[5]),
-                                            M::pack(x[6], x[7]));
-                const uint4 vw = *reinterpret_cast<const uint4*>(kh + a.KVH * HD + 8 * tid);
-                knew[tid] = kw;
-                vnew[tid] = vw;
-                if (have) {
+#pragma unroll
+            for (int n = 0; n < kNew; ++n) {
+                const int i = tid + n * NW * 64, hh = i / CPR, c = i - hh * CPR;
+                if (hh >= G + 2) continue;
+                const uint32_t none = M::pack(it.bad ? NAN : 0.0f, it.bad ? NAN : 0.0f);
+                uint4 w = make_uint4(none, none, none, none);
+                if (it.tokens > 0) w = hh == G + 1 ? rq[n].x : rq[n].packed();
+                heads[i] = w;
+                if (hh < G) {
+                    if (a.q_out != nullptr && it.chunk == 0)
+                        *reinterpret_cast<uint4*>(a.q_out + (b * a.QH + kvh * G + hh) * HD + 8 * c) = w;
+                } else if (holds_new && have) {
                     const int64_t off = (int64_t)page * a.ps_page + (int64_t)(pos & ps_mask) * a.ps_tok +
-                                        kvh * a.ps_head + 8 * tid;
-                    *reinterpret_cast<uint4*>(a.kp + off) = kw;
-                    *reinterpret_cast<uint4*>(a.vp + off) = vw;
+                                        kvh * a.ps_head + 8 * c;
+                    *reinterpret_cast<uint4*>((hh == G ? a.kp : a.vp) + off) = w;
                 }
             }
             lds_barrier();
         }
-    }
-    // B operand of S^T: q of head lr, dims 32 kk + 8 lq ..
-    uint4 qf[KK];
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        const int d0 = 32 * kk + 8 * lq;
-        if (lr < G) {
-            const int h = kvh * G + lr;
-            if constexpr (STEP) {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = it.bad ? NAN : 0.0f;
-                if (it.tokens > 0)
-                    paged_rope8(qrow + h * HD, a.cosv + (int64_t)pos * HD, a.sinv + (int64_t)pos * HD, d0, HD, x);
-                w = make_uint4(M::pack(x[0], x[1]), M::pack(x[2], x[3]), M::pack(x[4], x[5]), M::pack(x[6], x[7]));
-                if (a.q_out != nullptr && it.chunk == 0 && wave == 0)
-                    *reinterpret_cast<uint4*>(a.q_out + (b * a.QH + h) * HD + d0) = w;
-            } else {
-                w = *reinterpret_cast<const uint4*>(qrow + h * HD + d0);
-            }
+        for (int kk = 0; kk < KK; ++kk) {
+            qf[kk] = make_uint4(0, 0, 0, 0);
+            if (lr < G)
+                qf[kk] = STEP ? heads[lr * CPR + 4 * kk + lq]
+                              : *reinterpret_cast<const uint4*>(qrow + (kvh * G + lr) * HD + 32 * kk + 8 * lq);
         }
-        qf[kk] = w;
-    }
-    const gqa_u4* kn_lds = reinterpret_cast<const gqa_u4*>(knew);
-    const gqa_u4* vn_lds = reinterpret_cast<const gqa_u4*>(vnew);
-    float mh = -INFINITY, lh = 0.0f;
-    pg_f32x4 accC[DT], accK[DT];
+        const gqa_u4* kn_lds = reinterpret_cast<const gqa_u4*>(heads + G * CPR);
+        const gqa_u4* vn_lds = kn_lds + CPR;
+        float mh = -INFINITY, lh = 0.0f;
+        pg_f32x4 accC[DT], accK[DT];
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) accC[dt] = accK[dt] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int dt = 0; dt < DT; ++dt) accC[dt] = accK[dt] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
 
-    for (int s = 0; s < nstep; ++s) {
-        const int ts = __builtin_amdgcn_readfirstlane(ts0 + s * 4 * kPgTile);
-        if (ts >= t1) break;                 // wave-uniform: no tile left for this wave
-        wave_lds_fence();
-        if (holds_new && pos >= ts && pos < ts + kPgTile) {
+        for (int ts = ts0; ts < t1; ts += NW * kPgTile) {
+            wave_lds_fence();
+            if (holds_new && pos >= ts && pos < ts + kPgTile) {
+#pragma unroll
+                for (int i = 0; i < 2 * NH2; ++i) {
+                    const int j = i * 64 + lane, row = j / CPR, c = j - row * CPR;
+                    if (ts + row == pos) {
+                        kr[i] = kn_lds[c];
+                        vr[i] = vn_lds[c];
+                    }
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 2 * NH2; ++i) {
                 const int j = i * 64 + lane, row = j / CPR, c = j - row * CPR;
-                if (ts + row == pos) {
-                    kr[i] = kn_lds[c];
-                    vr[i] = vn_lds[c];
-                }
+                const int slot = row * CPR + (c ^ kv_swz(row));
+                tl.k[slot] = kr[i];
+                tl.v[slot] = vr[i];
             }
-        }
-#pragma unroll
-        for (int i = 0; i < 2 * NH2; ++i) {
-            const int j = i * 64 + lane, row = j / CPR, c = j - row * CPR;
-            const int slot = row * CPR + (c ^ kv_swz(row));
-            tl.k[slot] = kr[i];
-            tl.v[slot] = vr[i];
-        }
-        if (s + 1 < nstep) load_kv(ts + 4 * kPgTile);
-        wave_lds_fence();
-        // S^T[token 16 hf + 4 lq + r][head lr]
-        pg_f32x4 sc[2];
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-            sc[hf] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int kk = 0; kk < KK; ++kk)
-                sc[hf] = M::dot(__builtin_bit_cast(uint4, tile_s_frag<CPR>(tl.k, tln, hf, kk)), qf[kk], sc[hf]);
-        }
-        float mx = -INFINITY, sv[2][4];
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const bool ok = ts + 16 * hf + 4 * lq + r < t1;
-                sv[hf][r] = ok ? sc[hf][r] * a.qscale : -INFINITY;
-                mx = fmaxf(mx, sv[hf][r]);
+            const int tn = ts + NW * kPgTile;
+            if (tn < t1) {
+                load_kv(tn);
+                pages_of(tn + NW * kPgTile, pg);
             }
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float mnew = fmaxf(mh, mx);
-        const float corr = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mh - mnew);
-        float ls = 0.0f, pv[2][4];
+            wave_lds_fence();
+            // S^T[token 16 hf + 4 lq + r][head lr]
+            pg_f32x4 sc[2];
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf)
+            for (int hf = 0; hf < 2; ++hf) {
+                sc[hf] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                pv[hf][r] = sv[hf][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sv[hf][r] - mnew);
-                ls += pv[hf][r];
+                for (int kk = 0; kk < KK; ++kk)
+                    sc[hf] = M::dot(__builtin_bit_cast(uint4, tile_s_frag<CPR>(tl.k, tln, hf, kk)), qf[kk], sc[hf]);
             }
-        ls += __shfl_xor(ls, 16, 64);
-        ls += __shfl_xor(ls, 32, 64);
-        lh = fmaf(lh, corr, ls);
-        mh = mnew;
-        // the weights enter the products rounded to the storage type (half a step of
-        // it, relative, per weight: below the rounding of the outputs)
-        const uint4 pa = make_uint4(M::pack(pv[0][0], pv[0][1]), M::pack(pv[0][2], pv[0][3]),
-                                    M::pack(pv[1][0], pv[1][1]), M::pack(pv[1][2], pv[1][3]));
-        if (__any(corr != 1.0f)) {
-            float cf[4];
+            float mx = -INFINITY, sv[2][4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) cf[r] = __shfl(corr, 4 * lq + r, 64);
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
+            for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    accC[dt][r] *= cf[r];
-                    if constexpr (KCTX) accK[dt][r] *= cf[r];
+                    const bool ok = ts + 16 * hf + 4 * lq + r < t1;
+                    sv[hf][r] = ok ? sc[hf][r] * a.qscale : -INFINITY;
+                    mx = fmaxf(mx, sv[hf][r]);
                 }
-        }
+            mx = max_16_32(mx);
+            const float mnew = fmaxf(mh, mx);
+            const float corr = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mh - mnew);
+            float ls = 0.0f, pv[2][4];
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-            accC[dt] = M::dot(pa, tile_tr_frag<CPR>(tl.v, tln, dt), accC[dt]);
-            if constexpr (KCTX) accK[dt] = M::dot(pa, tile_tr_frag<CPR>(tl.k, tln, dt), accK[dt]);
-        }
-    }
-    broken = __syncthreads_or(broken);       // and every wave is done with its tiles
-    float* wm = reinterpret_cast<float*>(lds);
-    float* wl = wm + 4 * NH;
-    float* wacc = wl + 4 * NH;
-    if (lq == 0) {
-        wm[wave * NH + lr] = mh;
-        wl[wave * NH + lr] = lh;
-    }
+            for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+                for (int r = 0; r < 4; ++r) {
+                    pv[hf][r] = sv[hf][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sv[hf][r] - mnew);
+                    ls += pv[hf][r];
+                }
+            ls = sum_16_32(ls);
+            lh = fmaf(lh, corr, ls);
+            mh = mnew;
+            // the weights enter the products rounded to the storage type (half a step of
+            // it, relative, per weight: below the rounding of the outputs)
+            const uint4 pa = make_uint4(M::pack(pv[0][0], pv[0][1]), M::pack(pv[0][2], pv[0][3]),
+                                        M::pack(pv[1][0], pv[1][1]), M::pack(pv[1][2], pv[1][3]));
+            if (__any(corr != 1.0f)) {
+                float cf[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            float* acc = wacc + ((wave * NH + 4 * lq + r) * 2) * HD + 16 * dt + lr;
-            if (4 * lq + r < G) {
-                acc[0] = accC[dt][r];
-                if constexpr (KCTX) acc[HD] = accK[dt][r];
+                for (int r = 0; r < 4; ++r) cf[r] = __shfl(corr, 4 * lq + r, 64);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        accC[dt][r] *= cf[r];
+                        if constexpr (KCTX) accK[dt][r] *= cf[r];
+                    }
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                accC[dt] = M::dot(pa, tile_tr_frag<CPR>(tl.v, tln, dt), accC[dt]);
+                if constexpr (KCTX) accK[dt] = M::dot(pa, tile_tr_frag<CPR>(tl.k, tln, dt), accK[dt]);
             }
         }
-    __syncthreads();
-    paged_finish(a, it, kvh * G, G, NH, HD, KCTX, broken, wm, wl, wacc);
+        broken = __syncthreads_or(broken);           // and every wave is done with its tiles
+        float* wm = reinterpret_cast<float*>(lds);
+        float* wl = wm + NW * NH;
+        float* wacc = wl + NW * NH;
+        if (lq == 0) {
+            wm[lr * NW + wave] = mh;
+            wl[lr * NW + wave] = lh;
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float* acc = wacc + ((wave * NH + 4 * lq + r) * 2) * HD + 16 * dt + lr;
+                if (4 * lq + r < G) {
+                    acc[0] = accC[dt][r];
+                    if constexpr (KCTX) acc[HD] = accK[dt][r];
+                }
+            }
+        __syncthreads();
+        paged_finish<NW>(a, it, kvh * G, G, NH, HD, KCTX, broken, wm, wl, wacc);
+        __syncthreads();                             // before the next row's tiles
+    });
 }
 
 // ------------------------------------------------------------------ vector form
 // fp32 (whose products stay in fp32) and the head sizes the matrix-core form
 // does not take.  LPR lanes per token, each NV groups of four elements (group
-// j + LPR v of the row), GT heads per block; scores by a lane-group sum.
-constexpr int kPvUnroll = 2;
-
+// j + LPR v of the row), GT heads per block; scores by a lane-group sum.  The next
+// tokens' rows are in flight while the present ones are folded in.
 template <typename T>
 __device__ __forceinline__ void load4(const T* p, float v[4]) {
     if constexpr (sizeof(T) == 4) {
@@ -464,236 +570,312 @@ __device__ __forceinline__ void load4(const T* p, float v[4]) {
 }
 
 template <typename T, int LPR, int NV, int GT, bool STEP>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 paged_vec_kernel(PagedArgs<T> a) {
-    constexpr int HD = LPR * NV * 4, E = NV * 4;
-    constexpr int RPW = 64 / LPR, RPB = 4 * RPW;        // tokens of a wave / block step
-    __shared__ float wm[4 * GT], wl[4 * GT], wacc[4 * GT * 2 * HD];
+    constexpr int HD = LPR * NV * 4, E = NV * 4, NW = 4;
+    constexpr int RPW = 64 / LPR, RPB = NW * RPW;       // tokens of a wave / block step
+    __shared__ float wm[NW * GT], wl[NW * GT], wacc[NW * GT * 2 * HD];
+    __shared__ __align__(16) float heads[(GT + 2) * HD];   // the new token's q, k, v
     const int htiles = (a.G + GT - 1) / GT;
     const int kvh = blockIdx.y / htiles, g0 = (blockIdx.y % htiles) * GT;
     const int nh = min(GT, a.G - g0), h0 = kvh * a.G + g0;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int j = lane % LPR, grp = wave * RPW + lane / LPR;
-    const PlanItem it = plan_item<false>(a.lens, a.B, STEP, a.cap, a.n_pos, a.target, blockIdx.x);
-    if (it.row < 0) return;
-    const int64_t b = it.row;
-    const int pos = it.tokens - 1;
-    const int tiles = (it.tokens + kPgTile - 1) / kPgTile;
-    const int t0 = (int)((int64_t)it.chunk * tiles / it.nchunk) * kPgTile;
-    const int t1 = min((int)((int64_t)(it.chunk + 1) * tiles / it.nchunk) * kPgTile, it.tokens);
-    const int32_t* trow = a.table + b * a.table_ld;
     const int ps_mask = (1 << a.log_ps) - 1;
     const bool kctx = a.k_out != nullptr;
-    bool broken = it.bad;
-    const T* qrow = a.q + b * a.q_ld;
-    const float* cr = a.cosv + (int64_t)pos * HD;       // read only where tokens > 0
-    const float* sr = a.sinv + (int64_t)pos * HD;
-
-    float q[GT][E];
+    plan_walk<STEP>(a.lens, a.B, a.cap, a.n_pos, a.slots, blockIdx.x, [&](const PlanItem& it) {
+        const int64_t b = it.row;
+        const int pos = it.tokens - 1;
+        const int t0 = it.tile0 * kPgTile, t1 = min(it.tile1 * kPgTile, it.tokens);
+        const int32_t* trow = a.table + b * a.table_ld;
+        bool broken = it.bad;
+        // cached tokens; the new one is folded in from the projection row, first
+        const int tc = STEP ? min(t1, pos) : t1;
+        auto page_at = [&](int t) { return trow[min(t, a.cap - 1) >> a.log_ps]; };
+        const T* qrow = a.q + b * a.q_ld;
+        const float* cr = a.cosv + (int64_t)pos * HD;   // read only where tokens > 0
+        const float* sr = a.sinv + (int64_t)pos * HD;
+        int pg = page_at(t0 + grp);
+        // the new token's heads (q of the block's heads, then k, then v) by one thread
+        // per four elements; every lane takes what it needs from LDS
+        const bool holds_new = STEP && it.tokens > 0 && it.chunk == it.nchunk - 1;
+        constexpr int kG4 = HD / 4, kNew = (GT + 2) * kG4 / 256 + 1;
+        float xr[kNew][4], yr[kNew][4], cs[kNew][4], sn[kNew][4];
+        int pgn = -1;
+        if (holds_new) pgn = page_at(pos);
 #pragma unroll
-    for (int g = 0; g < GT; ++g)
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
+        for (int n = 0; n < kNew; ++n) {
+            const int i = tid + n * 256, hh = i / kG4, d = 4 * (i - hh * kG4);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int d = 4 * (j + LPR * v) + e;
-                float x = it.bad ? NAN : 0.0f;
-                if (g < nh) {
-                    if constexpr (STEP) {
-                        if (it.tokens > 0) x = round_to<T>(paged_rope(qrow + (h0 + g) * HD, cr, sr, d, HD));
-                        if (a.q_out != nullptr && it.chunk == 0 && grp == 0)
-                            st(a.q_out + (b * a.QH + h0 + g) * HD + d, x);
-                    } else {
-                        x = ld(qrow + (h0 + g) * HD + d);
-                    }
-                }
-                q[g][4 * v + e] = x * a.qscale;
+                xr[n][e] = it.bad ? NAN : 0.0f;
+                yr[n][e] = cs[n][e] = sn[n][e] = 0.0f;
             }
-    float m[GT], l[GT], ac[GT][E], ak[GT][E];
-#pragma unroll
-    for (int g = 0; g < GT; ++g) {
-        m[g] = -INFINITY;
-        l[g] = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) ac[g][e] = ak[g][e] = 0.0f;
-    }
-    auto fold = [&](const float (&kv)[kPvUnroll][E], const float (&vv)[kPvUnroll][E], const bool (&ok)[kPvUnroll]) {
-#pragma unroll
-        for (int g = 0; g < GT; ++g) {
-            float s[kPvUnroll], mx = m[g];
-#pragma unroll
-            for (int u = 0; u < kPvUnroll; ++u) {
-                float x = 0.0f;
-#pragma unroll
-                for (int e = 0; e < E; ++e) x = fmaf(q[g][e], kv[u][e], x);
-                x = group_sum<LPR>(x);
-                s[u] = ok[u] ? x : -INFINITY;
-                mx = fmaxf(mx, s[u]);
+            if (hh >= GT + (STEP ? 2 : 0) || (hh < GT && hh >= nh) || (STEP && it.tokens <= 0)) continue;
+            const T* head = qrow + (int64_t)(hh < GT ? h0 + hh : a.QH + kvh + (hh - GT) * a.KVH) * HD;
+            load4(head + d, xr[n]);
+            if constexpr (STEP) {
+                load4(head + (d < HD / 2 ? d + HD / 2 : d - HD / 2), yr[n]);
+                load4(cr + d, cs[n]);
+                load4(sr + d, sn[n]);
             }
-            const float corr = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[g] - mx);
-            l[g] *= corr;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                ac[g][e] *= corr;
-                ak[g][e] *= corr;
-            }
-#pragma unroll
-            for (int u = 0; u < kPvUnroll; ++u) {
-                const float p = s[u] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s[u] - mx);
-                l[g] += p;
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    ac[g][e] = fmaf(p, vv[u][e], ac[g][e]);
-                    ak[g][e] = fmaf(p, kv[u][e], ak[g][e]);
-                }
-            }
-            m[g] = mx;
         }
-    };
-    // cached tokens; the new one is folded in from the projection row below
-    const int tc = STEP ? min(t1, pos) : t1;
-    for (int t = t0 + grp; t < tc; t += RPB * kPvUnroll) {
-        float kv[kPvUnroll][E], vv[kPvUnroll][E];
-        bool ok[kPvUnroll];
-        int64_t off[kPvUnroll];
-#pragma unroll
-        for (int u = 0; u < kPvUnroll; ++u) {
-            const int tu = t + RPB * u;
-            const int page = tu < tc ? trow[tu >> a.log_ps] : -1;
-            ok[u] = (unsigned)page < (unsigned)a.n_pages;
-            broken |= tu < tc && !ok[u];
-            off[u] = ok[u] ? (int64_t)page * a.ps_page + (int64_t)(tu & ps_mask) * a.ps_tok + kvh * a.ps_head : 0;
-        }
-#pragma unroll
-        for (int u = 0; u < kPvUnroll; ++u)
+        float kv[E], vv[E], kn[E], vn[E];
+        // the row of token t, whose page is `page`; false where there is none: the
+        // lanes then hold some row of the pool, set to zeros before it is used
+        auto load_row = [&](int t, int page, float (&k)[E], float (&v_)[E]) __attribute__((always_inline)) {
+            const bool in = t < tc, have = in && (unsigned)page < (unsigned)a.n_pages;
+            broken |= in && !have;
+            const int64_t off = (have ? (int64_t)page * a.ps_page + (int64_t)(t & ps_mask) * a.ps_tok : 0) + kvh * a.ps_head;
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                if (ok[u]) {
-                    load4(a.kp + off[u] + 4 * (j + LPR * v), &kv[u][4 * v]);
-                    load4(a.vp + off[u] + 4 * (j + LPR * v), &vv[u][4 * v]);
-                } else {
+                load4(a.kp + off + 4 * (j + LPR * v), &k[4 * v]);
+                load4(a.vp + off + 4 * (j + LPR * v), &v_[4 * v]);
+            }
+            return have;
+        };
+        bool ok = load_row(t0 + grp, pg, kv, vv);
+        pg = page_at(t0 + grp + RPB);
+        const bool have_new = (unsigned)pgn < (unsigned)a.n_pages;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) kv[u][4 * v + e] = vv[u][4 * v + e] = 0.0f;
+        for (int n = 0; n < kNew; ++n) {
+            const int i = tid + n * 256, hh = i / kG4, d = 4 * (i - hh * kG4);
+            if (hh >= GT + 2) continue;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = xr[n][e];
+                if (STEP && hh <= GT && it.tokens > 0)
+                    v[e] = round_to<T>(fmaf(xr[n][e], cs[n][e], (d < HD / 2 ? -yr[n][e] : yr[n][e]) * sn[n][e]));
+                heads[4 * i + e] = v[e];
+            }
+            if constexpr (STEP) {
+                T* out = nullptr;
+                if (hh < nh && a.q_out != nullptr && it.chunk == 0) {
+                    out = a.q_out + (b * a.QH + h0 + hh) * HD + d;
+                } else if (hh >= GT && holds_new && have_new && g0 == 0) {
+                    out = (hh == GT ? a.kp : a.vp) + (int64_t)pgn * a.ps_page + (int64_t)(pos & ps_mask) * a.ps_tok +
+                          kvh * a.ps_head + d;
+                }
+                if (out != nullptr) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) st(out + e, v[e]);
                 }
             }
-        fold(kv, vv, ok);
-    }
-    if constexpr (STEP) {
-        if (it.tokens > 0 && it.chunk == it.nchunk - 1) {
-            const int page = trow[pos >> a.log_ps];
-            const bool have = (unsigned)page < (unsigned)a.n_pages;
-            broken |= !have;
-            if (grp == 0) {                  // one lane group of the block
-                float kv[kPvUnroll][E] = {}, vv[kPvUnroll][E] = {};
-                bool ok[kPvUnroll] = {};
-                const T* kh = qrow + (a.QH + kvh) * HD;
-                const T* vh = kh + a.KVH * HD;
-                const int64_t off = have ? (int64_t)page * a.ps_page + (int64_t)(pos & ps_mask) * a.ps_tok +
-                                               kvh * a.ps_head : 0;
+        }
+        lds_barrier();
+        auto take = [&](int hh, float (&o)[E]) __attribute__((always_inline)) {
 #pragma unroll
-                for (int v = 0; v < NV; ++v)
+            for (int v = 0; v < NV; ++v)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int d = 4 * (j + LPR * v) + e;
-                        kv[0][4 * v + e] = round_to<T>(paged_rope(kh, cr, sr, d, HD));
-                        vv[0][4 * v + e] = ld(vh + d);
-                        if (have && g0 == 0) {
-                            st(a.kp + off + d, kv[0][4 * v + e]);
-                            a.vp[off + d] = vh[d];
-                        }
+                for (int e = 0; e < 4; ++e) o[4 * v + e] = heads[hh * HD + 4 * (j + LPR * v) + e];
+        };
+        float q[GT][E];
+#pragma unroll
+        for (int g = 0; g < GT; ++g) {
+            take(g, q[g]);
+#pragma unroll
+            for (int e = 0; e < E; ++e) q[g][e] *= a.qscale;
+        }
+        float m[GT], l[GT], ac[GT][E], ak[GT][E];
+#pragma unroll
+        for (int g = 0; g < GT; ++g) {
+            m[g] = -INFINITY;
+            l[g] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) ac[g][e] = ak[g][e] = 0.0f;
+        }
+        auto fold = [&](const float (&k)[E], const float (&v_)[E], bool in) __attribute__((always_inline)) {
+#pragma unroll
+            for (int g = 0; g < GT; ++g) {
+                float s = 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) s = fmaf(q[g][e], k[e], s);
+                s = group_sum<LPR>(s);
+                s = in ? s : -INFINITY;
+                const float mx = fmaxf(m[g], s);
+                const float corr = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[g] - mx);
+                const float p = s == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s - mx);
+                if (__any(corr != 1.0f)) {
+                    l[g] *= corr;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        ac[g][e] *= corr;
+                        ak[g][e] *= corr;
                     }
-                ok[0] = true;
-                fold(kv, vv, ok);
+                }
+                l[g] += p;
+                m[g] = mx;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    ac[g][e] = fmaf(p, v_[e], ac[g][e]);
+                    ak[g][e] = fmaf(p, k[e], ak[g][e]);
+                }
+            }
+        };
+        if constexpr (STEP) {
+            if (holds_new) {
+                broken |= !have_new;
+                if (wave == 0) {                     // one lane group of the block
+                    take(GT, kn);
+                    take(GT + 1, vn);
+                    fold(kn, vn, grp == 0);
+                }
             }
         }
-    }
-    // join the wave's token groups (lanes LPR apart), then the waves through LDS
+        for (int t = t0 + grp; t - grp < tc; t += RPB) {           // block-uniform trip count
+            const bool okn = load_row(t + RPB, pg, kn, vn);
+            pg = page_at(t + 2 * RPB);
+            if (!__all(ok)) {
 #pragma unroll
-    for (int g = 0; g < GT; ++g) {
-        float mw = m[g];
-#pragma unroll
-        for (int d = LPR; d < 64; d <<= 1) mw = fmaxf(mw, __shfl_xor(mw, d, 64));
-        const float f = mw == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[g] - mw);
-        float lw = l[g] * f;
-#pragma unroll
-        for (int d = LPR; d < 64; d <<= 1) lw += __shfl_xor(lw, d, 64);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            float c = ac[g][e] * f, kx = ak[g][e] * f;
-#pragma unroll
-            for (int d = LPR; d < 64; d <<= 1) {
-                c += __shfl_xor(c, d, 64);
-                kx += __shfl_xor(kx, d, 64);
+                for (int e = 0; e < E; ++e) {
+                    kv[e] = ok ? kv[e] : 0.0f;
+                    vv[e] = ok ? vv[e] : 0.0f;
+                }
             }
-            if (lane < LPR) {
-                const int dd = 4 * (j + LPR * (e / 4)) + e % 4;
-                wacc[((wave * GT + g) * 2) * HD + dd] = c;
-                wacc[((wave * GT + g) * 2 + 1) * HD + dd] = kx;
+            fold(kv, vv, ok);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                kv[e] = kn[e];
+                vv[e] = vn[e];
+            }
+            ok = okn;
+        }
+        // join the wave's token groups (lanes LPR apart), then the waves through LDS:
+        // lanes 32 apart take the sums of C and of Kctx, lanes 16 apart those of the
+        // even and the odd elements, lanes of one row of 16 all of them
+        const int which = lane >> 5, odd = (lane >> 4) & 1;
+#pragma unroll
+        for (int g = 0; g < GT; ++g) {
+            float mw = m[g];
+            if constexpr (LPR <= 2) mw = fmaxf(mw, dpp<0x122>(mw));         // row_ror 2, 4, 8
+            if constexpr (LPR <= 4) mw = fmaxf(mw, dpp<0x124>(mw));
+            if constexpr (LPR <= 8) mw = fmaxf(mw, dpp<0x128>(mw));
+            mw = max_16_32(mw);
+            const float f = mw == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[g] - mw);
+            float lw = l[g] * f;
+            if constexpr (LPR <= 2) lw += dpp<0x122>(lw);
+            if constexpr (LPR <= 4) lw += dpp<0x124>(lw);
+            if constexpr (LPR <= 8) lw += dpp<0x128>(lw);
+            lw = sum_16_32(lw);
+            float h[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float2 p = pair32(ac[g][e] * f, ak[g][e] * f);
+                h[e] = p.x + p.y;
+            }
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                const float2 p = pair16(h[e], h[e + 1]);
+                float v = p.x + p.y;
+                if constexpr (LPR <= 8) v += dpp<0x128>(v);
+                if constexpr (LPR <= 4) v += dpp<0x124>(v);
+                if constexpr (LPR <= 2) v += dpp<0x122>(v);
+                if ((lane & 15) < LPR)
+                    wacc[((wave * GT + g) * 2 + which) * HD + 4 * (j + LPR * (e / 4)) + e % 4 + odd] = v;
+            }
+            if (lane == 0) {
+                wm[g * NW + wave] = mw;
+                wl[g * NW + wave] = lw;
             }
         }
-        if (lane == 0) {
-            wm[wave * GT + g] = mw;
-            wl[wave * GT + g] = lw;
-        }
-    }
-    broken = __syncthreads_or(broken);
-    paged_finish(a, it, h0, nh, GT, HD, kctx, broken, wm, wl, wacc);
+        broken = __syncthreads_or(broken);
+        paged_finish<NW>(a, it, h0, nh, GT, HD, kctx, broken, wm, wl, wacc);
+        __syncthreads();                             // before the next row's sums
+    });
 }
 
 // ------------------------------------------------------------------ the join
-// One block per (row, q head), a thread per element: the row's chunk records,
-// up to kPgJoin of them in flight.  Rows of one chunk are done already.
+// One block per (row, q head): wave w takes the row's chunk records w, w + 4, ..,
+// a whole record of 2 HD sums per load, kPgJoin of them in flight; the waves meet
+// in LDS.  Rows of one chunk are done already.
 constexpr int kPgJoin = 8;
 
-template <typename T>
-__global__ void paged_join_kernel(PagedArgs<T> a, int HD, int step) {
-    const PlanItem it = plan_item<true>(a.lens, a.B, step, a.cap, a.n_pos, a.target, blockIdx.x);
-    const int d = threadIdx.x, h = blockIdx.y;
-    if (it.nchunk == 1 || d >= HD) return;
-    const bool kctx = a.k_out != nullptr;
-    float M = -INFINITY, L = 0.0f, C = 0.0f, K = 0.0f;
-    for (int c0 = 0; c0 < it.nchunk; c0 += kPgJoin) {
-        float m[kPgJoin], l[kPgJoin], cv[kPgJoin], kv[kPgJoin], mx = M;
+template <typename T, int HD, bool STEP>
+__global__ void __launch_bounds__(256)
+paged_join_kernel(PagedArgs<T> a) {
+    constexpr int NV = HD > 128 ? 2 : 1, NL = HD / 2 / NV;     // lanes of four sums
+    __shared__ float wm[4], wl[4];
+    __shared__ __align__(16) float wacc[4][2 * HD];
+    const Plan p = make_plan<STEP>(a.lens, a.B, a.cap, a.n_pos, a.slots);
+    const PlanRow r0 = plan_find<STEP, true>(p, a.lens, a.B, a.cap, a.n_pos, blockIdx.x);
+    const PlanItem it = plan_item(p, r0, 0);
+    if (it.nchunk == 1) return;
+    const int h = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    float M = -INFINITY, L = 0.0f;
+    pg_f32x4 acc[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) acc[v] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c0 = wave; c0 < it.nchunk; c0 += 4 * kPgJoin) {
+        float2 ml[kPgJoin];
+        pg_f32x4 x[kPgJoin][NV];
 #pragma unroll
         for (int u = 0; u < kPgJoin; ++u) {
-            const int64_t r = (int64_t)(it.item0 + min(c0 + u, it.nchunk - 1)) * a.QH + h;
-            m[u] = a.rec[a.rec_ml + 2 * r];
-            l[u] = a.rec[a.rec_ml + 2 * r + 1];
-            cv[u] = a.rec[r * 2 * HD + d];
-            kv[u] = kctx ? a.rec[r * 2 * HD + HD + d] : 0.0f;
+            const int64_t r = (int64_t)(it.item0 + min(c0 + 4 * u, it.nchunk - 1)) * a.QH + h;
+            ml[u] = *reinterpret_cast<const float2*>(a.rec + a.rec_ml + 2 * r);
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                if (lane < NL) x[u][v] = *reinterpret_cast<const pg_f32x4*>(a.rec + r * 2 * HD + 4 * (lane + NL * v));
         }
+        float mx = M;
 #pragma unroll
         for (int u = 0; u < kPgJoin; ++u)
-            if (c0 + u < it.nchunk) mx = fmaxf(mx, m[u]);
+            if (c0 + 4 * u < it.nchunk) mx = fmaxf(mx, ml[u].x);
         const float f = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M - mx);
         L *= f;
-        C *= f;
-        K *= f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) acc[v] *= f;
 #pragma unroll
         for (int u = 0; u < kPgJoin; ++u) {
-            if (c0 + u >= it.nchunk) continue;
-            const float w = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[u] - mx);
-            L = fmaf(l[u], w, L);
-            C = fmaf(cv[u], w, C);
-            K = fmaf(kv[u], w, K);
+            if (c0 + 4 * u >= it.nchunk) continue;
+            const float w = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml[u].x - mx);
+            L = fmaf(ml[u].y, w, L);
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[v][e] = fmaf(x[u][v][e], w, acc[v][e]);
         }
         M = mx;
     }
-    const float inv = 1.0f / L;
-    const int64_t o = (int64_t)it.row * a.out_ld + (int64_t)h * HD + d;
-    st(a.c_out + o, L == 0.0f ? 0.0f : C * inv);
-    if (kctx) st(a.k_out + o, L == 0.0f ? 0.0f : K * inv);
+    if (lane == 0) {
+        wm[wave] = M;
+        wl[wave] = L;
+    }
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+        if (lane < NL) *reinterpret_cast<pg_f32x4*>(&wacc[wave][4 * (lane + NL * v)]) = acc[v];
+    __syncthreads();
+    const int n = a.k_out != nullptr ? 2 * HD : HD;
+    for (int k = threadIdx.x; k < n; k += 256) {
+        const float m = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+        float l = 0.0f, x = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(wm[w] - m);
+            l = fmaf(wl[w], f, l);
+            x = fmaf(wacc[w][k], f, x);
+        }
+        T* out = (k < HD ? a.c_out : a.k_out) + (int64_t)it.row * a.out_ld + (int64_t)h * HD + (k < HD ? k : k - HD);
+        st(out, l == 0.0f ? 0.0f : x / l);
+    }
 }
 
 // ------------------------------------------------------------------ host side
 
-// Chunks aimed at for each kv head: two blocks per CU in all.
-static int paged_target(int64_t KVH) { return (int)max((int64_t)1, 2 * (int64_t)device_cus() / KVH); }
+// Blocks per kv head that share the work: as many as the device holds at once
+// (two per CU); none where no row can be longer than kPgWhole tokens: then a
+// block per row does it in one launch.
+static int paged_slots(int64_t cap, int64_t KVH) {
+    if (cap <= kPgWhole) return 0;
+    const int64_t n = 2 * (int64_t)device_cus() / KVH;
+    return n < 1 ? 1 : (int)n;
+}
 
-// Most items (chunks over all rows): sum of max(1, ceil(tiles / ct)).
+// Blocks per kv head of a launch, and records of it: one for each pair of a block
+// and a row that it works on (at most slots + B, and ceil(tiles / kPgMinTiles) a row).
 static int64_t paged_items(int64_t B, int64_t cap, int64_t KVH) {
-    const int64_t per_row = max((int64_t)1, ceil_div(ceil_div(cap, kPgTile), kPgMinTiles));
-    return min(B * per_row, B + paged_target(KVH));
+    const int64_t slots = paged_slots(cap, KVH);
+    return slots == 0 ? B : B + slots;
 }
 
 template <typename T, bool STEP>
@@ -704,35 +886,42 @@ static int paged_launch(PagedArgs<T>& a, int64_t HD, hipStream_t st) {
     bool done = false;
     if constexpr (sizeof(T) == 2) {
         const dim3 grid((unsigned)items, (unsigned)a.KVH);
+        // a row that one block does alone has eight waves, its tiles in flight at once
+#define LOOM_PG_MF1(HDV, NW, KC)                                                                    \
+        hipLaunchKernelGGL((paged_mfma_kernel<T, HDV, NW, STEP, KC>), grid, dim3(NW * 64), 0, st, a)
 #define LOOM_PG_MF(HDV)                                                                             \
         if (!done && HD == HDV && a.G <= 16) {                                                      \
-            if (a.k_out != nullptr)                                                                 \
-                hipLaunchKernelGGL((paged_mfma_kernel<T, HDV, STEP, true>), grid, dim3(256), 0, st, a);  \
-            else                                                                                    \
-                hipLaunchKernelGGL((paged_mfma_kernel<T, HDV, STEP, false>), grid, dim3(256), 0, st, a); \
+            if (a.slots == 0 && a.k_out != nullptr) LOOM_PG_MF1(HDV, 8, true);                      \
+            else if (a.slots == 0) LOOM_PG_MF1(HDV, 8, false);                                      \
+            else if (a.k_out != nullptr) LOOM_PG_MF1(HDV, 4, true);                                 \
+            else LOOM_PG_MF1(HDV, 4, false);                                                        \
             done = true;                                                                            \
         }
         LOOM_PG_MF(96) LOOM_PG_MF(128) LOOM_PG_MF(64) LOOM_PG_MF(32)
 #undef LOOM_PG_MF
+#undef LOOM_PG_MF1
     }
-#define LOOM_PG_V(LPR, NV)                                                                          \
+#define LOOM_PG_V(LPR, NV, GT)                                                                      \
     if (!done && HD == LPR * NV * 4) {                                                              \
         if (a.G == 1)                                                                               \
             hipLaunchKernelGGL((paged_vec_kernel<T, LPR, NV, 1, STEP>), dim3((unsigned)items, (unsigned)a.KVH), \
                                dim3(256), 0, st, a);                                                \
         else                                                                                        \
-            hipLaunchKernelGGL((paged_vec_kernel<T, LPR, NV, 4, STEP>),                             \
-                               dim3((unsigned)items, (unsigned)(a.KVH * ((a.G + 3) / 4))), dim3(256), 0, st, a); \
+            hipLaunchKernelGGL((paged_vec_kernel<T, LPR, NV, GT, STEP>),                            \
+                               dim3((unsigned)items, (unsigned)(a.KVH * ((a.G + GT - 1) / GT))), dim3(256), 0, st, a); \
         done = true;                                                                                \
     }
-    LOOM_PG_V(8, 3) LOOM_PG_V(8, 4) LOOM_PG_V(8, 2) LOOM_PG_V(8, 1) LOOM_PG_V(4, 1) LOOM_PG_V(2, 1)
-    LOOM_PG_V(16, 4)
+    LOOM_PG_V(8, 3, 4) LOOM_PG_V(16, 2, 4) LOOM_PG_V(8, 2, 4) LOOM_PG_V(8, 1, 4) LOOM_PG_V(4, 1, 4)
+    LOOM_PG_V(2, 1, 4) LOOM_PG_V(16, 4, 2)
 #undef LOOM_PG_V
     LOOM_CHECK(done, "%s: unsupported head_dim %lld (8, 16, 32, 64, 96, 128 or 256)", who, (long long)HD);
     const int rc = launch_status(who);
-    if (rc != LOOM_OK || items <= a.B) return rc;      // one chunk per row: no join
-    hipLaunchKernelGGL((paged_join_kernel<T>), dim3((unsigned)a.B, (unsigned)a.QH),
-                       dim3((unsigned)(ceil_div(HD, 64) * 64)), 0, st, a, (int)HD, STEP ? 1 : 0);
+    if (rc != LOOM_OK || a.slots == 0) return rc;      // one chunk per row: no join
+#define LOOM_PG_J(HDV)                                                                              \
+    if (HD == HDV)                                                                                  \
+        hipLaunchKernelGGL((paged_join_kernel<T, HDV, STEP>), dim3((unsigned)a.B, (unsigned)a.QH), dim3(256), 0, st, a);
+    LOOM_PG_J(96) LOOM_PG_J(128) LOOM_PG_J(64) LOOM_PG_J(32) LOOM_PG_J(16) LOOM_PG_J(8) LOOM_PG_J(256)
+#undef LOOM_PG_J
     return launch_status(who);
 }
 
@@ -780,7 +969,7 @@ static int paged_typed(const PagedCall& c, hipStream_t st) {
     a.QH = (int)c.QH;
     a.KVH = (int)c.KVH;
     a.G = (int)(c.QH / c.KVH);
-    a.target = paged_target(c.KVH);
+    a.slots = paged_slots(a.cap, c.KVH);
     a.qscale = kLog2e / sqrtf((float)c.HD);
     return paged_launch<T, STEP>(a, c.HD, st);
 }
@@ -838,7 +1027,7 @@ extern "C" int64_t loom_paged_decode_workspace_bytes(int64_t B, int64_t capacity
                                                      int64_t HD) {
     if (B <= 0 || capacity <= 0 || KVH <= 0) return 0;
     const int64_t items = paged_items(B, capacity, KVH);
-    return items <= B ? 0 : items * QH * (2 + 2 * HD) * (int64_t)sizeof(float);
+    return paged_slots(capacity, KVH) == 0 ? 0 : items * QH * (2 + 2 * HD) * (int64_t)sizeof(float);
 }
 
 extern "C" int loom_paged_decode_step(int dtype, const void* qkv, int64_t qkv_ld, void* k_pages, void* v_pages,

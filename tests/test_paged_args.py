@@ -33,7 +33,7 @@ PAGED = [(dict(dtype=5), "unsupported dtype"), (dict(B=1025), "0 to 1024 rows"),
 
 
 def test_paged_decode_refuses():
-    # three rows of 80 tokens stay within one chunk each and need no workspace; 256 pages do
+    # rows of 80 tokens are not split and need no workspace; rows of 256 pages do
     base = dict(STEP, max_pages=256, table_ld=256, n_pos=4096)
     _refuses("loom_paged_decode_step", base, PAGED + [
         (dict(qkv_ld=1144), "qkv must be 16-byte aligned and hold 1152"), (dict(qkv_ld=1153), "qkv must be 16-byte"),
@@ -102,10 +102,11 @@ def test_beam_select_and_reorder_refuse():
 def test_workspace_queries():
     from loom_amd import _lib
     lib = _lib.load()
-    # 256 CUs assumed without a device: two blocks per CU over 2 kv heads = 256 chunks and one more per row at most
+    # 256 CUs assumed without a device: two blocks per CU over 2 kv heads = 256 blocks, a record for
+    # each row that one of them works on
     assert lib.loom_paged_decode_workspace_bytes(32, 4096, 8, 2, 96) == (32 + 256) * 8 * 2 * 97 * 4
-    assert lib.loom_paged_decode_workspace_bytes(2, 300, 8, 2, 96) == 2 * 3 * 8 * 2 * 97 * 4
-    assert lib.loom_paged_decode_workspace_bytes(2, 128, 8, 2, 96) == 0        # one chunk per row: no join
+    assert lib.loom_paged_decode_workspace_bytes(2, 528, 8, 2, 96) == (2 + 256) * 8 * 2 * 97 * 4
+    assert lib.loom_paged_decode_workspace_bytes(200, 512, 8, 2, 96) == 0      # one chunk per row: no join
     assert lib.loom_paged_update_workspace_bytes(7) == 7 * 16
     assert lib.loom_paged_compact_workspace_bytes(10) == 136
     assert lib.loom_beam_select_workspace_bytes(0, 4, 100, 4) == 0
