@@ -17,9 +17,11 @@ namespace loom {
 
 constexpr int kBeamMaxOut = 64, kBeamMaxBeams = 32;
 constexpr int kBeamVec = 8;                       // elements per load
-constexpr int kBeamPieces = 4;                    // loads in flight per thread
+constexpr int kBeamPieces = 4;                    // loads of a thread per step
 constexpr int kBeamTile = 256 * kBeamVec * kBeamPieces;   // logits of a block step
-constexpr int kBeamMaxCand = 2048;                // survivors of a group
+constexpr int kBeamMaxCand = 2048;                // survivors of a group, from all its slices
+constexpr int kBeamWhole = 32768;                 // logits of a group that one block of 1024 takes
+constexpr int kBeamWholeOut = 32, kBeamWholeBeams = 16;
 
 struct BeamArgs {
     const float* scores;        // [groups * W]
@@ -54,128 +56,223 @@ __device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int d) {
     const uint32_t lo = __shfl_xor((uint32_t)v, d, 64), hi = __shfl_xor((uint32_t)(v >> 32), d, 64);
     return ((uint64_t)hi << 32) | lo;
 }
+__device__ __forceinline__ uint64_t readlane_u64(uint64_t v, int l) {
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32) |
+           (uint32_t)__builtin_amdgcn_readlane((int)v, l);
+}
 
-// The K largest keys of a slice of one row: key 0 means no candidate (a NaN or
-// -inf logit).  Per step of kBeamTile logits: the best of each four threads'
-// keys; the K-th best of those 64 is a bound that at least K keys reach (each
-// is the best of its own four threads) and that only K of the fours can reach,
-// so at most K * 4 * 32 keys pass, with the kept ones of earlier steps.  They
-// are ranked by counting the larger ones.
+// Eight logits as loaded, from place v on; places from v1 on hold -inf.  Rows start
+// at any element: which thread sums what goes by the place alone, so that equal
+// rows have equal sums (and their candidates tie) wherever they lie.
 template <typename T>
-__global__ void __launch_bounds__(256)
-beam_row_kernel(const T* __restrict__ logits, BeamArgs a) {
-    extern __shared__ uint64_t found[];               // K * 128 + K
-    __shared__ uint64_t quad[64], kept[kBeamMaxOut];
-    __shared__ float wmax[4];
-    __shared__ double wsum[4];
-    __shared__ int nfound;
-    const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int K = a.K;
-    const int64_t rec = (int64_t)row * a.slices + slice;
-    if (a.finished != nullptr && a.finished[row]) return;     // its logits are not read
-    const T* x = logits + (int64_t)row * a.ld;
-    const int64_t v0 = (int64_t)slice * a.slice_len, v1 = min(v0 + a.slice_len, a.V);
-    // vector loads start at the last aligned address at or before v0; pieces that
-    // are not wholly inside the slice are read element by element
-    const int skew = (int)(((uintptr_t)(x + v0) / sizeof(T)) % kBeamVec);
-    float m = -INFINITY;                               // of this thread
-    double s = 0.0;
-    if (tid < K) kept[tid] = 0;
-    for (int64_t base = v0 - skew; base < v1; base += kBeamTile) {
-        float e[kBeamPieces][kBeamVec];
+struct BeamPiece {
+    static constexpr int NW = (int)sizeof(T) * kBeamVec / 4;
+    uint32_t w[NW];
+    __device__ __forceinline__ void load(const T* x, int64_t v, int64_t v1) {
+        if (v + kBeamVec <= v1) {
 #pragma unroll
-        for (int p = 0; p < kBeamPieces; ++p) {
-            const int64_t v = base + (int64_t)(p * 256 + tid) * kBeamVec;
-            if (v >= v0 && v + kBeamVec <= v1) {
-                Vec8<T>::load(x + v, e[p]);
+            for (int i = 0; i < NW / 4; ++i) {
+                u32x4 q;                             // one load, of any alignment
+                __builtin_memcpy(&q, reinterpret_cast<const char*>(x + v) + 16 * i, 16);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[4 * i + k] = q[k];
+            }
+            return;
+        }
+        constexpr uint32_t ninf = std::is_same<T, float>::value    ? 0xff800000u
+                                  : std::is_same<T, bf16_t>::value ? 0xff80ff80u
+                                                                   : 0xfc00fc00u;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) w[i] = ninf;
+#pragma unroll
+        for (int k = 0; k < kBeamVec; ++k) {
+            if (v + k >= v1) continue;
+            if constexpr (sizeof(T) == 4) {
+                w[k] = __float_as_uint(x[v + k]);
             } else {
-#pragma unroll
-                for (int k = 0; k < kBeamVec; ++k) e[p][k] = v + k >= v0 && v + k < v1 ? ld(x + v + k) : -INFINITY;
+                const uint32_t h = x[v + k].x;
+                w[k / 2] = (k & 1) ? (w[k / 2] & 0xffffu) | (h << 16) : (w[k / 2] & 0xffff0000u) | h;
             }
         }
-        // running sum of exponentials
+    }
+    __device__ __forceinline__ float get(int k) const {
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(w[k]);
+        } else {
+            const T t{(uint16_t)(w[k / 2] >> (16 * (k & 1)))};
+            return ld(&t);
+        }
+    }
+};
+
+// A thread's logits of one step: place of element k of piece p is v(p) + k.
+template <typename T>
+struct BeamStep {
+    BeamPiece<T> e[kBeamPieces];
+    // Running maximum and sum of exponentials.  A NaN makes the sum NaN, and so does
+    // +inf; the maximum stays -inf while there is no other logit.
+    __device__ __forceinline__ void sum(float& m, double& s) const {
         float mt = m;
-        bool nan = false;
 #pragma unroll
         for (int p = 0; p < kBeamPieces; ++p)
 #pragma unroll
-            for (int k = 0; k < kBeamVec; ++k) {
-                mt = fmaxf(mt, e[p][k]);
-                nan |= e[p][k] != e[p][k];
-            }
+            for (int k = 0; k < kBeamVec; ++k) mt = fmaxf(mt, e[p].get(k));
+        const float at = mt == -INFINITY ? 0.0f : mt;
         float st = 0.0f;
-        if (mt != -INFINITY) {
 #pragma unroll
-            for (int p = 0; p < kBeamPieces; ++p)
+        for (int p = 0; p < kBeamPieces; ++p)
 #pragma unroll
-                for (int k = 0; k < kBeamVec; ++k) st += __builtin_amdgcn_exp2f((e[p][k] - mt) * kLog2e);
-            s = s * (double)__builtin_amdgcn_exp2f((m - mt) * kLog2e) + (double)st;
-            m = mt;
-        }
-        if (nan) s = NAN;
-        // this thread's best
+            for (int k = 0; k < kBeamVec; ++k) st += __builtin_amdgcn_exp2f((e[p].get(k) - at) * kLog2e);
+        s = s * (double)(m == mt ? 1.0f : __builtin_amdgcn_exp2f((m - mt) * kLog2e)) + (double)st;
+        m = mt;
+    }
+    // The largest key (0: no candidate); piece p's first place is v + p * stride.
+    __device__ __forceinline__ uint64_t best(uint32_t v, uint32_t stride) const {
         float bx = -INFINITY;
-        int64_t bv = -1;
+        uint32_t at = 0;
 #pragma unroll
         for (int p = 0; p < kBeamPieces; ++p)
 #pragma unroll
             for (int k = 0; k < kBeamVec; ++k)
-                if (e[p][k] > bx) {
-                    bx = e[p][k];
-                    bv = base + (int64_t)(p * 256 + tid) * kBeamVec + k;
+                if (e[p].get(k) > bx) {
+                    bx = e[p].get(k);
+                    at = v + p * stride + k;
                 }
-        uint64_t best = bv < 0 ? 0 : beam_key(bx, (uint32_t)bv);
-#pragma unroll
-        for (int d = 1; d < 4; d <<= 1) {
-            const uint64_t o = shfl_xor_u64(best, d);
-            best = o > best ? o : best;
-        }
-        if ((tid & 3) == 0) quad[tid >> 2] = best;
-        if (tid == 0) nfound = 0;
-        __syncthreads();
-        // the K-th best of the 64 (0 when fewer hold a candidate)
-        const uint64_t mine = quad[lane];
-        int larger = 0;
-#pragma unroll 8
-        for (int i = 0; i < 64; ++i) larger += quad[i] > mine;
-        const unsigned long long at = __ballot(mine != 0 && larger == K - 1);
-        uint64_t bound = 1;                            // every candidate
-        if (at) {
-            const int l = __ffsll(at) - 1;
-            bound = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), l) << 32) |
-                    (uint32_t)__builtin_amdgcn_readlane((int)mine, l);
-        }
-        const uint64_t low = kept[K - 1];
-        bound = low > bound ? low : bound;
+        return bx > -INFINITY ? beam_key(bx, at) : 0;
+    }
+    // f(key) for every candidate whose key is at least `bound`
+    template <typename F>
+    __device__ __forceinline__ void passing(uint64_t bound, uint32_t v, uint32_t stride, F f) const {
+        const float low = beam_key_x(bound);            // (bound 1 or 0: NaN, which nothing is below)
 #pragma unroll
         for (int p = 0; p < kBeamPieces; ++p)
 #pragma unroll
             for (int k = 0; k < kBeamVec; ++k) {
-                if (!(e[p][k] > -INFINITY)) continue;
-                const uint64_t key = beam_key(e[p][k], (uint32_t)(base + (int64_t)(p * 256 + tid) * kBeamVec + k));
-                if (key >= bound) found[atomicAdd(&nfound, 1)] = key;
+                const float x = e[p].get(k);
+                if (!(x > -INFINITY) || x < low) continue;
+                const uint64_t key = beam_key(x, v + p * stride + k);
+                if (key >= bound) f(key);
             }
-        if (tid < K && kept[tid] >= bound) found[atomicAdd(&nfound, 1)] = kept[tid];
+    }
+};
+
+// Sum and maximum of a wave's lanes.
+__device__ __forceinline__ void beam_wave_sum(float& m, double& s) {
+    const float mw = wave_max(m);
+    s = m == mw ? s : s * (double)__builtin_amdgcn_exp2f((m - mw) * kLog2e);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d, 64);
+    m = mw;
+}
+
+// The K-th largest of 64 keys in LDS (1: fewer than K are candidates), by counting.
+__device__ __forceinline__ uint64_t beam_kth(const uint64_t* keys, int K) {
+    const uint64_t mine = keys[threadIdx.x & 63];
+    int larger = 0;
+#pragma unroll 8
+    for (int i = 0; i < 64; ++i) larger += keys[i] > mine;
+    const unsigned long long at = __ballot(mine != 0 && larger == K - 1);
+    return at ? readlane_u64(mine, __builtin_amdgcn_readfirstlane(__ffsll(at) - 1)) : 1;
+}
+
+// Threads that count for one of n entries among `threads` of them: a power of
+// two of at most 64.
+__device__ __forceinline__ int beam_counters(int n, int threads) {
+    int tp = 64;
+    while (tp > 1 && n * tp > threads) tp >>= 1;
+    return tp;
+}
+
+// The K largest keys of a slice of one row.  In the first step: the best key of
+// each four threads; the K-th best of those 64 is a bound that at least K keys
+// reach (each is the best of its own four threads) and that only K of the fours
+// can reach, so at most K * 4 * 32 keys pass into the list.  They are ranked by
+// counting the larger ones.  Later steps pass what reaches the K-th best so far;
+// only where the list would overflow are it and the step ranked again.
+template <typename T>
+__global__ void __launch_bounds__(256)
+beam_row_kernel(const T* __restrict__ logits, BeamArgs a) {
+    extern __shared__ uint64_t found[];               // cap = K * 128 + K
+    __shared__ uint64_t quad[64], kept[kBeamMaxOut];
+    __shared__ float wmax[4];
+    __shared__ double wsum[4];
+    __shared__ int count[2][4], nfound;
+    const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int K = a.K, cap = K * 129;
+    const int64_t rec = (int64_t)row * a.slices + slice;
+    if (a.finished != nullptr && a.finished[row]) return;     // its logits are not read
+    const T* x = logits + (int64_t)row * a.ld;
+    const int64_t v0 = (int64_t)slice * a.slice_len, v1 = min(v0 + a.slice_len, a.V);
+    constexpr int kStride = 256 * kBeamVec;
+    float m = -INFINITY;
+    double s = 0.0;
+    uint64_t bound = 0;                                // 0: no step was ranked yet
+    int listed = 0;                                    // entries of the list, in every thread
+    if (tid < K) kept[tid] = 0;
+    if (tid == 0) nfound = 0;
+    auto load = [&](BeamStep<T>& st, int64_t base) __attribute__((always_inline)) {
+#pragma unroll
+        for (int p = 0; p < kBeamPieces; ++p) st.e[p].load(x, base + (int64_t)p * kStride + tid * kBeamVec, v1);
+    };
+    auto push = [&](uint64_t key) __attribute__((always_inline)) { found[atomicAdd(&nfound, 1)] = key; };
+    // the K best of the list to kept, and the list down to them
+    auto rank = [&]() {
         __syncthreads();
-        const int n = nfound;
-        if (tid < K) kept[tid] = 0;
-        __syncthreads();
-        for (int i = tid; i < n; i += 256) {
+        const int n = nfound, tp = beam_counters(n, 256);
+        for (int i = tid / tp; i < n; i += 256 / tp) {
             const uint64_t key = found[i];
-            int rank = 0;
-            for (int q = 0; q < n; ++q) rank += found[q] > key;
-            if (rank < K) kept[rank] = key;
+            int larger = 0;
+            for (int q = tid & (tp - 1); q < n; q += tp) larger += found[q] > key;
+            for (int d = 1; d < tp; d <<= 1) larger += __shfl_xor(larger, d, 64);
+            if (larger < K) kept[larger] = key;        // (the tp threads of an entry alike)
         }
         __syncthreads();
+        listed = min(n, K);
+        if (tid < listed) found[tid] = kept[tid];
+        if (tid == 0) nfound = listed;
+        bound = max(kept[K - 1], (uint64_t)1);
+        __syncthreads();
+    };
+    BeamStep<T> cur, next;
+    load(cur, v0);
+    int step = 0;
+    for (int64_t base = v0; base < v1; base += kBeamTile, ++step) {
+        if (base + kBeamTile < v1) load(next, base + kBeamTile);
+        cur.sum(m, s);
+        const uint32_t v = (uint32_t)(base + tid * kBeamVec);
+        int all = cap + 1;
+        if (bound != 0) {
+            int n = 0;
+            cur.passing(bound, v, kStride, [&](uint64_t) __attribute__((always_inline)) { ++n; });
+            n = wave_sum_int(n);
+            if (lane == 0) count[step & 1][wave] = n;
+            __syncthreads();
+            all = count[step & 1][0] + count[step & 1][1] + count[step & 1][2] + count[step & 1][3];
+        }
+        const bool full = listed + all > cap;
+        uint64_t low = bound;
+        if (full) {
+            if (listed > 0) rank();
+            uint64_t best = cur.best(v, kStride);
+#pragma unroll
+            for (int d = 1; d < 4; d <<= 1) {
+                const uint64_t o = shfl_xor_u64(best, d);
+                best = o > best ? o : best;
+            }
+            if ((tid & 3) == 0) quad[tid >> 2] = best;
+            __syncthreads();
+            low = max(beam_kth(quad, K), bound);
+        }
+        if (all > 0) cur.passing(low, v, kStride, push);
+        listed += all;
+        if (full || base + kBeamTile >= v1) rank();
+        cur = next;
     }
     // the slice's sum: threads, then waves
-    const float mw = wave_max(m);
-    double sw = mw == -INFINITY ? s : s * (double)__builtin_amdgcn_exp2f((m - mw) * kLog2e);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) sw += __shfl_xor(sw, d, 64);
+    beam_wave_sum(m, s);
     if (lane == 0) {
-        wmax[wave] = mw;
-        wsum[wave] = sw;
+        wmax[wave] = m;
+        wsum[wave] = s;
     }
     __syncthreads();
     if (tid == 0) {
@@ -183,7 +280,7 @@ beam_row_kernel(const T* __restrict__ logits, BeamArgs a) {
         double sb = 0.0;
 #pragma unroll
         for (int w = 0; w < 4; ++w)
-            sb += mb == -INFINITY ? wsum[w] : wsum[w] * (double)__builtin_amdgcn_exp2f((wmax[w] - mb) * kLog2e);
+            sb += wmax[w] == mb ? wsum[w] : wsum[w] * (double)__builtin_amdgcn_exp2f((wmax[w] - mb) * kLog2e);
         a.part_m[rec] = mb;
         a.part_s[rec] = sb;
     }
@@ -194,137 +291,218 @@ beam_row_kernel(const T* __restrict__ logits, BeamArgs a) {
     }
 }
 
-struct BeamCand {
+// ------------------------------------------------------------------ groups
+
+struct __align__(16) BeamCand {
     double value;
-    uint32_t place;             // (row in group) * V + token
+    uint32_t place;             // (row in group) * V + token; kBeamNone: no candidate
     uint32_t pad;
 };
-// larger value first, then the lower place
-__device__ __forceinline__ bool beam_before(double v, uint32_t p, double w, uint32_t q) {
-    return v > w || (v == w && p < q);
+constexpr uint32_t kBeamNone = 0xffffffffu;
+// larger value first, then the lower place (a place that is none has value -inf)
+__device__ __forceinline__ bool beam_before(const BeamCand& a, const BeamCand& b) {
+    return a.value > b.value || (a.value == b.value && a.place < b.place);
 }
 
-__global__ void __launch_bounds__(256)
-beam_group_kernel(BeamArgs a, int cap) {
-    extern __shared__ BeamCand list[];                // cap
-    __shared__ double lse[kBeamMaxBeams], qv[64];
-    __shared__ float sc[kBeamMaxBeams];
-    __shared__ uint32_t qp[64];
-    __shared__ uint8_t fin[kBeamMaxBeams];
-    __shared__ int nfound;
-    const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-    const int W = a.W, K = a.K, S = a.slices;
-    constexpr uint32_t kNone = 0xffffffffu;
-    if (tid < W) {
-        const int row = g * W + tid;
-        const bool f = a.finished != nullptr && a.finished[row];
-        fin[tid] = f;
-        sc[tid] = a.scores[row];
-        double l = 0.0;
-        if (!f) {
-            float mb = -INFINITY;
-            for (int i = 0; i < S; ++i) mb = fmaxf(mb, a.part_m[(int64_t)row * S + i]);
-            for (int i = 0; i < S; ++i) {
-                const float mi = a.part_m[(int64_t)row * S + i];
-                l += a.part_s[(int64_t)row * S + i] * (mb == -INFINITY ? 1.0 : exp((double)mi - (double)mb));
-            }
-            l = (double)mb + log(l);                  // -inf: no logit; NaN: a NaN or +inf among them
-        }
-        lse[tid] = l;
+// A row's candidate as it enters the group: its value and place, or none where
+// the value is not finite (a score or a sum that is not; a logit that is ruled out).
+__device__ __forceinline__ BeamCand beam_cand(bool any, float x, double lse, float score, int w, int64_t V,
+                                              int64_t token) {
+    BeamCand c{-INFINITY, kBeamNone, 0};
+    const double value = ((double)x - lse) + (double)score;
+    if (any && value > -INFINITY && value < INFINITY) {
+        c.value = value;
+        c.place = (uint32_t)(w * V + token);
     }
-    if (tid == 0) nfound = 0;
-    __syncthreads();
-    const int n = W * S * K;
-    auto candidate = [&](int i, double* v, uint32_t* p) {
-        const int w = i / (S * K), k = i - w * S * K;
-        *v = -INFINITY;
-        *p = kNone;
-        double value;
-        uint32_t place;
-        if (fin[w]) {
-            if (k != 0) return;
-            value = (double)sc[w];
-            place = (uint32_t)(w * a.V + a.pad);
-        } else {
-            const int64_t r = (int64_t)(g * W + w) * S * K + k;
-            const int32_t tok = a.cand_v[r];
-            if (tok < 0) return;
-            value = ((double)a.cand_x[r] - lse[w]) + (double)sc[w];
-            place = (uint32_t)(w * a.V + tok);
-        }
-        if (!(value > -INFINITY && value < INFINITY)) return;     // NaN as well
-        *v = value;
-        *p = place;
-    };
-    double bv = -INFINITY;
-    uint32_t bp = kNone;
-    for (int i = tid; i < n; i += 256) {
-        double v;
-        uint32_t p;
-        candidate(i, &v, &p);
-        if (p != kNone && (bp == kNone || beam_before(v, p, bv, bp))) {
-            bv = v;
-            bp = p;
-        }
-    }
-#pragma unroll
-    for (int d = 1; d < 4; d <<= 1) {
-        const double ov = __shfl_xor(bv, d, 64);
-        const uint32_t op = __shfl_xor(bp, d, 64);
-        if (op != kNone && (bp == kNone || beam_before(ov, op, bv, bp))) {
-            bv = ov;
-            bp = op;
-        }
-    }
-    if ((tid & 3) == 0) {
-        qv[tid >> 2] = bv;
-        qp[tid >> 2] = bp;
-    }
-    __syncthreads();
-    const double mv = qv[lane];
-    const uint32_t mp = qp[lane];
-    int larger = 0;
-    for (int i = 0; i < 64; ++i) larger += qp[i] != kNone && beam_before(qv[i], qp[i], mv, mp);
-    const unsigned long long at = __ballot(mp != kNone && larger == K - 1);
-    double tv = -INFINITY;
-    uint32_t tp = kNone;
-    if (at) {
-        const int l = __ffsll(at) - 1;
-        tv = __shfl(mv, l, 64);
-        tp = __shfl(mp, l, 64);
-    }
-    for (int i = tid; i < n; i += 256) {
-        double v;
-        uint32_t p;
-        candidate(i, &v, &p);
-        if (p == kNone || beam_before(tv, tp, v, p)) continue;     // below the bound
-        const int k = atomicAdd(&nfound, 1);
-        if (k < cap) list[k] = BeamCand{v, p, 0};
-    }
-    __syncthreads();
-    const int m = min(nfound, cap);
-    for (int i = tid; i < m; i += 256) {
+    return c;
+}
+
+// The best K of n entries of `list` (LDS) to the group's outputs, and the places
+// behind the last candidate; all threads of the block, after a barrier.
+__device__ __forceinline__ void beam_write(const BeamArgs& a, const BeamCand* list, int n, int g, const uint8_t* fin) {
+    const int K = a.K, NT = blockDim.x, tid = threadIdx.x, tp = beam_counters(n, NT);
+    for (int i = tid / tp; i < n; i += NT / tp) {
         const BeamCand c = list[i];
-        int rank = 0;
-        for (int q = 0; q < m; ++q) rank += beam_before(list[q].value, list[q].place, c.value, c.place);
-        if (rank < K) {
-            const int64_t o = (int64_t)g * K + rank;
-            const int w = (int)(c.place / (uint32_t)a.V);
-            const int64_t tok = c.place - (int64_t)w * a.V;
-            a.out_scores[o] = (float)c.value;
-            a.out_parent[o] = g * W + w;
-            a.out_token[o] = tok;
-            if (a.out_finished != nullptr) a.out_finished[o] = fin[w] || tok == a.eos;
-        }
+        if (c.place == kBeamNone) continue;
+        int before = 0;
+        for (int q = tid & (tp - 1); q < n; q += tp) before += beam_before(list[q], c);
+        for (int d = 1; d < tp; d <<= 1) before += __shfl_xor(before, d, 64);
+        if (before >= K || (tid & (tp - 1)) != 0) continue;
+        const int64_t o = (int64_t)g * K + before;
+        const int w = (int)(c.place / (uint32_t)a.V);
+        const int64_t tok = c.place - (int64_t)w * a.V;
+        a.out_scores[o] = (float)c.value;
+        a.out_parent[o] = g * a.W + w;
+        a.out_token[o] = tok;
+        if (a.out_finished != nullptr) a.out_finished[o] = fin[w] || tok == a.eos;
     }
+    int some = 0;
+    for (int i = tid; i < n; i += NT) some += list[i].place != kBeamNone;
+    __shared__ int valid;
+    if (tid == 0) valid = 0;
+    __syncthreads();
+    some = wave_sum_int(some);
+    if ((tid & 63) == 0 && some > 0) atomicAdd(&valid, some);
+    __syncthreads();
     // fewer candidates than places: no parent but the group's first row
-    for (int k = m + tid; k < K; k += 256) {
+    for (int k = valid + tid; k < K; k += NT) {
         const int64_t o = (int64_t)g * K + k;
         a.out_scores[o] = -INFINITY;
-        a.out_parent[o] = g * W;
+        a.out_parent[o] = g * a.W;
         a.out_token[o] = a.pad;
         if (a.out_finished != nullptr) a.out_finished[o] = 0;
     }
+}
+
+// One block per group: the rows' sums from their slices', the survivors' values,
+// and the K best of them.  More than 256 survivors pass a bound first, as in
+// beam_row_kernel: the K-th best of the 64 bests of 16 threads each.
+__global__ void __launch_bounds__(1024)
+beam_group_kernel(BeamArgs a) {
+    __shared__ BeamCand list[kBeamMaxCand], top[64];
+    __shared__ double lse[kBeamMaxBeams];
+    __shared__ float sc[kBeamMaxBeams];
+    __shared__ uint8_t fin[kBeamMaxBeams];
+    __shared__ int nfound;
+    const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    const int W = a.W, K = a.K, S = a.slices, SK = S * K, n = W * SK;
+    // the survivors' logits are on their way while the sums are joined
+    float cx[2];
+    int32_t cv[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int i = tid + 1024 * k;
+        cx[k] = 0.0f;
+        cv[k] = -1;
+        if (i < n) {
+            const int64_t r = (int64_t)g * n + i;
+            cx[k] = a.cand_x[r];
+            cv[k] = a.cand_v[r];
+        }
+    }
+    if (tid < W) {
+        fin[tid] = a.finished != nullptr && a.finished[g * W + tid];
+        sc[tid] = a.scores[g * W + tid];
+    }
+    if (tid == 0) nfound = 0;
+    for (int w = tid >> 6; w < W; w += 16) {
+        const int64_t r = (int64_t)(g * W + w) * S;
+        float mb = -INFINITY;
+        for (int i = lane; i < S; i += 64) mb = fmaxf(mb, a.part_m[r + i]);
+        mb = wave_max(mb);
+        double l = 0.0;
+        for (int i = lane; i < S; i += 64) {
+            const float mi = a.part_m[r + i];
+            l += mi == mb ? a.part_s[r + i] : a.part_s[r + i] * exp((double)mi - (double)mb);
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
+        if (lane == 0) lse[w] = (double)mb + log(l);   // -inf: no logit; NaN: a NaN or +inf among them
+    }
+    __syncthreads();
+    BeamCand c[2], best{-INFINITY, kBeamNone, 0};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int i = tid + 1024 * k, w = i < n ? i / SK : 0;
+        const bool f = fin[w];                          // one candidate, its own score
+        c[k] = f ? beam_cand(i < n && i - w * SK == 0, 0.0f, 0.0, sc[w], w, a.V, a.pad)
+                 : beam_cand(i < n && cv[k] >= 0, cx[k], lse[w], sc[w], w, a.V, cv[k]);
+        if (beam_before(c[k], best)) best = c[k];
+    }
+    BeamCand bound{-INFINITY, kBeamNone, 0};
+    if (n > 256) {
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) {
+            const BeamCand o{__shfl_xor(best.value, d, 64), (uint32_t)__shfl_xor((int)best.place, d, 64), 0};
+            if (beam_before(o, best)) best = o;
+        }
+        if ((tid & 15) == 0) top[tid >> 4] = best;
+        __syncthreads();
+        const BeamCand mine = top[lane];
+        int before = 0;
+        for (int i = 0; i < 64; ++i) before += beam_before(top[i], mine);
+        const unsigned long long at = __ballot(mine.place != kBeamNone && before == K - 1);
+        if (at) bound = top[__builtin_amdgcn_readfirstlane(__ffsll(at) - 1)];
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        if (c[k].place != kBeamNone && !beam_before(bound, c[k])) list[atomicAdd(&nfound, 1)] = c[k];
+    __syncthreads();
+    beam_write(a, list, nfound, g, fin);
+}
+
+// ------------------------------------------------------------------ a whole group in one block
+
+// Groups of up to kBeamWhole logits (W rounded up to a power of two, times V):
+// 16 >> wl waves per row, 32 logits per thread, one launch.  A row's bound comes
+// from the bests of 64 equal parts of its threads, so that up to K * (16 >> wl) * 32
+// keys pass; ranked, its K best enter the group.
+template <typename T>
+__global__ void __launch_bounds__(1024)
+beam_whole_kernel(const T* __restrict__ logits, BeamArgs a, int wl, int cap) {
+    extern __shared__ uint64_t found[];               // cap per row of the power of two
+    __shared__ uint64_t part[kBeamWholeBeams * 64];
+    __shared__ BeamCand list[kBeamWholeBeams * kBeamWholeOut];
+    __shared__ float wmax[16];
+    __shared__ double wsum[16];
+    __shared__ int nfound[kBeamWholeBeams];
+    __shared__ uint8_t fin[kBeamWholeBeams];
+    const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int W = a.W, K = a.K, wpr = 16 >> wl;
+    const int w = wave >> (4 - wl), sub = wave & (wpr - 1), t = sub * 64 + lane, nt = wpr * 64;   // thread t of nt of row w
+    const int row = g * W + min(w, W - 1);
+    const bool dead = w >= W, fn = a.finished != nullptr && a.finished[row] != 0;
+    const float score = a.scores[row];
+    const T* x = logits + (int64_t)row * a.ld;
+    const int64_t v1 = dead || fn ? 0 : a.V;           // a finished row's logits are not read
+    const int stride = nt * kBeamVec, v = t * kBeamVec;
+    BeamStep<T> st;
+#pragma unroll
+    for (int p = 0; p < kBeamPieces; ++p) st.e[p].load(x, v + (int64_t)p * stride, v1);
+    if (t == 0 && !dead) fin[w] = fn;
+    if (tid < kBeamWholeBeams) nfound[tid] = 0;
+    float m = -INFINITY;
+    double s = 0.0;
+    st.sum(m, s);
+    beam_wave_sum(m, s);
+    if (lane == 0) {
+        wmax[wave] = m;
+        wsum[wave] = s;
+    }
+    uint64_t best = st.best((uint32_t)v, (uint32_t)stride);
+    for (int d = 1; d < wpr; d <<= 1) {
+        const uint64_t o = shfl_xor_u64(best, d);
+        best = o > best ? o : best;
+    }
+    if ((t & (wpr - 1)) == 0) part[w * 64 + t / wpr] = best;
+    for (int i = t; i < K; i += nt) list[w * K + i] = BeamCand{-INFINITY, kBeamNone, 0};
+    __syncthreads();
+    uint64_t* mine = found + (size_t)w * cap;
+    st.passing(beam_kth(part + w * 64, K), (uint32_t)v, (uint32_t)stride,
+               [&](uint64_t key) __attribute__((always_inline)) { mine[atomicAdd(&nfound[w], 1)] = key; });
+    // the row's logsumexp
+    float mb = -INFINITY;
+    for (int i = 0; i < wpr; ++i) mb = fmaxf(mb, wmax[w * wpr + i]);
+    double l = 0.0;
+    for (int i = 0; i < wpr; ++i) {
+        const float mi = wmax[w * wpr + i];
+        l += mi == mb ? wsum[w * wpr + i] : wsum[w * wpr + i] * exp((double)mi - (double)mb);
+    }
+    const double lse = (double)mb + log(l);
+    __syncthreads();
+    const int n = nfound[w];
+    const int tp = beam_counters(n, nt);
+    for (int i = t / tp; i < n; i += nt / tp) {
+        const uint64_t key = mine[i];
+        int larger = 0;
+        for (int q = t & (tp - 1); q < n; q += tp) larger += mine[q] > key;
+        for (int d = 1; d < tp; d <<= 1) larger += __shfl_xor(larger, d, 64);
+        if (larger < K && (t & (tp - 1)) == 0)
+            list[w * K + larger] = beam_cand(true, beam_key_x(key), lse, score, w, a.V, (uint32_t)~(uint32_t)key);
+    }
+    if (fn && !dead && t == 0) list[w * K] = beam_cand(true, 0.0f, 0.0, score, w, a.V, a.pad);
+    __syncthreads();
+    beam_write(a, list, W * K, g, fin);
 }
 
 // ------------------------------------------------------------------ reorder
@@ -385,6 +563,15 @@ reorder_rows_kernel(ReorderArgs a) {
 
 // ------------------------------------------------------------------ host side
 
+// Whether one block takes a whole group: the beams' power of two (its logarithm),
+// or -1.
+static int beam_whole(int64_t W, int64_t V, int64_t K) {
+    if (W > kBeamWholeBeams || K > kBeamWholeOut) return -1;
+    int wl = 0;
+    while ((1 << wl) < W) ++wl;
+    return (V << wl) <= kBeamWhole ? wl : -1;
+}
+
 // Slices of a row: enough blocks for the device, each at least a quarter of a
 // step's logits, and few enough that a group's survivors fit one block.
 static int64_t beam_slices(int64_t rows, int64_t W, int64_t V, int64_t K) {
@@ -400,7 +587,7 @@ static int64_t beam_slices(int64_t rows, int64_t W, int64_t V, int64_t K) {
 using namespace loom;
 
 extern "C" int64_t loom_beam_select_workspace_bytes(int64_t groups, int64_t beams, int64_t V, int64_t n_out) {
-    if (groups <= 0 || beams <= 0 || V <= 0 || n_out <= 0) return 0;
+    if (groups <= 0 || beams <= 0 || V <= 0 || n_out <= 0 || beam_whole(beams, V, n_out) >= 0) return 0;
     const int64_t recs = groups * beams * beam_slices(groups * beams, beams, V, n_out);
     return recs * (8 + 4 + 8 * n_out) + 16;
 }
@@ -423,6 +610,7 @@ extern "C" int loom_beam_select(int dtype, const void* logits, int64_t logits_ld
     LOOM_CHECK(pad_id >= 0 && pad_id < V, "%s: pad_id must lie in [0, %lld), got %lld", who, (long long)V, (long long)pad_id);
     LOOM_CHECK(logits && scores && out_scores && out_parent && out_token, "%s: a required pointer is NULL", who);
     const int64_t need = loom_beam_select_workspace_bytes(groups, beams, V, n_out);
+    const int wl = beam_whole(beams, V, n_out);
     LOOM_CHECK(workspace_bytes >= need && (workspace != nullptr || need == 0) && ((uintptr_t)workspace % 16) == 0,
                "%s: a 16-byte aligned workspace of %lld bytes is needed, got %lld", who, (long long)need,
                (long long)workspace_bytes);
@@ -439,16 +627,28 @@ extern "C" int loom_beam_select(int dtype, const void* logits, int64_t logits_ld
     a.W = (int)beams;
     a.K = (int)n_out;
     a.groups = (int)groups;
+    a.eos = eos_id;
+    a.pad = pad_id;
+    hipStream_t st = (hipStream_t)stream;
+    if (wl >= 0) {
+        // (at most K of a row's 64 parts reach its bound, each of (16 >> wl) * 32 logits)
+        const int cap = (int)n_out * (16 >> wl) * 32;
+        const unsigned lds = (unsigned)((size_t)cap * beams * sizeof(uint64_t));
+#define LOOM_BEAM_WHOLE(T) \
+        hipLaunchKernelGGL((beam_whole_kernel<T>), dim3((unsigned)groups), dim3(1024), lds, st, (const T*)logits, a, wl, cap)
+        if (dtype == LOOM_F32) LOOM_BEAM_WHOLE(float);
+        else if (dtype == LOOM_BF16) LOOM_BEAM_WHOLE(bf16_t);
+        else LOOM_BEAM_WHOLE(f16_t);
+#undef LOOM_BEAM_WHOLE
+        return launch_status("loom_beam_select");
+    }
     const int64_t rows = groups * beams, S = beam_slices(rows, beams, V, n_out), recs = rows * S;
     a.slice_len = ceil_div(ceil_div(V, S), kBeamVec) * kBeamVec;
     a.slices = (int)S;
-    a.eos = eos_id;
-    a.pad = pad_id;
     a.part_s = (double*)workspace;
     a.part_m = (float*)(a.part_s + recs);
     a.cand_x = a.part_m + recs;
     a.cand_v = (int32_t*)(a.cand_x + recs * n_out);
-    hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)S, (unsigned)rows);
     const unsigned lds = (unsigned)((n_out * 128 + n_out) * sizeof(uint64_t));
     if (dtype == LOOM_F32)
@@ -458,10 +658,7 @@ extern "C" int loom_beam_select(int dtype, const void* logits, int64_t logits_ld
     else
         hipLaunchKernelGGL((beam_row_kernel<f16_t>), grid, dim3(256), lds, st, (const f16_t*)logits, a);
     if (int rc = launch_status("loom_beam_select(rows)")) return rc;
-    // at most K fours of threads reach the bound, each with its share of the survivors
-    const int64_t n = beams * S * n_out, pass = n_out * 4 * ceil_div(n, 256), cap = pass < n ? pass : n;
-    hipLaunchKernelGGL(beam_group_kernel, dim3((unsigned)groups), dim3(256), (unsigned)(cap * sizeof(BeamCand)), st, a,
-                       (int)cap);
+    hipLaunchKernelGGL(beam_group_kernel, dim3((unsigned)groups), dim3(1024), 0, st, a);
     return launch_status("loom_beam_select(groups)");
 }
 

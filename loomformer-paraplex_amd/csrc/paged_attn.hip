@@ -21,7 +21,7 @@ typedef _Float16 pg_f16x8 __attribute__((ext_vector_type(8)));
 constexpr int kPgTile = 32;       // tokens of one wave step of the matrix-core form
 constexpr int kPgMinTiles = 4;    // tiles of a chunk at least: one per wave
 constexpr int kPgStream = 16;     // tiles per block from which the rows are laid end to end
-constexpr int kPgRowCost = 2;     // what starting on a row costs a block, in tiles
+constexpr int kPgRowCost = 6;     // what starting on a row costs a block, in tiles
 constexpr int kPgWhole = 512;     // rows of up to so many tokens are not split
 constexpr int kPgMaxRows = 1024;
 
@@ -56,15 +56,6 @@ __device__ __forceinline__ int row_tokens(const int32_t* lens, int b, int step, 
     const int n = lens[b];
     *bad = n >= 0 && (n > cap - step || (step && n >= n_pos));
     return n < 0 || *bad ? 0 : n + step;
-}
-
-__device__ __forceinline__ int wave_sum_int(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, kDppQuad1032, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, kDppQuad2301, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, kDppHalfMirror, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, kDppMirror, 0xF, 0xF, false);
-    return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) +
-           __builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48);
 }
 
 // inclusive scan over the wave

@@ -404,7 +404,10 @@ def _check_select(x, sc, K, finished=None, eos=-1, pad=0):
 
 @pytest.mark.parametrize("dt", [BF, HF, FP])
 @pytest.mark.parametrize("S,W,V,K", [(1, 1, 1, 1), (1, 4, 4096, 4), (3, 5, 777, 10), (2, 8, 8193, 16), (1, 32, 501, 64),
-                                     (2, 3, 20000, 3), (1, 1, 70, 64), (1, 2, 9, 18)])
+                                     (2, 3, 20000, 3), (1, 1, 70, 64), (1, 2, 9, 18),
+                                     # one block per group: its largest sizes, and one more
+                                     (2, 1, 32768, 32), (2, 1, 32769, 32), (1, 16, 2048, 32), (1, 9, 2047, 7), (1, 16, 2049, 5),
+                                     (2, 2, 16383, 31), (1, 17, 300, 4), (1, 5, 4095, 33)])
 def test_select(dt, S, W, V, K):
     g = torch.Generator().manual_seed(V + K)
     x = (torch.randn(S * W, V, generator=g) * 3).to(DEV, dt)
@@ -426,13 +429,14 @@ def test_select_many_rows_steps_through_long_slices():
 
 
 @pytest.mark.parametrize("kind", ["ascending", "descending", "constant", "steps", "blocks"])
-def test_select_ties_and_orders(kind):
+@pytest.mark.parametrize("V", [24001, 24000, 8185])
+def test_select_ties_and_orders(kind, V):
     """Logits whose largest values lie together, rise towards the end or are all
     the same; ties inside a row and between rows go to the lowest (beam, token)."""
-    V, W = 24000, 4
+    W = 4
     i = torch.arange(V, dtype=torch.float64)
     x = {"ascending": i / 1000, "descending": -i / 1000, "constant": 0 * i, "steps": (i // 300) / 8,
-         "blocks": torch.where((i >= 9000) & (i < 9128), 5.0, 0.0)}[kind]
+         "blocks": torch.where((i >= 7000) & (i < 7128), 5.0, 0.0)}[kind]
     x = x.float().expand(512, V).contiguous().to(DEV)   # 512 rows: several steps per slice
     sc = torch.zeros(128, W, device=DEV)
     from loom_amd import ops
@@ -451,8 +455,8 @@ def test_select_ties_and_orders(kind):
 
 def test_select_finished_dead_and_ruled_out():
     g = torch.Generator().manual_seed(12)
-    for dt in (BF, FP):
-        S, W, V = 7, 4, 3000
+    for dt, V in ((BF, 3000), (FP, 3000), (BF, 30000)):
+        S, W = 7, 4
         x = (torch.randn(S * W, V, generator=g) * 2).to(DEV, dt)
         sc = (-2 * torch.rand(S, W, generator=g)).to(DEV)
         fin = torch.zeros(S * W, dtype=torch.bool, device=DEV)

@@ -81,13 +81,13 @@ def test_paged_update_write_compact_refuse():
 
 
 def test_beam_select_and_reorder_refuse():
-    sel = dict(dtype=1, logits=P, ld=100, scores=P, finished=None, os=P, op=P, ot=P, of=None, groups=2, beams=4, V=100,
-               n_out=4, eos=-1, pad=0, ws=P, ws_bytes=1 << 24, stream=None)
+    sel = dict(dtype=1, logits=P, ld=20000, scores=P, finished=None, os=P, op=P, ot=P, of=None, groups=2, beams=4,
+               V=20000, n_out=4, eos=-1, pad=0, ws=P, ws_bytes=1 << 24, stream=None)
     _refuses("loom_beam_select", sel, [
         (dict(dtype=9), "unsupported dtype"), (dict(beams=33), "1 to 32 beams"), (dict(beams=0), "1 to 32 beams"),
         (dict(groups=-1), "1 to 32 beams"), (dict(groups=65535), "at most 65535 rows"), (dict(V=0, n_out=0), "vocabulary"),
-        (dict(V=(1 << 24) + 1, ld=1 << 25), "vocabulary"), (dict(ld=99), "row stride 99"), (dict(n_out=0), "n_out"),
-        (dict(n_out=65), "n_out"), (dict(V=10, n_out=41), "n_out"), (dict(pad=100), "pad_id"), (dict(pad=-1), "pad_id"),
+        (dict(V=(1 << 24) + 1, ld=1 << 25), "vocabulary"), (dict(ld=19999), "row stride 19999"), (dict(n_out=0), "n_out"),
+        (dict(n_out=65), "n_out"), (dict(V=10, n_out=41), "n_out"), (dict(pad=20000), "pad_id"), (dict(pad=-1), "pad_id"),
         (dict(logits=None), "required pointer"), (dict(ot=None), "required pointer"), (dict(ws_bytes=10), "workspace"),
         (dict(ws=ctypes.c_void_p(260)), "workspace")])
     one = lambda v: (ctypes.c_int64 * 1)(v)  # noqa: E731
@@ -110,7 +110,8 @@ def test_workspace_queries():
     assert lib.loom_paged_update_workspace_bytes(7) == 7 * 16
     assert lib.loom_paged_compact_workspace_bytes(10) == 136
     assert lib.loom_beam_select_workspace_bytes(0, 4, 100, 4) == 0
-    assert lib.loom_beam_select_workspace_bytes(2, 4, 100, 4) >= 8 * (12 + 8 * 4)
+    assert lib.loom_beam_select_workspace_bytes(2, 4, 100, 4) == 0              # one block per group
+    assert lib.loom_beam_select_workspace_bytes(2, 4, 100000, 4) >= 8 * (12 + 8 * 4)
 
 
 def test_mirror_refuses_cpu_tensors():
