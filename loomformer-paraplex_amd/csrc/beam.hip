@@ -523,42 +523,59 @@ struct ReorderArgs {
 // Row r of every tensor becomes the former row parent[r].  A block owns a slice
 // of columns of one tensor for all rows: every thread reads its rows' new
 // values, the block meets, every thread writes, so no second buffer is needed.
-// Rows that stay, and rows whose parent is no row, are not touched.
+// Rows that stay, and rows whose parent is no row, are not touched: the block
+// first lists the rows that move.
 template <typename V, int RPT, int NT>
-__device__ __forceinline__ void reorder_slice(const ReorderSeg& s, const int32_t* parent, int R, int tx_log,
-                                              int slice, int64_t outer) {
+__device__ __forceinline__ void reorder_slice(const ReorderSeg& s, const int2* moves, int n, int tx_log, int slice,
+                                              int64_t outer) {
     const int TX = 1 << tx_log, TY = NT >> tx_log;
     const int tx = threadIdx.x & (TX - 1), ty = threadIdx.x >> tx_log;
     const int64_t col = ((int64_t)slice * TX + tx) * sizeof(V);
     char* base = s.p + outer * s.outer_stride + col;
     const bool in = col < s.row_bytes;
     V val[RPT];
-    bool move[RPT];
+    if (in) {
 #pragma unroll
-    for (int k = 0; k < RPT; ++k) {
-        const int r = ty + k * TY;
-        const int p = in && r < R ? parent[r] : -1;
-        move[k] = p >= 0 && p < R && p != r;
-        if (move[k]) val[k] = *reinterpret_cast<const V*>(base + p * s.row_stride);
+        for (int k = 0; k < RPT; ++k)
+            if (ty + k * TY < n) val[k] = *reinterpret_cast<const V*>(base + moves[ty + k * TY].y * s.row_stride);
     }
     __syncthreads();
+    if (in) {
 #pragma unroll
-    for (int k = 0; k < RPT; ++k)
-        if (move[k]) *reinterpret_cast<V*>(base + (int64_t)(ty + k * TY) * s.row_stride) = val[k];
+        for (int k = 0; k < RPT; ++k)
+            if (ty + k * TY < n) *reinterpret_cast<V*>(base + moves[ty + k * TY].x * s.row_stride) = val[k];
+    }
 }
 
 template <int RPT, int NT>
 __global__ void __launch_bounds__(NT)
 reorder_rows_kernel(ReorderArgs a) {
+    __shared__ int2 moves[kReorderRows];
+    __shared__ int counts[NT / 64];
     int i = 0;
     while (i + 1 < a.nseg && (int)blockIdx.x >= a.seg[i + 1].block0) ++i;
     const ReorderSeg& s = a.seg[i];
     const int k = blockIdx.x - s.block0;
     const int slice = k % s.slices;
     const int64_t outer = k / s.slices;
-    if (s.vec == 16) reorder_slice<u32x4, RPT, NT>(s, a.parent, a.R, a.tx_log, slice, outer);
-    else if (s.vec == 4) reorder_slice<uint32_t, RPT, NT>(s, a.parent, a.R, a.tx_log, slice, outer);
-    else reorder_slice<uint8_t, RPT, NT>(s, a.parent, a.R, a.tx_log, slice, outer);
+    const int tid = threadIdx.x, wave = tid >> 6;     // (at most NT rows)
+    const int p = tid < a.R ? a.parent[tid] : -1;
+    const bool move = p >= 0 && p < a.R && p != tid;
+    const unsigned long long who = __ballot(move);
+    if ((tid & 63) == 0) counts[wave] = __popcll(who);
+    __syncthreads();
+    int at = __popcll(who & ((1ull << (tid & 63)) - 1)), n = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) {
+        if (w < wave) at += counts[w];
+        n += counts[w];
+    }
+    if (move) moves[at] = make_int2(tid, p);
+    __syncthreads();
+    if (n == 0) return;
+    if (s.vec == 16) reorder_slice<u32x4, RPT, NT>(s, moves, n, a.tx_log, slice, outer);
+    else if (s.vec == 4) reorder_slice<uint32_t, RPT, NT>(s, moves, n, a.tx_log, slice, outer);
+    else reorder_slice<uint8_t, RPT, NT>(s, moves, n, a.tx_log, slice, outer);
 }
 
 // ------------------------------------------------------------------ host side
