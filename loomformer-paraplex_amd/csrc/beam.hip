@@ -105,18 +105,26 @@ struct BeamPiece {
     }
 };
 
-// A thread's logits of one step: place of element k of piece p is v(p) + k.
+// A thread's logits of one step: place of element k of piece p is v + p * stride + k.
 template <typename T>
 struct BeamStep {
     BeamPiece<T> e[kBeamPieces];
+    float top[kBeamPieces];                            // largest of each piece (NaNs apart)
+    __device__ __forceinline__ void maxima() {
+#pragma unroll
+        for (int p = 0; p < kBeamPieces; ++p) {
+            top[p] = e[p].get(0);
+#pragma unroll
+            for (int k = 1; k < kBeamVec; ++k) top[p] = fmaxf(top[p], e[p].get(k));
+        }
+    }
+    __device__ __forceinline__ float most() const {
+        return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    }
     // Running maximum and sum of exponentials.  A NaN makes the sum NaN, and so does
     // +inf; the maximum stays -inf while there is no other logit.
     __device__ __forceinline__ void sum(float& m, double& s) const {
-        float mt = m;
-#pragma unroll
-        for (int p = 0; p < kBeamPieces; ++p)
-#pragma unroll
-            for (int k = 0; k < kBeamVec; ++k) mt = fmaxf(mt, e[p].get(k));
+        const float mt = fmaxf(m, most());
         const float at = mt == -INFINITY ? 0.0f : mt;
         float st = 0.0f;
 #pragma unroll
@@ -126,33 +134,33 @@ struct BeamStep {
         s = s * (double)(m == mt ? 1.0f : __builtin_amdgcn_exp2f((m - mt) * kLog2e)) + (double)st;
         m = mt;
     }
-    // The largest key (0: no candidate); piece p's first place is v + p * stride.
+    // The largest key (0: no candidate)
     __device__ __forceinline__ uint64_t best(uint32_t v, uint32_t stride) const {
-        float bx = -INFINITY;
+        const float x = most();
         uint32_t at = 0;
 #pragma unroll
-        for (int p = 0; p < kBeamPieces; ++p)
+        for (int p = kBeamPieces - 1; p >= 0; --p)
 #pragma unroll
-            for (int k = 0; k < kBeamVec; ++k)
-                if (e[p].get(k) > bx) {
-                    bx = e[p].get(k);
-                    at = v + p * stride + k;
-                }
-        return bx > -INFINITY ? beam_key(bx, at) : 0;
+            for (int k = kBeamVec - 1; k >= 0; --k)
+                if (e[p].get(k) == x) at = v + p * stride + k;
+        return x > -INFINITY ? beam_key(x, at) : 0;
     }
-    // f(key) for every candidate whose key is at least `bound`
+    // f(key) for every candidate whose key is at least `bound`; a piece whose largest
+    // is below it is passed over
     template <typename F>
     __device__ __forceinline__ void passing(uint64_t bound, uint32_t v, uint32_t stride, F f) const {
-        const float low = beam_key_x(bound);            // (bound 1 or 0: NaN, which nothing is below)
+        const float low = bound > 1 ? beam_key_x(bound) : -3.402823466e38f;      // (1: every candidate)
 #pragma unroll
-        for (int p = 0; p < kBeamPieces; ++p)
+        for (int p = 0; p < kBeamPieces; ++p) {
+            if (!(top[p] >= low)) continue;
 #pragma unroll
             for (int k = 0; k < kBeamVec; ++k) {
                 const float x = e[p].get(k);
-                if (!(x > -INFINITY) || x < low) continue;
+                if (!(x >= low)) continue;
                 const uint64_t key = beam_key(x, v + p * stride + k);
                 if (key >= bound) f(key);
             }
+        }
     }
 };
 
@@ -238,6 +246,7 @@ beam_row_kernel(const T* __restrict__ logits, BeamArgs a) {
     int step = 0;
     for (int64_t base = v0; base < v1; base += kBeamTile, ++step) {
         if (base + kBeamTile < v1) load(next, base + kBeamTile);
+        cur.maxima();
         cur.sum(m, s);
         const uint32_t v = (uint32_t)(base + tid * kBeamVec);
         int all = cap + 1;
@@ -445,6 +454,8 @@ beam_whole_kernel(const T* __restrict__ logits, BeamArgs a, int wl, int cap) {
     __shared__ BeamCand list[kBeamWholeBeams * kBeamWholeOut];
     __shared__ float wmax[16];
     __shared__ double wsum[16];
+    __shared__ uint64_t bound[kBeamWholeBeams];
+    __shared__ double lse_of[kBeamWholeBeams];
     __shared__ int nfound[kBeamWholeBeams];
     __shared__ uint8_t fin[kBeamWholeBeams];
     const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -463,6 +474,7 @@ beam_whole_kernel(const T* __restrict__ logits, BeamArgs a, int wl, int cap) {
     if (tid < kBeamWholeBeams) nfound[tid] = 0;
     float m = -INFINITY;
     double s = 0.0;
+    st.maxima();
     st.sum(m, s);
     beam_wave_sum(m, s);
     if (lane == 0) {
@@ -477,18 +489,24 @@ beam_whole_kernel(const T* __restrict__ logits, BeamArgs a, int wl, int cap) {
     if ((t & (wpr - 1)) == 0) part[w * 64 + t / wpr] = best;
     for (int i = t; i < K; i += nt) list[w * K + i] = BeamCand{-INFINITY, kBeamNone, 0};
     __syncthreads();
-    uint64_t* mine = found + (size_t)w * cap;
-    st.passing(beam_kth(part + w * 64, K), (uint32_t)v, (uint32_t)stride,
-               [&](uint64_t key) __attribute__((always_inline)) { mine[atomicAdd(&nfound[w], 1)] = key; });
-    // the row's logsumexp
-    float mb = -INFINITY;
-    for (int i = 0; i < wpr; ++i) mb = fmaxf(mb, wmax[w * wpr + i]);
-    double l = 0.0;
-    for (int i = 0; i < wpr; ++i) {
-        const float mi = wmax[w * wpr + i];
-        l += mi == mb ? wsum[w * wpr + i] : wsum[w * wpr + i] * exp((double)mi - (double)mb);
+    // one wave of the row finds the bound, another the row's logsumexp
+    if (sub == 0) {
+        const uint64_t kth = beam_kth(part + w * 64, K);
+        if (lane == 0) bound[w] = kth;
     }
-    const double lse = (double)mb + log(l);
+    if (sub == wpr - 1) {
+        const float mi = lane < wpr ? wmax[w * wpr + lane] : -INFINITY, mb = wave_max(mi);
+        double l = lane < wpr ? wsum[w * wpr + lane] : 0.0;
+        l = mi == mb ? l : l * exp((double)mi - (double)mb);
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) l += __shfl_xor(l, d, 64);
+        if (lane == 0) lse_of[w] = (double)mb + log(l);
+    }
+    __syncthreads();
+    uint64_t* mine = found + (size_t)w * cap;
+    st.passing(bound[w], (uint32_t)v, (uint32_t)stride,
+               [&](uint64_t key) __attribute__((always_inline)) { mine[atomicAdd(&nfound[w], 1)] = key; });
+    const double lse = lse_of[w];
     __syncthreads();
     const int n = nfound[w];
     const int tp = beam_counters(n, nt);

@@ -120,15 +120,23 @@ paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* _
     // (r + 1024 k) as (row, column), without a division per entry
     const int step_r = 1024 / MP, step_c = 1024 - step_r * MP;
     if constexpr (FORK) {
+        constexpr int kU = 8;                        // loads in flight
         int er = r / MP, ec = r - er * MP;
-        for (int i = r; i < R * MP; i += 1024) {
-            old[i] = table[(int64_t)er * ld + ec];
-            er += step_r;
-            ec += step_c;
-            if (ec >= MP) {
-                ec -= MP;
-                ++er;
+        for (int i0 = r; i0 < R * MP; i0 += 1024 * kU) {
+            int32_t v[kU];
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                v[u] = i0 + 1024 * u < R * MP ? table[(int64_t)er * ld + ec] : -1;
+                er += step_r;
+                ec += step_c;
+                if (ec >= MP) {
+                    ec -= MP;
+                    ++er;
+                }
             }
+#pragma unroll
+            for (int u = 0; u < kU; ++u)
+                if (i0 + 1024 * u < R * MP) old[i0 + 1024 * u] = v[u];
         }
     }
     int len = -1, p = -1;
