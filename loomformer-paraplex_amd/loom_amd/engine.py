@@ -31,11 +31,62 @@ from typing import Dict, Optional
 
 import torch
 
-from . import _lib
+from . import _lib, ops
 from .config import ModelConfig
+from .paged import PagedKVCache
 from .weights import rope_tables
 
 _P = _lib.addr
+
+
+class _BeamState:
+    """What a beam search keeps on the device beside the engine's own state: the paged
+    cache, the scores and ends of the beams, the chosen parents, workspaces, and the
+    captured step of each pair of eos and pad ids."""
+
+    def __init__(self, eng: "LoomDecoder", beams: int, page_size: int, n_pages: Optional[int]):
+        c, dev = eng.cfg, eng.dev
+        self.beams, self.n_pages = beams, n_pages
+        self.cache = PagedKVCache(c.L, eng.B, eng.max_len, c.KVH, c.HD, eng.dtype, dev, page_size, n_pages)
+        self.ws = self.cache.workspace(c.QH)
+        self.scores = torch.empty(eng.B // beams, beams, dtype=torch.float32, device=dev)
+        self.finished = torch.empty(eng.B, dtype=torch.bool, device=dev)
+        self.parent = torch.empty(eng.B, dtype=torch.int32, device=dev)
+        n = eng.lib.loom_beam_select_workspace_bytes(eng.B // beams, beams, c.V, beams)
+        self.select_ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        self.first = torch.arange(eng.B, device=dev) % beams == 0      # the rows that take the prompt's pages
+        self.eos_id, self.pad_id = -1, 0
+        self._graphs: Dict[object, torch.cuda.CUDAGraph] = {}
+
+    def fits(self, beams: int, page_size: int, n_pages: Optional[int]) -> bool:
+        return (self.beams, self.cache.page_size, self.n_pages) == (beams, page_size, n_pages)
+
+    def begin(self, eng: "LoomDecoder", P: int, eos_id: int, pad_id: int) -> None:
+        """The first beam of every prompt holds the P tokens of the dense cache and is
+        the only one alive.  lens counts the last of them as written since (the
+        steps advance by one before they fork)."""
+        self.eos_id, self.pad_id = eos_id, pad_id
+        kc = self.cache
+        kc.reset()
+        kc.start(self.first)
+        kc.update(n_new=P)
+        last = torch.where(self.first, P, 0).to(torch.int32)
+        kc.load(eng.k_cache, eng.v_cache, torch.zeros_like(last), last)
+        kc.lens.copy_(torch.where(self.first, P - 1, -1))
+        self.scores.fill_(-math.inf)
+        self.scores[:, 0] = 0.0
+        self.finished.zero_()
+
+    def graph(self, eng: "LoomDecoder") -> torch.cuda.CUDAGraph:
+        key = (self.eos_id, self.pad_id)
+        g = self._graphs.get(key)
+        if g is None:
+            torch.cuda.synchronize(eng.dev)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                eng._launch_beam_step(self)
+            self._graphs[key] = g
+        return g
 
 
 class LoomDecoder:
@@ -213,6 +264,9 @@ class LoomDecoder:
         # (≈1 GB at B = 32, 128-token chunks, H = 3072); free_prefill_buffers()
         # drops them
         self._prefill_buffers: Dict[str, torch.Tensor] = {}
+        # the beam search's paged cache, choices and captured steps, kept from one
+        # search to the next; free_beam_buffers() drops them
+        self._beams: Optional[_BeamState] = None
 
     # ------------------------------------------------------------------ helpers
 
@@ -306,6 +360,11 @@ class LoomDecoder:
         (the next prefill allocates them again)."""
         self._prefill_buffers.clear()
 
+    def free_beam_buffers(self) -> None:
+        """Release the paged cache and the captured steps that the beam search keeps
+        (the next search builds them again)."""
+        self._beams = None
+
     def reset(self) -> None:
         """Forget all sequence state (Model.step at pos 0 starts afresh)."""
         self.pos = 0
@@ -317,12 +376,14 @@ class LoomDecoder:
 
     # ------------------------------------------------------------------ the step
 
-    def _launch_step(self, first: bool, prompt_len: int, argmax: bool = False) -> None:
+    def _launch_step(self, first: bool, prompt_len: int, argmax: bool = False,
+                     paged: Optional["_BeamState"] = None) -> None:
         """Enqueue one Model.step for position *pos_dev (device-resident).  `first`
         selects the position-0 variant (no seed, no previous temporal state);
         `argmax`: the step's token is the greedy pick of the current logits
         (infer's argmax, loomformer.py:5306) once the prompt is consumed, else the
-        id the caller wrote into self.ids."""
+        id the caller wrote into self.ids; `paged`: the attention's cache is the
+        beam search's paged one instead of the dense caches."""
         c, B, N, H, L = self.cfg, self.B, self.cfg.N, self.cfg.H, self.cfg.L
         st = self._stream()
         carry_id = -1 if self.carry_token_id is None else int(self.carry_token_id)
@@ -363,7 +424,13 @@ class LoomDecoder:
             # ---- attention step (loomformer.py:3300-3332): RoPE + cache append +
             # attention + chunk merge, one launch
             # with the depth read 2*bi of this token (loomformer.py:3999) in the same launch
-            if self.depth_pair:
+            if paged is not None:
+                self._paged_attention(paged, bi, st)
+                if self.depth_pair:
+                    self._depth_read_pair(sub, _P(self.hist), _P(self.d), _P(self.part_d), _P(self.part_lse), B, st)
+                else:
+                    self.depth_read(sub, self.hist, self.d, B)
+            elif self.depth_pair:
                 # with the FFN sublayer's read (query sub + 1) over the same slots
                 self._call("loom_gqa_decode_step_depth2", self.code, _P(self.qkv), _P(kc), _P(vc),
                            cache_sb, cache_st, cache_sh, _P(self.cos), _P(self.sin), _P(self.q),
@@ -471,6 +538,16 @@ class LoomDecoder:
                    _P(self.ca_len), N, float(N ** -0.5), st)
         self.head_logits(self.h2, self.logits, B)
 
+    def _paged_attention(self, bs: "_BeamState", bi: int, st) -> None:
+        """The attention step of block bi over the paged cache: each row at its own
+        length (the q, c and kctx buffers as the dense step leaves them)."""
+        c, kc = self.cfg, bs.cache
+        k, v = kc.k_pages[bi], kc.v_pages[bi]
+        self._call("loom_paged_decode_step", self.code, _P(self.qkv), self.qkv.stride(0), _P(k), _P(v), k.stride(0),
+                   k.stride(2), k.stride(1), kc.n_pages, kc.page_size, _P(kc.table), kc.table.stride(0),
+                   kc.table.shape[1], _P(kc.lens), _P(self.cos), _P(self.sin), self.max_len, _P(self.q), _P(self.c),
+                   _P(self.kctx), c.N, _P(bs.ws), bs.ws.numel() * 4, self.B, c.QH, c.KVH, c.HD, st)
+
     def _argmax(self) -> None:
         """ids = argmax(logits) per row (infer's greedy pick, loomformer.py:5306)."""
         self._call("loom_argmax_rows", self.code, _P(self.logits), self.B, self.cfg.V, _P(self.ids),
@@ -562,6 +639,85 @@ class LoomDecoder:
         if return_logits:
             return out, torch.stack(logits_all, 1)
         return out
+
+    # ------------------------------------------------------------------ beam search
+
+    def _beam_choose(self, bs: "_BeamState", states) -> None:
+        """One choice over beams and vocabulary from self.logits: scores, ends and
+        token ids in place, and `states` ((tensor, row dimension) pairs) following
+        the chosen parents."""
+        st = self._stream()
+        self._call("loom_beam_select", self.code, _P(self.logits), self.cfg.V, _P(bs.scores), _P(bs.finished),
+                   _P(bs.scores), _P(bs.parent), _P(self.ids), _P(bs.finished), self.B // bs.beams, bs.beams,
+                   self.cfg.V, bs.beams, bs.eos_id, bs.pad_id, _P(bs.select_ws), bs.select_ws.numel(), st)
+        ops.reorder_rows([t for t, _ in states], bs.parent, [d for _, d in states])
+
+    def _launch_beam_step(self, bs: "_BeamState") -> None:
+        """A token of every beam: the choice, the states and the cache of the chosen
+        parents, one Model.step of the chosen tokens."""
+        self._beam_choose(bs, [(self.trace, 1), (self.doc, 0), (self.pending, 0), (self.ca_k, 0), (self.ca_v, 0),
+                               (self.ca_valid, 0), (self.tokens, 0)])
+        bs.cache.update(parent=bs.parent, n_new=1, advance=1)
+        self._launch_step(first=False, prompt_len=0, paged=bs)
+
+    @torch.no_grad()
+    def beam_search(self, prompt: torch.Tensor, n_new: int, beams: int, eos_id: Optional[int] = None, pad_id: int = 0,
+                    chunked_prefill: bool = False, use_graph: bool = True, page_size: int = 64,
+                    n_pages: Optional[int] = None):
+        """The `beams` best continuations of `n_new` tokens of each prompt [S, P] by
+        beam search over the sum of log-probabilities (infer's loop,
+        loomformer.py:5290-5311, with a choice over beams in place of the argmax):
+        returns (ids [S, beams, n_new], scores [S, beams] float32), best first.  The
+        engine's batch is S * beams.  A beam that chose eos_id has ended: it keeps
+        its score and is filled up with pad_id.
+
+        The prompt runs through the dense cache as in ``generate``; its keys and
+        values then go into pages (page_size tokens each) once per prompt, and the
+        beams share them: a step forks the rows by their parents and copies only a
+        partly filled last page.  n_pages: pages of the pool (default: enough for
+        beams that share nothing); running out raises.  One step is captured into
+        a graph and replayed.  Afterwards the engine holds no sequence to continue
+        (its dense cache ends with the prompt)."""
+        S, P = prompt.shape
+        if beams < 1 or beams > 32 or S * beams != self.B:
+            raise ValueError(f"{S} prompts of {beams} beams (1 to 32) need an engine batch of {S * beams}, not {self.B}")
+        if P < 1 or n_new < 1:
+            raise ValueError("the prompt and the continuation must hold at least one token")
+        eos = -1 if eos_id is None else int(eos_id)
+        if eos >= self.cfg.V or not 0 <= pad_id < self.cfg.V:
+            raise ValueError(f"eos_id and pad_id must lie in [0, {self.cfg.V})")
+        if beams > self.cfg.V:
+            raise ValueError(f"{beams} beams over a vocabulary of {self.cfg.V}")
+        total = P + n_new
+        self._check_capacity(total - 1)
+        bs = self._beams
+        if bs is None or not bs.fits(beams, page_size, n_pages):
+            self._beams = None                       # frees the old pool first
+            bs = self._beams = _BeamState(self, beams, page_size, n_pages)
+        rows = prompt.repeat_interleave(beams, 0)
+        if chunked_prefill:
+            self.prefill(rows)
+        else:
+            self.start(rows)
+            if P > 1:
+                self.replay_steps(P - 1) if use_graph else self._eager_steps(P, P - 1)
+        bs.begin(self, P, eos, int(pad_id))
+        graph = bs.graph(self) if use_graph and n_new > 1 else None
+        for _ in range(n_new - 1):
+            if graph is not None:
+                graph.replay()
+            else:
+                self._launch_beam_step(bs)
+        self._beam_choose(bs, [(self.tokens, 0)])
+        self.tokens[:, total - 1] = self.ids
+        self.pos = self.max_len                      # nothing to continue from
+        bs.cache.check()
+        return self.tokens[:, P:total].reshape(S, beams, n_new).clone(), bs.scores.clone()
+
+    def _eager_steps(self, prompt_len: int, n: int) -> None:
+        for _ in range(n):
+            self._launch_step(first=False, prompt_len=prompt_len, argmax=True)
+        self.pos += n
 
     @torch.no_grad()
     def start(self, prompt: torch.Tensor) -> None:
