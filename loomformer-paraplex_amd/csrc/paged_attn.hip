@@ -58,17 +58,6 @@ __device__ __forceinline__ int row_tokens(const int32_t* lens, int b, int step, 
     return n < 0 || *bad ? 0 : n + step;
 }
 
-// inclusive scan over the wave
-__device__ __forceinline__ int wave_scan_int(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);      // row_shr 1, 2, 4, 8
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);      // lane 15 to row 1, 47 to row 3
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);      // lane 31 to rows 2, 3
-    return v;
-}
-
 // Lanes 16 and 32 apart: the two values of each pair in every lane of it
 __device__ __forceinline__ float2 pair16(float a, float b) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);

@@ -12,7 +12,7 @@ namespace loom {
 
 constexpr int kPcMaxRows = 1024;
 constexpr int kForkCols = 8;        // table columns of a fork block
-constexpr int kForkOne = 32768;     // table entries that the reserving block forks itself
+constexpr int kForkOne = 8192;      // table entries that the reserving block forks itself
 
 struct PageCopy {                   // one copy on write: the first `tokens` tokens of a page
     int32_t src, dst, tokens, pad;
@@ -73,28 +73,26 @@ paged_fork_kernel(int32_t* __restrict__ table, int64_t ld, int MP, const int32_t
 
 // ------------------------------------------------------------------ reserve
 
-// Exclusive scan over the 1024 threads of a block; *total: the sum.
-template <typename V>
-__device__ __forceinline__ V block_scan(V v, V* waves, V* total) {
+// Exclusive scan of N counts over the 1024 threads of a block; total: their sums.
+template <int N>
+__device__ __forceinline__ void block_scan(const int (&v)[N], int (*waves)[N], int (&before)[N], int (&total)[N]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    V incl = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const V o = __shfl_up(incl, d, 64);
-        if (lane >= d) incl += o;
-    }
+    int incl[N];
     __syncthreads();                                 // the previous use of `waves` is over
-    if (lane == 63) waves[wave] = incl;
-    __syncthreads();
-    V before = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < 16; ++w) {
-        const V x = waves[w];
-        if (w < wave) before += x;
-        all += x;
+    for (int k = 0; k < N; ++k) {
+        incl[k] = wave_scan_int(v[k]);
+        if (lane == 63) waves[wave][k] = incl[k];
     }
-    *total = all;
-    return before + incl - v;
+    __syncthreads();
+    // lane w of every wave holds wave w's sums
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int mine = lane < 16 ? waves[lane][k] : 0;
+        const int upto = wave_scan_int(mine);
+        total[k] = __builtin_amdgcn_readlane(upto, 15);
+        before[k] = __builtin_amdgcn_readlane(upto - mine, __builtin_amdgcn_readfirstlane(wave)) + incl[k] - v[k];
+    }
 }
 
 constexpr int kScanIds = 4;         // groups of four page ids per thread and round
@@ -105,8 +103,9 @@ constexpr int kScanIds = 4;         // groups of four page ids per thread and ro
 // row in turn copies while others hold it), and pages that are missing are
 // appended.  The free pages are taken lowest id first, in row order, by one
 // scan over refs: a free page's rank among the free ones names its row.
-// FORK: the block also forks the table, staged whole in LDS (a launch less:
-// 4 rows of 23 pages 12.2 -> .. us, 256 of 67 34.7 -> .. us for all of the call).
+// FORK: the block also forks the table, staged whole in LDS: a launch less, but
+// one CU's work.  All of a call in both forms (us, one launch / two): 92 entries
+// 7.9 / 9.9, 4352 16.0 / 17.1, 17152 21.3 / 17.8, 32512 19.6 / 13.0.
 template <bool FORK>
 __global__ void __launch_bounds__(1024)
 paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* __restrict__ lens,
@@ -115,10 +114,12 @@ paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* _
     extern __shared__ int32_t old[];                 // FORK: [R][MP]
     __shared__ __align__(16) int32_t tail[kPcMaxRows];
     __shared__ int32_t base[kPcMaxRows], slot0[kPcMaxRows], len_of[kPcMaxRows];
-    __shared__ int64_t waves[16];
+    __shared__ int waves[16][2];
     const int r = threadIdx.x, PS = 1 << log_ps;
     // (r + 1024 k) as (row, column), without a division per entry
     const int step_r = 1024 / MP, step_c = 1024 - step_r * MP;
+    int len = -1, p = -1;
+    if (r < R) p = parent != nullptr ? parent[r] : r;
     if constexpr (FORK) {
         constexpr int kU = 8;                        // loads in flight
         int er = r / MP, ec = r - er * MP;
@@ -139,12 +140,8 @@ paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* _
                 if (i0 + 1024 * u < R * MP) old[i0 + 1024 * u] = v[u];
         }
     }
-    int len = -1, p = -1;
-    if (r < R) {
-        p = parent != nullptr ? parent[r] : r;
-        if (in_range(p, R)) len = lens[p];
-        len = len >= 0 ? len + advance : -1;
-    }
+    if (in_range(p, R)) len = lens[p];
+    len = len >= 0 ? len + advance : -1;
     // base: the row's parent, slot0: the pages it takes from it (both until the scan)
     base[r] = p;
     slot0[r] = held_pages(len, 0, log_ps);
@@ -203,17 +200,18 @@ paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* _
         }
     }
     const int want = nmiss + (copy ? 1 : 0);
-    int64_t total64;
-    const int first = (int)block_scan<int64_t>(want, waves, &total64);
+    int want1[1] = {want}, first1[1], total1[1];
+    block_scan<1>(want1, reinterpret_cast<int(*)[1]>(waves), first1, total1);
+    const int first = first1[0];
     base[r] = first;
     slot0[r] = copy ? ~miss0 : miss0;                // (the sign says whether the first page is a copy's)
     if (r < R) copies[r] = PageCopy{-1, -1, 0, 0};
-    const int64_t need = total64;
-    int64_t given = 0;                               // free pages handed out so far
+    const int need = total1[0];
+    int given = 0;                                   // free pages handed out so far
     __syncthreads();
     for (int64_t seg = 0; seg < NP && given < need; seg += 1024 * 4 * kScanIds) {
         uint32_t mask = 0;                           // bit 4 j + e: page seg + 4096 j + 4 r + e is free
-        int64_t count = 0;                           // 16 bits per j
+        int count[2] = {0, 0}, before[2], all[2];    // 16 bits per j
 #pragma unroll
         for (int j = 0; j < kScanIds; ++j) {
             const int64_t id = seg + 4096 * j + 4 * r;
@@ -225,14 +223,13 @@ paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* _
                 for (int e = 0; e < 4 && id + e < NP; ++e)
                     if (refs[id + e] <= 0) mask |= 1u << (4 * j + e);
             }
-            count |= (int64_t)__popc((mask >> (4 * j)) & 15u) << (16 * j);
         }
-        int64_t all;
-        const int64_t before = block_scan<int64_t>(count, waves, &all);
-        int64_t at = given;
+#pragma unroll
+        for (int j = 0; j < kScanIds; ++j) count[j / 2] |= __popc((mask >> (4 * j)) & 15u) << (16 * (j & 1));
+        block_scan<2>(count, waves, before, all);
 #pragma unroll
         for (int j = 0; j < kScanIds; ++j) {
-            int64_t rank = at + ((before >> (16 * j)) & 0xffff);
+            int rank = given + ((before[j / 2] >> (16 * (j & 1))) & 0xffff);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if (!((mask >> (4 * j + e)) & 1u)) continue;
@@ -244,7 +241,7 @@ paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* _
                         if (base[mid] <= rank) lo = mid; else hi = mid - 1;
                     }
                     const bool cp = slot0[lo] < 0;
-                    const int k = (int)rank - base[lo], m0 = cp ? ~slot0[lo] : slot0[lo];
+                    const int k = rank - base[lo], m0 = cp ? ~slot0[lo] : slot0[lo];
                     refs[id] = 1;
                     if (cp && k == 0) {
                         const int l = len_of[lo], sl = l >> log_ps;
@@ -257,9 +254,8 @@ paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* _
                 }
                 ++rank;
             }
-            at += (all >> (16 * j)) & 0xffff;
+            given += (all[j / 2] >> (16 * (j & 1))) & 0xffff;
         }
-        given = at;
     }
     // a row whose copy found no page must not write into the shared one
     if (copy && first >= given) {
@@ -267,22 +263,37 @@ paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* _
         atomicSub(refs + page, 1);
     }
     if (short_of) atomicAdd(status, 1);
-    if (r == 0 && given < need) atomicAdd(status, (int)(need - given));
+    if (r == 0 && given < need) atomicAdd(status, need - given);
 }
 
-// Copies of `copies[r]`, both pools of all layers: grid (rows, 2 * layers).
+// Copies of `copies[r]`, both pools of all layers: block (r, y) takes every
+// gridDim.y-th of the row's 2 * layers pages, as one run of pieces, kCowUnroll in
+// flight per thread.
+constexpr int kCowUnroll = 4;
+
 __global__ void __launch_bounds__(256)
 paged_cow_kernel(PoolArgs a, const PageCopy* __restrict__ copies) {
     const PageCopy c = copies[blockIdx.x];
     if (c.src < 0) return;
-    char* pool = (blockIdx.y & 1 ? a.v : a.k) + (int64_t)(blockIdx.y >> 1) * a.layer;
-    const char* src = pool + c.src * a.page;
-    char* dst = pool + c.dst * a.page;
-    const int pieces = a.row_bytes / 16, per_head = c.tokens * pieces;
-    for (int i = threadIdx.x; i < a.KVH * per_head; i += 256) {
-        const int h = i / per_head, k = i - h * per_head, t = k / pieces;
-        const int64_t off = h * a.head + t * a.tok + (int64_t)(k - t * pieces) * 16;
-        *reinterpret_cast<u32x4*>(dst + off) = *reinterpret_cast<const u32x4*>(src + off);
+    const uint32_t pieces = a.row_bytes / 16, per_head = c.tokens * pieces, per_page = a.KVH * per_head;
+    const uint32_t pages = (2 * a.layers - blockIdx.y + gridDim.y - 1) / gridDim.y;
+    for (uint32_t i0 = threadIdx.x; i0 < pages * per_page; i0 += 256 * kCowUnroll) {
+        u32x4 v[kCowUnroll];
+        char* to[kCowUnroll];
+#pragma unroll
+        for (int u = 0; u < kCowUnroll; ++u) {
+            const uint32_t i = i0 + 256 * u;
+            if (i >= pages * per_page) continue;
+            const uint32_t n = i / per_page, k = i - n * per_page, h = k / per_head, m = k - h * per_head, t = m / pieces;
+            const uint32_t lp = blockIdx.y + n * gridDim.y;
+            char* pool = (lp & 1 ? a.v : a.k) + (int64_t)(lp >> 1) * a.layer + h * a.head + t * a.tok +
+                         (int64_t)(m - t * pieces) * 16;
+            to[u] = pool + c.dst * a.page;
+            v[u] = *reinterpret_cast<const u32x4*>(pool + c.src * a.page);
+        }
+#pragma unroll
+        for (int u = 0; u < kCowUnroll; ++u)
+            if (i0 + 256 * u < pages * per_page) *reinterpret_cast<u32x4*>(to[u]) = v[u];
     }
 }
 
@@ -323,17 +334,16 @@ paged_write_kernel(PoolArgs a, const char* __restrict__ kd, const char* __restri
 // number of moves, then movers [NP], holes [NP], map [NP].
 __global__ void __launch_bounds__(1024)
 paged_compact_plan_kernel(int32_t* refs, int NP, int32_t* __restrict__ used, int32_t* ws) {
-    __shared__ int64_t waves[16];
+    __shared__ int waves[16][2];
     int32_t *movers = ws + 4, *holes = movers + NP, *map = holes + NP;
     const int r = threadIdx.x;
-    int mine = 0;
-    for (int64_t i = r; i < NP; i += 1024) mine += refs[i] > 0;
-    int64_t total;
-    block_scan<int64_t>(mine, waves, &total);
-    const int U = (int)total;
+    int mine[1] = {0}, ignore[1], total[1];
+    for (int64_t i = r; i < NP; i += 1024) mine[0] += refs[i] > 0;
+    block_scan<1>(mine, reinterpret_cast<int(*)[1]>(waves), ignore, total);
+    const int U = total[0];
     int nm = 0, nh = 0;
     for (int64_t seg = 0; seg < NP; seg += 4096) {
-        int64_t count = 0;                           // movers low, holes high
+        int count[2] = {0, 0}, before[2], all[2];    // movers, holes
         uint32_t bits = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -341,20 +351,19 @@ paged_compact_plan_kernel(int32_t* refs, int NP, int32_t* __restrict__ used, int
             if (id >= NP) continue;
             const bool inuse = refs[id] > 0;
             map[id] = (int)id;
-            if (inuse && id >= U) { count += 1; bits |= 1u << e; }
-            if (!inuse && id < U) { count += (int64_t)1 << 32; bits |= 16u << e; }
+            if (inuse && id >= U) { ++count[0]; bits |= 1u << e; }
+            if (!inuse && id < U) { ++count[1]; bits |= 16u << e; }
         }
-        int64_t all;
-        const int64_t before = block_scan<int64_t>(count, waves, &all);
-        int m = nm + (int)(before & 0xffffffff), h = nh + (int)(before >> 32);
+        block_scan<2>(count, waves, before, all);
+        int m = nm + before[0], h = nh + before[1];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int id = (int)(seg + 4 * r + e);
             if (bits >> e & 1u) movers[m++] = id;
             if (bits >> (4 + e) & 1u) holes[h++] = id;
         }
-        nm += (int)(all & 0xffffffff);
-        nh += (int)(all >> 32);
+        nm += all[0];
+        nh += all[1];
     }
     __syncthreads();                                 // the lists and the map are written
     for (int i = r; i < nm; i += 1024) {             // (as many holes as movers)
@@ -368,6 +377,8 @@ paged_compact_plan_kernel(int32_t* refs, int NP, int32_t* __restrict__ used, int
         *used = U;
     }
 }
+
+constexpr int kMoveUnroll = 6;      // 16-byte pieces in flight per thread
 
 // The moves (a page of one layer's K or V pool each) and, in the blocks of
 // y = 1, the tables' new ids.
@@ -383,17 +394,30 @@ paged_compact_move_kernel(PoolArgs a, int PS, const int32_t* __restrict__ ws, in
         }
         return;
     }
+    // a page as runs of bytes that lie together: the whole page where heads and
+    // tokens follow each other, else a head's tokens, else a token
     const int64_t units = (int64_t)ws[0] * 2 * a.layers;
-    const int pieces = a.row_bytes / 16, per_head = PS * pieces;
+    const bool head_run = a.tok == a.row_bytes, page_run = head_run && a.head == (int64_t)PS * a.row_bytes;
+    const int runs = page_run ? 1 : head_run ? a.KVH : a.KVH * PS;
+    const int run = page_run ? a.KVH * PS * a.row_bytes : head_run ? PS * a.row_bytes : a.row_bytes;
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-        const int i = (int)(u / (2 * a.layers)), lp = (int)(u % (2 * a.layers));
+        const int i = (int)(u / (2 * a.layers)), lp = (int)(u - (int64_t)i * 2 * a.layers);
         char* pool = (lp & 1 ? a.v : a.k) + (int64_t)(lp >> 1) * a.layer;
         const char* src = pool + movers[i] * a.page;
         char* dst = pool + holes[i] * a.page;
-        for (int k0 = threadIdx.x; k0 < a.KVH * per_head; k0 += 256) {
-            const int h = k0 / per_head, k = k0 - h * per_head, t = k / pieces;
-            const int64_t off = h * a.head + t * a.tok + (int64_t)(k - t * pieces) * 16;
-            *reinterpret_cast<u32x4*>(dst + off) = *reinterpret_cast<const u32x4*>(src + off);
+        for (int n = 0; n < runs; ++n) {
+            const int64_t off = page_run ? 0 : head_run ? n * a.head : (n / PS) * a.head + (n % PS) * a.tok;
+            for (int b0 = threadIdx.x * 16; b0 < run; b0 += 256 * 16 * kMoveUnroll) {
+                u32x4 v[kMoveUnroll];
+#pragma unroll
+                for (int k = 0; k < kMoveUnroll; ++k)
+                    if (b0 + 4096 * k < run)
+                        v[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + off + b0 + 4096 * k));
+#pragma unroll
+                for (int k = 0; k < kMoveUnroll; ++k)
+                    if (b0 + 4096 * k < run)
+                        __builtin_nontemporal_store(v[k], reinterpret_cast<u32x4*>(dst + off + b0 + 4096 * k));
+            }
         }
     }
 }
@@ -477,7 +501,9 @@ extern "C" int loom_paged_update(int dtype, void* k_pages, void* v_pages, int64_
                            (PageCopy*)workspace, status);
     if (int rc = launch_status("loom_paged_update(reserve)")) return rc;
     if (n_new == 0) return LOOM_OK;
-    hipLaunchKernelGGL(paged_cow_kernel, dim3((unsigned)rows, (unsigned)(2 * layers)), dim3(256), 0, st, a,
+    // (about 2048 blocks, and no more than a block per page)
+    const int64_t y = ceil_div((int64_t)2048, rows);
+    hipLaunchKernelGGL(paged_cow_kernel, dim3((unsigned)rows, (unsigned)(y < 2 * layers ? y : 2 * layers)), dim3(256), 0, st, a,
                        (const PageCopy*)workspace);
     return launch_status("loom_paged_update(copy)");
 }
