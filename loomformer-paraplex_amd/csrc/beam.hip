@@ -52,13 +52,51 @@ __device__ __forceinline__ float beam_key_x(uint64_t k) {
     return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
 }
 
-__device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int d) {
-    const uint32_t lo = __shfl_xor((uint32_t)v, d, 64), hi = __shfl_xor((uint32_t)(v >> 32), d, 64);
-    return ((uint64_t)hi << 32) | lo;
+// Lane permutations of 64-bit values inside rows of 16 lanes (see dpp): each step
+// pairs the halves of twice the group, so reductions over 2, 4, 8, 16 lanes are
+// the first 1, 2, 3, 4 of them.
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp_u64(uint64_t v) {
+    const int lo = (int)v, hi = (int)(v >> 32);
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_update_dpp(hi, hi, CTRL, 0xF, 0xF, false) << 32) |
+           (uint32_t)__builtin_amdgcn_update_dpp(lo, lo, CTRL, 0xF, 0xF, false);
+}
+template <int CTRL>
+__device__ __forceinline__ int dpp_i32(int v) {
+    return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xF, 0xF, false);
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+    return __builtin_bit_cast(double, dpp_u64<CTRL>(__builtin_bit_cast(uint64_t, v)));
 }
 __device__ __forceinline__ uint64_t readlane_u64(uint64_t v, int l) {
     return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32) |
            (uint32_t)__builtin_amdgcn_readlane((int)v, l);
+}
+__device__ __forceinline__ double readlane_f64(double v, int l) {
+    return __builtin_bit_cast(double, readlane_u64(__builtin_bit_cast(uint64_t, v), l));
+}
+// the largest of each aligned group of g = 1, 2, 4, 8 or 16 lanes
+__device__ __forceinline__ uint64_t group_max_u64(uint64_t v, int g) {
+    if (g >= 2) v = max(v, dpp_u64<kDppQuad1032>(v));
+    if (g >= 4) v = max(v, dpp_u64<kDppQuad2301>(v));
+    if (g >= 8) v = max(v, dpp_u64<kDppHalfMirror>(v));
+    if (g >= 16) v = max(v, dpp_u64<kDppMirror>(v));
+    return v;
+}
+__device__ __forceinline__ int group_sum_int(int v, int g) {
+    if (g >= 2) v += __builtin_amdgcn_update_dpp(0, v, kDppQuad1032, 0xF, 0xF, false);
+    if (g >= 4) v += __builtin_amdgcn_update_dpp(0, v, kDppQuad2301, 0xF, 0xF, false);
+    if (g >= 8) v += __builtin_amdgcn_update_dpp(0, v, kDppHalfMirror, 0xF, 0xF, false);
+    if (g >= 16) v += __builtin_amdgcn_update_dpp(0, v, kDppMirror, 0xF, 0xF, false);
+    return v;
+}
+__device__ __forceinline__ double wave_sum_f64(double v) {
+    v += dpp_f64<kDppQuad1032>(v);
+    v += dpp_f64<kDppQuad2301>(v);
+    v += dpp_f64<kDppHalfMirror>(v);
+    v += dpp_f64<kDppMirror>(v);
+    return (readlane_f64(v, 0) + readlane_f64(v, 16)) + (readlane_f64(v, 32) + readlane_f64(v, 48));
 }
 
 // Eight logits as loaded, from place v on; places from v1 on hold -inf.  Rows start
@@ -68,12 +106,12 @@ template <typename T>
 struct BeamPiece {
     static constexpr int NW = (int)sizeof(T) * kBeamVec / 4;
     uint32_t w[NW];
-    __device__ __forceinline__ void load(const T* x, int64_t v, int64_t v1) {
+    __device__ __forceinline__ void load(const T* x, int v, int v1) {
         if (v + kBeamVec <= v1) {
 #pragma unroll
             for (int i = 0; i < NW / 4; ++i) {
                 u32x4 q;                             // one load, of any alignment
-                __builtin_memcpy(&q, reinterpret_cast<const char*>(x + v) + 16 * i, 16);
+                __builtin_memcpy(&q, reinterpret_cast<const char*>(x) + ((uint32_t)v * (uint32_t)sizeof(T) + 16 * i), 16);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) w[4 * i + k] = q[k];
             }
@@ -167,26 +205,33 @@ struct BeamStep {
 // Sum and maximum of a wave's lanes.
 __device__ __forceinline__ void beam_wave_sum(float& m, double& s) {
     const float mw = wave_max(m);
-    s = m == mw ? s : s * (double)__builtin_amdgcn_exp2f((m - mw) * kLog2e);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d, 64);
+    s = wave_sum_f64(m == mw ? s : s * (double)__builtin_amdgcn_exp2f((m - mw) * kLog2e));
     m = mw;
 }
 
-// The K-th largest of 64 keys in LDS (1: fewer than K are candidates), by counting.
-__device__ __forceinline__ uint64_t beam_kth(const uint64_t* keys, int K) {
-    const uint64_t mine = keys[threadIdx.x & 63];
-    int larger = 0;
-#pragma unroll 8
-    for (int i = 0; i < 64; ++i) larger += keys[i] > mine;
-    const unsigned long long at = __ballot(mine != 0 && larger == K - 1);
+// The K-th largest of 64 keys in LDS, by counting the larger ones: each of `nw`
+// waves (this one is number w) counts among its 64 / nw keys for all 64, into
+// larger[64] (zero before).  After a barrier beam_kth reads it: 1 if fewer than K
+// are candidates.
+__device__ __forceinline__ void beam_count(const uint64_t* keys, int* larger, int w, int nw) {
+    const int lane = threadIdx.x & 63, n = 64 / nw;
+    const uint64_t mine = keys[lane];
+    int c = 0;
+#pragma unroll 4
+    for (int i = w * n; i < (w + 1) * n; ++i) c += keys[i] > mine;
+    atomicAdd(larger + lane, c);
+}
+__device__ __forceinline__ uint64_t beam_kth(const uint64_t* keys, const int* larger, int K) {
+    const int lane = threadIdx.x & 63;
+    const uint64_t mine = keys[lane];
+    const unsigned long long at = __ballot(mine != 0 && larger[lane] == K - 1);
     return at ? readlane_u64(mine, __builtin_amdgcn_readfirstlane(__ffsll(at) - 1)) : 1;
 }
 
 // Threads that count for one of n entries among `threads` of them: a power of
-// two of at most 64.
+// two of at most 16.
 __device__ __forceinline__ int beam_counters(int n, int threads) {
-    int tp = 64;
+    int tp = 16;
     while (tp > 1 && n * tp > threads) tp >>= 1;
     return tp;
 }
@@ -198,19 +243,19 @@ __device__ __forceinline__ int beam_counters(int n, int threads) {
 // counting the larger ones.  Later steps pass what reaches the K-th best so far;
 // only where the list would overflow are it and the step ranked again.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4)))
 beam_row_kernel(const T* __restrict__ logits, BeamArgs a) {
     extern __shared__ uint64_t found[];               // cap = K * 128 + K
     __shared__ uint64_t quad[64], kept[kBeamMaxOut];
     __shared__ float wmax[4];
     __shared__ double wsum[4];
-    __shared__ int count[2][4], nfound;
+    __shared__ int count[2][4], larger64[64], nfound;
     const int row = blockIdx.y, slice = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int K = a.K, cap = K * 129;
     const int64_t rec = (int64_t)row * a.slices + slice;
     if (a.finished != nullptr && a.finished[row]) return;     // its logits are not read
     const T* x = logits + (int64_t)row * a.ld;
-    const int64_t v0 = (int64_t)slice * a.slice_len, v1 = min(v0 + a.slice_len, a.V);
+    const int v0 = slice * (int)a.slice_len, v1 = min(v0 + (int)a.slice_len, (int)a.V);   // (V <= 2^24)
     constexpr int kStride = 256 * kBeamVec;
     float m = -INFINITY;
     double s = 0.0;
@@ -218,9 +263,9 @@ beam_row_kernel(const T* __restrict__ logits, BeamArgs a) {
     int listed = 0;                                    // entries of the list, in every thread
     if (tid < K) kept[tid] = 0;
     if (tid == 0) nfound = 0;
-    auto load = [&](BeamStep<T>& st, int64_t base) __attribute__((always_inline)) {
+    auto load = [&](BeamStep<T>& st, int base) __attribute__((always_inline)) {
 #pragma unroll
-        for (int p = 0; p < kBeamPieces; ++p) st.e[p].load(x, base + (int64_t)p * kStride + tid * kBeamVec, v1);
+        for (int p = 0; p < kBeamPieces; ++p) st.e[p].load(x, base + p * kStride + tid * kBeamVec, v1);
     };
     auto push = [&](uint64_t key) __attribute__((always_inline)) { found[atomicAdd(&nfound, 1)] = key; };
     // the K best of the list to kept, and the list down to them
@@ -231,7 +276,7 @@ beam_row_kernel(const T* __restrict__ logits, BeamArgs a) {
             const uint64_t key = found[i];
             int larger = 0;
             for (int q = tid & (tp - 1); q < n; q += tp) larger += found[q] > key;
-            for (int d = 1; d < tp; d <<= 1) larger += __shfl_xor(larger, d, 64);
+            larger = group_sum_int(larger, tp);
             if (larger < K) kept[larger] = key;        // (the tp threads of an entry alike)
         }
         __syncthreads();
@@ -244,7 +289,7 @@ beam_row_kernel(const T* __restrict__ logits, BeamArgs a) {
     BeamStep<T> cur, next;
     load(cur, v0);
     int step = 0;
-    for (int64_t base = v0; base < v1; base += kBeamTile, ++step) {
+    for (int base = v0; base < v1; base += kBeamTile, ++step) {
         if (base + kBeamTile < v1) load(next, base + kBeamTile);
         cur.maxima();
         cur.sum(m, s);
@@ -262,15 +307,13 @@ beam_row_kernel(const T* __restrict__ logits, BeamArgs a) {
         uint64_t low = bound;
         if (full) {
             if (listed > 0) rank();
-            uint64_t best = cur.best(v, kStride);
-#pragma unroll
-            for (int d = 1; d < 4; d <<= 1) {
-                const uint64_t o = shfl_xor_u64(best, d);
-                best = o > best ? o : best;
-            }
+            const uint64_t best = group_max_u64(cur.best(v, kStride), 4);
             if ((tid & 3) == 0) quad[tid >> 2] = best;
+            if (tid < 64) larger64[tid] = 0;
             __syncthreads();
-            low = max(beam_kth(quad, K), bound);
+            beam_count(quad, larger64, wave, 4);
+            __syncthreads();
+            low = max(beam_kth(quad, larger64, K), bound);
         }
         if (all > 0) cur.passing(low, v, kStride, push);
         listed += all;
@@ -326,16 +369,18 @@ __device__ __forceinline__ BeamCand beam_cand(bool any, float x, double lse, flo
     return c;
 }
 
-// The best K of n entries of `list` (LDS) to the group's outputs, and the places
-// behind the last candidate; all threads of the block, after a barrier.
-__device__ __forceinline__ void beam_write(const BeamArgs& a, const BeamCand* list, int n, int g, const uint8_t* fin) {
+// The best K of n entries of `list` (LDS), `valid` of them candidates, to the
+// group's outputs, and the places behind the last candidate; all threads of the
+// block, after a barrier.
+__device__ __forceinline__ void beam_write(const BeamArgs& a, const BeamCand* list, int n, int valid, int g,
+                                           const uint8_t* fin) {
     const int K = a.K, NT = blockDim.x, tid = threadIdx.x, tp = beam_counters(n, NT);
     for (int i = tid / tp; i < n; i += NT / tp) {
         const BeamCand c = list[i];
         if (c.place == kBeamNone) continue;
         int before = 0;
         for (int q = tid & (tp - 1); q < n; q += tp) before += beam_before(list[q], c);
-        for (int d = 1; d < tp; d <<= 1) before += __shfl_xor(before, d, 64);
+        before = group_sum_int(before, tp);
         if (before >= K || (tid & (tp - 1)) != 0) continue;
         const int64_t o = (int64_t)g * K + before;
         const int w = (int)(c.place / (uint32_t)a.V);
@@ -345,14 +390,6 @@ __device__ __forceinline__ void beam_write(const BeamArgs& a, const BeamCand* li
         a.out_token[o] = tok;
         if (a.out_finished != nullptr) a.out_finished[o] = fin[w] || tok == a.eos;
     }
-    int some = 0;
-    for (int i = tid; i < n; i += NT) some += list[i].place != kBeamNone;
-    __shared__ int valid;
-    if (tid == 0) valid = 0;
-    __syncthreads();
-    some = wave_sum_int(some);
-    if ((tid & 63) == 0 && some > 0) atomicAdd(&valid, some);
-    __syncthreads();
     // fewer candidates than places: no parent but the group's first row
     for (int k = valid + tid; k < K; k += NT) {
         const int64_t o = (int64_t)g * K + k;
@@ -372,8 +409,8 @@ beam_group_kernel(BeamArgs a) {
     __shared__ double lse[kBeamMaxBeams];
     __shared__ float sc[kBeamMaxBeams];
     __shared__ uint8_t fin[kBeamMaxBeams];
-    __shared__ int nfound;
-    const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    __shared__ int nfound, larger64[64];
+    const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int W = a.W, K = a.K, S = a.slices, SK = S * K, n = W * SK;
     // the survivors' logits are on their way while the sums are joined
     float cx[2];
@@ -394,7 +431,8 @@ beam_group_kernel(BeamArgs a) {
         sc[tid] = a.scores[g * W + tid];
     }
     if (tid == 0) nfound = 0;
-    for (int w = tid >> 6; w < W; w += 16) {
+    if (tid < 64) larger64[tid] = 0;
+    for (int w = wave; w < W; w += 16) {
         const int64_t r = (int64_t)(g * W + w) * S;
         float mb = -INFINITY;
         for (int i = lane; i < S; i += 64) mb = fmaxf(mb, a.part_m[r + i]);
@@ -404,8 +442,7 @@ beam_group_kernel(BeamArgs a) {
             const float mi = a.part_m[r + i];
             l += mi == mb ? a.part_s[r + i] : a.part_s[r + i] * exp((double)mi - (double)mb);
         }
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
+        l = wave_sum_f64(l);
         if (lane == 0) lse[w] = (double)mb + log(l);   // -inf: no logit; NaN: a NaN or +inf among them
     }
     __syncthreads();
@@ -420,24 +457,31 @@ beam_group_kernel(BeamArgs a) {
     }
     BeamCand bound{-INFINITY, kBeamNone, 0};
     if (n > 256) {
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) {
-            const BeamCand o{__shfl_xor(best.value, d, 64), (uint32_t)__shfl_xor((int)best.place, d, 64), 0};
+        auto better = [&](double v, int p) __attribute__((always_inline)) {
+            const BeamCand o{v, (uint32_t)p, 0};
             if (beam_before(o, best)) best = o;
-        }
+        };
+        better(dpp_f64<kDppQuad1032>(best.value), dpp_i32<kDppQuad1032>((int)best.place));
+        better(dpp_f64<kDppQuad2301>(best.value), dpp_i32<kDppQuad2301>((int)best.place));
+        better(dpp_f64<kDppHalfMirror>(best.value), dpp_i32<kDppHalfMirror>((int)best.place));
+        better(dpp_f64<kDppMirror>(best.value), dpp_i32<kDppMirror>((int)best.place));
         if ((tid & 15) == 0) top[tid >> 4] = best;
         __syncthreads();
+        // each wave counts among four of the 64 for all of them
         const BeamCand mine = top[lane];
         int before = 0;
-        for (int i = 0; i < 64; ++i) before += beam_before(top[i], mine);
-        const unsigned long long at = __ballot(mine.place != kBeamNone && before == K - 1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) before += beam_before(top[4 * wave + i], mine);
+        atomicAdd(larger64 + lane, before);
+        __syncthreads();
+        const unsigned long long at = __ballot(mine.place != kBeamNone && larger64[lane] == K - 1);
         if (at) bound = top[__builtin_amdgcn_readfirstlane(__ffsll(at) - 1)];
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k)
         if (c[k].place != kBeamNone && !beam_before(bound, c[k])) list[atomicAdd(&nfound, 1)] = c[k];
     __syncthreads();
-    beam_write(a, list, nfound, g, fin);
+    beam_write(a, list, nfound, nfound, g, fin);
 }
 
 // ------------------------------------------------------------------ a whole group in one block
@@ -454,7 +498,7 @@ beam_whole_kernel(const T* __restrict__ logits, BeamArgs a, int wl, int cap) {
     __shared__ BeamCand list[kBeamWholeBeams * kBeamWholeOut];
     __shared__ float wmax[16];
     __shared__ double wsum[16];
-    __shared__ uint64_t bound[kBeamWholeBeams];
+    __shared__ int larger[kBeamWholeBeams * 64];
     __shared__ double lse_of[kBeamWholeBeams];
     __shared__ int nfound[kBeamWholeBeams];
     __shared__ uint8_t fin[kBeamWholeBeams];
@@ -465,13 +509,14 @@ beam_whole_kernel(const T* __restrict__ logits, BeamArgs a, int wl, int cap) {
     const bool dead = w >= W, fn = a.finished != nullptr && a.finished[row] != 0;
     const float score = a.scores[row];
     const T* x = logits + (int64_t)row * a.ld;
-    const int64_t v1 = dead || fn ? 0 : a.V;           // a finished row's logits are not read
+    const int v1 = dead || fn ? 0 : (int)a.V;          // a finished row's logits are not read
     const int stride = nt * kBeamVec, v = t * kBeamVec;
     BeamStep<T> st;
 #pragma unroll
-    for (int p = 0; p < kBeamPieces; ++p) st.e[p].load(x, v + (int64_t)p * stride, v1);
+    for (int p = 0; p < kBeamPieces; ++p) st.e[p].load(x, v + p * stride, v1);
     if (t == 0 && !dead) fin[w] = fn;
     if (tid < kBeamWholeBeams) nfound[tid] = 0;
+    larger[tid] = 0;                                  // (16 rows of 64: one for each thread)
     float m = -INFINITY;
     double s = 0.0;
     st.maxima();
@@ -481,30 +526,21 @@ beam_whole_kernel(const T* __restrict__ logits, BeamArgs a, int wl, int cap) {
         wmax[wave] = m;
         wsum[wave] = s;
     }
-    uint64_t best = st.best((uint32_t)v, (uint32_t)stride);
-    for (int d = 1; d < wpr; d <<= 1) {
-        const uint64_t o = shfl_xor_u64(best, d);
-        best = o > best ? o : best;
-    }
+    const uint64_t best = group_max_u64(st.best((uint32_t)v, (uint32_t)stride), wpr);
     if ((t & (wpr - 1)) == 0) part[w * 64 + t / wpr] = best;
     for (int i = t; i < K; i += nt) list[w * K + i] = BeamCand{-INFINITY, kBeamNone, 0};
     __syncthreads();
-    // one wave of the row finds the bound, another the row's logsumexp
-    if (sub == 0) {
-        const uint64_t kth = beam_kth(part + w * 64, K);
-        if (lane == 0) bound[w] = kth;
-    }
+    // the row's waves count for the bound; one of them joins the row's sum
+    beam_count(part + w * 64, larger + w * 64, sub, wpr);
     if (sub == wpr - 1) {
         const float mi = lane < wpr ? wmax[w * wpr + lane] : -INFINITY, mb = wave_max(mi);
         double l = lane < wpr ? wsum[w * wpr + lane] : 0.0;
-        l = mi == mb ? l : l * exp((double)mi - (double)mb);
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) l += __shfl_xor(l, d, 64);
+        l = wave_sum_f64(mi == mb ? l : l * exp((double)mi - (double)mb));
         if (lane == 0) lse_of[w] = (double)mb + log(l);
     }
     __syncthreads();
     uint64_t* mine = found + (size_t)w * cap;
-    st.passing(bound[w], (uint32_t)v, (uint32_t)stride,
+    st.passing(beam_kth(part + w * 64, larger + w * 64, K), (uint32_t)v, (uint32_t)stride,
                [&](uint64_t key) __attribute__((always_inline)) { mine[atomicAdd(&nfound[w], 1)] = key; });
     const double lse = lse_of[w];
     __syncthreads();
@@ -512,15 +548,16 @@ beam_whole_kernel(const T* __restrict__ logits, BeamArgs a, int wl, int cap) {
     const int tp = beam_counters(n, nt);
     for (int i = t / tp; i < n; i += nt / tp) {
         const uint64_t key = mine[i];
-        int larger = 0;
-        for (int q = t & (tp - 1); q < n; q += tp) larger += mine[q] > key;
-        for (int d = 1; d < tp; d <<= 1) larger += __shfl_xor(larger, d, 64);
-        if (larger < K && (t & (tp - 1)) == 0)
-            list[w * K + larger] = beam_cand(true, beam_key_x(key), lse, score, w, a.V, (uint32_t)~(uint32_t)key);
+        int above = 0;
+        for (int q = t & (tp - 1); q < n; q += tp) above += mine[q] > key;
+        above = group_sum_int(above, tp);
+        if (above < K && (t & (tp - 1)) == 0)
+            list[w * K + above] = beam_cand(true, beam_key_x(key), lse, score, w, a.V, (uint32_t)~(uint32_t)key);
     }
     if (fn && !dead && t == 0) list[w * K] = beam_cand(true, 0.0f, 0.0, score, w, a.V, a.pad);
     __syncthreads();
-    beam_write(a, list, W * K, g, fin);
+    const int valid = __syncthreads_count(tid < W * K && list[tid].place != kBeamNone);    // (at most 512)
+    beam_write(a, list, W * K, valid, g, fin);
 }
 
 // ------------------------------------------------------------------ reorder
