@@ -252,34 +252,33 @@ template <int NW, typename T>
 __device__ __forceinline__ void paged_finish(const PagedArgs<T>& a, const PlanItem& it, int h0, int nh,
                                              int NH, int HD, bool kctx, bool broken, const float* wm,
                                              const float* wl, const float* wacc) {
-    for (int k = threadIdx.x; k < nh * HD; k += blockDim.x) {
-        const int j = k / HD, d = k - j * HD, h = h0 + j;
+    // four sums per thread: of head j, C (which = 0) or Kctx, from d on
+    const int quads = HD / 4, per_head = kctx ? 2 * quads : quads;
+    for (int k = threadIdx.x; k < nh * per_head; k += blockDim.x) {
+        const int j = k / per_head, e = k - j * per_head, which = e >= quads, d = 4 * (e - which * quads), h = h0 + j;
         float m = -INFINITY;
 #pragma unroll
         for (int w = 0; w < NW; ++w) m = fmaxf(m, wm[j * NW + w]);
-        float l = 0.0f, c = 0.0f, kx = 0.0f;
+        float l = 0.0f;
+        pg_f32x4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
             const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(wm[j * NW + w] - m);
-            const float* acc = wacc + (size_t)((w * NH + j) * 2) * HD + d;
+            const pg_f32x4 x = *reinterpret_cast<const pg_f32x4*>(wacc + (size_t)((w * NH + j) * 2 + which) * HD + d);
             l = fmaf(wl[j * NW + w], f, l);
-            c = fmaf(acc[0], f, c);
-            if (kctx) kx = fmaf(acc[HD], f, kx);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[i] = fmaf(x[i], f, c[i]);
         }
         if (broken) l = NAN;
         if (it.nchunk == 1) {
             const float inv = 1.0f / l;
-            const int64_t o = (int64_t)it.row * a.out_ld + (int64_t)h * HD + d;
-            st(a.c_out + o, l == 0.0f ? 0.0f : c * inv);
-            if (kctx) st(a.k_out + o, l == 0.0f ? 0.0f : kx * inv);
+            T* out = (which ? a.k_out : a.c_out) + (int64_t)it.row * a.out_ld + (int64_t)h * HD + d;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st(out + i, l == 0.0f ? 0.0f : c[i] * inv);
         } else {
             const int64_t r = (int64_t)(it.item0 + it.chunk) * a.QH + h;
-            a.rec[r * 2 * HD + d] = c;
-            if (kctx) a.rec[r * 2 * HD + HD + d] = kx;
-            if (d == 0) {
-                a.rec[a.rec_ml + 2 * r] = m;
-                a.rec[a.rec_ml + 2 * r + 1] = l;
-            }
+            *reinterpret_cast<pg_f32x4*>(a.rec + (r * 2 + which) * HD + d) = c;
+            if (e == 0) *reinterpret_cast<float2*>(a.rec + a.rec_ml + 2 * r) = make_float2(m, l);
         }
     }
 }
@@ -554,7 +553,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 paged_vec_kernel(PagedArgs<T> a) {
     constexpr int HD = LPR * NV * 4, E = NV * 4, NW = 4;
     constexpr int RPW = 64 / LPR, RPB = NW * RPW;       // tokens of a wave / block step
-    __shared__ float wm[NW * GT], wl[NW * GT], wacc[NW * GT * 2 * HD];
+    __shared__ __align__(16) float wm[NW * GT], wl[NW * GT], wacc[NW * GT * 2 * HD];
     __shared__ __align__(16) float heads[(GT + 2) * HD];   // the new token's q, k, v
     const int htiles = (a.G + GT - 1) / GT;
     const int kvh = blockIdx.y / htiles, g0 = (blockIdx.y % htiles) * GT;
