@@ -845,7 +845,8 @@ int loom_paged_write(int dtype, void* k_pages, void* v_pages, int64_t layers, in
 
 /* Moves the pages in use to the lowest ids: with U of them in use, the k-th one
  * with id >= U goes to the k-th free id below U (pools of all layers, tables and
- * refs follow), and *used = U.  Pages U.. are free afterwards.  workspace:
+ * refs follow), and *used = U.  Pages U.. are free afterwards.  Pages that refs
+ * count but the table does not hold move as well.  workspace:
  * loom_paged_compact_workspace_bytes(n_pages), scratch. */
 int64_t loom_paged_compact_workspace_bytes(int64_t n_pages);
 int loom_paged_compact(int dtype, void* k_pages, void* v_pages, int64_t layers, int64_t layer_stride,
@@ -878,7 +879,8 @@ int loom_beam_select(int dtype, const void* logits, int64_t logits_ld, const flo
  * parent is outside [0, rows) stay as they are).  n <= 16 tensors; tensor i has
  * outer[i] slices, outer_stride[i] bytes apart, of `rows` rows of row_bytes[i]
  * bytes, row_stride[i] bytes apart.  The arrays are host arrays, read before the
- * call returns; rows of different tensors, slices or places must not overlap. */
+ * call returns; rows of different tensors, slices or places, and parent, must
+ * not overlap. */
 int loom_reorder_rows(int64_t n, void* const* tensors, const int64_t* outer, const int64_t* outer_stride,
                       const int64_t* row_stride, const int64_t* row_bytes, const int32_t* parent, int64_t rows,
                       void* stream);

@@ -205,6 +205,7 @@ PyObject* attention(const Args& a, bool step) {
     at::Tensor c = at::empty({B, QH, HD}, opt), kx, qo;
     if (kctx) kx = at::empty({B, QH, HD}, opt);
     if (step) qo = at::empty({B, QH, HD}, opt);
+    if (B == 0) return step ? list_of({&c, &kx, &qo}) : list_of({&c, &kx});
     const int64_t need = loom_paged_decode_workspace_bytes(B, t.pages * PS, QH, KVH, HD);
     at::Tensor ws;
     if (need > 0) ws = bytes(need, p.dev);
@@ -246,6 +247,7 @@ PyObject* paged_update(PyObject* const* x, Py_ssize_t n) {
                      &status = i32(a, 5, "status", 1, p.dev);
     const int32_t* parent = a.none(6) ? nullptr : (const int32_t*)i32(a, 6, "parent", t.rows, p.dev).data_ptr();
     const int64_t n_new = a.integer(7), advance = a.integer(8);
+    if (t.rows == 0) Py_RETURN_NONE;
     OnDevice on(p.dev.index());
     const int64_t need = loom_paged_update_workspace_bytes(t.rows);
     const at::Tensor ws = bytes(need, p.dev);
@@ -272,6 +274,7 @@ PyObject* paged_write(PyObject* const* x, Py_ssize_t n) {
           a.name, ": k_rows and v_rows must be [layers, rows, kv_heads, positions, head_dim] tensors of the pools' "
                   "dtype and one layout");
     const at::Tensor &first = i32(a, 5, "first", t.rows, p.dev), &last = i32(a, 6, "last", t.rows, p.dev);
+    if (kr.numel() == 0) Py_RETURN_NONE;
     OnDevice on(p.dev.index());
     void* st = stream_of(p.dev.index());
     launch([&] {
@@ -410,7 +413,12 @@ PyObject* reorder_rows(PyObject* const* x, Py_ssize_t n) {
         CHECK(row >= inner && (outer == 1 || step >= row * (R - 1) + inner ||
                                (row >= step * (outer - 1) + inner && step >= inner)),
               a.name, ": the rows of a tensor must not overlap");
-        segs.push_back({t.data_ptr(), outer, step * es, row * es, inner * es});
+        char* lo = (char*)t.data_ptr();
+        char* hi = lo + (step * (outer - 1) + row * (R - 1) + inner) * es;
+        const char* p = (const char*)parent.data_ptr();
+        CHECK(hi <= p || lo >= p + 4 * R, a.name, ": parent must not lie in one of the tensors");
+        for (const Seg& s : segs) CHECK(s.p != lo, a.name, ": a tensor is there twice");
+        segs.push_back({lo, outer, step * es, row * es, inner * es});
     }
     for (size_t i = 0; i < segs.size(); i += kMax) {
         const int m = (int)std::min<size_t>(kMax, segs.size() - i);

@@ -438,6 +438,9 @@ static int pool_checks(const char* who, int dtype, const void* k, const void* v,
     LOOM_CHECK((tok * es) % 16 == 0 && (page * es) % 16 == 0 && (head * es) % 16 == 0 && (layer * es) % 16 == 0 &&
                    k != nullptr && v != nullptr && (((uintptr_t)k | (uintptr_t)v) % 16) == 0,
                "%s: the pools must be given, they and their strides multiples of 16 bytes", who);
+    LOOM_CHECK(KVH * PS * HD * es < ((int64_t)1 << 31) && 2 * L * KVH * PS * HD * es / 16 < ((int64_t)1 << 31),
+               "%s: a page of %lld bytes in %lld layers is more than a copy takes at once", who,
+               (long long)(KVH * PS * HD * es), (long long)L);
     *out = PoolArgs{(char*)k, (char*)v, layer * es, page * es, tok * es, head * es, (int)L, (int)KVH, (int)(HD * es)};
     return LOOM_OK;
 }

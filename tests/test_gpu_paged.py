@@ -153,6 +153,17 @@ def test_step_long_rows_split_and_joined(dt):
     _check_step(dt, [5000, 3, 1, 4097, -1, 900], 8, 2, 96, 64, 79, 5)
 
 
+@pytest.mark.parametrize("dt", [BF, HF, FP])
+@pytest.mark.parametrize("lens", [[5000, 3, -1, 4000, 0, 900, 77], [0, -1, 1, 8191, -1, -1], [511] * 17, [8200]])
+def test_step_rows_laid_end_to_end(dt, lens):
+    """32 kv heads leave 16 blocks to each: enough tiles per block that the blocks take
+    equal stretches of all rows laid end to end (from 256 tiles of 32 tokens)."""
+    assert sum(-(-(n + 1) // 32) if n >= 0 else 1 for n in lens) >= 256
+    _check_step(dt, lens, 32, 32, 32, 64, 130, 15)
+    if dt == BF:
+        _check_step(dt, lens, 32, 32, 96, 16, 520, 16, kctx=False)
+
+
 def test_step_many_rows():
     _check_step(BF, [(37 * i) % 90 - 1 for i in range(1, 301)], 4, 2, 32, 16, 8, 6)
 
@@ -511,6 +522,54 @@ def test_reorder_more_than_sixteen_tensors():
     want = [t[[4, 0, 0, 3, 1]].clone() for t in ts]
     ops.reorder_rows(ts, _i32([4, 0, 0, 3, 1]))
     assert all(torch.equal(a, b) for a, b in zip(ts, want))
+
+
+def test_empty_calls_and_refusals():
+    from loom_amd import ops
+    z = lambda *s, dt=BF: torch.zeros(*s, dtype=dt, device=DEV)  # noqa: E731
+    i = lambda *s: z(*s, dt=torch.int32)  # noqa: E731
+    kp, vp, pool = z(10, 2, 16, 96), z(10, 2, 16, 96), z(2, 10, 2, 16, 96)
+    co = z(80, 96, dt=FP)
+    c, kx, q = ops.paged_decode_step(z(0, 1152), kp, vp, i(0, 5), i(0), co, co)
+    assert c.shape == kx.shape == q.shape == (0, 8, 96)
+    ops.paged_update(pool, pool, i(0, 5), i(0), i(10), i(1), n_new=1)
+    ops.reorder_rows([], i(4))
+    ops.reorder_rows([z(0, 3)], i(0))
+    step = lambda **k: ops.paged_decode_step(*{**dict(q=z(3, 1152), k=kp, v=vp, t=i(3, 5), n=i(3), c=co, s=co), **k}.values())  # noqa: E731
+    upd = lambda **k: ops.paged_update(*{**dict(k=pool, v=pool, t=i(3, 5), n=i(3), r=i(10), s=i(1)), **k}.values())  # noqa: E731
+    x, sc = z(8, 100), z(2, 4, dt=FP)
+    bad = [(lambda: step(q=z(3, 1150)), "qkv must be"), (lambda: step(q=z(3, 1152, dt=FP)), "dtype"), (lambda: step(q=z(4, 1152)), "rows of"),
+           (lambda: step(q=z(3, 384)), "qkv must be"), (lambda: step(q=z(3, 1248)), "9 query heads"),
+           (lambda: step(k=z(10, 2, 16, 96, dt=HF)), "one dtype"), (lambda: step(v=z(9, 2, 16, 96)), "same layout"),
+           (lambda: step(v=z(10, 16, 2, 96).transpose(1, 2)), "same layout"), (lambda: step(k=pool, v=pool), "pages, kv_heads"),
+           (lambda: step(t=i(3, 5).long()), "table must be"), (lambda: step(n=i(4)), "lens must be"), (lambda: step(n=i(3).long()), "lens must be"),
+           (lambda: step(c=z(80, 96)), "cos and sin"), (lambda: step(s=z(81, 96, dt=FP)), "cos and sin"), (lambda: step(t=i(3, 5).t()), "table must be"),
+           (lambda: step(q=z(3, 80 * 12), k=z(10, 2, 16, 80), v=z(10, 2, 16, 80), c=z(80, 80, dt=FP), s=z(80, 80, dt=FP)), "head_dim 80"),
+           (lambda: step(k=z(10, 2, 24, 96), v=z(10, 2, 24, 96)), "power of two"), (lambda: step(q=torch.zeros(3, 1152)), "CUDA"),
+           (lambda: step(t=i(1, 5).expand(3, 5)), "row stride 0"),
+           (lambda: upd(k=kp, v=kp), "layers, pages"), (lambda: upd(r=i(9)), "refs must be"), (lambda: upd(s=i(2)), "status must be"),
+           (lambda: ops.paged_update(pool, pool, i(3, 5), i(3), i(10), i(1), parent=i(2)), "parent must be"),
+           (lambda: ops.paged_update(pool, pool, i(3, 5), i(3), i(10), i(1), n_new=81), "n_new=81"),
+           (lambda: ops.paged_write(pool, pool, i(3, 5), z(2, 3, 2, 40, 64), z(2, 3, 2, 40, 64), i(3), i(3)), "k_rows and v_rows"),
+           (lambda: ops.paged_compact(pool, pool, i(3, 5), i(10), i(2)), "used must be"),
+           (lambda: ops.beam_select(x, sc.double()), "float32"), (lambda: ops.beam_select(x, sc[:1]), "each row"), (lambda: ops.beam_select(x, sc, 0), "n_out"),
+           (lambda: ops.beam_select(x, sc, 65), "n_out"), (lambda: ops.beam_select(x, sc, finished=z(8)), "bool"), (lambda: ops.beam_select(x.long(), sc), "logits must be"),
+           (lambda: ops.beam_select(x, sc, pad_id=100), "pad_id"), (lambda: ops.beam_select(z(33, 50), z(1, 33, dt=FP)), "beams"),
+           (lambda: ops.beam_select(z(0, 50), z(0, 4, dt=FP)), "a group"),
+           (lambda: ops.reorder_rows([x], i(7)), "7 rows"), (lambda: ops.reorder_rows([x.t()], i(100)), "dense"),
+           (lambda: ops.reorder_rows([x, x], i(8)), "twice"), (lambda: ops.reorder_rows([x], i(8), [0, 1]), "one dimension"),
+           (lambda: ops.reorder_rows([x[:1].expand(8, 100)], i(8)), "overlap"), (lambda: ops.reorder_rows([x], i(8).long()), "int32"),
+           (lambda: ops.reorder_rows([z(1100, 4)], i(1100)), "0 to 1024 rows"), (lambda: ops.reorder_rows([5], i(8)), "tensors")]
+    p = i(8)
+    bad.append((lambda: ops.reorder_rows([p], p), "parent must not"))
+    for n, (f, msg) in enumerate(bad):
+        with pytest.raises(RuntimeError, match=msg):
+            f()
+            print("not refused:", n, msg)
+    with pytest.raises(TypeError):
+        ops.paged_update(pool, pool, i(3, 5), i(3), i(10), i(1), n_new=1.5)
+    with pytest.raises(TypeError):
+        ops.reorder_rows(7, i(8))
 
 
 # ------------------------------------------------------------------ together

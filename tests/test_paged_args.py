@@ -56,7 +56,7 @@ POOL = dict(dtype=1, k=P, v=P, layers=2, layer=10 * 2 * 16 * 96, page=2 * 16 * 9
 POOLS = [(dict(dtype=3), "unsupported dtype"), (dict(k=None), "pools must be given"), (dict(v=ctypes.c_void_p(8)), "multiples of 16 bytes"),
          (dict(tok=100), "multiples of 16 bytes"), (dict(tok=64), "bad pool strides"), (dict(layer=-8), "bad pool strides"),
          (dict(layers=0), "bad pool shape"), (dict(HD=4, tok=8), "bad pool shape"), (dict(HD=2048, tok=2048), "bad pool shape"),
-         (dict(KVH=0), "bad pool shape"), (dict(n_pages=0), "n_pages"), (dict(page_size=100), "power of two"),
+         (dict(KVH=0), "bad pool shape"), (dict(layers=4096, KVH=4096, HD=1024, tok=1024), "more than a copy takes"), (dict(n_pages=0), "n_pages"), (dict(page_size=100), "power of two"),
          (dict(table=None), "required pointer"), (dict(rows=1025), "0 to 1024 rows"), (dict(max_pages=0), "1 page to 2\\^24"),
          (dict(table_ld=3), "row stride 3")]
 
