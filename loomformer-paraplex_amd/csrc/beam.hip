@@ -52,6 +52,11 @@ __device__ __forceinline__ float beam_key_x(uint64_t k) {
     return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
 }
 
+// the least logit that reaches a bound (1: every candidate does)
+__device__ __forceinline__ float beam_low(uint64_t bound) {
+    return bound > 1 ? beam_key_x(bound) : -3.402823466e38f;
+}
+
 // Lane permutations of 64-bit values inside rows of 16 lanes (see dpp): each step
 // pairs the halves of twice the group, so reductions over 2, 4, 8, 16 lanes are
 // the first 1, 2, 3, 4 of them.
@@ -106,15 +111,18 @@ template <typename T>
 struct BeamPiece {
     static constexpr int NW = (int)sizeof(T) * kBeamVec / 4;
     uint32_t w[NW];
+    __device__ __forceinline__ void load_whole(const T* x, int v) {
+#pragma unroll
+        for (int i = 0; i < NW / 4; ++i) {
+            u32x4 q;                                 // one load, of any alignment
+            __builtin_memcpy(&q, reinterpret_cast<const char*>(x) + ((uint32_t)v * (uint32_t)sizeof(T) + 16 * i), 16);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[4 * i + k] = q[k];
+        }
+    }
     __device__ __forceinline__ void load(const T* x, int v, int v1) {
         if (v + kBeamVec <= v1) {
-#pragma unroll
-            for (int i = 0; i < NW / 4; ++i) {
-                u32x4 q;                             // one load, of any alignment
-                __builtin_memcpy(&q, reinterpret_cast<const char*>(x) + ((uint32_t)v * (uint32_t)sizeof(T) + 16 * i), 16);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) w[4 * i + k] = q[k];
-            }
+            load_whole(x, v);
             return;
         }
         constexpr uint32_t ninf = std::is_same<T, float>::value    ? 0xff800000u
@@ -183,11 +191,20 @@ struct BeamStep {
                 if (e[p].get(k) == x) at = v + p * stride + k;
         return x > -INFINITY ? beam_key(x, at) : 0;
     }
+    // Logits of the wave that may reach `bound`, at most: those of the pieces whose
+    // largest does
+    __device__ __forceinline__ int reaching(uint64_t bound) const {
+        const float low = beam_low(bound);
+        int n = 0;
+#pragma unroll
+        for (int p = 0; p < kBeamPieces; ++p) n += __popcll(__ballot(top[p] >= low));
+        return n * kBeamVec;
+    }
     // f(key) for every candidate whose key is at least `bound`; a piece whose largest
     // is below it is passed over
     template <typename F>
     __device__ __forceinline__ void passing(uint64_t bound, uint32_t v, uint32_t stride, F f) const {
-        const float low = bound > 1 ? beam_key_x(bound) : -3.402823466e38f;      // (1: every candidate)
+        const float low = beam_low(bound);
 #pragma unroll
         for (int p = 0; p < kBeamPieces; ++p) {
             if (!(top[p] >= low)) continue;
@@ -260,12 +277,17 @@ beam_row_kernel(const T* __restrict__ logits, BeamArgs a) {
     float m = -INFINITY;
     double s = 0.0;
     uint64_t bound = 0;                                // 0: no step was ranked yet
-    int listed = 0;                                    // entries of the list, in every thread
+    int listed = 0;                                    // entries of the list, at most (in every thread)
     if (tid < K) kept[tid] = 0;
     if (tid == 0) nfound = 0;
     auto load = [&](BeamStep<T>& st, int base) __attribute__((always_inline)) {
+        if (base + kBeamTile <= v1) {
 #pragma unroll
-        for (int p = 0; p < kBeamPieces; ++p) st.e[p].load(x, base + p * kStride + tid * kBeamVec, v1);
+            for (int p = 0; p < kBeamPieces; ++p) st.e[p].load_whole(x, base + p * kStride + tid * kBeamVec);
+        } else {
+#pragma unroll
+            for (int p = 0; p < kBeamPieces; ++p) st.e[p].load(x, base + p * kStride + tid * kBeamVec, v1);
+        }
     };
     auto push = [&](uint64_t key) __attribute__((always_inline)) { found[atomicAdd(&nfound, 1)] = key; };
     // the K best of the list to kept, and the list down to them
@@ -296,9 +318,7 @@ beam_row_kernel(const T* __restrict__ logits, BeamArgs a) {
         const uint32_t v = (uint32_t)(base + tid * kBeamVec);
         int all = cap + 1;
         if (bound != 0) {
-            int n = 0;
-            cur.passing(bound, v, kStride, [&](uint64_t) __attribute__((always_inline)) { ++n; });
-            n = wave_sum_int(n);
+            const int n = cur.reaching(bound);
             if (lane == 0) count[step & 1][wave] = n;
             __syncthreads();
             all = count[step & 1][0] + count[step & 1][1] + count[step & 1][2] + count[step & 1][3];
@@ -306,7 +326,7 @@ beam_row_kernel(const T* __restrict__ logits, BeamArgs a) {
         const bool full = listed + all > cap;
         uint64_t low = bound;
         if (full) {
-            if (listed > 0) rank();
+            if (step > 0) rank();
             const uint64_t best = group_max_u64(cur.best(v, kStride), 4);
             if ((tid & 3) == 0) quad[tid >> 2] = best;
             if (tid < 64) larger64[tid] = 0;
