@@ -151,6 +151,15 @@ struct BeamPiece {
     }
 };
 
+// The largest of three; a NaN gives way.  (fmaxf would first pass each loaded value
+// through an instruction of its own that quiets signalling NaNs; here such a one
+// may come out instead, in a row whose sum is NaN and that has no candidate.)
+__device__ __forceinline__ float beam_max3(float a, float b, float c) {
+    float d;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
+}
+
 // A thread's logits of one step: place of element k of piece p is v + p * stride + k.
 template <typename T>
 struct BeamStep {
@@ -159,24 +168,27 @@ struct BeamStep {
     __device__ __forceinline__ void maxima() {
 #pragma unroll
         for (int p = 0; p < kBeamPieces; ++p) {
-            top[p] = e[p].get(0);
+            top[p] = beam_max3(e[p].get(0), e[p].get(1), e[p].get(1));
 #pragma unroll
-            for (int k = 1; k < kBeamVec; ++k) top[p] = fmaxf(top[p], e[p].get(k));
+            for (int k = 2; k < kBeamVec; k += 2) top[p] = beam_max3(top[p], e[p].get(k), e[p].get(k + 1));
         }
     }
     __device__ __forceinline__ float most() const {
-        return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        return beam_max3(beam_max3(top[0], top[1], top[2]), top[3], top[3]);
     }
     // Running maximum and sum of exponentials.  A NaN makes the sum NaN, and so does
-    // +inf; the maximum stays -inf while there is no other logit.
-    __device__ __forceinline__ void sum(float& m, double& s) const {
+    // +inf; the maximum stays -inf while there is no other logit.  A wave passes over
+    // pieces that lie behind v1.
+    __device__ __forceinline__ void sum(float& m, double& s, int v, int stride, int v1) const {
+        const int first = __builtin_amdgcn_readfirstlane(v);
         const float mt = fmaxf(m, most());
         const float at = mt == -INFINITY ? 0.0f : mt;
         float st = 0.0f;
 #pragma unroll
         for (int p = 0; p < kBeamPieces; ++p)
+            if (first + p * stride < v1)
 #pragma unroll
-            for (int k = 0; k < kBeamVec; ++k) st += __builtin_amdgcn_exp2f((e[p].get(k) - at) * kLog2e);
+                for (int k = 0; k < kBeamVec; ++k) st += __builtin_amdgcn_exp2f((e[p].get(k) - at) * kLog2e);
         s = s * (double)(m == mt ? 1.0f : __builtin_amdgcn_exp2f((m - mt) * kLog2e)) + (double)st;
         m = mt;
     }
@@ -314,8 +326,8 @@ beam_row_kernel(const T* __restrict__ logits, BeamArgs a) {
     for (int base = v0; base < v1; base += kBeamTile, ++step) {
         if (base + kBeamTile < v1) load(next, base + kBeamTile);
         cur.maxima();
-        cur.sum(m, s);
         const uint32_t v = (uint32_t)(base + tid * kBeamVec);
+        cur.sum(m, s, (int)v, kStride, v1);
         int all = cap + 1;
         if (bound != 0) {
             const int n = cur.reaching(bound);
@@ -540,7 +552,7 @@ beam_whole_kernel(const T* __restrict__ logits, BeamArgs a, int wl, int cap) {
     float m = -INFINITY;
     double s = 0.0;
     st.maxima();
-    st.sum(m, s);
+    st.sum(m, s, v, stride, v1);
     beam_wave_sum(m, s);
     if (lane == 0) {
         wmax[wave] = m;
