@@ -22,7 +22,8 @@ constexpr int kPgTile = 32;       // tokens of one wave step of the matrix-core 
 constexpr int kPgMinTiles = 4;    // tiles of a chunk at least: one per wave
 constexpr int kPgStream = 16;     // tiles per block from which the rows are laid end to end
 constexpr int kPgRowCost = 6;     // what starting on a row costs a block, in tiles
-constexpr int kPgWhole = 512;     // rows of up to so many tokens are not split
+constexpr int kPgWhole = 512;     // rows of up to so many tokens are not split,
+constexpr int kPgWholeVec = 256;  // in the vector form of up to so many, if there are few rows
 constexpr int kPgMaxRows = 1024;
 
 template <typename T>
@@ -842,36 +843,53 @@ paged_join_kernel(PagedArgs<T> a) {
 // ------------------------------------------------------------------ host side
 
 // Blocks per kv head that share the work: as many as the device holds at once
-// (two per CU); none where no row can be longer than kPgWhole tokens: then a
-// block per row does it in one launch.
-static int paged_slots(int64_t cap, int64_t KVH) {
-    if (cap <= kPgWhole) return 0;
+// (two per CU; 32 rows of 2176 tokens in us with 1, 1.5, 2, 3, 4 per CU: 24.1, 20.2,
+// 21.3, 27.9, 27.8, and 64 rows of 2048, 8 kv heads of 128: 94.5, 94.3, 96.5, 99.7,
+// 100).  None where no row can be long: a block per row then does it in one launch.
+// Both ways in us, whole rows / split and joined, at 120, 250, 370, 500 tokens:
+//   bf16, 4 rows, 2 kv heads of 96      6.8 / 7.7, 7.5 / 10.7,  8.8 / 10.8,  9.9 / 10.9
+//   bf16, 4 rows, 8 kv heads of 128     7.3 / 8.9, 9.2 / 10.5, 11.0 / 10.7, 12.8 / 10.8
+//   bf16, 32 rows, 8 kv heads of 128    8.9 / 11.9, 11.4 / 16.0, 14.0 / 19.3, 16.8 / 21.1
+//   fp32, 5 rows, 2 kv heads of 96     10.6 / 12.5, 14.4 / 15.9, 17.6 / 15.9, 20.8 / 16.0
+// (fp32, 2 kv heads of 96: 32 rows of 300 15.9 / 16.0, 128 rows of 440 20.9 / 26.5)
+// and at 900: 1 row 12.7 / 10.7, 32 rows of 2 kv heads of 96 14.2 / 12.5.
+static int paged_slots(int64_t cap, int64_t KVH, bool vec, int64_t B) {
+    if (cap <= (vec && 2 * B * KVH < device_cus() ? kPgWholeVec : kPgWhole)) return 0;
     const int64_t n = 2 * (int64_t)device_cus() / KVH;
     return n < 1 ? 1 : (int)n;
 }
 
+// Whether the matrix cores do not take the case (see paged_mfma_kernel)
+static bool paged_vec(int64_t es, int64_t HD, int64_t G) {
+    return es != 2 || G > 16 || !(HD == 32 || HD == 64 || HD == 96 || HD == 128);
+}
+
 // Blocks per kv head of a launch, and records of it: one for each pair of a block
 // and a row that it works on (at most slots + B, and ceil(tiles / kPgMinTiles) a row).
-static int64_t paged_items(int64_t B, int64_t cap, int64_t KVH) {
-    const int64_t slots = paged_slots(cap, KVH);
-    return slots == 0 ? B : B + slots;
-}
+static int64_t paged_items(int64_t B, int64_t slots) { return slots == 0 ? B : B + slots; }
+
+// Waves of a block that does a row alone: eight, so that its tiles are in flight at
+// once, but four where a row has no more tiles than that or where the blocks fill
+// the device (two of four waves fit a CU, one of eight).  In us, eight / four: 4 rows,
+// 2 kv heads of 96, 120 tokens 6.8 / 5.8; 1 row of 450 8.3 / 9.2; 8 kv heads of 128,
+// 4 rows of 440 11.8 / 12.9, 32 of 500 16.8 / 16.1, 64 of 440 29.0 / 24.7.
+static bool paged_eight(int64_t cap, int64_t blocks) { return cap > 4 * kPgTile && blocks < device_cus(); }
 
 template <typename T, bool STEP>
 static int paged_launch(PagedArgs<T>& a, int64_t HD, hipStream_t st) {
-    const int64_t items = paged_items(a.B, a.cap, a.KVH);
+    const int64_t items = paged_items(a.B, a.slots);
     a.rec_ml = items * a.QH * 2 * HD;
     const char* who = STEP ? "loom_paged_decode_step" : "loom_paged_decode_attention";
     bool done = false;
     if constexpr (sizeof(T) == 2) {
         const dim3 grid((unsigned)items, (unsigned)a.KVH);
-        // a row that one block does alone has eight waves, its tiles in flight at once
+        const bool eight = a.slots == 0 && paged_eight(a.cap, (int64_t)a.B * a.KVH);
 #define LOOM_PG_MF1(HDV, NW, KC)                                                                    \
         hipLaunchKernelGGL((paged_mfma_kernel<T, HDV, NW, STEP, KC>), grid, dim3(NW * 64), 0, st, a)
 #define LOOM_PG_MF(HDV)                                                                             \
-        if (!done && HD == HDV && a.G <= 16) {                                                      \
-            if (a.slots == 0 && a.k_out != nullptr) LOOM_PG_MF1(HDV, 8, true);                      \
-            else if (a.slots == 0) LOOM_PG_MF1(HDV, 8, false);                                      \
+        if (HD == HDV && !paged_vec(sizeof(T), HD, a.G)) {                                          \
+            if (eight && a.k_out != nullptr) LOOM_PG_MF1(HDV, 8, true);                             \
+            else if (eight) LOOM_PG_MF1(HDV, 8, false);                                             \
             else if (a.k_out != nullptr) LOOM_PG_MF1(HDV, 4, true);                                 \
             else LOOM_PG_MF1(HDV, 4, false);                                                        \
             done = true;                                                                            \
@@ -948,7 +966,7 @@ static int paged_typed(const PagedCall& c, hipStream_t st) {
     a.QH = (int)c.QH;
     a.KVH = (int)c.KVH;
     a.G = (int)(c.QH / c.KVH);
-    a.slots = paged_slots(a.cap, c.KVH);
+    a.slots = paged_slots(a.cap, c.KVH, paged_vec(sizeof(T), c.HD, a.G), c.B);
     a.qscale = kLog2e / sqrtf((float)c.HD);
     return paged_launch<T, STEP>(a, c.HD, st);
 }
@@ -1005,8 +1023,9 @@ using namespace loom;
 extern "C" int64_t loom_paged_decode_workspace_bytes(int64_t B, int64_t capacity, int64_t QH, int64_t KVH,
                                                      int64_t HD) {
     if (B <= 0 || capacity <= 0 || KVH <= 0) return 0;
-    const int64_t items = paged_items(B, capacity, KVH);
-    return paged_slots(capacity, KVH) == 0 ? 0 : items * QH * (2 + 2 * HD) * (int64_t)sizeof(float);
+    // (whatever the type: as for the form that splits first)
+    const int64_t slots = paged_slots(capacity, KVH, true, 0);
+    return slots == 0 ? 0 : paged_items(B, slots) * QH * (2 + 2 * HD) * (int64_t)sizeof(float);
 }
 
 extern "C" int loom_paged_decode_step(int dtype, const void* qkv, int64_t qkv_ld, void* k_pages, void* v_pages,

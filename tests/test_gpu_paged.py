@@ -168,6 +168,16 @@ def test_step_many_rows():
     _check_step(BF, [(37 * i) % 90 - 1 for i in range(1, 301)], 4, 2, 32, 16, 8, 6)
 
 
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("B", [3, 140])
+@pytest.mark.parametrize("cap", [112, 128, 144, 256, 272, 512, 528])
+def test_step_around_the_capacities_that_split(dt, B, cap):
+    """Whether a row is split, and by how many waves it is done, goes by the capacity
+    and the number of rows: both sides of each bound."""
+    lens = [cap - 1, 0, cap // 2] + [(29 * i) % cap - 1 for i in range(B - 3)]
+    _check_step(dt, lens, 4, 2, 96, 16, cap // 16, 17, kctx=cap % 32 == 0)
+
+
 def test_step_equals_dense_step():
     """Rows of one length: loom_gqa_decode_step over the dense cache with the same rows."""
     from loom_amd import _lib, ops

@@ -106,7 +106,7 @@ def test_workspace_queries():
     # each row that one of them works on
     assert lib.loom_paged_decode_workspace_bytes(32, 4096, 8, 2, 96) == (32 + 256) * 8 * 2 * 97 * 4
     assert lib.loom_paged_decode_workspace_bytes(2, 528, 8, 2, 96) == (2 + 256) * 8 * 2 * 97 * 4
-    assert lib.loom_paged_decode_workspace_bytes(200, 512, 8, 2, 96) == 0      # one chunk per row: no join
+    assert lib.loom_paged_decode_workspace_bytes(200, 256, 8, 2, 96) == 0      # one chunk per row: no join
     assert lib.loom_paged_update_workspace_bytes(7) == 7 * 16
     assert lib.loom_paged_compact_workspace_bytes(10) == 136
     assert lib.loom_beam_select_workspace_bytes(0, 4, 100, 4) == 0
