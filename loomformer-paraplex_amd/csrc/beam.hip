@@ -676,12 +676,16 @@ static int beam_whole(int64_t W, int64_t V, int64_t K) {
     return (V << wl) <= kBeamWhole ? wl : -1;
 }
 
-// Slices of a row: enough blocks for the device, each at least a quarter of a
-// step's logits, and few enough that a group's survivors fit one block.
+// Slices of a row: four blocks per CU (as many as it holds) as long as a slice has
+// a step's logits, two per CU down to a quarter of that, and few enough that a
+// group's survivors fit one block.
 static int64_t beam_slices(int64_t rows, int64_t W, int64_t V, int64_t K) {
-    int64_t s = ceil_div(4 * (int64_t)device_cus(), rows);
-    const int64_t most = ceil_div(V, kBeamTile / 4), fit = kBeamMaxCand / (W * K);
-    s = s < most ? s : most;
+    const int64_t cus = device_cus(), fit = kBeamMaxCand / (W * K);
+    int64_t s = ceil_div(4 * cus, rows), least = ceil_div(2 * cus, rows);
+    const int64_t full = ceil_div(V, kBeamTile), quarter = ceil_div(V, kBeamTile / 4);
+    s = s < full ? s : full;
+    least = least < quarter ? least : quarter;
+    s = s > least ? s : least;
     s = s < fit ? s : fit;
     return s < 1 ? 1 : s;
 }
