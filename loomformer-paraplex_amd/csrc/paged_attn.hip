@@ -90,6 +90,13 @@ __device__ __forceinline__ int row_tiles(int n) { return n > 0 ? (n + kPgTile - 
 // kPgMinTiles or more), one block each: no more chunks than slots, but for rows
 // of less than a chunk (a block more than the device holds at once would run
 // after all others).
+// End to end no block waits for a longer one, but a block that starts on a row pays
+// its rope, its join record and an empty pipeline again (about six tiles: 64 rows of
+// 1 to 16384 tokens, 8 kv heads of 128, in us with kPgRowCost 2, 4, 6: 90.9, 86.8,
+// 85.7); equal chunks have one start per block.  From how many tiles per block the
+// former pays, in us with kPgStream 8, 16, 32: 32 rows of 2176 tokens, 2 kv heads of
+// 96, 19.6, 18.3, 18.3; the same in fp32 30.6, 28.2, 28.2; 1 row of 16384, 8 kv heads
+// of 128, 22.5, 21.7, 21.7.
 struct Plan {
     int q, slots, total;
 };
@@ -291,6 +298,13 @@ __device__ __forceinline__ void paged_finish(const PagedArgs<T>& a, const PlanIt
 // the transposing LDS read.  A 16-token half of a tile lies in one page (pages
 // hold a multiple of 16 tokens), so its base address and its bound are scalar:
 // rows past the chunk's end and pages that are missing load zeros.
+// Long rows are bound by the reading of K and V, each once for all of a kv head's
+// query heads and for both sums: 64 rows of 1 to 16384 tokens, 8 kv heads of 128,
+// bf16, 442 MB: 77 us here and 7 in the join, 5.2 TB/s over both (a large copy runs
+// at 5.2); 64 rows of 2048 5.9 TB/s.  Short ones by the chain of first loads: lens,
+// table, the row's K; scores; the waves' join: 1 row of 300, 2 kv heads of 96, 7 us of
+// which an empty launch is 2.  Two waves per SIMD leave 256 registers, so that the
+// next tile's K and V are in flight in registers while the present one is multiplied.
 template <typename T, int HD, int NW, bool STEP, bool KCTX>
 __global__ void __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 paged_mfma_kernel(PagedArgs<T> a) {
@@ -530,7 +544,11 @@ paged_mfma_kernel(PagedArgs<T> a) {
 // fp32 (whose products stay in fp32) and the head sizes the matrix-core form
 // does not take.  LPR lanes per token, each NV groups of four elements (group
 // j + LPR v of the row), GT heads per block; scores by a lane-group sum.  The next
-// tokens' rows are in flight while the present ones are folded in.
+// tokens' rows are in flight while the present ones are folded in.  fp32, 32 rows of
+// 2176 tokens, 2 kv heads of 96, 107 MB: 27 us with the join, 3.9 TB/s; bound by its
+// arithmetic, 2 G + 2 G products per K and V element with no matrix instruction.
+// 5 rows of 1 to 1001: 12 us here, of which about 8 are the first loads, the rope
+// and the waves' join.
 template <typename T>
 __device__ __forceinline__ void load4(const T* p, float v[4]) {
     if constexpr (sizeof(T) == 4) {
@@ -768,7 +786,9 @@ paged_vec_kernel(PagedArgs<T> a) {
 // ------------------------------------------------------------------ the join
 // One block per (row, q head): wave w takes the row's chunk records w, w + 4, ..,
 // a whole record of 2 HD sums per load, kPgJoin of them in flight; the waves meet
-// in LDS.  Rows of one chunk are done already.
+// in LDS.  Rows of one chunk are done already.  Bound by the chain plan, records,
+// sums: 32 rows of 2176 tokens, 8 heads, 3.9 us with a launch's 2; eight records
+// in flight and four sums per load took 0.5 us off one and one.
 constexpr int kPgJoin = 8;
 
 template <typename T, int HD, bool STEP>
