@@ -81,6 +81,11 @@ __device__ __forceinline__ float sum_16_32(float v) {
     return p.x + p.y;
 }
 
+// The exponents' running reference: it follows the maximum (in powers of two) only
+// where that is 2^8 beyond it.  Weights of up to 2^8 lose nothing in fp32, nor in a
+// 16-bit type's relative step, and the sums are hardly ever rescaled.
+__device__ __forceinline__ float raised(float ref, float most) { return most > ref + 8.0f ? most : ref; }
+
 // Tiles of a row of n tokens; a row of none counts as one, which writes its outputs.
 __device__ __forceinline__ int row_tiles(int n) { return n > 0 ? (n + kPgTile - 1) / kPgTile : 1; }
 
@@ -481,7 +486,7 @@ paged_mfma_kernel(PagedArgs<T> a) {
                     mx = fmaxf(mx, sv[hf][r]);
                 }
             mx = max_16_32(mx);
-            const float mnew = fmaxf(mh, mx);
+            const float mnew = raised(mh, mx);
             const float corr = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mh - mnew);
             float ls = 0.0f, pv[2][4];
 #pragma unroll
@@ -493,12 +498,13 @@ paged_mfma_kernel(PagedArgs<T> a) {
                 }
             ls = sum_16_32(ls);
             lh = fmaf(lh, corr, ls);
+            const bool rescale = corr != 1.0f && mh != -INFINITY;      // (before, the sums are zero)
             mh = mnew;
             // the weights enter the products rounded to the storage type (half a step of
             // it, relative, per weight: below the rounding of the outputs)
             const uint4 pa = make_uint4(M::pack(pv[0][0], pv[0][1]), M::pack(pv[0][2], pv[0][3]),
                                         M::pack(pv[1][0], pv[1][1]), M::pack(pv[1][2], pv[1][3]));
-            if (__any(corr != 1.0f)) {
+            if (__any(rescale)) {
                 float cf[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) cf[r] = __shfl(corr, 4 * lq + r, 64);
@@ -691,10 +697,10 @@ paged_vec_kernel(PagedArgs<T> a) {
                 for (int e = 0; e < E; ++e) s = fmaf(q[g][e], k[e], s);
                 s = group_sum<LPR>(s);
                 s = in ? s : -INFINITY;
-                const float mx = fmaxf(m[g], s);
-                const float corr = mx == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[g] - mx);
+                const float mx = raised(m[g], s);
                 const float p = s == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s - mx);
-                if (__any(corr != 1.0f)) {
+                if (__any(mx != m[g] && m[g] != -INFINITY)) {          // (before, the sums are zero)
+                    const float corr = mx == m[g] ? 1.0f : __builtin_amdgcn_exp2f(m[g] - mx);
                     l[g] *= corr;
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
