@@ -19,11 +19,11 @@ typedef __bf16 pg_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 pg_f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kPgTile = 32;       // tokens of one wave step of the matrix-core form
-constexpr int kPgMinTiles = 4;    // tiles of a chunk at least: one per wave
+constexpr int kPgLeast = 1;       // a chunk has 2^kPgLeast tiles at least, one in the vector form
 constexpr int kPgStream = 16;     // tiles per block from which the rows are laid end to end
 constexpr int kPgRowCost = 6;     // what starting on a row costs a block, in tiles
 constexpr int kPgWhole = 512;     // rows of up to so many tokens are not split,
-constexpr int kPgWholeVec = 256;  // in the vector form of up to so many, if there are few rows
+constexpr int kPgWholeVec = 8;    // in the vector form of up to so many steps, if there are few rows
 constexpr int kPgMaxRows = 1024;
 
 template <typename T>
@@ -47,6 +47,7 @@ struct PagedArgs {
     int n_pages, log_ps, cap, n_pos;
     int B, QH, KVH, G;
     int slots;             // blocks per kv head to share the work among; 0: a block per row
+    int least;             // tiles of a chunk at least: 2^least
     float qscale;
 };
 
@@ -92,7 +93,7 @@ __device__ __forceinline__ int row_tiles(int n) { return n > 0 ? (n + kPgTile - 
 // How the rows' tiles are shared out.  q > 0: block j takes units j q .. (j+1) q - 1
 // of the rows laid end to end, a row being kPgRowCost units and its tiles.  Else a
 // row of t tiles is cut into slots * t / total equal chunks (at least one, each of
-// kPgMinTiles or more), one block each: no more chunks than slots, but for rows
+// 2^least or more), one block each: no more chunks than slots, but for rows
 // of less than a chunk (a block more than the device holds at once would run
 // after all others).
 // End to end no block waits for a longer one, but a block that starts on a row pays
@@ -102,25 +103,29 @@ __device__ __forceinline__ int row_tiles(int n) { return n > 0 ? (n + kPgTile - 
 // former pays, in us with kPgStream 8, 16, 32: 32 rows of 2176 tokens, 2 kv heads of
 // 96, 19.6, 18.3, 18.3; the same in fp32 30.6, 28.2, 28.2; 1 row of 16384, 8 kv heads
 // of 128, 22.5, 21.7, 21.7.
+// The least chunk, in us with 1, 2, 4 tiles: bf16, 1 row of 2000 tokens, 2 kv heads of
+// 96, 11.2, 10.3, 10.7, 4 rows of 900, 8 kv heads of 128, 12.6, 12.6, 13.0 (a wave of
+// the block without a tile costs nothing); in the vector form, whose blocks do one
+// tile at a time, fp32, 5 rows to 1001, 11.8, 12.8, 14.0.
 struct Plan {
-    int q, slots, total;
+    int q, slots, total, least;
 };
 
 template <bool STEP>
-__device__ __forceinline__ Plan make_plan(const int32_t* lens, int B, int cap, int n_pos, int slots) {
-    if (slots == 0) return Plan{0, 0, 1};
+__device__ __forceinline__ Plan make_plan(const int32_t* lens, int B, int cap, int n_pos, int slots, int least) {
+    if (slots == 0) return Plan{0, 0, 1, 0};
     int total = 0;
     bool bad;
     for (int b = threadIdx.x & 63; b < B; b += 64) total += row_tiles(row_tokens(lens, b, STEP, cap, n_pos, &bad));
     total = wave_sum_int(total);
     const bool stream = total >= kPgStream * slots;
-    return Plan{stream ? (total + B * kPgRowCost + slots - 1) / slots : 0, slots, total};
+    return Plan{stream ? (total + B * kPgRowCost + slots - 1) / slots : 0, slots, total, least};
 }
 
 __device__ __forceinline__ int plan_units(const Plan& p, int tiles) {
     if (p.q > 0) return tiles + kPgRowCost;
     const uint32_t n = (uint32_t)tiles * (uint32_t)p.slots / (uint32_t)p.total;      // (< 2^19 * 2^9)
-    return max(1, (int)min(n, (uint32_t)(tiles + kPgMinTiles - 1) / kPgMinTiles));
+    return max(1, (int)min(n, (uint32_t)(tiles + (1 << p.least) - 1) >> p.least));
 }
 
 // A row's place in the plan: the units before it, its tokens
@@ -187,8 +192,9 @@ __device__ __forceinline__ PlanItem plan_item(const Plan& p, const PlanRow& r, i
 
 // The rows of block j, one after the other: f(PlanItem).
 template <bool STEP, typename F>
-__device__ __forceinline__ void plan_walk(const int32_t* lens, int B, int cap, int n_pos, int slots, int j, F f) {
-    const Plan p = make_plan<STEP>(lens, B, cap, n_pos, slots);
+__device__ __forceinline__ void plan_walk(const int32_t* lens, int B, int cap, int n_pos, int slots, int least, int j,
+                                          F f) {
+    const Plan p = make_plan<STEP>(lens, B, cap, n_pos, slots, least);
     PlanRow r = plan_find<STEP, false>(p, lens, B, cap, n_pos, p.q > 0 ? j * p.q : j);
     if (r.row < 0) return;
     while (true) {
@@ -338,7 +344,7 @@ paged_mfma_kernel(PagedArgs<T> a) {
         const int j = i * 64 + lane, row = j / CPR, c = j - row * CPR;
         loff[i] = (uint32_t)(row * a.ps_tok * (int)sizeof(T)) + 16 * c;
     }
-    plan_walk<STEP>(a.lens, a.B, a.cap, a.n_pos, a.slots, blockIdx.x, [&](const PlanItem& it) {
+    plan_walk<STEP>(a.lens, a.B, a.cap, a.n_pos, a.slots, a.least, blockIdx.x, [&](const PlanItem& it) {
         const int64_t b = it.row;
         const int pos = it.tokens - 1;
         const int t1 = min(it.tile1 * kPgTile, it.tokens);
@@ -551,10 +557,10 @@ paged_mfma_kernel(PagedArgs<T> a) {
 // does not take.  LPR lanes per token, each NV groups of four elements (group
 // j + LPR v of the row), GT heads per block; scores by a lane-group sum.  The next
 // tokens' rows are in flight while the present ones are folded in.  fp32, 32 rows of
-// 2176 tokens, 2 kv heads of 96, 107 MB: 27 us with the join, 3.9 TB/s; bound by its
-// arithmetic, 2 G + 2 G products per K and V element with no matrix instruction.
-// 5 rows of 1 to 1001: 12 us here, of which about 8 are the first loads, the rope
-// and the waves' join.
+// 2176 tokens, 2 kv heads of 96, 107 MB: 27 us with the join, 4.0 TB/s; bound by its
+// arithmetic, 2 G products per K and G per V element with no matrix instruction (a
+// step of 32 tokens takes 0.8 us).  5 rows of 1 to 1001: 12 us with the join, of which
+// about 8 are the first loads, the rope and the waves' join.
 template <typename T>
 __device__ __forceinline__ void load4(const T* p, float v[4]) {
     if constexpr (sizeof(T) == 4) {
@@ -587,7 +593,7 @@ paged_vec_kernel(PagedArgs<T> a) {
     const int j = lane % LPR, grp = wave * RPW + lane / LPR;
     const int ps_mask = (1 << a.log_ps) - 1;
     const bool kctx = a.k_out != nullptr;
-    plan_walk<STEP>(a.lens, a.B, a.cap, a.n_pos, a.slots, blockIdx.x, [&](const PlanItem& it) {
+    plan_walk<STEP>(a.lens, a.B, a.cap, a.n_pos, a.slots, a.least, blockIdx.x, [&](const PlanItem& it) {
         const int64_t b = it.row;
         const int pos = it.tokens - 1;
         const int t0 = it.tile0 * kPgTile, t1 = min(it.tile1 * kPgTile, it.tokens);
@@ -803,7 +809,7 @@ paged_join_kernel(PagedArgs<T> a) {
     constexpr int NV = HD > 128 ? 2 : 1, NL = HD / 2 / NV;     // lanes of four sums
     __shared__ float wm[4], wl[4];
     __shared__ __align__(16) float wacc[4][2 * HD];
-    const Plan p = make_plan<STEP>(a.lens, a.B, a.cap, a.n_pos, a.slots);
+    const Plan p = make_plan<STEP>(a.lens, a.B, a.cap, a.n_pos, a.slots, a.least);
     const PlanRow r0 = plan_find<STEP, true>(p, a.lens, a.B, a.cap, a.n_pos, blockIdx.x);
     const PlanItem it = plan_item(p, r0, 0);
     if (it.nchunk == 1) return;
@@ -876,11 +882,15 @@ paged_join_kernel(PagedArgs<T> a) {
 //   bf16, 4 rows, 2 kv heads of 96      6.8 / 7.7, 7.5 / 10.7,  8.8 / 10.8,  9.9 / 10.9
 //   bf16, 4 rows, 8 kv heads of 128     7.3 / 8.9, 9.2 / 10.5, 11.0 / 10.7, 12.8 / 10.8
 //   bf16, 32 rows, 8 kv heads of 128    8.9 / 11.9, 11.4 / 16.0, 14.0 / 19.3, 16.8 / 21.1
-//   fp32, 5 rows, 2 kv heads of 96     10.6 / 12.5, 14.4 / 15.9, 17.6 / 15.9, 20.8 / 16.0
-// (fp32, 2 kv heads of 96: 32 rows of 300 15.9 / 16.0, 128 rows of 440 20.9 / 26.5)
-// and at 900: 1 row 12.7 / 10.7, 32 rows of 2 kv heads of 96 14.2 / 12.5.
-static int paged_slots(int64_t cap, int64_t KVH, bool vec, int64_t B) {
-    if (cap <= (vec && 2 * B * KVH < device_cus() ? kPgWholeVec : kPgWhole)) return 0;
+// and at 900: 1 row 12.7 / 10.7, 32 rows of 2 kv heads of 96 14.2 / 12.5.  The vector
+// form takes a block's 4 waves times 64 / LPR tokens per step, so its bound is in steps:
+//   fp32, 5 rows, 2 kv heads of 96, 100, 180, 250 tokens   9.9 / 12.2, 11.5 / 12.4, 12.8 / 12.3
+//   bf16, 4 rows, 4 kv heads of 256, the same             11.9 / 12.9, 15.8 / 13.5, 18.6 / 13.7
+// unless the rows fill the device: fp32, 128 rows of 440, 2 kv heads of 96, 20.9 / 26.5.
+static int paged_slots(int64_t cap, int64_t HD, int64_t KVH, bool vec, int64_t B) {
+    const int64_t step = HD <= 8 ? 128 : HD <= 16 ? 64 : HD <= 96 ? 32 : 16;     // tokens of a vector block's step
+    const int64_t few = kPgWholeVec * step < kPgWhole ? kPgWholeVec * step : kPgWhole;
+    if (cap <= (vec && 2 * B * KVH < device_cus() ? few : kPgWhole)) return 0;
     const int64_t n = 2 * (int64_t)device_cus() / KVH;
     return n < 1 ? 1 : (int)n;
 }
@@ -891,7 +901,7 @@ static bool paged_vec(int64_t es, int64_t HD, int64_t G) {
 }
 
 // Blocks per kv head of a launch, and records of it: one for each pair of a block
-// and a row that it works on (at most slots + B, and ceil(tiles / kPgMinTiles) a row).
+// and a row that it works on (at most slots + B, and ceil(tiles / 2^least) a row).
 static int64_t paged_items(int64_t B, int64_t slots) { return slots == 0 ? B : B + slots; }
 
 // Waves of a block that does a row alone: eight, so that its tiles are in flight at
@@ -992,7 +1002,9 @@ static int paged_typed(const PagedCall& c, hipStream_t st) {
     a.QH = (int)c.QH;
     a.KVH = (int)c.KVH;
     a.G = (int)(c.QH / c.KVH);
-    a.slots = paged_slots(a.cap, c.KVH, paged_vec(sizeof(T), c.HD, a.G), c.B);
+    const bool vec = paged_vec(sizeof(T), c.HD, a.G);
+    a.slots = paged_slots(a.cap, c.HD, c.KVH, vec, c.B);
+    a.least = vec ? 0 : kPgLeast;
     a.qscale = kLog2e / sqrtf((float)c.HD);
     return paged_launch<T, STEP>(a, c.HD, st);
 }
@@ -1050,7 +1062,7 @@ extern "C" int64_t loom_paged_decode_workspace_bytes(int64_t B, int64_t capacity
                                                      int64_t HD) {
     if (B <= 0 || capacity <= 0 || KVH <= 0) return 0;
     // (whatever the type: as for the form that splits first)
-    const int64_t slots = paged_slots(capacity, KVH, true, 0);
+    const int64_t slots = paged_slots(capacity, HD, KVH, true, 0);
     return slots == 0 ? 0 : paged_items(B, slots) * QH * (2 + 2 * HD) * (int64_t)sizeof(float);
 }
 

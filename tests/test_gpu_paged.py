@@ -176,6 +176,9 @@ def test_step_around_the_capacities_that_split(dt, B, cap):
     and the number of rows: both sides of each bound."""
     lens = [cap - 1, 0, cap // 2] + [(29 * i) % cap - 1 for i in range(B - 3)]
     _check_step(dt, lens, 4, 2, 96, 16, cap // 16, 17, kctx=cap % 32 == 0)
+    if B == 3:
+        for HD in (8, 16, 256):                     # the vector form's steps are 128, 64 and 16 tokens
+            _check_step(dt, lens, 2, 2, HD, 16, cap // 16, 18)
 
 
 def test_step_equals_dense_step():
