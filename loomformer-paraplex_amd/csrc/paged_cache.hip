@@ -120,6 +120,25 @@ paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* _
     __shared__ int32_t base[kPcMaxRows], slot0[kPcMaxRows], len_of[kPcMaxRows];
     __shared__ int waves[16][2];
     const int r = threadIdx.x, PS = 1 << log_ps;
+    // bit 4 j + e: page seg + 4096 j + 4 r + e is free
+    auto free_ids = [&](int64_t seg) __attribute__((always_inline)) {
+        uint32_t mask = 0;
+#pragma unroll
+        for (int j = 0; j < kScanIds; ++j) {
+            const int64_t id = seg + 4096 * j + 4 * r;
+            if (id + 4 <= NP) {
+                int4 q;                              // one load, aligned to a word
+                __builtin_memcpy(&q, refs + id, 16);
+                mask |= (uint32_t)((q.x <= 0) | (q.y <= 0) << 1 | (q.z <= 0) << 2 | (q.w <= 0) << 3) << (4 * j);
+            } else {
+                for (int e = 0; e < 4 && id + e < NP; ++e)
+                    if (refs[id + e] <= 0) mask |= 1u << (4 * j + e);
+            }
+        }
+        return mask;
+    };
+    uint32_t mask = 0;                               // of the first pages, with the row's first loads
+    if constexpr (!FORK) mask = free_ids(0);
     // (r + 1024 k) as (row, column), without a division per entry
     const int step_r = 1024 / MP, step_c = 1024 - step_r * MP;
     int len = -1, p = -1;
@@ -190,19 +209,30 @@ paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* _
     }
     tail[r] = page;
     __syncthreads();                                 // (and the fork's changes of refs are done)
-    if (page >= 0) {
-        const int held_by = refs[page];
-        if (held_by > 1) {
-            int before = 0, i = 0;
+    const int held_by = page >= 0 ? refs[page] : 0;
+    // rows before this one with the same tail: `share` threads count for a row
+    int share = 16;
+    while (share > 1 && R * share > 1024) share >>= 1;
+    const int of = r / share, part = r & (share - 1);
+    if (of < R) {
+        const int mine = tail[of];
+        int before = 0;
+        if (mine >= 0) {
 #pragma unroll 4
-            for (; i + 4 <= r; i += 4) {
+            for (int i = 4 * part; i < of; i += 4 * share) {
                 const int4 t = *reinterpret_cast<const int4*>(tail + i);
-                before += (t.x == page) + (t.y == page) + (t.z == page) + (t.w == page);
+                before += (t.x == mine) + (i + 1 < of && t.y == mine) + (i + 2 < of && t.z == mine) +
+                          (i + 3 < of && t.w == mine);
             }
-            for (; i < r; ++i) before += tail[i] == page;
-            copy = held_by - before > 1;
         }
+        if (share >= 2) before += __builtin_amdgcn_update_dpp(0, before, kDppQuad1032, 0xF, 0xF, false);
+        if (share >= 4) before += __builtin_amdgcn_update_dpp(0, before, kDppQuad2301, 0xF, 0xF, false);
+        if (share >= 8) before += __builtin_amdgcn_update_dpp(0, before, kDppHalfMirror, 0xF, 0xF, false);
+        if (share >= 16) before += __builtin_amdgcn_update_dpp(0, before, kDppMirror, 0xF, 0xF, false);
+        if (part == 0) base[of] = before;
     }
+    __syncthreads();
+    copy = page >= 0 && held_by - base[r] > 1;
     const int want = nmiss + (copy ? 1 : 0);
     int want1[1] = {want}, first1[1], total1[1];
     block_scan<1>(want1, reinterpret_cast<int(*)[1]>(waves), first1, total1);
@@ -214,20 +244,8 @@ paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* _
     int given = 0;                                   // free pages handed out so far
     __syncthreads();
     for (int64_t seg = 0; seg < NP && given < need; seg += 1024 * 4 * kScanIds) {
-        uint32_t mask = 0;                           // bit 4 j + e: page seg + 4096 j + 4 r + e is free
+        if (FORK || seg > 0) mask = free_ids(seg);
         int count[2] = {0, 0}, before[2], all[2];    // 16 bits per j
-#pragma unroll
-        for (int j = 0; j < kScanIds; ++j) {
-            const int64_t id = seg + 4096 * j + 4 * r;
-            if (id + 4 <= NP) {
-                int4 q;                              // one load, aligned to a word
-                __builtin_memcpy(&q, refs + id, 16);
-                mask |= (uint32_t)((q.x <= 0) | (q.y <= 0) << 1 | (q.z <= 0) << 2 | (q.w <= 0) << 3) << (4 * j);
-            } else {
-                for (int e = 0; e < 4 && id + e < NP; ++e)
-                    if (refs[id + e] <= 0) mask |= 1u << (4 * j + e);
-            }
-        }
 #pragma unroll
         for (int j = 0; j < kScanIds; ++j) count[j / 2] |= __popc((mask >> (4 * j)) & 15u) << (16 * (j & 1));
         block_scan<2>(count, waves, before, all);
