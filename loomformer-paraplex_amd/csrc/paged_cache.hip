@@ -251,17 +251,19 @@ paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* _
         block_scan<2>(count, waves, before, all);
 #pragma unroll
         for (int j = 0; j < kScanIds; ++j) {
+            const uint32_t bits = (mask >> (4 * j)) & 15u;
             int rank = given + ((before[j / 2] >> (16 * (j & 1))) & 0xffff);
+            if (bits != 0 && rank < need) {
+                int lo = 0, hi = R - 1;              // the last row whose base is at most `rank`
+                while (lo < hi) {
+                    const int mid = (lo + hi + 1) >> 1;
+                    if (base[mid] <= rank) lo = mid; else hi = mid - 1;
+                }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (!((mask >> (4 * j + e)) & 1u)) continue;
-                if (rank < need) {
+                for (int e = 0; e < 4; ++e) {
+                    if (!((bits >> e) & 1u) || rank >= need) continue;
+                    while (lo + 1 < R && base[lo + 1] <= rank) ++lo;
                     const int id = (int)(seg + 4096 * j + 4 * r + e);
-                    int lo = 0, hi = R - 1;          // the last row whose base is at most `rank`
-                    while (lo < hi) {
-                        const int mid = (lo + hi + 1) >> 1;
-                        if (base[mid] <= rank) lo = mid; else hi = mid - 1;
-                    }
                     const bool cp = slot0[lo] < 0;
                     const int k = rank - base[lo], m0 = cp ? ~slot0[lo] : slot0[lo];
                     refs[id] = 1;
@@ -273,8 +275,8 @@ paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* _
                     } else {
                         table[(int64_t)lo * ld + m0 + k - (cp ? 1 : 0)] = id;
                     }
+                    ++rank;
                 }
-                ++rank;
             }
             given += (all[j / 2] >> (16 * (j & 1))) & 0xffff;
         }
