@@ -230,6 +230,15 @@ template <> struct Mfma16<f16_t> {
     }
 };
 
+// x c + y s of the rotation.  For the 16-bit types in 64 bits, where both products
+// are exact: the stored value is the exact one's rounding (in fp32 one in some 10000
+// comes out a step beside it).
+template <typename T>
+__device__ __forceinline__ float turn(float x, float c, float y, float s) {
+    if constexpr (sizeof(T) == 2) return (float)fma((double)x, (double)c, (double)y * (double)s);
+    else return fmaf(x, c, y * s);
+}
+
 // Eight elements of a head from d0 on (a multiple of 8, as HD / 2 is) as they are
 // loaded for the rotation x cos + rotate_half(x) sin: all loads first, so that a
 // row's are one wait.
@@ -255,7 +264,7 @@ struct Rope8 {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const T xe{(uint16_t)(xs[k] >> (16 * h))}, ye{(uint16_t)(ys[k] >> (16 * h))};
-                v[h] = fmaf(ld(&xe), c[2 * k + h], (low ? -ld(&ye) : ld(&ye)) * s[2 * k + h]);
+                v[h] = turn<T>(ld(&xe), c[2 * k + h], low ? -ld(&ye) : ld(&ye), s[2 * k + h]);
             }
             o[k] = Mfma16<T>::pack(v[0], v[1]);
         }
@@ -656,7 +665,7 @@ paged_vec_kernel(PagedArgs<T> a) {
             for (int e = 0; e < 4; ++e) {
                 v[e] = xr[n][e];
                 if (STEP && hh <= GT && it.tokens > 0)
-                    v[e] = round_to<T>(fmaf(xr[n][e], cs[n][e], (d < HD / 2 ? -yr[n][e] : yr[n][e]) * sn[n][e]));
+                    v[e] = round_to<T>(turn<T>(xr[n][e], cs[n][e], d < HD / 2 ? -yr[n][e] : yr[n][e], sn[n][e]));
                 heads[4 * i + e] = v[e];
             }
             if constexpr (STEP) {

@@ -181,6 +181,23 @@ def test_step_around_the_capacities_that_split(dt, B, cap):
             _check_step(dt, lens, 2, 2, HD, 16, cap // 16, 18)
 
 
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("HD", [96, 16])
+def test_step_ropes_to_the_exact_values_rounding(dt, HD):
+    """The products of a 16-bit and a 32-bit value are exact in 64 bits."""
+    from loom_amd import ops
+    g = torch.Generator().manual_seed(19)
+    lens = [(31 * i) % 96 for i in range(256)]
+    kp, vp, table, ln = _cache(g, lens, 6, 2, 16, HD, dt)
+    qkv = torch.randn(256, 12 * HD, generator=g).to(DEV, dt)
+    cos, sin = _tables(HD, 96)
+    q = ops.paged_decode_step(qkv, kp, vp, table, ln, cos, sin)[2]
+    x = qkv.view(256, 12, HD)[:, :8].double()
+    co, si = cos[ln.long()][:, None].double(), sin[ln.long()][:, None].double()
+    turned = torch.cat([-x[..., HD // 2:], x[..., :HD // 2]], -1)
+    assert torch.equal(q, (x * co + turned * si).float().to(dt))
+
+
 def test_step_equals_dense_step():
     """Rows of one length: loom_gqa_decode_step over the dense cache with the same rows."""
     from loom_amd import _lib, ops
