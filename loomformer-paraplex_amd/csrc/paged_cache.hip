@@ -105,11 +105,11 @@ constexpr int kScanIds = 4;         // groups of four page ids per thread and ro
 // appended.  The free pages are taken lowest id first, in row order, by one
 // scan over refs: a free page's rank among the free ones names its row.
 // Bound by the latency of its stages, each a pass over the rows or over refs with a
-// block scan behind it: 256 rows and 17152 pages 10.4 us.  One block and not a launch
+// block scan behind it: 256 rows and 17152 pages 8.6 us.  One block and not a launch
 // per stage, since each stage needs the whole of the one before.
 // FORK: the block also forks the table, staged whole in LDS: a launch less, but
 // one CU's work.  All of a call in both forms (us, one launch / two): 92 entries
-// 7.9 / 9.9, 4352 16.0 / 17.1, 17152 21.3 / 17.8, 32512 19.6 / 13.0.
+// 7.7 / 9.9, 4352 15.8 / 16.9, 17152 20.8 / 16.8, 32512 18.1 / 11.6.
 template <bool FORK>
 __global__ void __launch_bounds__(1024)
 paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* __restrict__ lens,
