@@ -41,9 +41,11 @@ struct BeamArgs {
     double* part_s;
 };
 
-// Order of a logit and its place: larger logit first, then the lower place.
+// Order of a logit and its place: larger logit first, then the lower place.  The two
+// zeros are one value: their keys differ by the place alone, as the comparisons of
+// floats (the bests, the bound) take them.
 __device__ __forceinline__ uint64_t beam_key(float x, uint32_t place) {
-    const uint32_t u = __float_as_uint(x);
+    const uint32_t u = x == 0.0f ? 0u : __float_as_uint(x);
     const uint32_t o = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);   // ascending with x
     return ((uint64_t)o << 32) | (uint32_t)~place;
 }

@@ -1,0 +1,75 @@
+"""Edges of the paged cache's operators, the beam selection and the row reordering:
+values, sizes and layouts at which they could go wrong, against plain
+implementations in 64 bits (oracle.paged)."""
+import math
+
+import pytest
+import torch
+
+from oracle import paged as ref
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no HIP device")
+
+
+def _i32(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+# ------------------------------------------------------------------ selection
+
+def _mixed_zeros(n, seed):
+    """Zeros of both signs in random order, the first one negative."""
+    z = torch.zeros(n)
+    z[torch.rand(n, generator=torch.Generator().manual_seed(seed)) < 0.5] = -0.0
+    z[0] = -0.0
+    z[-1] = 0.0
+    return z
+
+
+@pytest.mark.parametrize("dt", [BF, HF, FP])
+@pytest.mark.parametrize("S,W,V,K", [(1, 1, 2, 1), (1, 1, 2, 2), (1, 1, 9, 3), (2, 4, 700, 4), (1, 4, 8192, 8), (1, 16, 2048, 32),
+                                     (1, 1, 40000, 1), (1, 3, 20011, 64)])
+def test_select_zeros_of_both_signs_are_one_value(dt, S, W, V, K):
+    """A row of nothing but zeros, zeros as the largest values, and zeros on the last
+    place that is chosen: -0.0 and +0.0 tie, the lowest place goes first."""
+    from loom_amd import ops
+    zero = torch.stack([_mixed_zeros(V, 7 * r + V) for r in range(S * W)])
+    below = torch.where(torch.rand(S * W, V, generator=torch.Generator().manual_seed(K)) < 0.9, -2.0, zero)
+    some = below.clone()
+    some[:, V // 2:V // 2 + (K + 1) // 2] = 1.5
+    apart = -torch.arange(S * W, device=DEV).float().view(S, W) / 8
+    for x, sc in ((zero, torch.zeros_like(apart)), (zero, apart), (below, apart), (some, apart)):
+        x = x.to(DEV, dt)
+        s, p, t, f = ops.beam_select(x, sc, K)
+        ws, wp, wt, _ = ref.beam_select(x, sc, K)
+        assert torch.equal(p.cpu(), wp) and torch.equal(t.cpu(), wt)
+        # the value's rounding, and the sum of V exponentials of arguments of at most
+        # 3.5: 32 additions and the exponentials' own two units
+        tol = 2.0 ** -24 * ws.abs() + 40 * 2.0 ** -24 + 2.0 ** -22 * 3.5
+        assert ((s.cpu().double() - ws).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_select_zeros_of_both_signs_over_many_steps(dt):
+    """512 rows: a slice takes several steps, whose bounds are zeros."""
+    from loom_amd import ops
+    V, K = 30011, 6
+    g = torch.Generator().manual_seed(3)
+    x = torch.where(torch.rand(512, V, generator=g) < 0.5, 0.0, -0.0)
+    x[torch.rand(512, V, generator=g) < 0.3] = -1.0
+    x = x.to(DEV, dt)
+    sc = torch.zeros(128, 4, device=DEV)
+    sc[:, 1:] = -3.0                                  # only the first beam's tokens are chosen
+    s, p, t, f = ops.beam_select(x, sc, K)
+    want = torch.sort(x[::4].cpu().double() + 0.0, dim=1, descending=True, stable=True)     # (-0.0 + 0.0 is +0.0)
+    assert torch.equal(t.cpu(), want.indices[:, :K])
+    assert torch.equal(p, (4 * torch.arange(128, device=DEV)).int()[:, None].expand(128, K))
