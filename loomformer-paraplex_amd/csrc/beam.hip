@@ -154,8 +154,10 @@ struct BeamPiece {
 };
 
 // The largest of three; a NaN gives way.  (fmaxf would first pass each loaded value
-// through an instruction of its own that quiets signalling NaNs; here such a one
-// may come out instead, in a row whose sum is NaN and that has no candidate.)
+// through an instruction of its own that quiets signalling NaNs; here such a one may
+// come out instead, or hide what came before it, in a row whose sum is NaN and that
+// has no candidate.  What passes in such a row may be more than the bound promises,
+// so the lists take no key behind their end.)
 __device__ __forceinline__ float beam_max3(float a, float b, float c) {
     float d;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
@@ -310,11 +312,14 @@ beam_row_kernel(const T* __restrict__ logits, BeamArgs a) {
             for (int p = 0; p < kBeamPieces; ++p) st.e[p].load(x, base + p * kStride + tid * kBeamVec, v1);
         }
     };
-    auto push = [&](uint64_t key) __attribute__((always_inline)) { found[atomicAdd(&nfound, 1)] = key; };
+    auto push = [&](uint64_t key) __attribute__((always_inline)) {
+        const int at = atomicAdd(&nfound, 1);
+        if (at < cap) found[at] = key;                 // (always, in a row without a signalling NaN)
+    };
     // the K best of the list to kept, and the list down to them
     auto rank = [&]() {
         __syncthreads();
-        const int n = nfound, tp = beam_counters(n, 256);
+        const int n = min(nfound, cap), tp = beam_counters(n, 256);
         for (int i = tid / tp; i < n; i += 256 / tp) {
             const uint64_t key = found[i];
             int larger = 0;
@@ -586,10 +591,13 @@ beam_whole_kernel(const T* __restrict__ logits, BeamArgs a, int wl, int cap) {
     __syncthreads();
     uint64_t* mine = found + (size_t)w * cap;
     st.passing(beam_kth(part + w * 64, larger + w * 64, K), (uint32_t)v, (uint32_t)stride,
-               [&](uint64_t key) __attribute__((always_inline)) { mine[atomicAdd(&nfound[w], 1)] = key; });
+               [&](uint64_t key) __attribute__((always_inline)) {
+                   const int at = atomicAdd(&nfound[w], 1);
+                   if (at < cap) mine[at] = key;       // (always, in a row without a signalling NaN)
+               });
     const double lse = lse_of[w];
     __syncthreads();
-    const int n = nfound[w];
+    const int n = min(nfound[w], cap);
     const int tp = beam_counters(n, nt);
     for (int i = t / tp; i < n; i += nt / tp) {
         const uint64_t key = mine[i];

@@ -73,3 +73,29 @@ def test_select_zeros_of_both_signs_over_many_steps(dt):
     want = torch.sort(x[::4].cpu().double() + 0.0, dim=1, descending=True, stable=True)     # (-0.0 + 0.0 is +0.0)
     assert torch.equal(t.cpu(), want.indices[:, :K])
     assert torch.equal(p, (4 * torch.arange(128, device=DEV)).int()[:, None].expand(128, K))
+
+
+@pytest.mark.parametrize("dt,snan", [(BF, 0x7F81), (HF, 0x7D01), (FP, 0x7F800001)])
+@pytest.mark.parametrize("V,K", [(16000, 1), (8192, 4), (30000, 1), (100000, 3)])
+def test_select_rows_with_signalling_nans(dt, snan, V, K):
+    """A NaN that is not quiet, with larger logits before it and a tie behind it in
+    every eight: the row has no candidate, and the rows beside it keep theirs."""
+    from loom_amd import ops
+    g = torch.Generator().manual_seed(V)
+    W = 2 if V <= 16384 else 3
+    x = (torch.randn(2 * W, V, generator=g) * 3).to(DEV, dt)
+    bits = torch.int32 if dt == FP else torch.int16
+    for row in (0, W + 1):                           # the first of a group, and one in the middle or at the end
+        x[row] = 5.0
+        x[row, :V // 8 * 8].view(-1, 8)[:, :5] = 7.0
+        x[row, :V // 8 * 8].view(-1, 8)[:, 5].copy_(torch.tensor(snan, dtype=bits, device=DEV).view(dt))
+    assert int(torch.isnan(x[0].float()).sum()) == V // 8
+    sc = torch.zeros(2, W, device=DEV)
+    s, p, t, f = ops.beam_select(x, sc, K)
+    dead = sc.clone()
+    dead[0, 0] = dead[1, 1] = -math.inf
+    y = torch.where(torch.isnan(x.float()), 0.0, x.float()).to(dt)
+    s2, p2, t2, f2 = ops.beam_select(y, dead, K)     # the same with those rows ruled out
+    ws, wp, wt, _ = ref.beam_select(y, dead, K)
+    assert torch.equal(p.cpu(), wp) and torch.equal(t.cpu(), wt)
+    assert torch.equal(s, s2) and torch.equal(p, p2) and torch.equal(t, t2)
