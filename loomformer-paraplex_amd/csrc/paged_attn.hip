@@ -195,6 +195,8 @@ template <bool STEP, typename F>
 __device__ __forceinline__ void plan_walk(const int32_t* lens, int B, int cap, int n_pos, int slots, int least, int j,
                                           F f) {
     const Plan p = make_plan<STEP>(lens, B, cap, n_pos, slots, least);
+    // end to end, `slots` blocks have all units (and only their j q stays within 32 bits)
+    if (p.q > 0 && j >= slots) return;
     PlanRow r = plan_find<STEP, false>(p, lens, B, cap, n_pos, p.q > 0 ? j * p.q : j);
     if (r.row < 0) return;
     while (true) {

@@ -99,3 +99,20 @@ def test_select_rows_with_signalling_nans(dt, snan, V, K):
     ws, wp, wt, _ = ref.beam_select(y, dead, K)
     assert torch.equal(p.cpu(), wp) and torch.equal(t.cpu(), wt)
     assert torch.equal(s, s2) and torch.equal(p, p2) and torch.equal(t, t2)
+
+
+# ------------------------------------------------------------------ attention
+
+def test_rows_end_to_end_of_more_units_than_32_bits_name():
+    """1024 rows of 131072 tokens (two pages shared by all) over 512 kv heads: one
+    block of each head has all the work, and the numbers of those behind it, times its
+    units, pass 2^32.  Half of the values are ones, so a part of a row's sum shows."""
+    from loom_amd import ops
+    KVH, HD, PS, MP, B = 512, 32, 1024, 128, 1024
+    kp = torch.zeros(2, KVH, PS, HD, dtype=BF, device=DEV)
+    vp = torch.zeros_like(kp)
+    vp[0] = 1.0
+    table = (torch.arange(MP, device=DEV) >= MP // 2).int().expand(B, MP).contiguous()
+    q = torch.ones(B, KVH, HD, dtype=BF, device=DEV)
+    c, _ = ops.paged_decode_attention(q, kp, vp, table, _i32([MP * PS] * B), want_kctx=False)
+    assert (c == 0.5).all()
