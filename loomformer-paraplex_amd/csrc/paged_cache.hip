@@ -429,7 +429,8 @@ paged_compact_move_kernel(PoolArgs a, int PS, const int32_t* __restrict__ ws, in
     const int64_t units = (int64_t)ws[0] * 2 * a.layers;
     const bool head_run = a.tok == a.row_bytes, page_run = head_run && a.head == (int64_t)PS * a.row_bytes;
     const int runs = page_run ? 1 : head_run ? a.KVH : a.KVH * PS;
-    const int run = page_run ? a.KVH * PS * a.row_bytes : head_run ? PS * a.row_bytes : a.row_bytes;
+    // (a page may have almost 2^31 bytes, so places in it plus a step need the 32nd bit)
+    const uint32_t run = page_run ? a.KVH * PS * a.row_bytes : head_run ? PS * a.row_bytes : a.row_bytes;
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
         const int i = (int)(u / (2 * a.layers)), lp = (int)(u - (int64_t)i * 2 * a.layers);
         char* pool = (lp & 1 ? a.v : a.k) + (int64_t)(lp >> 1) * a.layer;
@@ -437,7 +438,7 @@ paged_compact_move_kernel(PoolArgs a, int PS, const int32_t* __restrict__ ws, in
         char* dst = pool + holes[i] * a.page;
         for (int n = 0; n < runs; ++n) {
             const int64_t off = page_run ? 0 : head_run ? n * a.head : (n / PS) * a.head + (n % PS) * a.tok;
-            for (int b0 = threadIdx.x * 16; b0 < run; b0 += 256 * 16 * kMoveUnroll) {
+            for (uint32_t b0 = threadIdx.x * 16; b0 < run; b0 += 256 * 16 * kMoveUnroll) {
                 u32x4 v[kMoveUnroll];
 #pragma unroll
                 for (int k = 0; k < kMoveUnroll; ++k)

@@ -116,3 +116,19 @@ def test_rows_end_to_end_of_more_units_than_32_bits_name():
     q = torch.ones(B, KVH, HD, dtype=BF, device=DEV)
     c, _ = ops.paged_decode_attention(q, kp, vp, table, _i32([MP * PS] * B), want_kctx=False)
     assert (c == 0.5).all()
+
+
+# ------------------------------------------------------------------ pages
+
+def test_compact_a_page_of_almost_two_gib():
+    """A page of 2^31 - 32768 bytes, the largest that this shape allows."""
+    from loom_amd import ops
+    KVH, PS, HD = 771, 1024, 680
+    assert KVH * PS * HD * 4 == 2 ** 31 - 32768
+    pools = [torch.randint(-2 ** 31, 2 ** 31 - 1, (1, 2, KVH, PS, HD), dtype=torch.int32, device=DEV) for _ in range(2)]
+    want = [p[:, 1].clone() for p in pools]
+    table, refs, used = _i32([[1]]), _i32([0, 1]), _i32([0])
+    ops.paged_compact(pools[0].view(FP), pools[1].view(FP), table, refs, used)
+    assert table.tolist() == [[0]] and refs.tolist() == [1, 0] and int(used) == 1
+    for p, w in zip(pools, want):
+        assert torch.equal(p[:, 0], w) and torch.equal(p[:, 1], w)
