@@ -83,9 +83,10 @@ __device__ __forceinline__ float sum_16_32(float v) {
 }
 
 // The exponents' running reference: it follows the maximum (in powers of two) only
-// where that is 2^8 beyond it.  Weights of up to 2^8 lose nothing in fp32, nor in a
-// 16-bit type's relative step, and the sums are hardly ever rescaled.
-__device__ __forceinline__ float raised(float ref, float most) { return most > ref + 8.0f ? most : ref; }
+// where that is LAG beyond it, so that the sums are hardly ever rescaled.  A factor of
+// 2^8 costs nothing where the weights keep an fp32's range of exponents.
+constexpr float kPgLag = 8.0f;
+__device__ __forceinline__ float raised(float ref, float most, float lag = kPgLag) { return most > ref + lag ? most : ref; }
 
 // Tiles of a row of n tokens; a row of none counts as one, which writes its outputs.
 __device__ __forceinline__ int row_tiles(int n) { return n > 0 ? (n + kPgTile - 1) / kPgTile : 1; }
@@ -213,6 +214,7 @@ __device__ __forceinline__ void plan_walk(const int32_t* lens, int B, int cap, i
 // Element pair helpers by type
 template <typename T> struct Mfma16;
 template <> struct Mfma16<bf16_t> {
+    static constexpr float kLag = kPgLag, kShift = 0.0f;
     __device__ __forceinline__ static pg_f32x4 dot(uint4 a, uint4 b, pg_f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pg_bf16x8, a),
                                                        __builtin_bit_cast(pg_bf16x8, b), c, 0, 0, 0);
@@ -220,6 +222,11 @@ template <> struct Mfma16<bf16_t> {
     __device__ __forceinline__ static uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
 };
 template <> struct Mfma16<f16_t> {
+    // half's exponents end at 2^15 and its normal values at 2^-14, so the reference lies
+    // 2^13 below the maximum it follows and lags by 2^2 at most: weights from 2^-27 of
+    // the largest on keep their 11 bits, and what a smaller one loses is at most 2^-38
+    // of the largest (2^-14 in a row of 2^24 tokens)
+    static constexpr float kLag = 2.0f, kShift = 13.0f;
     __device__ __forceinline__ static pg_f32x4 dot(uint4 a, uint4 b, pg_f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pg_f16x8, a),
                                                       __builtin_bit_cast(pg_f16x8, b), c, 0, 0, 0);
@@ -503,7 +510,7 @@ paged_mfma_kernel(PagedArgs<T> a) {
                     mx = fmaxf(mx, sv[hf][r]);
                 }
             mx = max_16_32(mx);
-            const float mnew = raised(mh, mx);
+            const float mnew = raised(mh, mx - M::kShift, M::kLag);
             const float corr = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mh - mnew);
             float ls = 0.0f, pv[2][4];
 #pragma unroll
@@ -518,7 +525,8 @@ paged_mfma_kernel(PagedArgs<T> a) {
             const bool rescale = corr != 1.0f && mh != -INFINITY;      // (before, the sums are zero)
             mh = mnew;
             // the weights enter the products rounded to the storage type (half a step of
-            // it, relative, per weight: below the rounding of the outputs)
+            // it, relative, per weight, down to Mfma16's smallest: below the rounding of
+            // the outputs); their sum l is that of the unrounded ones
             const uint4 pa = make_uint4(M::pack(pv[0][0], pv[0][1]), M::pack(pv[0][2], pv[0][3]),
                                         M::pack(pv[1][0], pv[1][1]), M::pack(pv[1][2], pv[1][3]));
             if (__any(rescale)) {

@@ -132,3 +132,38 @@ def test_compact_a_page_of_almost_two_gib():
     assert table.tolist() == [[0]] and refs.tolist() == [1, 0] and int(used) == 1
     for p, w in zip(pools, want):
         assert torch.equal(p[:, 0], w) and torch.equal(p[:, 1], w)
+
+
+@pytest.mark.parametrize("dt", [BF, HF, FP])
+@pytest.mark.parametrize("n", [700, 131072, 1 << 20])
+@pytest.mark.parametrize("down", [14.3, 20.3, 24.6, 25.1, 28.7])
+def test_one_dominant_token_and_a_long_tail(dt, n, down):
+    """All tokens but one have a weight 2^-down of the largest, of value one: their sum
+    is what a long row keeps of them, however small each of them is."""
+    from loom_amd import ops
+    HD, PS = 64, 64
+    MP = n // PS + 1
+    kp, vp = torch.zeros(3, 1, PS, HD), torch.ones(3, 1, PS, HD)
+    q = torch.zeros(3, 2, HD)
+    q[..., 0] = torch.tensor([8.0, 7.75])            # the score is k / sqrt(64) times this
+    kp[1, 0, 5, 0] = kp[2, 0, 50, 0] = down * math.log(2)
+    vp[1, 0, 5] = vp[2, 0, 50] = 0.0
+    table = torch.zeros(3, MP, dtype=torch.int32)
+    table[0, 0], table[1, (n - 1) // PS - 1], table[2, MP // 2] = 1, 2, 1     # early, at the end, in the middle
+    kp, vp, q = kp.to(DEV, dt), vp.to(DEV, dt), q.to(DEV, dt)
+    c, kx = ops.paged_decode_attention(q, kp, vp, table.to(DEV), _i32([n] * 3))
+    top = kp[1, 0, 5, 0].double()
+    s = q[:, :, 0].double() * top / 8
+    rest = (n - 1) * torch.exp(-s)
+    want_c, want_k = (rest / (1 + rest)).cpu(), (top / (1 + rest)).cpu()
+    # roundings: of the output and of each weight (half a step each; of half's small ones
+    # 2^-38 of the largest), of the score (a product, 64 additions, the scaling; its
+    # exponential's argument and result), and one per tile of 32 tokens and per chunk of
+    # the sums, in the numerator and the denominator
+    half, u = torch.finfo(dt).eps / 2, 2.0 ** -24
+    rel = half + (0 if dt == FP else half) + 2 * (72 * float(s.max()) + 8) * u + 2 * (n / 32 + 512) * u
+    least = n * 2.0 ** -38 + 2.0 ** -24 if dt == HF else 2.0 ** -126
+    over_c = ((c.cpu().double() - want_c[..., None]).abs() / (rel * want_c + least)[..., None]).max()
+    over_k = ((kx[..., 0].cpu().double() - want_k).abs() / (rel * want_k)).max()
+    assert float(over_c) <= 1 and float(over_k) <= 1
+    assert not kx[..., 1:].float().any()
