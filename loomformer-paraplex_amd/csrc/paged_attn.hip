@@ -284,7 +284,8 @@ struct Rope8 {
 // The end of a chunk: the NW waves' (m, l, C, Kctx) of nh heads from LDS (wave w,
 // head j: wm[j][w], wl[j][w], and wacc + ((w * NH + j) * 2 + which) * HD)
 // joined into the chunk's record, or into the outputs when it is the row's only
-// chunk.  A sum of 0 (no token) gives zeros; NaN weights stay NaN.
+// chunk.  A row of no token gives zeros; NaN weights stay NaN, and a sum of 0 (every
+// score is -inf) gives NaN, as the softmax does.
 template <int NW, typename T>
 __device__ __forceinline__ void paged_finish(const PagedArgs<T>& a, const PlanItem& it, int h0, int nh,
                                              int NH, int HD, bool kctx, bool broken, const float* wm,
@@ -309,9 +310,10 @@ __device__ __forceinline__ void paged_finish(const PagedArgs<T>& a, const PlanIt
         if (broken) l = NAN;
         if (it.nchunk == 1) {
             const float inv = 1.0f / l;
+            const bool none = it.tokens <= 0 && !broken;
             T* out = (which ? a.k_out : a.c_out) + (int64_t)it.row * a.out_ld + (int64_t)h * HD + d;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) st(out + i, l == 0.0f ? 0.0f : c[i] * inv);
+            for (int i = 0; i < 4; ++i) st(out + i, none ? 0.0f : c[i] * inv);
         } else {
             const int64_t r = (int64_t)(it.item0 + it.chunk) * a.QH + h;
             *reinterpret_cast<pg_f32x4*>(a.rec + (r * 2 + which) * HD + d) = c;
@@ -887,7 +889,7 @@ paged_join_kernel(PagedArgs<T> a) {
             x = fmaf(wacc[w][k], f, x);
         }
         T* out = (k < HD ? a.c_out : a.k_out) + (int64_t)it.row * a.out_ld + (int64_t)h * HD + (k < HD ? k : k - HD);
-        st(out, l == 0.0f ? 0.0f : x / l);
+        st(out, x / l);                              // (a row of more than one chunk has tokens)
     }
 }
 

@@ -118,6 +118,30 @@ def test_rows_end_to_end_of_more_units_than_32_bits_name():
     assert (c == 0.5).all()
 
 
+@pytest.mark.parametrize("dt,HD", [(BF, 64), (HF, 96), (FP, 64), (HF, 8), (BF, 256)])
+@pytest.mark.parametrize("n", [1, 45, 3000])
+def test_scores_of_minus_infinity(dt, HD, n):
+    """Row 0: every score is -inf, the softmax of which is NaN; row 1: all but the last;
+    row 2: none; row 3 holds no token, row 4 no sequence: zeros."""
+    from loom_amd import ops
+    PS, MP = 16, -(-n // 16)
+    g = torch.Generator().manual_seed(n)
+    kp, vp = torch.randn(3 * MP, 1, PS, HD, generator=g), torch.randn(3 * MP, 1, PS, HD, generator=g)
+    q = torch.randn(5, 2, HD, generator=g)
+    q[:2] = 0.0
+    q[:2, :, 1] = 1.0
+    kp[:2 * MP, :, :, 1] = -math.inf
+    kp[MP + (n - 1) // PS, :, (n - 1) % PS, 1] = 0.5
+    table = torch.cat([torch.arange(3 * MP).view(3, MP), torch.zeros(2, MP).long()]).int()
+    kp, vp, q = kp.to(DEV, dt), vp.to(DEV, dt), q.to(DEV, dt)
+    c, kx = ops.paged_decode_attention(q, kp, vp, table.to(DEV), _i32([n, n, n, 0, -1]))
+    assert torch.isnan(c[0].float()).all() and torch.isnan(kx[0].float()).all()
+    last = vp[MP + (n - 1) // PS, 0, (n - 1) % PS]
+    assert torch.equal(c[1], last.expand(2, HD))
+    assert torch.isfinite(c[2].float()).all() and torch.isfinite(kx[2].float()).all()
+    assert not c[3:].float().any() and not kx[3:].float().any()
+
+
 # ------------------------------------------------------------------ pages
 
 def test_compact_a_page_of_almost_two_gib():
