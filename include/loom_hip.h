@@ -771,7 +771,8 @@ int loom_decode_epilogue(int dtype, const void* stage_k, const void* stage_v, vo
  * [0, n_pages) are no page.  refs[p] counts the table entries that hold page p
  * (0: the page is free).  table, lens, refs, parent: int32 on the device, read
  * there, so that every call can be captured into a graph.  Pages may be shared
- * by rows; tokens behind lens[r] in them are never read.  At most 1024 rows and
+ * by rows; tokens behind lens[r] in them are never read, and a row's last tokens
+ * are dropped by lowering lens[r].  At most 1024 rows and
  * 2^24 tokens per row (max_pages * page_size).
  * ------------------------------------------------------------------------ */
 
@@ -818,7 +819,10 @@ int loom_paged_decode_attention(int dtype, const void* q, int64_t q_ld, const vo
  *   tokens lens[r] .. lens[r] + n_new - 1 are made writable: missing pages are
  *     taken from the free ones, and a partly filled last page that is held more
  *     than once is copied (its tokens below lens[r], all layers) to a free page,
- *     by each of its rows in row order for as long as others hold it.  Free pages
+ *     by each of its rows in row order for as long as others hold it.  A page in
+ *     the place of these tokens that holds none of the row's and that others hold
+ *     (lens[r] was lowered) is let go, as are the row's pages behind it up to the
+ *     last of these tokens, and another takes its place.  Free pages
  *     go lowest id first, in row order, a row's copy before its new pages.
  * status[0] is raised by the number of pages that could not be had (a row whose
  * copy failed loses its last page: its outputs are NaN, never another row's

@@ -4,8 +4,9 @@
 //
 // A pool has n_pages pages; refs[p] counts the table entries that hold page p
 // (0: free).  Row r holds lens[r] tokens (-1: no sequence); its table entries
-// below ceil(lens[r] / PS) are its pages, entries behind them are -1 or pages
-// reserved ahead, which only this row holds.
+// below ceil(lens[r] / PS) are its pages, entries behind them are -1, pages
+// reserved ahead, which only this row holds, or, where the caller lowered lens[r],
+// pages that others may hold too.
 #include "loom_common.h"
 
 namespace loom {
@@ -102,7 +103,8 @@ constexpr int kScanIds = 4;         // groups of four page ids per thread and ro
 // lens[r] + n_new - 1 get pages of their own: where the row's last page is
 // partly filled and held more than once, row order decides who copies it (each
 // row in turn copies while others hold it), and pages that are missing are
-// appended.  The free pages are taken lowest id first, in row order, by one
+// appended.  A row lets go of pages in their places that others hold too (they hold
+// none of its tokens), and of what lies behind the first of them.  The free pages are taken lowest id first, in row order, by one
 // scan over refs: a free page's rank among the free ones names its row.
 // Bound by the latency of its stages, each a pass over the rows or over refs with a
 // block scan behind it: 256 rows and 17152 pages 8.6 us.  One block and not a launch
@@ -118,15 +120,22 @@ paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* _
     extern __shared__ int32_t old[];                 // FORK: [R][MP]
     __shared__ __align__(16) int32_t tail[kPcMaxRows];
     __shared__ int32_t base[kPcMaxRows], slot0[kPcMaxRows], len_of[kPcMaxRows];
-    __shared__ int waves[16][2];
+    __shared__ int waves[16][2], ahead;              // ahead: a row has a page behind its tokens
     const int r = threadIdx.x, PS = 1 << log_ps;
+    // a page's count where this block may have changed it since it was last read
+    auto count_of = [&](int64_t id) __attribute__((always_inline)) {
+        return __hip_atomic_load(refs + id, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    };
     // bit 4 j + e: page seg + 4096 j + 4 r + e is free
-    auto free_ids = [&](int64_t seg) __attribute__((always_inline)) {
+    auto free_ids = [&](int64_t seg, bool changed) __attribute__((always_inline)) {
         uint32_t mask = 0;
 #pragma unroll
         for (int j = 0; j < kScanIds; ++j) {
             const int64_t id = seg + 4096 * j + 4 * r;
-            if (id + 4 <= NP) {
+            if (changed) {
+                for (int e = 0; e < 4 && id + e < NP; ++e)
+                    if (count_of(id + e) <= 0) mask |= 1u << (4 * j + e);
+            } else if (id + 4 <= NP) {
                 int4 q;                              // one load, aligned to a word
                 __builtin_memcpy(&q, refs + id, 16);
                 mask |= (uint32_t)((q.x <= 0) | (q.y <= 0) << 1 | (q.z <= 0) << 2 | (q.w <= 0) << 3) << (4 * j);
@@ -138,7 +147,8 @@ paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* _
         return mask;
     };
     uint32_t mask = 0;                               // of the first pages, with the row's first loads
-    if constexpr (!FORK) mask = free_ids(0);
+    if constexpr (!FORK) mask = free_ids(0, false);
+    if (r == 0) ahead = 0;
     // (r + 1024 k) as (row, column), without a division per entry
     const int step_r = 1024 / MP, step_c = 1024 - step_r * MP;
     int len = -1, p = -1;
@@ -196,20 +206,36 @@ paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* _
     const int cap = MP * PS;
     const int n = len >= 0 ? max(min(n_new, cap - len), 0) : 0;
     if (len >= 0 && n < n_new) short_of = 1;
-    int miss0 = 0, nmiss = 0;
+    int miss0 = 0, last = -1;
     if (n > 0) {
         if (len & (PS - 1)) {
             page = entry(len >> log_ps);
             if (!in_range(page, NP)) page = -1;
         }
-        const int last = (len + n - 1) >> log_ps;
+        last = (len + n - 1) >> log_ps;
         miss0 = (len + PS - 1) >> log_ps;
-        while (miss0 <= last && in_range(entry(miss0), NP)) ++miss0;
-        nmiss = last + 1 - miss0;
+        bool any = false;
+#pragma unroll 4
+        for (int s = miss0; s <= last; ++s) any |= in_range(entry(s), NP);
+        if (any) ahead = 1;
     }
     tail[r] = page;
     __syncthreads();                                 // (and the fork's changes of refs are done)
-    const int held_by = page >= 0 ? refs[page] : 0;
+    const bool let_go = ahead != 0;
+    if (let_go) {                                    // (the same in all threads)
+        while (miss0 <= last && in_range(entry(miss0), NP) && count_of(entry(miss0)) <= 1) ++miss0;
+        __syncthreads();                             // every row goes by the counts as they were
+        for (int s = miss0; s <= last; ++s) {
+            const int e = entry(s);
+            if (!in_range(e, NP)) continue;
+            row[s] = -1;
+            atomicSub(refs + e, 1);
+        }
+        __syncthreads();
+        if constexpr (!FORK) mask = free_ids(0, true);
+    }
+    const int nmiss = last + 1 - miss0;
+    const int held_by = page >= 0 ? count_of(page) : 0;
     // rows before this one with the same tail: `share` threads count for a row
     int share = 16;
     while (share > 1 && R * share > 1024) share >>= 1;
@@ -244,7 +270,7 @@ paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* _
     int given = 0;                                   // free pages handed out so far
     __syncthreads();
     for (int64_t seg = 0; seg < NP && given < need; seg += 1024 * 4 * kScanIds) {
-        if (FORK || seg > 0) mask = free_ids(seg);
+        if (FORK || seg > 0) mask = free_ids(seg, let_go);
         int count[2] = {0, 0}, before[2], all[2];    // 16 bits per j
 #pragma unroll
         for (int j = 0; j < kScanIds; ++j) count[j / 2] |= __popc((mask >> (4 * j)) & 15u) << (16 * (j & 1));

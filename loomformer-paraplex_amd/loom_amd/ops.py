@@ -606,7 +606,8 @@ def paged_update(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tens
     kv_heads, page_size, head_dim]: row r takes the pages and length of row
     parent[r] (int32; outside [0, rows): row r becomes empty), lens += advance,
     and the next n_new tokens of every row are made writable (missing pages
-    taken from the free ones, a shared last page copied).  refs [pages] counts
+    taken from the free ones, a shared last page copied, shared pages behind a
+    row's tokens, left by a lens that was lowered, replaced).  refs [pages] counts
     the holders of each page; status [1] is raised where pages ran out.  All
     bookkeeping is on the device."""
     (_host_module or _host()).paged_update(k_pages, v_pages, table, lens, refs, status, parent, n_new, advance)

@@ -24,7 +24,7 @@ class PagedKVCache:
       refs  [n_pages] int32           table entries that hold each page
       status [1] int32                pages that could not be had (see check)
 
-    n_pages defaults to what rows that share nothing need, which never runs out.
+    A row's last tokens are dropped by lowering its entry of lens.  n_pages defaults to what rows that share nothing need, which never runs out.
     """
 
     def __init__(self, layers: int, rows: int, max_len: int, kv_heads: int, head_dim: int, dtype: torch.dtype,

@@ -75,6 +75,17 @@ def update(k_pages, v_pages, table, lens, refs, parent=None, n_new=0, advance=0)
                     if valid(b):
                         rf[b] += 1
     ln = [n + advance if n >= 0 else -1 for n in ln]
+    held, gone = list(rf), []
+    for r in range(R):                                # pages behind the tokens that are not the row's alone
+        n = min(n_new, MP * PS - ln[r]) if ln[r] >= 0 else 0
+        kept = True
+        for s in range(-(-ln[r] // PS), (ln[r] + n - 1) // PS + 1) if n > 0 else ():
+            kept = kept and valid(rows[r][s]) and held[rows[r][s]] <= 1
+            if not kept and valid(rows[r][s]):
+                gone.append(rows[r][s])
+                rows[r][s] = -1
+    for p in gone:
+        rf[p] -= 1
     free = [p for p in range(NP) if rf[p] <= 0]
     for r in range(R):
         if ln[r] < 0 or n_new == 0:

@@ -191,3 +191,68 @@ def test_one_dominant_token_and_a_long_tail(dt, n, down):
     over_k = ((kx[..., 0].cpu().double() - want_k).abs() / (rel * want_k)).max()
     assert float(over_c) <= 1 and float(over_k) <= 1
     assert not kx[..., 1:].float().any()
+
+
+def _shared_rows(g, R, MP, PS, tokens, NP, KVH=1, HD=8, dt=FP):
+    """R rows that hold the same pages of `tokens` tokens."""
+    n = -(-tokens // PS)
+    order = torch.randperm(NP, generator=g)[:n].int()
+    table = torch.full((R, MP), -1, dtype=torch.int32)
+    table[:, :n] = order
+    refs = torch.zeros(NP, dtype=torch.int32)
+    refs[order.long()] = R
+    pools = [torch.randn(2, NP, KVH, PS, HD, generator=g).to(dt) for _ in range(2)]
+    return [t.to(DEV) for t in (*pools, table, torch.full((R,), tokens, dtype=torch.int32), refs)]
+
+
+def _update_as_the_oracle(s, **kw):
+    """paged_update against the plain restatement; every page of the tokens made
+    writable is its row's alone."""
+    from loom_amd import ops
+    status, PS = _i32([0]), s[0].shape[3]
+    par = kw.get("parent")
+    want = ref.update(*[t.cpu() for t in s], **dict(kw, parent=None if par is None else par.cpu()))
+    ops.paged_update(*s, status, **kw)
+    for name, a, b in zip(("k", "v", "table", "lens", "refs"), s, want):
+        assert torch.equal(a.cpu(), b), (name, kw)
+    assert int(status) == want[5]
+    t, refs, lens = s[2].tolist(), s[4].tolist(), s[3].tolist()
+    assert refs == torch.bincount(s[2].cpu()[s[2].cpu() >= 0].long(), minlength=len(refs)).tolist()
+    for r, n in enumerate(lens):
+        if n >= 0 and kw.get("n_new", 0) > 0:
+            for at in range(n // PS, min((n + kw["n_new"] - 1) // PS + 1, len(t[r]))):
+                assert t[r][at] < 0 or refs[t[r][at]] == 1, (r, at, kw)
+
+
+@pytest.mark.parametrize("lens", [[64, 32], [64, 40], [32, 33], [0, 64], [1, 0], [48, 16], [64, -1]])
+@pytest.mark.parametrize("n_new", [1, 20, 48])
+@pytest.mark.parametrize("forked", [False, True])
+def test_update_behind_lowered_lengths(lens, n_new, forked):
+    """Two rows of the same four pages, whose last tokens are dropped: what is made
+    writable is no page that the other holds."""
+    s = _shared_rows(torch.Generator().manual_seed(1), 2, 8, 16, 64, 40)
+    s[3].copy_(_i32(lens))
+    _update_as_the_oracle(s, n_new=n_new, **({"parent": _i32([0, 1])} if forked else {}))
+    _update_as_the_oracle(s, n_new=1, advance=n_new, parent=_i32([1, 0]))
+
+
+@pytest.mark.parametrize("R,MP,pool", [(6, 9, 200), (6, 9, 25), (300, 30, 20000), (300, 30, 3000)])
+@pytest.mark.parametrize("seed", [1, 2])
+def test_update_random_walk_with_lowered_lengths(R, MP, pool, seed):
+    """Forks, advances, reservations and dropped tokens in a row, in pools that suffice
+    and that do not; the table's fork in its own launch and not."""
+    g = torch.Generator().manual_seed(seed)
+    s = _shared_rows(g, R, MP, 16, 50, pool)
+    for step in range(10):
+        kw = dict(n_new=int(torch.randint(0, 60, (1,), generator=g)), advance=0)
+        if step % 2:
+            par = torch.randint(-1, R + 1, (R,), generator=g).int()
+            keep = torch.rand(R, generator=g) < 0.4
+            par[keep] = torch.arange(R).int()[keep]
+            kw["parent"] = par.to(DEV)
+        _update_as_the_oracle(s, **kw)
+        # some of the reserved tokens are written, and some rows drop tokens again
+        add = torch.randint(0, kw["n_new"] + 1, (R,), generator=g).to(DEV)
+        down = (torch.randint(0, 40, (R,), generator=g) * (torch.rand(R, generator=g) < 0.5)).to(DEV)
+        grown = torch.minimum(s[3] + add, torch.tensor(MP * 16, device=DEV))
+        s[3].copy_(torch.where(s[3] >= 0, (grown - down).clamp(min=0), s[3]))
