@@ -507,7 +507,7 @@ static int table_checks(const char* who, const int32_t* table, int64_t ld, int64
     LOOM_CHECK(MP >= 1 && MP * PS <= ((int64_t)1 << 24) && ld >= MP,
                "%s: the table must hold 1 page to 2^24 tokens per row (max_pages=%lld, row stride %lld)", who,
                (long long)MP, (long long)ld);
-    LOOM_CHECK(table != nullptr, "%s: a required pointer is NULL", who);
+    LOOM_CHECK(table != nullptr || R == 0, "%s: a required pointer is NULL", who);
     return LOOM_OK;
 }
 
@@ -532,7 +532,7 @@ extern "C" int loom_paged_update(int dtype, void* k_pages, void* v_pages, int64_
                              head_stride, n_pages, page_size, KVH, HD, &a))
         return rc;
     if (int rc = table_checks(who, table, table_ld, max_pages, page_size, rows)) return rc;
-    LOOM_CHECK(lens && refs && status, "%s: a required pointer is NULL", who);
+    LOOM_CHECK((lens && refs && status) || rows == 0, "%s: a required pointer is NULL", who);
     LOOM_CHECK(n_new >= 0 && n_new <= max_pages * page_size && advance >= 0 && advance <= max_pages * page_size,
                "%s: n_new=%lld and advance=%lld must lie in 0..%lld", who, (long long)n_new, (long long)advance,
                (long long)(max_pages * page_size));
@@ -583,7 +583,7 @@ extern "C" int loom_paged_write(int dtype, void* k_pages, void* v_pages, int64_t
         return rc;
     if (int rc = table_checks(who, table, table_ld, max_pages, page_size, rows)) return rc;
     const int64_t es = dtype == LOOM_F32 ? 4 : 2;
-    LOOM_CHECK(k_rows && v_rows && first && last, "%s: a required pointer is NULL", who);
+    LOOM_CHECK((k_rows && v_rows && first && last) || rows == 0, "%s: a required pointer is NULL", who);
     LOOM_CHECK(src_tokens >= 0 && src_tokens <= ((int64_t)1 << 24) && src_token_stride >= HD &&
                    src_layer_stride >= 0 && src_row_stride >= 0 && src_head_stride >= 0,
                "%s: bad source shape", who);

@@ -256,3 +256,18 @@ def test_update_random_walk_with_lowered_lengths(R, MP, pool, seed):
         down = (torch.randint(0, 40, (R,), generator=g) * (torch.rand(R, generator=g) < 0.5)).to(DEV)
         grown = torch.minimum(s[3] + add, torch.tensor(MP * 16, device=DEV))
         s[3].copy_(torch.where(s[3] >= 0, (grown - down).clamp(min=0), s[3]))
+
+
+def test_compact_a_cache_of_no_rows():
+    """Pages that refs count but no table holds move too."""
+    from loom_amd import ops
+    g = torch.Generator().manual_seed(2)
+    pools = [torch.randn(2, 7, 2, 16, 32, generator=g).to(DEV, BF) for _ in range(2)]
+    want = [p.clone() for p in pools]
+    refs, used = _i32([0, 2, 0, 0, 1, 0, 1]), _i32([0])
+    for p in want:
+        p[:, 0], p[:, 2] = p[:, 4].clone(), p[:, 6].clone()
+    table = torch.empty(0, 5, dtype=torch.int32, device=DEV)
+    ops.paged_compact(*pools, table, refs, used)
+    assert refs.tolist() == [1, 2, 1, 0, 0, 0, 0] and int(used) == 3
+    assert torch.equal(pools[0], want[0]) and torch.equal(pools[1], want[1])
