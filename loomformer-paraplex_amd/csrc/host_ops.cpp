@@ -118,21 +118,35 @@ Table table_of(const Args& a, int i, c10::Device dev) {
     return {(int32_t*)t.data_ptr(), t.size(0), t.size(0) > 1 ? t.stride(0) : std::max(w, t.stride(0)), w};
 }
 
+// The stride of a dimension of one entry says nothing: it is not compared, and
+// `one` stands for it.
+int64_t stride_of(const at::Tensor& t, int64_t d, int64_t one = 0) { return t.size(d) > 1 ? t.stride(d) : one; }
+
+bool same_layout(const at::Tensor& a, const at::Tensor& b) {
+    if (a.sizes() != b.sizes()) return false;
+    for (int64_t d = 0; d < a.dim(); ++d)
+        if (stride_of(a, d) != stride_of(b, d)) return false;
+    return true;
+}
+
+// layer (0 without one), page, token and head strides
 struct Pools {
     const at::Tensor &k, &v;
     int dtype;
     c10::Device dev;
+    int64_t layer, page, tok, head;
 };
 
 Pools pools_of(const Args& a, int i, int64_t dim) {
     const at::Tensor &k = a.tensor(i, "k_pages"), &v = a.tensor(i + 1, "v_pages");
-    CHECK(k.dim() == dim && k.sizes() == v.sizes() && k.strides() == v.strides() && k.stride(dim - 1) == 1, a.name,
+    CHECK(k.dim() == dim && v.dim() == dim && same_layout(k, v) && stride_of(k, dim - 1, 1) == 1, a.name,
           ": k_pages and v_pages must be [", dim == 5 ? "layers, " : "",
           "pages, kv_heads, page_size, head_dim] tensors of the same layout with dense heads");
     const int code = dtype_code(k);
     CHECK(code >= 0 && v.scalar_type() == k.scalar_type() && v.device() == k.device(), a.name,
           ": k_pages and v_pages must be float32, bfloat16 or float16 and have one dtype and one device");
-    return {k, v, code, k.device()};
+    return {k, v, code, k.device(), dim == 5 ? stride_of(k, 0) : 0, stride_of(k, dim - 4), stride_of(k, dim - 2, k.size(dim - 1)),
+            stride_of(k, dim - 3)};
 }
 
 at::Tensor bytes(int64_t n, c10::Device dev) {
@@ -215,12 +229,12 @@ PyObject* attention(const Args& a, bool step) {
     const int32_t* lp = (const int32_t*)lens.data_ptr();
     launch([&] {
         if (step)
-            return loom_paged_decode_step(p.dtype, q.data_ptr(), ld, p.k.data_ptr(), p.v.data_ptr(), p.k.stride(0),
-                                          p.k.stride(2), p.k.stride(1), NP, PS, t.p, t.ld, t.pages, lp,
+            return loom_paged_decode_step(p.dtype, q.data_ptr(), ld, p.k.data_ptr(), p.v.data_ptr(), p.page, p.tok,
+                                          p.head, NP, PS, t.p, t.ld, t.pages, lp,
                                           (const float*)cos->data_ptr(), (const float*)sin->data_ptr(), cos->size(0),
                                           qo.data_ptr(), c.data_ptr(), kxp, QH * HD, w, need, B, QH, KVH, HD, st);
-        return loom_paged_decode_attention(p.dtype, q.data_ptr(), ld, p.k.data_ptr(), p.v.data_ptr(), p.k.stride(0),
-                                           p.k.stride(2), p.k.stride(1), NP, PS, t.p, t.ld, t.pages, lp, c.data_ptr(),
+        return loom_paged_decode_attention(p.dtype, q.data_ptr(), ld, p.k.data_ptr(), p.v.data_ptr(), p.page, p.tok,
+                                           p.head, NP, PS, t.p, t.ld, t.pages, lp, c.data_ptr(),
                                            kxp, QH * HD, w, need, B, QH, KVH, HD, st);
     });
     return step ? list_of({&c, &kx, &qo}) : list_of({&c, &kx});
@@ -253,8 +267,8 @@ PyObject* paged_update(PyObject* const* x, Py_ssize_t n) {
     const at::Tensor ws = bytes(need, p.dev);
     void* st = stream_of(p.dev.index());
     launch([&] {
-        return loom_paged_update(p.dtype, p.k.data_ptr(), p.v.data_ptr(), p.k.size(0), p.k.stride(0), p.k.stride(1),
-                                 p.k.stride(3), p.k.stride(2), p.k.size(1), p.k.size(3), p.k.size(2), p.k.size(4), t.p,
+        return loom_paged_update(p.dtype, p.k.data_ptr(), p.v.data_ptr(), p.k.size(0), p.layer, p.page, p.tok, p.head,
+                                 p.k.size(1), p.k.size(3), p.k.size(2), p.k.size(4), t.p,
                                  t.ld, t.pages, (int32_t*)lens.data_ptr(), (int32_t*)refs.data_ptr(),
                                  (int32_t*)status.data_ptr(), parent, n_new, advance, ws.data_ptr(), need, t.rows, st);
     });
@@ -268,9 +282,9 @@ PyObject* paged_write(PyObject* const* x, Py_ssize_t n) {
     const Table t = table_of(a, 2, p.dev);
     const at::Tensor &kr = a.tensor(3, "k_rows"), &vr = a.tensor(4, "v_rows");
     CHECK(kr.device() == p.dev && vr.device() == p.dev && kr.scalar_type() == p.k.scalar_type() &&
-              vr.scalar_type() == p.k.scalar_type() && kr.dim() == 5 && kr.sizes() == vr.sizes() &&
-              kr.strides() == vr.strides() && kr.size(0) == p.k.size(0) && kr.size(1) == t.rows &&
-              kr.size(2) == p.k.size(2) && kr.size(4) == p.k.size(4) && kr.stride(4) == 1,
+              vr.scalar_type() == p.k.scalar_type() && kr.dim() == 5 && vr.dim() == 5 && same_layout(kr, vr) &&
+              kr.size(0) == p.k.size(0) && kr.size(1) == t.rows &&
+              kr.size(2) == p.k.size(2) && kr.size(4) == p.k.size(4) && stride_of(kr, 4, 1) == 1,
           a.name, ": k_rows and v_rows must be [layers, rows, kv_heads, positions, head_dim] tensors of the pools' "
                   "dtype and one layout");
     const at::Tensor &first = i32(a, 5, "first", t.rows, p.dev), &last = i32(a, 6, "last", t.rows, p.dev);
@@ -278,10 +292,10 @@ PyObject* paged_write(PyObject* const* x, Py_ssize_t n) {
     OnDevice on(p.dev.index());
     void* st = stream_of(p.dev.index());
     launch([&] {
-        return loom_paged_write(p.dtype, p.k.data_ptr(), p.v.data_ptr(), p.k.size(0), p.k.stride(0), p.k.stride(1),
-                                p.k.stride(3), p.k.stride(2), p.k.size(1), p.k.size(3), p.k.size(2), p.k.size(4), t.p,
-                                t.ld, t.pages, kr.data_ptr(), vr.data_ptr(), kr.stride(0), kr.stride(1), kr.stride(2),
-                                kr.stride(3), kr.size(3), (const int32_t*)first.data_ptr(),
+        return loom_paged_write(p.dtype, p.k.data_ptr(), p.v.data_ptr(), p.k.size(0), p.layer, p.page, p.tok, p.head,
+                                p.k.size(1), p.k.size(3), p.k.size(2), p.k.size(4), t.p,
+                                t.ld, t.pages, kr.data_ptr(), vr.data_ptr(), stride_of(kr, 0), stride_of(kr, 1),
+                                stride_of(kr, 2), stride_of(kr, 3, kr.size(4)), kr.size(3), (const int32_t*)first.data_ptr(),
                                 (const int32_t*)last.data_ptr(), t.rows, st);
     });
     Py_RETURN_NONE;
@@ -298,8 +312,8 @@ PyObject* paged_compact(PyObject* const* x, Py_ssize_t n) {
     const at::Tensor ws = bytes(need, p.dev);
     void* st = stream_of(p.dev.index());
     launch([&] {
-        return loom_paged_compact(p.dtype, p.k.data_ptr(), p.v.data_ptr(), p.k.size(0), p.k.stride(0), p.k.stride(1),
-                                  p.k.stride(3), p.k.stride(2), p.k.size(1), p.k.size(3), p.k.size(2), p.k.size(4), t.p,
+        return loom_paged_compact(p.dtype, p.k.data_ptr(), p.v.data_ptr(), p.k.size(0), p.layer, p.page, p.tok, p.head,
+                                  p.k.size(1), p.k.size(3), p.k.size(2), p.k.size(4), t.p,
                                   t.ld, t.pages, (int32_t*)refs.data_ptr(), (int32_t*)used.data_ptr(), ws.data_ptr(),
                                   need, t.rows, st);
     });

@@ -271,3 +271,41 @@ def test_compact_a_cache_of_no_rows():
     ops.paged_compact(*pools, table, refs, used)
     assert refs.tolist() == [1, 2, 1, 0, 0, 0, 0] and int(used) == 3
     assert torch.equal(pools[0], want[0]) and torch.equal(pools[1], want[1])
+
+
+# ------------------------------------------------------------------ layouts
+
+def _odd(t, d):
+    """The same tensor with another stride in its dimension d of one entry."""
+    assert t.shape[d] == 1
+    return t.as_strided(t.shape, [s + 3 if k == d else s for k, s in enumerate(t.stride())], t.storage_offset())
+
+
+def test_strides_of_dimensions_of_one_entry_say_nothing():
+    from loom_amd import ops
+    g = torch.Generator().manual_seed(4)
+    for L, NP, KVH in ((1, 6, 2), (2, 1, 2), (2, 6, 1)):
+        k, v = (torch.randn(L, NP, KVH, 16, 32, generator=g).to(DEV, BF) for _ in range(2))
+        k2, v2 = k.clone(), v.clone()
+        for d in range(3):
+            if k2.shape[d] == 1:
+                v2 = _odd(v2, d)
+        n = 10 if NP == 1 else 30
+        start = lambda: [torch.full((1, 3), -1, dtype=torch.int32, device=DEV), _i32([0]), _i32([0] * NP), _i32([0])]  # noqa: E731
+        rows = [torch.randn(L, 1, KVH, 40, 32, generator=g).to(DEV, BF) for _ in range(2)]
+        q = torch.randn(1, 4, 32, generator=g).to(DEV, BF)
+        out = []
+        for kp, vp, kr, vr in ((k, v, *rows), (k2, v2, rows[0], _odd(rows[1], 1))):
+            table, lens, refs, status = start()
+            ops.paged_update(kp, vp, table, lens, refs, status, n_new=n)
+            ops.paged_write(kp, vp, table, kr, vr, _i32([0]), _i32([n]))
+            used = _i32([0])
+            ops.paged_compact(kp, vp, table, refs, used)
+            out.append([kp, vp, table, used, *ops.paged_decode_attention(q, kp[-1], vp[-1], table, _i32([n]))])
+        assert int(out[0][3]) == -(-n // 16)
+        for a, b in zip(*out):
+            assert torch.equal(a, b)
+        one = [r[:, :, :, 4:5].contiguous() for r in rows]      # a source of one position
+        for kp, vp, kr, vr in ((k, v, *one), (k2, v2, _odd(one[0], 3), one[1])):
+            ops.paged_write(kp, vp, out[0][2], kr, vr, _i32([0]), _i32([1]))
+        assert torch.equal(k, k2) and torch.equal(v, v2)
