@@ -1043,10 +1043,10 @@ static int paged_call(const char* who, int dtype, const PagedCall& c, void* stre
     LOOM_CHECK(c.page_size >= 16 && c.page_size <= 1024 && (c.page_size & (c.page_size - 1)) == 0,
                "%s: page_size must be a power of two from 16 to 1024, got %lld", who, (long long)c.page_size);
     LOOM_CHECK(c.n_pages >= 1 && c.n_pages < ((int64_t)1 << 31), "%s: bad n_pages %lld", who, (long long)c.n_pages);
-    LOOM_CHECK(c.max_pages >= 1 && c.max_pages * c.page_size <= ((int64_t)1 << 24) && c.table_ld >= c.max_pages,
+    LOOM_CHECK(c.max_pages >= 1 && c.max_pages <= ((int64_t)1 << 24) / c.page_size && c.table_ld >= c.max_pages,
                "%s: the table must hold 1 page to 2^24 tokens per row (max_pages=%lld, row stride %lld)", who,
                (long long)c.max_pages, (long long)c.table_ld);
-    LOOM_CHECK(c.token_stride >= c.HD && c.token_stride * 16 * es < ((int64_t)1 << 31) && c.page_stride >= 0 &&
+    LOOM_CHECK(c.token_stride >= c.HD && c.token_stride < ((int64_t)1 << 31) / (16 * es) && c.page_stride >= 0 &&
                    c.head_stride >= 0,
                "%s: bad page strides", who);
     LOOM_CHECK((c.token_stride * es) % 16 == 0 && (c.page_stride * es) % 16 == 0 && (c.head_stride * es) % 16 == 0 &&

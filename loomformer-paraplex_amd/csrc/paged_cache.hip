@@ -504,7 +504,7 @@ static int pool_checks(const char* who, int dtype, const void* k, const void* v,
 
 static int table_checks(const char* who, const int32_t* table, int64_t ld, int64_t MP, int64_t PS, int64_t R) {
     LOOM_CHECK(R >= 0 && R <= kPcMaxRows, "%s: 0 to %d rows, got %lld", who, kPcMaxRows, (long long)R);
-    LOOM_CHECK(MP >= 1 && MP * PS <= ((int64_t)1 << 24) && ld >= MP,
+    LOOM_CHECK(MP >= 1 && MP <= ((int64_t)1 << 24) / PS && ld >= MP,
                "%s: the table must hold 1 page to 2^24 tokens per row (max_pages=%lld, row stride %lld)", who,
                (long long)MP, (long long)ld);
     LOOM_CHECK(table != nullptr || R == 0, "%s: a required pointer is NULL", who);

@@ -14,3 +14,24 @@ def test_a_batch_of_no_rows_needs_no_pointers():
     _lib.call("loom_paged_write", *pool, None, 5, 5, None, None, 0, 0, 0, 96, 40, None, None, 0, None)
     with pytest.raises(RuntimeError, match="required pointer"):
         _lib.call("loom_paged_compact", *pool, None, 5, 5, None, P, P, 136, 0, None)
+
+
+def _refused(name, args, message):
+    from loom_amd import _lib
+    with pytest.raises(RuntimeError, match=message):
+        _lib.call(name, *args.values())
+
+
+def test_sizes_whose_products_pass_64_bits_are_refused():
+    step = dict(dtype=1, qkv=P, qkv_ld=1152, k=P, v=P, page=2 * 16 * 96, tok=96, head=16 * 96, n_pages=10, page_size=16, table=P,
+                table_ld=5, max_pages=5, lens=P, cos=P, sin=P, n_pos=80, q_out=P, c=P, kctx=P, out_ld=768, ws=P,
+                ws_bytes=1 << 30, B=3, QH=8, KVH=2, HD=96, stream=None)
+    for n in (1 << 60, (1 << 60) + 1, 1 << 59):
+        _refused("loom_paged_decode_step", dict(step, max_pages=n, table_ld=n), "1 page to 2\\^24")
+    for n in (1 << 59, 1 << 60, (1 << 59) + 96):
+        _refused("loom_paged_decode_step", dict(step, tok=n), "page strides")
+    pool = dict(dtype=1, k=P, v=P, layers=2, layer=10 * 2 * 16 * 96, page=2 * 16 * 96, tok=96, head=16 * 96, n_pages=10,
+                page_size=16, KVH=2, HD=96, table=P, table_ld=1 << 60, max_pages=1 << 60)
+    _refused("loom_paged_update", dict(pool, lens=P, refs=P, status=P, parent=P, n_new=0, advance=0, ws=P, ws_bytes=1 << 20,
+                                       rows=3, stream=None), "1 page to 2\\^24")
+    _refused("loom_paged_compact", dict(pool, refs=P, used=P, ws=P, ws_bytes=1 << 20, rows=3, stream=None), "1 page to 2\\^24")
