@@ -827,11 +827,11 @@ extern "C" int loom_reorder_rows(int64_t n, void* const* tensors, const int64_t*
         s.outer_stride = outer_stride[i];
         s.row_bytes = row_bytes[i];
         s.vec = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
-        s.slices = (int)ceil_div(row_bytes[i], (int64_t)s.vec * tx);
+        const int64_t slices = ceil_div(row_bytes[i], (int64_t)s.vec * tx), most = ((int64_t)1 << 31) - 1 - blocks;
+        LOOM_CHECK(slices <= most && outer[i] <= most / slices, "%s: too much data for one call", who);
+        s.slices = (int)slices;
         s.block0 = (int)blocks;
-        blocks += s.slices * outer[i];
-        LOOM_CHECK(blocks < ((int64_t)1 << 31) && ceil_div(row_bytes[i], (int64_t)s.vec * tx) < ((int64_t)1 << 31),
-                   "%s: too much data for one call", who);
+        blocks += slices * outer[i];
     }
     if (blocks == 0) return LOOM_OK;
     const int rpt = (int)ceil_div(rows, ty);

@@ -35,3 +35,11 @@ def test_sizes_whose_products_pass_64_bits_are_refused():
     _refused("loom_paged_update", dict(pool, lens=P, refs=P, status=P, parent=P, n_new=0, advance=0, ws=P, ws_bytes=1 << 20,
                                        rows=3, stream=None), "1 page to 2\\^24")
     _refused("loom_paged_compact", dict(pool, refs=P, used=P, ws=P, ws_bytes=1 << 20, rows=3, stream=None), "1 page to 2\\^24")
+
+
+def test_reorder_of_slices_whose_number_passes_64_bits_is_refused():
+    one = lambda v: (ctypes.c_int64 * 1)(v)  # noqa: E731
+    p1 = (ctypes.c_void_p * 1)(256)
+    for outer, rb in ((1 << 62, 1 << 10), (1 << 31, 16), (1 << 62, 1 << 40), (4, 1 << 50)):
+        _refused("loom_reorder_rows", dict(n=1, t=p1, outer=one(outer), os=one(0), rs=one(rb), rb=one(rb), parent=P, rows=4, stream=None),
+                 "too much data")
