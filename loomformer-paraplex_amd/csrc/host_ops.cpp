@@ -335,7 +335,7 @@ PyObject* beam_select(PyObject* const* x, Py_ssize_t n) {
           a.name, ": scores must be a float32 [groups, beams] tensor, a value for each row of logits");
     const int64_t S = scores.size(0), W = scores.size(1), V = logits.size(1);
     const int64_t K = a.none(2) ? W : a.integer(2);
-    CHECK(K >= 1 && S >= 1, a.name, ": n_out must be at least 1, and there must be a group");
+    CHECK(K >= 1 && K <= 64 && S >= 1, a.name, ": n_out must be 1 to 64, got ", K, ", and there must be a group");
     const int64_t eos = a.integer(4), pad = a.integer(5);
     at::Tensor lg = logits;
     int64_t ld = S * W > 1 ? lg.stride(0) : V;

@@ -101,6 +101,14 @@ def test_select_rows_with_signalling_nans(dt, snan, V, K):
     assert torch.equal(s, s2) and torch.equal(p, p2) and torch.equal(t, t2)
 
 
+def test_select_refuses_more_places_before_it_makes_outputs():
+    from loom_amd import ops
+    x, sc = torch.zeros(8, 100, device=DEV), torch.zeros(2, 4, device=DEV)
+    for n in (65, 1 << 40, 1 << 62, -1):
+        with pytest.raises(RuntimeError, match="n_out must be 1 to 64"):
+            ops.beam_select(x, sc, n)
+
+
 # ------------------------------------------------------------------ attention
 
 def test_rows_end_to_end_of_more_units_than_32_bits_name():
