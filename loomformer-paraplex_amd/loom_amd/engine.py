@@ -42,7 +42,9 @@ _P = _lib.addr
 class _BeamState:
     """What a beam search keeps on the device beside the engine's own state: the paged
     cache, the scores and ends of the beams, the chosen parents, workspaces, and the
-    captured step of each pair of eos and pad ids."""
+    captured steps of the last MAX_GRAPHS pairs of eos and pad ids."""
+
+    MAX_GRAPHS = 4
 
     def __init__(self, eng: "LoomDecoder", beams: int, page_size: int, n_pages: Optional[int]):
         c, dev = eng.cfg, eng.dev
@@ -79,13 +81,15 @@ class _BeamState:
 
     def graph(self, eng: "LoomDecoder") -> torch.cuda.CUDAGraph:
         key = (self.eos_id, self.pad_id)
-        g = self._graphs.get(key)
+        g = self._graphs.pop(key, None)
         if g is None:
-            torch.cuda.synchronize(eng.dev)
+            torch.cuda.synchronize(eng.dev)          # (also: no replay of a dropped one is under way)
+            while len(self._graphs) >= self.MAX_GRAPHS:
+                del self._graphs[next(iter(self._graphs))]
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g):
                 eng._launch_beam_step(self)
-            self._graphs[key] = g
+        self._graphs[key] = g                        # the last used goes last
         return g
 
 
