@@ -239,9 +239,10 @@ template <> struct Mfma16<f16_t> {
     }
 };
 
-// x c + y s of the rotation.  For the 16-bit types in 64 bits, where both products
-// are exact: the stored value is the exact one's rounding (in fp32 one in some 10000
-// comes out a step beside it).
+// x c + y s of the rotation.  For the 16-bit types in 64 bits, where both products are
+// exact; rounded to fp32 here and to the type when it is stored, the value is the exact
+// one's rounding but where fp32's falls on the middle of two values: of 2^24 random ones
+// 1058 of half and 114 of bf16 come out a step beside it (all in fp32 2966 and 477).
 template <typename T>
 __device__ __forceinline__ float turn(float x, float c, float y, float s) {
     if constexpr (sizeof(T) == 2) return (float)fma((double)x, (double)c, (double)y * (double)s);

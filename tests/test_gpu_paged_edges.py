@@ -150,6 +150,31 @@ def test_scores_of_minus_infinity(dt, HD, n):
     assert not c[3:].float().any() and not kx[3:].float().any()
 
 
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_step_ropes_to_the_nearest_value_but_for_ties_of_fp32(dt):
+    """The rotation is computed in 64 bits, rounded to fp32 and then to the type: it is
+    the nearest value of the type, or beside it where fp32's rounding falls on the
+    middle of two (one in some 16000 values of half, one in 150000 of bf16)."""
+    from loom_amd import ops
+    g = torch.Generator().manual_seed(20)
+    HD, B = 128, 256
+    kp, vp = (torch.zeros(B, 2, 16, HD, dtype=dt, device=DEV) for _ in range(2))
+    table = torch.arange(B, dtype=torch.int32, device=DEV)[:, None].contiguous()
+    ang = torch.rand(16, HD, generator=g, dtype=torch.float64) * 6
+    cos, sin = ang.cos().float().to(DEV), ang.sin().float().to(DEV)
+    lens = torch.arange(B, dtype=torch.int32, device=DEV) % 16
+    x = torch.randn(B, 20, HD, generator=g).to(DEV, dt)
+    q = ops.paged_decode_step(x.view(B, -1), kp, vp, table, lens, cos, sin)[2]
+    xd = x[:, :16].double()
+    turned = torch.cat([-xd[..., HD // 2:], xd[..., :HD // 2]], -1)
+    d = xd * cos[lens.long()][:, None].double() + turned * sin[lens.long()][:, None].double()
+    err, bits = (q.double() - d).abs(), q.view(torch.int16).int()
+    beside = torch.minimum(*[((bits + k).to(torch.int16).view(dt).double() - d).abs() for k in (-1, 1)])
+    off = beside < err
+    assert float(off.double().mean()) <= 2.0 ** -12
+    assert (err[off] <= beside[off] + 2 * 2.0 ** -24 * d.abs()[off]).all()
+
+
 # ------------------------------------------------------------------ pages
 
 def test_compact_a_page_of_almost_two_gib():
