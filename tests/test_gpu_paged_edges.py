@@ -101,6 +101,31 @@ def test_select_rows_with_signalling_nans(dt, snan, V, K):
     assert torch.equal(s, s2) and torch.equal(p, p2) and torch.equal(t, t2)
 
 
+@pytest.mark.parametrize("kind", ["ascending", "descending", "constant", "steps", "blocks"])
+@pytest.mark.parametrize("V,K", [(24001, 8), (24000, 9), (8185, 16), (4096, 8)])
+def test_select_every_place_of_ties_and_orders(kind, V, K):
+    """Equal rows of one group: the K places are the first of all candidates by (value,
+    beam, token), scores too."""
+    from loom_amd import ops
+    W, S = 4, 128
+    i = torch.arange(V, dtype=torch.float64)
+    x = {"ascending": i / 1000, "descending": -i / 1000, "constant": 0 * i, "steps": (i // 300) / 8,
+         "blocks": torch.where((i >= 3000) & (i < 3003), 5.0, 0.0)}[kind].float()
+    s, p, t, f = ops.beam_select(x.expand(S * W, V).contiguous().to(DEV), torch.zeros(S, W, device=DEV), K)
+    top = torch.sort(x, descending=True, stable=True)
+    each = [(-float(top.values[k]), w, int(top.indices[k])) for k in range(K) for w in range(W)]
+    want = sorted(each)[:K]
+    xd = x.double()
+    lse = float(torch.logsumexp(xd, 0))
+    ws = torch.tensor([-v - lse for v, _, _ in want], dtype=torch.float64)
+    assert torch.equal(p.cpu(), torch.tensor([w for _, w, _ in want]).int()[None] + 4 * torch.arange(S).int()[:, None])
+    assert torch.equal(t.cpu(), torch.tensor([k for _, _, k in want])[None].expand(S, K))
+    # the value's rounding, the sum's 40 units, and its arguments' on sum p |x - max|
+    far = float((torch.softmax(xd, 0) * (xd - xd.max()).abs()).sum())
+    tol = 2.0 ** -24 * ws.abs() + 40 * 2.0 ** -24 + 2.0 ** -22 * far
+    assert ((s.cpu().double() - ws).abs() <= tol).all()
+
+
 def test_select_refuses_more_places_before_it_makes_outputs():
     from loom_amd import ops
     x, sc = torch.zeros(8, 100, device=DEV), torch.zeros(2, 4, device=DEV)
