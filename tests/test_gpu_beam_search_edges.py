@@ -50,3 +50,61 @@ def test_captured_steps_of_many_eos_and_pad_ids_are_bounded():
     kept = list(eng._beams._graphs)
     eng.beam_search(prompt, 6, 3, eos_id=kept[0][0] if kept[0][0] >= 0 else None, pad_id=kept[0][1], page_size=16)
     assert sorted(eng._beams._graphs) == sorted(kept) and list(eng._beams._graphs)[-1] == kept[0]
+
+
+@pytest.mark.parametrize("dt,chunked,page", [(torch.bfloat16, False, 16), (torch.bfloat16, True, 64), (torch.float32, False, 16)])
+def test_hypotheses_run_alone_give_the_same_bits(dt, chunked, page):
+    """The checkpoint's shape, over a fire of the document state: every hypothesis run
+    by itself, in a row that never forks and holds pages of its own, gives the search's
+    last logits to the bit (a row's sums do not depend on the rows beside it), and its
+    log-probabilities sum up to the score.  A page or a state of another hypothesis
+    anywhere would show."""
+    from loom_amd.engine import LoomDecoder, _BeamState
+    from loom_amd.weights import init_state_dict
+    cfg = _cfg("nano_chk", seq_len=512)
+    state = init_state_dict(cfg, 2)
+    S, W, P, n = 2, 4, 125, 12
+    prompt = torch.randint(0, cfg.V, (S, P), generator=torch.Generator().manual_seed(5))
+    eng = LoomDecoder(cfg, state, batch=S * W, dtype=dt)
+    ids, scores = eng.beam_search(prompt, n, W, chunked_prefill=chunked, page_size=page)
+    logits, parent = eng.logits.clone(), eng._beams.parent.long()
+    moved = eng._beams.cache.refs.max()
+    assert int(moved) == W                                    # the prompt's pages are still shared
+
+    rows = prompt.repeat_interleave(W, 0)
+    hyp = ids.view(S * W, n)
+    if chunked:
+        eng.prefill(rows)
+    else:
+        eng.start(rows)
+        eng.replay_steps(P - 1)
+    bs = _BeamState(eng, W, page, None)
+    kc = bs.cache
+    kc.reset()
+    kc.start(torch.ones(S * W, dtype=torch.bool, device=eng.dev))
+    kc.update(n_new=P)
+    full = torch.full((S * W,), P, dtype=torch.int32, device=eng.dev)
+    kc.load(eng.k_cache, eng.v_cache, torch.zeros_like(full), full)
+    kc.lens.copy_(full - 1)
+    total = torch.zeros(S * W, dtype=torch.float64, device=eng.dev)
+    for t in range(n):
+        total += torch.log_softmax(eng.logits.double(), 1).gather(1, hyp[:, t:t + 1])[:, 0]
+        if t == n - 1:
+            break
+        eng.ids.copy_(hyp[:, t])
+        kc.update(n_new=1, advance=1)
+        eng._launch_step(first=False, prompt_len=0, paged=bs)
+    assert int(kc.refs.max()) == 1
+    assert torch.equal(eng.logits, logits[parent])
+    # a choice's error in its score (the value's rounding, 40 units of the sum's, and the
+    # exponentials' arguments of up to 8), n times
+    tol = n * (2.0 ** -24 * float(scores.abs().max()) + 40 * 2.0 ** -24 + 2.0 ** -22 * 8)
+    assert float((scores.view(-1).double() - total).abs().max()) <= tol
+    # and another hypothesis' history would: the rows are not alike
+    for s in range(S):
+        own = logits[parent][s * W:(s + 1) * W]
+        hist = [tuple(h) for h in hyp[s * W:(s + 1) * W, :-1].tolist()]
+        assert len(set(hist)) > 1
+        for a in range(W):
+            for b in range(a):
+                assert torch.equal(own[a], own[b]) == (hist[a] == hist[b])
