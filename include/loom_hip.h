@@ -871,8 +871,9 @@ int loom_paged_compact(int dtype, void* k_pages, void* v_pages, int64_t layers, 
  * logit is a token ruled out); places without a candidate come out as score
  * -inf, token pad_id, parent g*beams, not finished.  Logits [groups*beams, V]
  * dtype, row stride logits_ld, any alignment; at most 32 beams, V <= 2^24.
- * Values are ranked in fp64.  out_scores / out_finished may be scores / finished
- * where n_out == beams.  workspace: loom_beam_select_workspace_bytes. */
+ * The two zeros are one value.  Values are ranked in fp64, a row's logsumexp in
+ * fp32 exponentials and 32-term sums (some 1e-7).  out_scores / out_finished may
+ * be scores / finished where n_out == beams.  workspace: loom_beam_select_workspace_bytes. */
 int64_t loom_beam_select_workspace_bytes(int64_t groups, int64_t beams, int64_t V, int64_t n_out);
 int loom_beam_select(int dtype, const void* logits, int64_t logits_ld, const float* scores,
                      const uint8_t* finished, float* out_scores, int32_t* out_parent, int64_t* out_token,

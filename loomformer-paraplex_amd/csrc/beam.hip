@@ -278,9 +278,9 @@ __device__ __forceinline__ int beam_counters(int n, int threads) {
 // A full sort or a heap per thread would cost several operations per logit; here a
 // logit costs its exponential (a quarter of the rate), a subtraction, two products
 // or sums and half a maximum, and a piece of eight one comparison with the bound.
-// 512 rows of 65537 bf16, 67 MB: 24 us, 2.8 TB/s, bound by those operations (the
-// vector units are busy for 60% of it) and the selection of the first step; fp32,
-// 134 MB, 36 us.  Four blocks per CU: the loads of one step are in flight while the
+// 512 rows of 65537 bf16, 67 MB: 24 us, 2.8 TB/s, bound by those operations (12 vector
+// instructions per logit; they are at work in 59% of a busy CU's cycles) and the
+// selection of the first step; fp32, 134 MB, 36 us.  Four blocks per CU: the loads of one step are in flight while the
 // present one is summed.
 template <typename T>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4)))
@@ -449,7 +449,7 @@ __device__ __forceinline__ void beam_write(const BeamArgs& a, const BeamCand* li
 // One block per group: the rows' sums from their slices', the survivors' values,
 // and the K best of them.  More than 256 survivors pass a bound first, as in
 // beam_row_kernel: the K-th best of the 64 bests of 16 threads each.  Bound by the
-// chain of loads, logarithm, bound and ranking: 64 groups of 8 beams, 5.9 us.
+// chain of loads, logarithm, bound and ranking: 64 groups of 8 beams, 5.6 us.
 __global__ void __launch_bounds__(1024)
 beam_group_kernel(BeamArgs a) {
     __shared__ BeamCand list[kBeamMaxCand], top[64];
@@ -537,8 +537,8 @@ beam_group_kernel(BeamArgs a) {
 // 16 >> wl waves per row, 32 logits per thread, one launch.  A row's bound comes
 // from the bests of 64 equal parts of its threads, so that up to K * (16 >> wl) * 32
 // keys pass; ranked, its K best enter the group.  Bound by the latency of that
-// chain.  One launch / the two above, in us: 4 beams of 8192 fp32 9.3 / 10.4, 16
-// groups of 4 of 4096 bf16 9.2 / 9.8, 1 of 30000 7.2 / 8.9; the host's share of a
+// chain.  One launch / the two above, in us: 4 beams of 8192 fp32 9.7 / 10.9, 16
+// groups of 4 of 4096 bf16 9.3 / 9.9, 1 of 30000 7.4 / 9.0; the host's share of a
 // second launch and of a workspace comes on top (2 us).
 template <typename T>
 __global__ void __launch_bounds__(1024)
@@ -702,8 +702,8 @@ static int beam_whole(int64_t W, int64_t V, int64_t K) {
 // Slices of a row: four blocks per CU (as many as it holds) as long as a slice has
 // a step's logits, two per CU down to a quarter of that, and few enough that a
 // group's survivors fit one block.  In us with the first number two, four, eight per
-// CU: 512 rows of 65537 bf16 36.6, 29.8, 37.7, fp32 45.8, 41.1, 44.3; slices of half a
-// step or of a whole one: 512 rows of 8192 13.2, 10.9, 64 rows of 65537 13.6, 13.4.
+// CU: 512 rows of 65537 bf16 37.5, 30.0, 37.7, fp32 45.3, 41.7, 44.2; slices of half a
+// step or of a whole one: 512 rows of 8192 13.4, 11.1, 64 rows of 65537 13.7, 13.6.
 static int64_t beam_slices(int64_t rows, int64_t W, int64_t V, int64_t K) {
     const int64_t cus = device_cus(), fit = kBeamMaxCand / (W * K);
     int64_t s = ceil_div(4 * cus, rows), least = ceil_div(2 * cus, rows);

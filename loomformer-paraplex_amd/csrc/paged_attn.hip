@@ -99,15 +99,15 @@ __device__ __forceinline__ int row_tiles(int n) { return n > 0 ? (n + kPgTile - 
 // after all others).
 // End to end no block waits for a longer one, but a block that starts on a row pays
 // its rope, its join record and an empty pipeline again (about six tiles: 64 rows of
-// 1 to 16384 tokens, 8 kv heads of 128, in us with kPgRowCost 2, 4, 6: 90.9, 86.8,
-// 85.7); equal chunks have one start per block.  From how many tiles per block the
+// 1 to 16384 tokens, 8 kv heads of 128, in us with kPgRowCost 2, 4, 6: 87.9, 85.1,
+// 84.1); equal chunks have one start per block.  From how many tiles per block the
 // former pays, in us with kPgStream 8, 16, 32: 32 rows of 2176 tokens, 2 kv heads of
-// 96, 19.6, 18.3, 18.3; the same in fp32 30.6, 28.2, 28.2; 1 row of 16384, 8 kv heads
-// of 128, 22.5, 21.7, 21.7.
+// 96, 17.2, 17.6, 17.6; the same in fp32 26.4, 27.2, 26.8; 1 row of 16384, 8 kv heads
+// of 128, 21.8, 21.0, 21.0.
 // The least chunk, in us with 1, 2, 4 tiles: bf16, 1 row of 2000 tokens, 2 kv heads of
-// 96, 11.2, 10.3, 10.7, 4 rows of 900, 8 kv heads of 128, 12.6, 12.6, 13.0 (a wave of
+// 96, 11.3, 10.4, 10.5, 4 rows of 900, 8 kv heads of 128, 12.6, 12.5, 12.6 (a wave of
 // the block without a tile costs nothing); in the vector form, whose blocks do one
-// tile at a time, fp32, 5 rows to 1001, 11.8, 12.8, 14.0.
+// tile at a time, fp32, 5 rows to 1001, 11.5, 12.3, 14.0.
 struct Plan {
     int q, slots, total, least;
 };
@@ -333,7 +333,7 @@ __device__ __forceinline__ void paged_finish(const PagedArgs<T>& a, const PlanIt
 // Long rows are bound by the reading of K and V, each once for all of a kv head's
 // query heads and for both sums: 64 rows of 1 to 16384 tokens, 8 kv heads of 128,
 // bf16, 442 MB: 77 us here and 7 in the join, 5.2 TB/s over both (a large copy runs
-// at 5.2); 64 rows of 2048 5.9 TB/s.  Short ones by the chain of first loads: lens,
+// at 5.2); half the same; 64 rows of 2048 5.9 TB/s.  Short ones by the chain of first loads: lens,
 // table, the row's K; scores; the waves' join: 1 row of 300, 2 kv heads of 96, 7 us of
 // which an empty launch is 2.  Two waves per SIMD leave 256 registers, so that the
 // next tile's K and V are in flight in registers while the present one is multiplied.
@@ -581,7 +581,9 @@ paged_mfma_kernel(PagedArgs<T> a) {
 // tokens' rows are in flight while the present ones are folded in.  fp32, 32 rows of
 // 2176 tokens, 2 kv heads of 96, 107 MB: 27 us with the join, 4.0 TB/s; bound by its
 // arithmetic, 2 G products per K and G per V element with no matrix instruction (a
-// step of 32 tokens takes 0.8 us).  5 rows of 1 to 1001: 12 us with the join, of which
+// step of 32 tokens takes 0.8 us).  bf16 heads of 256, 4 kv heads, 285 MB, 54 us, as a
+// large copy; 24 query heads on one kv head of 64, 18 MB, 66 us, far from that: six
+// blocks of four heads read the rows again and multiply them in fp32.  5 rows of 1 to 1001: 12 us with the join, of which
 // about 8 are the first loads, the rope and the waves' join.
 template <typename T>
 __device__ __forceinline__ void load4(const T* p, float v[4]) {
@@ -897,18 +899,18 @@ paged_join_kernel(PagedArgs<T> a) {
 // ------------------------------------------------------------------ host side
 
 // Blocks per kv head that share the work: as many as the device holds at once
-// (two per CU; 32 rows of 2176 tokens in us with 1, 1.5, 2, 3, 4 per CU: 24.1, 20.2,
-// 21.3, 27.9, 27.8, and 64 rows of 2048, 8 kv heads of 128: 94.5, 94.3, 96.5, 99.7,
-// 100).  None where no row can be long: a block per row then does it in one launch.
+// (two per CU; 32 rows of 2176 tokens in us with 1, 1.5, 2, 3, 4 per CU: 21.0, 17.5,
+// 17.4, 20.1, 22.5, and 64 rows of 2048, 8 kv heads of 128: 120.0, 103.3, 90.5, 100.1,
+// 95.4).  None where no row can be long: a block per row then does it in one launch.
 // Both ways in us, whole rows / split and joined, at 120, 250, 370, 500 tokens:
-//   bf16, 4 rows, 2 kv heads of 96      6.8 / 7.7, 7.5 / 10.7,  8.8 / 10.8,  9.9 / 10.9
-//   bf16, 4 rows, 8 kv heads of 128     7.3 / 8.9, 9.2 / 10.5, 11.0 / 10.7, 12.8 / 10.8
-//   bf16, 32 rows, 8 kv heads of 128    8.9 / 11.9, 11.4 / 16.0, 14.0 / 19.3, 16.8 / 21.1
-// and at 900: 1 row 12.7 / 10.7, 32 rows of 2 kv heads of 96 14.2 / 12.5.  The vector
+//   bf16, 4 rows, 2 kv heads of 96      6.0 / 10.0, 7.0 / 10.2,  8.0 / 10.3,  8.7 / 10.3
+//   bf16, 4 rows, 8 kv heads of 128     6.8 / 9.9, 8.6 / 10.0, 10.3 / 11.5, 12.0 / 11.7
+//   bf16, 32 rows, 8 kv heads of 128    7.6 / 14.2, 10.5 / 15.6, 12.8 / 18.6, 15.1 / 20.3
+// and at 900, 2 kv heads of 96: 1 row 11.2 / 10.3, 32 rows 14.2 / 12.5.  The vector
 // form takes a block's 4 waves times 64 / LPR tokens per step, so its bound is in steps:
-//   fp32, 5 rows, 2 kv heads of 96, 100, 180, 250 tokens   9.9 / 12.2, 11.5 / 12.4, 12.8 / 12.3
-//   bf16, 4 rows, 4 kv heads of 256, the same             11.9 / 12.9, 15.8 / 13.5, 18.6 / 13.7
-// unless the rows fill the device: fp32, 128 rows of 440, 2 kv heads of 96, 20.9 / 26.5.
+//   fp32, 5 rows, 2 kv heads of 96, 100, 180, 250 tokens   9.6 / 11.6, 10.7 / 11.7, 12.2 / 11.6
+//   bf16, 4 rows, 4 kv heads of 256, the same             10.2 / 12.6, 13.3 / 13.0, 17.1 / 13.4
+// unless the rows fill the device: fp32, 128 rows of 440, 2 kv heads of 96, 19.8 / 25.7.
 static int paged_slots(int64_t cap, int64_t HD, int64_t KVH, bool vec, int64_t B) {
     const int64_t step = HD <= 8 ? 128 : HD <= 16 ? 64 : HD <= 96 ? 32 : 16;     // tokens of a vector block's step
     const int64_t few = kPgWholeVec * step < kPgWhole ? kPgWholeVec * step : kPgWhole;
@@ -929,8 +931,8 @@ static int64_t paged_items(int64_t B, int64_t slots) { return slots == 0 ? B : B
 // Waves of a block that does a row alone: eight, so that its tiles are in flight at
 // once, but four where a row has no more tiles than that or where the blocks fill
 // the device (two of four waves fit a CU, one of eight).  In us, eight / four: 4 rows,
-// 2 kv heads of 96, 120 tokens 6.8 / 5.8; 1 row of 450 8.3 / 9.2; 8 kv heads of 128,
-// 4 rows of 440 11.8 / 12.9, 32 of 500 16.8 / 16.1, 64 of 440 29.0 / 24.7.
+// 2 kv heads of 96, 120 tokens 6.6 / 6.0; 1 row of 450 8.5 / 9.6; 8 kv heads of 128,
+// 4 rows of 440 10.4 / 11.8, 32 of 500 16.0 / 15.2, 64 of 440 28.2 / 23.8.
 static bool paged_eight(int64_t cap, int64_t blocks) { return cap > 4 * kPgTile && blocks < device_cus(); }
 
 template <typename T, bool STEP>

@@ -107,11 +107,11 @@ constexpr int kScanIds = 4;         // groups of four page ids per thread and ro
 // none of its tokens), and of what lies behind the first of them.  The free pages are taken lowest id first, in row order, by one
 // scan over refs: a free page's rank among the free ones names its row.
 // Bound by the latency of its stages, each a pass over the rows or over refs with a
-// block scan behind it: 256 rows and 17152 pages 8.6 us.  One block and not a launch
+// block scan behind it: 256 rows, 67 places each, 8.8 us.  One block and not a launch
 // per stage, since each stage needs the whole of the one before.
 // FORK: the block also forks the table, staged whole in LDS: a launch less, but
 // one CU's work.  All of a call in both forms (us, one launch / two): 92 entries
-// 7.7 / 9.9, 4352 15.8 / 16.9, 17152 20.8 / 16.8, 32512 18.1 / 11.6.
+// 8.0 / 9.9, 4384 10.6 / 11.1, 17152 20.5 / 17.2, 32512 19.6 / 13.7.
 template <bool FORK>
 __global__ void __launch_bounds__(1024)
 paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* __restrict__ lens,
@@ -355,6 +355,8 @@ paged_cow_kernel(PoolArgs a, const PageCopy* __restrict__ copies) {
 // head, t) at the strides given) into the row's pages: grid (token tiles of
 // kWriteTile, rows, layers * KVH * 2).  Tokens without a page are left out.  A copy:
 // each 16 bytes are read once and written once, a run of a head's tokens per block.
+// 32 rows of 2048 tokens, 10 layers, 2 kv heads of 96, bf16, 1.0 GB read and written:
+// 183 us, 5.5 TB/s; one row of 512, 4.8 us.
 constexpr int kWriteTile = 64;
 
 __global__ void __launch_bounds__(256)
@@ -437,7 +439,7 @@ constexpr int kMoveUnroll = 6;      // 16-byte pieces in flight per thread
 // The moves (a page of one layer's K or V pool each) and, in the blocks of
 // y = 1, the tables' new ids.  Bound by the copy, read and written once: 6000 pages
 // of 64 tokens, 10 layers, 2 kv heads of 96, bf16, a third of them in use, 1.31 GB read
-// and written: 258 us, 5.1 TB/s (a large copy: 5.2).  2, 6 or 8 pieces in flight: 270, 268, 268 us with the plan.
+// and written: 257 us, 5.1 TB/s (a large copy: 5.2).  2, 6 or 8 pieces in flight: 269, 271, 269 us with the plan.
 __global__ void __launch_bounds__(256)
 paged_compact_move_kernel(PoolArgs a, int PS, const int32_t* __restrict__ ws, int NP, int32_t* __restrict__ table,
                           int64_t ld, int MP, int R) {

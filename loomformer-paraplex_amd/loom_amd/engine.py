@@ -675,9 +675,9 @@ class LoomDecoder:
         engine's batch is S * beams.  A beam that chose eos_id has ended: it keeps
         its score and is filled up with pad_id.
 
-        The prompt runs through the dense cache as in ``generate``; its keys and
-        values then go into pages (page_size tokens each) once per prompt, and the
-        beams share them: a step forks the rows by their parents and copies only a
+        The prompt runs through the dense cache as in ``generate``, in all of its
+        beams' rows; its keys and values then go into pages (page_size tokens each)
+        once per prompt, and the beams share them: a step forks the rows by their parents and copies only a
         partly filled last page.  n_pages: pages of the pool (default: enough for
         beams that share nothing); running out raises.  One step is captured into
         a graph and replayed.  Afterwards the engine holds no sequence to continue
