@@ -367,3 +367,73 @@ def test_strides_of_dimensions_of_one_entry_say_nothing():
         for kp, vp, kr, vr in ((k, v, *one), (k2, v2, _odd(one[0], 3), one[1])):
             ops.paged_write(kp, vp, out[0][2], kr, vr, _i32([0]), _i32([1]))
         assert torch.equal(k, k2) and torch.equal(v, v2)
+
+
+def _laid_out(t, how):
+    """The values of a pool [L, NP, KVH, PS, HD] in another layout, and in memory behind it."""
+    L, NP, KVH, PS, HD = t.shape
+    if how == "token":
+        return t.transpose(2, 3).contiguous().transpose(2, 3)
+    if how == "page":                                # a page of all layers together
+        return t.transpose(0, 1).contiguous().transpose(0, 1)
+    wide = torch.full((L, NP, KVH + 1, PS, HD + 8), 3.0, dtype=t.dtype, device=t.device)      # rows and pages apart
+    wide[:, :, :KVH, :, :HD] = t
+    return wide[:, :, :KVH, :, :HD]
+
+
+@pytest.mark.parametrize("how", ["token", "page", "wide"])
+@pytest.mark.parametrize("R,MP", [(5, 9), (300, 28)])
+def test_bookkeeping_of_other_layouts_and_table_views(how, R, MP):
+    """Update, dense rows and compaction over pools of other strides and a table that is
+    a view of a wider one: as over dense ones, and nothing between the rows changes."""
+    from loom_amd import ops
+    g = torch.Generator().manual_seed(R)
+    a = _shared_rows(g, R, MP, 16, 40, 12 + 3 * R, KVH=2, HD=24, dt=BF)
+    b = [t.clone() for t in a]
+    b[0], b[1] = _laid_out(a[0], how), _laid_out(a[1], how)
+    table = torch.full((R, MP + 5), 77, dtype=torch.int32, device=DEV)
+    table[:, :MP] = a[2]
+    b[2] = table[:, :MP]
+    par = torch.randint(-1, R, (R,), generator=g).int().to(DEV)
+    rows = [torch.randn(2, R, 40, 2, 24, generator=g).to(DEV, BF).transpose(2, 3) for _ in range(2)]
+    first, last = torch.full((R,), 35, device=DEV).int(), torch.full((R,), 38, device=DEV).int()
+    for s in (a, b):
+        status, used = _i32([0]), _i32([0])
+        ops.paged_update(*s, status, n_new=1)
+        ops.paged_write(s[0], s[1], s[2], *rows, first, last)
+        ops.paged_update(*s, status, parent=par, n_new=10)
+        ops.paged_compact(s[0], s[1], s[2], s[4], used)
+        s += [status, used]
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+    assert (table[:, MP:] == 77).all()
+    if how == "wide":
+        for t in b[:2]:
+            whole = t.as_strided((2, t.shape[1], 3, 16, 32), t.stride())
+            assert (whole[:, :, 2] == 3.0).all() and (whole[..., 24:] == 3.0).all()
+
+
+@pytest.mark.parametrize("dt,V,W,K", [(BF, 1 << 24, 2, 64), (FP, (1 << 24) - 3, 1, 1), (HF, 1 << 24, 1, 5)])
+def test_select_over_the_largest_vocabularies(dt, V, W, K):
+    from loom_amd import ops
+    g = torch.Generator(device=DEV).manual_seed(K)
+    x = torch.empty(W, V, dtype=dt, device=DEV)
+    for r in range(W):
+        x[r] = torch.randn(V, generator=g, device=DEV).clamp(max=3).to(dt)
+    at = torch.randperm(V, generator=g, device=DEV)[:40 * W].view(W, 40)
+    at[:, 0], at[:, 1] = V - 1, 0
+    x.scatter_(1, at, (4 + torch.arange(40, device=DEV) % 7).to(dt).expand(W, 40).contiguous())       # with ties
+    sc = torch.zeros(1, W, device=DEV)
+    s, p, t, f = ops.beam_select(x, sc, K)
+    each = []
+    for r in range(W):
+        xr = x[r].double()
+        lse = float(torch.logsumexp(xr, 0))
+        least = float(torch.topk(x[r].float(), K).values[-1])
+        tok = (x[r].float() >= least).nonzero().view(-1)
+        each += [(lse - float(v), r, int(k)) for v, k in zip(xr[tok].tolist(), tok.tolist())]
+    want = sorted(each)[:K]
+    assert p.tolist() == [[r for _, r, _ in want]] and t.tolist() == [[k for _, _, k in want]]
+    # the value's rounding, 40 units of the sums, and the arguments' (at most 16) two units
+    ws = torch.tensor([-v for v, _, _ in want], dtype=torch.float64)
+    assert ((s[0].cpu().double() - ws).abs() <= 2.0 ** -24 * ws.abs() + 40 * 2.0 ** -24 + 2.0 ** -22 * 16).all()
