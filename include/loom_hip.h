@@ -836,6 +836,61 @@ int loom_paged_update(int dtype, void* k_pages, void* v_pages, int64_t layers, i
                       int64_t n_new, int64_t advance, void* workspace, int64_t workspace_bytes, int64_t rows,
                       void* stream);
 
+/* The reservation of loom_paged_update alone, with a count per row: tokens lens[r]
+ * .. lens[r] + new_tokens[r] - 1 of every row that holds a sequence are made
+ * writable (new_tokens[r] <= 0: none).  lens is not changed.  workspace:
+ * loom_paged_update_workspace_bytes(rows). */
+int loom_paged_reserve(int dtype, void* k_pages, void* v_pages, int64_t layers, int64_t layer_stride,
+                       int64_t page_stride, int64_t token_stride, int64_t head_stride, int64_t n_pages,
+                       int64_t page_size, int64_t KVH, int64_t HD, int32_t* table, int64_t table_ld,
+                       int64_t max_pages, int32_t* lens, int32_t* refs, int32_t* status,
+                       const int32_t* new_tokens, void* workspace, int64_t workspace_bytes, int64_t rows,
+                       void* stream);
+
+/* A serving step: every row r that holds a sequence brings new_tokens[r] tokens
+ * (none, one, a prompt or a piece of one), which lie one row behind the other in
+ * a flat batch of n_tokens (at most 2^20) places.  Places behind the last are padding.
+ *
+ * loom_paged_plan makes the maps of the flat batch:
+ *   starts [rows + 1]    the place of each row's first token, then their number
+ *   rows_of [n_tokens]   each place's row (-1: padding)
+ *   positions [n_tokens] its position lens[r] + i in the row (-1: padding)
+ *   slots [n_tokens]     int64: page * page_size + place in the page (-1: none)
+ * shared [rows]: how many of the row's first tokens lie in pages that other rows of
+ * the batch hold too and are read once for all of them (0: none), and `plan`, for
+ * loom_paged_batch_step: the step's work cut into equal shares.  It holds for
+ * the layers of one step, until table, lens or new_tokens change.  A row without a
+ * page for each of its tokens, those to come included, with more than its
+ * table takes, or whose tokens do not all fit into the batch, has no slots.
+ * plan: loom_paged_plan_bytes, 64-byte aligned, no initial contents. */
+int64_t loom_paged_plan_bytes(int64_t rows, int64_t n_tokens, int64_t QH, int64_t KVH);
+int loom_paged_plan(const int32_t* table, int64_t table_ld, int64_t max_pages, int64_t n_pages, int64_t page_size,
+                    const int32_t* lens, const int32_t* new_tokens, int64_t rows, int64_t n_tokens, int64_t QH,
+                    int64_t KVH, int32_t* starts, int32_t* rows_of, int32_t* positions, int64_t* slots,
+                    int32_t* shared, void* plan, int64_t plan_bytes, void* stream);
+
+/* A layer of a serving step (the attention of GroupedQueryCausalSelfAttention,
+ * loomformer.py:3215-3332, over a paged cache and a ragged batch): qkv
+ * [n_tokens, (QH + 2 KVH) HD] projection rows; q and k are roped at the token's
+ * position, k and v written to its slot, and the token attends to positions 0 ..
+ * its own of its row.  q_out [n_tokens, QH, HD] the roped q, c_out = A.V, kctx_out = A.K
+ * (or NULL), rows out_ld apart.  Pages that a new token is written to must be held
+ * by its row alone (loom_paged_reserve).  Later tokens of the row and
+ * whatever else lies in its pages have no influence, infinities and NaN included.
+ * Padding gives zeros; tokens of a row without slots, and those whose position
+ * lies past the rotary tables, give NaN and are not written.  A plan of other
+ * sizes gives NaN.  workspace: loom_paged_batch_workspace_bytes, 16-byte aligned,
+ * no initial contents; not for two calls at once. */
+int64_t loom_paged_batch_workspace_bytes(int64_t rows, int64_t n_tokens, int64_t QH, int64_t KVH, int64_t HD);
+int loom_paged_batch_step(int dtype, const void* qkv, int64_t qkv_ld, void* k_pages, void* v_pages,
+                          int64_t page_stride, int64_t token_stride, int64_t head_stride, int64_t n_pages,
+                          int64_t page_size, const int32_t* table, int64_t table_ld, int64_t max_pages,
+                          int64_t rows, const int32_t* rows_of, const int32_t* positions, const int64_t* slots,
+                          const void* plan, int64_t plan_bytes, const float* cos_table, const float* sin_table,
+                          int64_t n_pos, void* q_out, void* c_out, void* kctx_out, int64_t out_ld,
+                          void* workspace, int64_t workspace_bytes, int64_t n_tokens, int64_t QH, int64_t KVH,
+                          int64_t HD, void* stream);
+
 /* Copies tokens first[r] .. last[r] - 1 of every row r of a dense cache
  * (src_tokens positions, element (layer, r, kv head, t, d) at the four source
  * strides + d; the decode engine's cache after a prefill) into the row's pages.

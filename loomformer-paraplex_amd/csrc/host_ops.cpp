@@ -275,6 +275,119 @@ PyObject* paged_update(PyObject* const* x, Py_ssize_t n) {
     Py_RETURN_NONE;
 }
 
+// (k_pages, v_pages, table, lens, refs, status, new)
+PyObject* paged_reserve(PyObject* const* x, Py_ssize_t n) {
+    const Args a("paged_reserve", x, n, 7);
+    const Pools p = pools_of(a, 0, 5);
+    const Table t = table_of(a, 2, p.dev);
+    const at::Tensor &lens = i32(a, 3, "lens", t.rows, p.dev), &refs = i32(a, 4, "refs", p.k.size(1), p.dev),
+                     &status = i32(a, 5, "status", 1, p.dev), &fresh = i32(a, 6, "new", t.rows, p.dev);
+    if (t.rows == 0) Py_RETURN_NONE;
+    OnDevice on(p.dev.index());
+    const int64_t need = loom_paged_update_workspace_bytes(t.rows);
+    const at::Tensor ws = bytes(need, p.dev);
+    void* st = stream_of(p.dev.index());
+    launch([&] {
+        return loom_paged_reserve(p.dtype, p.k.data_ptr(), p.v.data_ptr(), p.k.size(0), p.layer, p.page, p.tok, p.head,
+                                  p.k.size(1), p.k.size(3), p.k.size(2), p.k.size(4), t.p, t.ld, t.pages,
+                                  (int32_t*)lens.data_ptr(), (int32_t*)refs.data_ptr(), (int32_t*)status.data_ptr(),
+                                  (const int32_t*)fresh.data_ptr(), ws.data_ptr(), need, t.rows, st);
+    });
+    Py_RETURN_NONE;
+}
+
+// ------------------------------------------------------------------ a ragged batch's step
+
+// (k_pages, table, lens, new, n_tokens, q_heads) -> starts, rows, positions, slots, shared, work, sizes
+PyObject* paged_plan(PyObject* const* x, Py_ssize_t n) {
+    const Args a("paged_plan", x, n, 6);
+    const at::Tensor& k = a.tensor(0, "k_pages");
+    const int64_t d = k.dim();
+    CHECK(d == 4 || d == 5, a.name, ": k_pages must be [pages, kv_heads, page_size, head_dim], or that of all layers");
+    const c10::Device dev = k.device();
+    const Table t = table_of(a, 1, dev);
+    const at::Tensor &lens = i32(a, 2, "lens", t.rows, dev), &fresh = i32(a, 3, "new", t.rows, dev);
+    const int64_t NP = k.size(d - 4), KVH = k.size(d - 3), PS = k.size(d - 2), N = a.integer(4), QH = a.integer(5), R = t.rows;
+    CHECK(N >= 0 && N <= (1 << 20), a.name, ": n_tokens must be 0 to 2^20, got ", N);
+    OnDevice on(dev.index());
+    const int64_t need = loom_paged_plan_bytes(R, N, QH, KVH);
+    CHECK(need > 0, a.name, ": ", QH, " query heads over ", KVH, " kv heads, ", R, " rows (at most 1024)");
+    const auto opt = at::TensorOptions().device(dev);
+    const at::Tensor starts = at::empty({R + 1}, opt.dtype(at::kInt)), rows = at::empty({N}, opt.dtype(at::kInt)),
+                     pos = at::empty({N}, opt.dtype(at::kInt)), slots = at::empty({N}, opt.dtype(at::kLong)),
+                     shared = at::empty({R}, opt.dtype(at::kInt)), work = bytes(need, dev);
+    void* st = stream_of(dev.index());
+    launch([&] {
+        return loom_paged_plan(t.p, t.ld, t.pages, NP, PS, (const int32_t*)lens.data_ptr(), (const int32_t*)fresh.data_ptr(),
+                               R, N, QH, KVH, (int32_t*)starts.data_ptr(), (int32_t*)rows.data_ptr(), (int32_t*)pos.data_ptr(),
+                               (int64_t*)slots.data_ptr(), (int32_t*)shared.data_ptr(), work.data_ptr(), need, st);
+    });
+    PyObject* l = list_of({&starts, &rows, &pos, &slots, &shared, &work, nullptr});
+    PyObject* sizes = Py_BuildValue("(LLLLL)", (long long)NP, (long long)KVH, (long long)PS, (long long)t.pages, (long long)QH);
+    if (sizes == nullptr) {
+        Py_DECREF(l);
+        throw PyError{};
+    }
+    PyList_SetItem(l, 6, sizes);
+    return l;
+}
+
+// (starts, rows, positions, slots, shared, work, sizes, qkv, k_pages, v_pages, table, cos, sin, want_kctx)
+PyObject* paged_batch_step(PyObject* const* x, Py_ssize_t n) {
+    const Args a("paged_batch_step", x, n, 14);
+    const Pools p = pools_of(a, 8, 4);
+    const int64_t NP = p.k.size(0), KVH = p.k.size(1), PS = p.k.size(2), HD = p.k.size(3);
+    at::Tensor q = a.tensor(7, "qkv");
+    CHECK(q.device() == p.dev && q.scalar_type() == p.k.scalar_type(), a.name, ": qkv must have the pools' dtype and device");
+    CHECK(q.dim() == 2 && HD > 0 && q.size(1) % HD == 0 && q.size(1) / HD > 2 * KVH, a.name,
+          ": qkv must be [n_tokens, (q_heads + 2 kv_heads) * head_dim]");
+    const int64_t N = q.size(0), QH = q.size(1) / HD - 2 * KVH;
+    CHECK(KVH > 0 && QH % KVH == 0, a.name, ": ", QH, " query heads over ", KVH, " kv heads");
+    const Table t = table_of(a, 10, p.dev);
+    const at::Tensor &rows = i32(a, 1, "plan.rows", N, p.dev), &pos = i32(a, 2, "plan.positions", N, p.dev),
+                     &slots = a.tensor(3, "plan.slots"), &work = a.tensor(5, "plan.work");
+    CHECK(slots.device() == p.dev && slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.size(0) == N &&
+              slots.is_contiguous() && work.device() == p.dev && work.scalar_type() == at::kByte && work.is_contiguous(),
+          a.name, ": the plan is not one of paged_plan for ", N, " tokens");
+    long long made[5];
+    if (!PyTuple_Check(a.a[6]) || !PyArg_ParseTuple(a.a[6], "LLLLL", made, made + 1, made + 2, made + 3, made + 4)) {
+        PyErr_Clear();
+        fail(a.name, ": the plan is not one of paged_plan");
+    }
+    CHECK(made[0] == NP && made[1] == KVH && made[2] == PS && made[3] == t.pages && made[4] == QH &&
+              a.tensor(0, "plan.starts").numel() == t.rows + 1,
+          a.name, ": the plan was made for other sizes (", made[0], " pages of ", made[2], " tokens, ", made[1],
+          " kv heads, ", made[4], " q heads, ", a.tensor(0, "plan.starts").numel() - 1, " rows of ", made[3], " pages)");
+    const at::Tensor &cos = a.tensor(11, "cos"), &sin = a.tensor(12, "sin");
+    for (const at::Tensor* c : {&cos, &sin})
+        CHECK(c->device() == p.dev && c->scalar_type() == at::kFloat && c->dim() == 2 && c->size(1) == HD &&
+                  c->size(0) == cos.size(0) && c->is_contiguous(),
+              a.name, ": cos and sin must be contiguous float32 [positions, head_dim] tables");
+    const bool kctx = a.truth(13);
+    int64_t ld = N > 1 ? q.stride(0) : q.size(1);
+    if (q.stride(1) != 1 || ld < q.size(1) || (ld * q.element_size()) % 16 != 0 || (uintptr_t)q.data_ptr() % 16 != 0) {
+        q = q.clone(at::MemoryFormat::Contiguous);
+        ld = q.size(1);
+    }
+    OnDevice on(p.dev.index());
+    const auto opt = p.k.options();
+    at::Tensor c = at::empty({N, QH, HD}, opt), kx, qo = at::empty({N, QH, HD}, opt);
+    if (kctx) kx = at::empty({N, QH, HD}, opt);
+    if (N == 0) return list_of({&c, &kx, &qo});
+    const int64_t need = loom_paged_batch_workspace_bytes(t.rows, N, QH, KVH, HD);
+    const at::Tensor ws = bytes(need, p.dev);
+    void* st = stream_of(p.dev.index());
+    launch([&] {
+        return loom_paged_batch_step(p.dtype, q.data_ptr(), ld, p.k.data_ptr(), p.v.data_ptr(), p.page, p.tok, p.head, NP,
+                                     PS, t.p, t.ld, t.pages, t.rows, (const int32_t*)rows.data_ptr(),
+                                     (const int32_t*)pos.data_ptr(), (const int64_t*)slots.data_ptr(), work.data_ptr(),
+                                     work.numel(), (const float*)cos.data_ptr(), (const float*)sin.data_ptr(), cos.size(0),
+                                     qo.data_ptr(), c.data_ptr(), kctx ? kx.data_ptr() : nullptr, QH * HD, ws.data_ptr(),
+                                     need, N, QH, KVH, HD, st);
+    });
+    return list_of({&c, &kx, &qo});
+}
+
 // (k_pages, v_pages, table, k_rows, v_rows, first, last)
 PyObject* paged_write(PyObject* const* x, Py_ssize_t n) {
     const Args a("paged_write", x, n, 7);
@@ -473,7 +586,8 @@ PyObject* guarded(PyObject*, PyObject* const* x, Py_ssize_t n) {
 #define ENTRY(f) {#f, (PyCFunction)(void (*)(void))guarded<f>, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {ENTRY(paged_decode_step), ENTRY(paged_decode_attention), ENTRY(paged_update),
                          ENTRY(paged_write),       ENTRY(paged_compact),          ENTRY(beam_select),
-                         ENTRY(reorder_rows),      {nullptr, nullptr, 0, nullptr}};
+                         ENTRY(reorder_rows),      ENTRY(paged_reserve),          ENTRY(paged_plan),
+                         ENTRY(paged_batch_step),  {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

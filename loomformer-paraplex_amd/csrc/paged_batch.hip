@@ -1,0 +1,1366 @@
+// A serving step over a paged key-value cache, for gfx950: every row of the batch
+// brings a number of new tokens of its own (none, one, a whole prompt), and pages
+// that rows have in common are read once for all of them.
+//
+// Token t of row r, the i-th of its new ones, stands at position p = lens[r] + i and
+// attends to positions 0 .. p of its row.  With s_j = q . k_j / sqrt(HD):
+//   C = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  Kctx = the same of k_j.
+// The sums split over any partition of the positions: each part leaves (m, l, C, Kctx)
+// with its own maximum m and sum l, and the join weighs them by e^(m - max m).  The
+// partition is that of the work: the positions that rows share against all those
+// rows' queries at once, then each row's own.
+//
+// Which rows share what only the device knows, so a step is planned there, once for
+// all layers:
+//   rows     which rows begin with the same pages, and how many (paged_rows_kernel)
+//   plan     segments (a block of up to 64 queries and the positions they read), cut
+//            into items of about equal work, one block each (paged_plan_kernel)
+// and a layer is three launches: rope and append, the items, the join.
+#include "attn_tile.h"
+#include "paged_math.h"
+
+#include <type_traits>
+
+namespace loom {
+
+constexpr int kPbMaxRows = 1024;
+constexpr int kPbQ = 64;            // queries (a token's heads of one kv head) of a block
+constexpr int kPbTile = 64;         // positions of a step of a block
+constexpr int kPbLeast = 2;         // an item has so many tiles at least
+constexpr int kPbAlone = 32;        // rows with more queries fill a block by themselves and share nothing
+constexpr int kPbShare = 64;        // common positions from which reading them once pays
+constexpr int kPbMagic = 0x4c50424c;
+constexpr int64_t kPbMaxTokens = (int64_t)1 << 20;
+
+// A block of queries and the positions they read.  Query x (0 .. nq - 1) is query x0 +
+// x of a list of tokens times the kv head's G heads: token list entry (x0 + x) / G,
+// head (x0 + x) % G.
+struct alignas(64) PbSeg {
+    int row;                        // whose table entries name the pages
+    int key0, key1;                 // positions key0 .. key1 - 1, key0 a multiple of 16
+    int base;                       // the list's first token (common: its place in toks)
+    int x0, nq;
+    int lens;                       // own: tokens the row held before the step
+    int common;                     // the positions that a group of rows shares
+    int nchunk, rec0;               // items; record of (chunk, x) is rec0 + chunk nq + x (rec0 < 0: none)
+    int tiles;
+    int pseg0, gx0;                 // own, of a group: the group's first segment, x = 0's place in its list
+    int pad[3];
+};
+struct alignas(16) PbItem {
+    int seg, chunk, tile0, tile1;
+};
+
+// The plan's parts, in ints from its start
+struct PbLayout {
+    int64_t rows, segs, items, joins, toks, total;      // rows: 4 ints each
+    int cap_segs, cap_items, cap_joins, cap_toks;
+    int64_t cap_recs;               // records of a kv head
+    int slots;
+};
+// header: 0 magic, 1 items, 2 joins, 3.. the sizes it was made for
+constexpr int kPbHeader = 16;
+
+static int pb_slots(int64_t KVH) {
+    const int64_t n = 2 * (int64_t)device_cus() / KVH;
+    return n < 1 ? 1 : (int)n;
+}
+
+// What a plan can need at most.  Own segments: a row's last may be partly filled;
+// common ones: of the rows that share, at least two to a group.  An item is
+// ceil(tiles / c) of a segment where c >= all tiles / slots, so all items are at most
+// slots + segments, and segments of more than one item have at most 2 slots of them.
+static PbLayout pb_layout(int64_t R, int64_t N, int64_t QH, int64_t KVH) {
+    PbLayout p{};
+    const int64_t G = QH / KVH, NG = N * G, some = NG < kPbAlone * R ? NG : kPbAlone * R;
+    p.slots = pb_slots(KVH);
+    p.cap_segs = (int)(R + NG / kPbQ + R / 2 + some / kPbQ + 2);
+    p.cap_items = p.cap_segs + p.slots;
+    const int64_t split = kPbQ < NG ? kPbQ : NG;          // queries of a split segment
+    p.cap_joins = (int)(p.slots * ((split + 3) / 4) + some / 4 + R + 1);
+    p.cap_toks = (int)some + 1;
+    p.cap_recs = 2 * p.slots * split + 2 * some;
+    p.rows = kPbHeader;
+    p.segs = (p.rows + 4 * R + 15) / 16 * 16;
+    p.items = p.segs + (int64_t)p.cap_segs * (sizeof(PbSeg) / 4);
+    p.joins = p.items + (int64_t)p.cap_items * (sizeof(PbItem) / 4);
+    p.toks = p.joins + 2 * (int64_t)p.cap_joins;
+    p.total = (p.toks + p.cap_toks + 3) / 4 * 4;
+    return p;
+}
+
+struct PlanArgs {
+    const int32_t* table;
+    int64_t table_ld;
+    const int32_t* lens;
+    const int32_t* fresh;           // new tokens of each row
+    int32_t *starts, *rows_of, *positions, *shared;
+    int64_t* slots_of;
+    int32_t* plan;
+    PbLayout at;
+    int R, N, QH, KVH, G, log_ps, cap, n_pages;
+};
+
+// A row's new tokens.  More than the batch holds is one more than it holds (its row
+// then does not fit), so that all rows' sum stays within 32 bits.
+__device__ __forceinline__ int pb_fresh(const PlanArgs& a, int r) {
+    return a.lens[r] < 0 ? 0 : min(max(a.fresh[r], 0), a.N + 1);
+}
+
+// ------------------------------------------------------------------ rows
+
+// A wave per row: whether the row has a page for each of its tokens, the ones to come
+// included, and with which other row it shares how many leading pages.  Rows that
+// start with the same page belong together; the lowest of them leads, found in a hash
+// table in LDS that every block fills from all rows' first entries.  rows[r] = (the
+// leader or -1, whole pages in common with it, pages all there, 0).  Bound by the chain
+// first entries, hash, the two rows' entries, 256 of each in flight per wave.
+constexpr int kPbHash = 2048;
+
+__global__ void __launch_bounds__(1024)
+paged_rows_kernel(PlanArgs a) {
+    __shared__ int key[kPbHash], low[kPbHash];
+    const int tid = threadIdx.x, lane = tid & 63, PS = 1 << a.log_ps;
+    for (int i = tid; i < kPbHash; i += 1024) {
+        key[i] = -1;
+        low[i] = kPbMaxRows;
+    }
+    auto candidate = [&](int r, int m, int n, int page) {
+        return m > 0 && (int64_t)m * a.G <= kPbAlone && n >= PS && (unsigned)page < (unsigned)a.n_pages;
+    };
+    // (at most 1024 different keys in 2048 places: every search ends)
+    auto place = [&](int page) { return (int)(((uint32_t)page * 2654435761u) >> 21); };
+    __syncthreads();
+    if (tid < a.R) {
+        const int page = a.table[(int64_t)tid * a.table_ld];
+        if (candidate(tid, pb_fresh(a, tid), a.lens[tid], page)) {
+            for (int h = place(page);; h = (h + 1) & (kPbHash - 1)) {
+                const int was = atomicCAS(&key[h], -1, page);
+                if (was == -1 || was == page) {
+                    atomicMin(&low[h], tid);
+                    break;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    const int r = blockIdx.x * 16 + __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (r >= a.R) return;
+    const int n = a.lens[r], m = pb_fresh(a, r);
+    const int32_t* row = a.table + (int64_t)r * a.table_ld;
+    const int first = row[0];
+    int lead = -1;
+    if (candidate(r, m, n, first)) {
+        int h = place(first);
+        while (key[h] != first) h = (h + 1) & (kPbHash - 1);
+        lead = low[h];
+    }
+    lead = __builtin_amdgcn_readfirstlane(lead);
+    const bool fits = n >= 0 && n <= a.cap && m <= a.cap - n;
+    const int need = m > 0 && fits ? (n + m + PS - 1) >> a.log_ps : 0, whole = lead >= 0 ? n >> a.log_ps : 0;
+    const int32_t* other = a.table + (int64_t)max(lead, 0) * a.table_ld;
+    bool there = fits;
+    int same = whole;
+    for (int c0 = 0; c0 < need; c0 += 256) {
+        int v[4], w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int c = c0 + 64 * u + lane;
+            v[u] = c < need ? row[c] : 0;
+            w[u] = c < whole && lead != r ? other[c] : v[u];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            there &= !__any((unsigned)v[u] >= (unsigned)a.n_pages);
+            const unsigned long long differ = __ballot(v[u] != w[u]);
+            if (differ) same = min(same, c0 + 64 * u + (int)__ffsll(differ) - 1);
+        }
+    }
+    if (lane == 0) *reinterpret_cast<int4*>(a.plan + a.at.rows + 4 * r) = make_int4(lead, same, there, 0);
+}
+
+// ------------------------------------------------------------------ plan
+
+// Exclusive scan of N counts over the 1024 threads of a block; total: their sums.
+template <int N>
+__device__ __forceinline__ void pb_scan(const int (&v)[N], int (*waves)[N], int (&before)[N], int (&total)[N]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int incl[N];
+    __syncthreads();                                 // the previous use of `waves` is over
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        incl[k] = wave_scan_int(v[k]);
+        if (lane == 63) waves[wave][k] = incl[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int mine = lane < 16 ? waves[lane][k] : 0;
+        const int upto = wave_scan_int(mine);
+        total[k] = __builtin_amdgcn_readlane(upto, 15);
+        before[k] = __builtin_amdgcn_readlane(upto - mine, __builtin_amdgcn_readfirstlane(wave)) + incl[k] - v[k];
+    }
+}
+
+// The last of `n` ascending values that is at most x (values[0] <= x)
+__device__ __forceinline__ int pb_find(const int* values, int n, int x) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (values[mid] <= x) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// Block 0: groups, segments, items, joins.  The others, 1024 flat tokens each: the
+// tokens' rows, positions and slots.  Both begin with a scan over the rows' counts.
+// Block 0 is one block because each stage needs the whole of the one before; it is
+// bound by their latency, a pass over the rows or the segments with a block scan each.
+__global__ void __launch_bounds__(1024)
+paged_plan_kernel(PlanArgs a) {
+    __shared__ int first[kPbMaxRows], m_of[kPbMaxRows], lead_of[kPbMaxRows];
+    __shared__ int gpages[kPbMaxRows], gtoks[kPbMaxRows], gbase[kPbMaxRows], pbase[kPbMaxRows], sbase[kPbMaxRows];
+    __shared__ int rowx[kPbMaxRows];
+    __shared__ int waves[16][3];
+    const int tid = threadIdx.x, r = tid, PS = 1 << a.log_ps;
+    int m = 0;
+    int4 info = make_int4(-1, 0, 0, 0);
+    if (r < a.R) {
+        m = pb_fresh(a, r);
+        info = *reinterpret_cast<const int4*>(a.plan + a.at.rows + 4 * r);
+    }
+    int m1[1] = {m}, start1[1], all1[1];
+    pb_scan<1>(m1, reinterpret_cast<int(*)[1]>(waves), start1, all1);
+    const int start = start1[0];
+    const bool ok = m > 0 && info.z != 0 && start + m <= a.N;
+    first[r] = r < a.R ? start : 0x7fffffff;
+    m_of[r] = ok ? m : 0;
+    if (blockIdx.x > 0) {
+        __syncthreads();
+        const int t = (blockIdx.x - 1) * 1024 + tid;
+        if (t >= a.N) return;
+        int row = -1, pos = -1;
+        int64_t slot = -1;
+        if (t < all1[0]) {
+            row = pb_find(first, a.R, t);
+            pos = a.lens[row] + t - first[row];
+            if (m_of[row] > 0)
+                slot = ((int64_t)a.table[(int64_t)row * a.table_ld + (pos >> a.log_ps)] << a.log_ps) + (pos & (PS - 1));
+            if (pos < 0) pos = 0x7fffffff;           // (a row that has no room for its tokens)
+        }
+        a.rows_of[t] = row;
+        a.positions[t] = pos;
+        a.slots_of[t] = slot;
+        return;
+    }
+    if (r < a.R) a.starts[r] = start;
+    if (r == 0) a.starts[a.R] = all1[0];
+
+    // groups: rows of one leader; what all of them have in common
+    const int lead = ok && info.x >= 0 ? info.x : -1;
+    lead_of[r] = lead;
+    gpages[r] = 0x7fffffff;
+    gtoks[r] = 0;
+    gbase[r] = 0;                                    // rows of the group, for now
+    __syncthreads();
+    if (lead >= 0) {
+        atomicMin(&gpages[lead], info.y);
+        atomicAdd(&gtoks[lead], m);
+        atomicAdd(&gbase[lead], 1);
+    }
+    __syncthreads();
+    // common positions of the group that row r leads
+    const bool pays = gbase[r] >= 2 && gpages[r] << a.log_ps >= kPbShare;
+    const int npre = pays ? (gtoks[r] * a.G + kPbQ - 1) / kPbQ : 0;
+    const int nown = ok ? (int)(((int64_t)m * a.G + kPbQ - 1) / kPbQ) : 0;
+    __syncthreads();
+    if (!pays) gpages[r] = 0;
+    int three[3] = {pays ? gtoks[r] : 0, npre, nown}, before[3], total[3];
+    pb_scan<3>(three, waves, before, total);
+    gbase[r] = before[0];
+    pbase[r] = before[1];
+    sbase[r] = total[1] + before[2];
+    __syncthreads();
+    const int shared = lead >= 0 ? gpages[lead] << a.log_ps : 0;
+    int ahead = 0;                                   // tokens of the group's rows before this one
+    if (shared > 0) {
+        for (int i = lead; i < r; ++i) ahead += lead_of[i] == lead ? m_of[i] : 0;
+        for (int i = 0; i < m; ++i) a.plan[a.at.toks + gbase[lead] + ahead + i] = start + i;
+    }
+    rowx[r] = ahead;
+    if (r < a.R) a.shared[r] = shared;
+    __syncthreads();
+
+    const int nseg = total[1] + total[2];
+    // a segment without its share of the work
+    auto segment = [&](int i) __attribute__((always_inline)) {
+        PbSeg s;
+        s.common = i < total[1];
+        const int row = pb_find(s.common ? pbase : sbase, a.R, i), x0 = (i - (s.common ? pbase : sbase)[row]) * kPbQ;
+        s.row = row;
+        s.x0 = x0;
+        s.pseg0 = -1;
+        s.gx0 = 0;
+        if (s.common) {
+            s.nq = min(kPbQ, gtoks[row] * a.G - x0);
+            s.base = gbase[row];
+            s.key0 = 0;
+            s.key1 = gpages[row] << a.log_ps;
+            s.lens = s.key1;
+        } else {
+            s.nq = (int)min((int64_t)kPbQ, (int64_t)m_of[row] * a.G - x0);
+            s.base = first[row];
+            s.lens = a.lens[row];
+            const int l = lead_of[row];
+            s.key0 = l >= 0 ? gpages[l] << a.log_ps : 0;
+            s.key1 = s.lens + (x0 + s.nq - 1) / a.G + 1;
+            if (s.key0 > 0) {
+                s.pseg0 = pbase[l];
+                s.gx0 = rowx[row] * a.G;
+            }
+        }
+        s.tiles = (s.key1 - s.key0 + kPbTile - 1) / kPbTile;
+        return s;
+    };
+    // (up to 2^24 segments of 2^18 tiles: the sum's upper and lower 20 bits apart)
+    int64_t mine = 0;
+    for (int i = tid; i < nseg; i += 1024) mine += segment(i).tiles;
+    int sum[2] = {(int)(mine >> 20), (int)(mine & 0xfffff)}, none[2], tiles[2];
+    pb_scan<2>(sum, reinterpret_cast<int(*)[2]>(waves), none, tiles);
+    const int64_t all_tiles = ((int64_t)tiles[0] << 20) + tiles[1];
+    const int chunk = max(kPbLeast, (int)min((all_tiles + a.at.slots - 1) / a.at.slots, (int64_t)1 << 30));
+    int item0 = 0, rec0 = 0, join0 = 0;
+    for (int i0 = 0; i0 < nseg; i0 += 1024) {
+        const int i = i0 + tid;
+        PbSeg s{};
+        int want[3] = {0, 0, 0}, at[3], all[3];
+        bool rec = false;
+        if (i < nseg) {
+            s = segment(i);
+            s.nchunk = (s.tiles + chunk - 1) / chunk;
+            rec = s.nchunk > 1 || s.common || s.pseg0 >= 0;
+            want[0] = s.nchunk;
+            want[1] = rec ? s.nchunk * s.nq : 0;
+            want[2] = rec && !s.common ? (s.nq + 3) / 4 : 0;
+        }
+        pb_scan<3>(want, waves, at, all);
+        if (i < nseg) {
+            s.rec0 = rec ? rec0 + at[1] : -1;
+            reinterpret_cast<PbSeg*>(a.plan + a.at.segs)[i] = s;
+            PbItem* items = reinterpret_cast<PbItem*>(a.plan + a.at.items) + item0 + at[0];
+            for (int k = 0; k < s.nchunk; ++k)
+                items[k] = PbItem{i, k, (int)((int64_t)k * s.tiles / s.nchunk), (int)((int64_t)(k + 1) * s.tiles / s.nchunk)};
+            int2* joins = reinterpret_cast<int2*>(a.plan + a.at.joins) + join0 + at[2];
+            for (int k = 0; k < want[2]; ++k) joins[k] = make_int2(i, 4 * k);
+        }
+        item0 += all[0];
+        rec0 += all[1];
+        join0 += all[2];
+    }
+    if (tid == 0) {
+        a.plan[0] = kPbMagic;
+        a.plan[1] = item0;
+        a.plan[2] = join0;
+        a.plan[3] = a.R;
+        a.plan[4] = a.N;
+        a.plan[5] = a.QH;
+        a.plan[6] = a.KVH;
+        a.plan[7] = a.cap;
+        a.plan[8] = a.log_ps;
+        a.plan[9] = a.at.slots;
+        a.plan[10] = a.n_pages;
+    }
+}
+
+// ------------------------------------------------------------------ a layer's step
+
+template <typename T>
+struct BatchArgs {
+    const T* qkv;                   // projection rows [q | k | v] of the flat tokens
+    int64_t qkv_ld;
+    T* kp;
+    T* vp;
+    int64_t ps_page, ps_tok, ps_head;
+    const int32_t* table;
+    int64_t table_ld;
+    const int32_t *positions, *rows_of;
+    const int64_t* slots_of;
+    const float *cosv, *sinv;
+    T *q_out, *c_out, *k_out;
+    int64_t out_ld;
+    const int32_t* plan;
+    PbLayout at;
+    uint8_t* odd;                   // tokens whose k or v holds an infinity or NaN
+    float* rec;                     // [KVH, cap_recs, 2 HD], then [KVH, cap_recs, 2]
+    int64_t rec_ml;
+    int R, N, QH, KVH, G, HD, log_ps, cap, n_pages, n_pos;
+    float qscale;
+};
+
+// Whether the plan is one of these sizes (another one's numbers could lie anywhere)
+template <typename T>
+__device__ __forceinline__ bool plan_fits(const BatchArgs<T>& a) {
+    const int32_t* h = a.plan;
+    return h[0] == kPbMagic && h[3] == a.R && h[4] == a.N && h[5] == a.QH && h[6] == a.KVH && h[7] == a.cap &&
+           h[8] == a.log_ps && h[9] == a.at.slots && h[10] == a.n_pages;
+}
+
+template <typename T, int E>
+__device__ __forceinline__ void load_e(const T* p, float (&v)[E]) {
+    if constexpr (E == 8) {
+        Vec8<T>::load(p, v);
+    } else if constexpr (sizeof(T) == 4) {
+        const float4 w = *reinterpret_cast<const float4*>(p);
+        v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+    } else {
+        RowIO<T, 4>::load(p, v);
+    }
+}
+template <typename T, int E>
+__device__ __forceinline__ void store_e(T* p, const float (&v)[E]) {
+    if constexpr (E == 8) {
+        Vec8<T>::store(p, v);
+    } else if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+        T t[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st(t + e, v[e]);
+        *reinterpret_cast<uint2*>(p) = make_uint2((uint32_t)t[0].x | ((uint32_t)t[1].x << 16),
+                                                  (uint32_t)t[2].x | ((uint32_t)t[3].x << 16));
+    }
+}
+
+// A wave per token: q and k roped and rounded, q to q_out, k and v into the token's
+// slot.  A lane takes E elements of a head and their partners half a head on, so that
+// each is loaded once.  Tokens behind the last give zeros, tokens of a row without room
+// or a page NaN; both are done here.  A copy with a little arithmetic: bound by the
+// bytes in and out.
+template <typename T, int E>
+__global__ void __launch_bounds__(256)
+paged_append_kernel(BatchArgs<T> a) {
+    const int t = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (t >= a.N) return;
+    const int row = a.rows_of[t], pos = a.positions[t], half = a.HD / 2;
+    const int64_t slot = a.slots_of[t], page = slot >> a.log_ps;
+    const bool fits = plan_fits(a);
+    const bool in = fits && row >= 0 && slot >= 0 && page < a.n_pages, turned = in && pos < a.n_pos && pos >= 0;
+    if (!turned) {
+        const float fill = row >= 0 || !fits ? NAN : 0.0f;
+        float v[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = fill;
+        for (int i = lane; i < a.QH * a.HD / E; i += 64) {
+            const int h = i * E / a.HD, d = i * E - h * a.HD;
+            store_e<T, E>(a.q_out + ((int64_t)t * a.QH + h) * a.HD + d, v);
+            // (the items write those of tokens that the plan has)
+            if (in) continue;
+            store_e<T, E>(a.c_out + t * a.out_ld + i * E, v);
+            if (a.k_out != nullptr) store_e<T, E>(a.k_out + t * a.out_ld + i * E, v);
+        }
+        if (lane == 0) a.odd[t] = 1;
+        return;
+    }
+    const T* x = a.qkv + t * a.qkv_ld;
+    const float *cr = a.cosv + (int64_t)pos * a.HD, *sr = a.sinv + (int64_t)pos * a.HD;
+    const int64_t at = page * a.ps_page + (slot & ((1 << a.log_ps) - 1)) * a.ps_tok;
+    const int per = half / E;
+    bool odd = false;
+    for (int i = lane; i < (a.QH + a.KVH) * per; i += 64) {
+        const int h = i / per, d = (i - h * per) * E;
+        float u[E], w[E], c0[E], s0[E], c1[E], s1[E], lo[E], hi[E];
+        load_e<T, E>(x + h * a.HD + d, u);
+        load_e<T, E>(x + h * a.HD + d + half, w);
+        load_e<float, E>(cr + d, c0);
+        load_e<float, E>(sr + d, s0);
+        load_e<float, E>(cr + d + half, c1);
+        load_e<float, E>(sr + d + half, s1);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            lo[e] = turn<T>(u[e], c0[e], -w[e], s0[e]);
+            hi[e] = turn<T>(w[e], c1[e], u[e], s1[e]);
+        }
+        T* out = h < a.QH ? a.q_out + ((int64_t)t * a.QH + h) * a.HD : a.kp + at + (h - a.QH) * a.ps_head;
+        store_e<T, E>(out + d, lo);
+        store_e<T, E>(out + d + half, hi);
+        if (h >= a.QH) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                odd |= !(fabsf(round_to<T>(lo[e])) < INFINITY) || !(fabsf(round_to<T>(hi[e])) < INFINITY);
+        }
+    }
+    const int vper = a.HD / E;
+    for (int i = lane; i < a.KVH * vper; i += 64) {
+        const int h = i / vper, d = (i - h * vper) * E;
+        float u[E];
+        load_e<T, E>(x + (a.QH + a.KVH + h) * a.HD + d, u);
+        store_e<T, E>(a.vp + at + h * a.ps_head + d, u);
+#pragma unroll
+        for (int e = 0; e < E; ++e) odd |= !(fabsf(u[e]) < INFINITY);
+    }
+    odd = __any(odd);
+    if (lane == 0) a.odd[t] = odd;
+}
+
+// What a block works on: its item, or nothing (seg < 0)
+struct PbWork {
+    PbSeg s;
+    PbItem it;
+    int kvh;
+    bool any;
+};
+
+template <typename T>
+__device__ __forceinline__ PbWork pb_work(const BatchArgs<T>& a) {
+    PbWork w;
+    const int n_items = min(a.plan[1], a.at.cap_items);
+    const int n = n_items * a.KVH, L = (int)blockIdx.x;
+    w.any = L < n && plan_fits(a);
+    if (!w.any) return w;
+    const int k = xcd_contiguous(L, n);
+    w.kvh = k / n_items;
+    auto uniform = [](auto v) {                      // the same in all lanes, which the compiler may not see
+        int* p = reinterpret_cast<int*>(&v);
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(v) / sizeof(int)); ++i) p[i] = __builtin_amdgcn_readfirstlane(p[i]);
+        return v;
+    };
+    w.it = uniform(reinterpret_cast<const PbItem*>(a.plan + a.at.items)[k - w.kvh * n_items]);
+    w.s = uniform(reinterpret_cast<const PbSeg*>(a.plan + a.at.segs)[w.it.seg]);
+    return w;
+}
+
+// Flat token of query x of a segment
+template <typename T>
+__device__ __forceinline__ int pb_token(const BatchArgs<T>& a, const PbSeg& s, int x) {
+    const int i = (s.x0 + x) / a.G;
+    return s.common ? a.plan[a.at.toks + s.base + i] : s.base + i;
+}
+
+// Positions that query x sees: all of a common segment, up to itself of its own row's
+template <typename T>
+__device__ __forceinline__ int pb_sees(const BatchArgs<T>& a, const PbSeg& s, int x) {
+    return s.common ? s.key1 : s.lens + (s.x0 + x) / a.G + 1;
+}
+
+// Whether a new token that some query of the block must not see, but others read with
+// it in one tile, holds an infinity or NaN: zero weights do not silence those in a
+// matrix product.  Such tokens lie from the first query's position on.
+template <typename T>
+__device__ __forceinline__ bool pb_odd(const BatchArgs<T>& a, const PbSeg& s) {
+    bool odd = false;
+    if (!s.common) {
+        const int last = (s.x0 + s.nq - 1) / a.G;
+        for (int i = s.x0 / a.G + 1 + threadIdx.x; i <= last; i += 256) odd |= a.odd[s.base + i] != 0;
+    }
+    return odd;
+}
+
+// The end of an item: the waves' (m, l, C, Kctx) from LDS joined into records, or into
+// the outputs where the queries have no other part.  part(w): the sums of wave w's 16
+// queries as its lanes hold them, C then Kctx, four queries' of one dimension side by
+// side; ml[w][16]: (m, l).  Query x is in the waves x / 16 + QW k.
+template <int HDP, bool KCTX, typename T, typename P>
+__device__ __forceinline__ void pb_finish(const BatchArgs<T>& a, const PbWork& w, int QW, const float2 (*ml)[16], P part) {
+    const PbSeg& s = w.s;
+    constexpr int quads = HDP / 4, per = KCTX ? 2 * quads : quads;
+    const int KW = 4 / QW;
+    for (int k = threadIdx.x; k < s.nq * per; k += 256) {
+        const int x = k / per, e = k - x * per, which = e >= quads, d = 4 * (e - which * quads);
+        const int w0 = x >> 4, j = x & 15;
+        float m = -INFINITY, l = 0.0f;
+        for (int g = 0; g < KW; ++g) m = fmaxf(m, ml[w0 + QW * g][j].x);
+        pg_f32x4 c = {0.f, 0.f, 0.f, 0.f};
+        for (int g = 0; g < KW; ++g) {
+            const float2 p = ml[w0 + QW * g][j];
+            const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(p.x - m);
+            // query j, dimension d: lane 16 (j / 4) + d % 16, element j % 4
+            const float* v = part(w0 + QW * g) + ((which * (HDP / 16) + (d >> 4)) * 64 + (j >> 2) * 16 + (d & 15)) * 4 + (j & 3);
+            l = fmaf(p.y, f, l);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[i] = fmaf(v[4 * i], f, c[i]);
+        }
+        if (s.rec0 < 0) {
+            if (HDP > a.HD && d >= a.HD) continue;
+            const int h = w.kvh * a.G + (s.x0 + x) % a.G;
+            T* out = (which ? a.k_out : a.c_out) + (int64_t)pb_token(a, s, x) * a.out_ld + (int64_t)h * a.HD + d;
+            const float inv = 1.0f / l;
+            const float o[4] = {c[0] * inv, c[1] * inv, c[2] * inv, c[3] * inv};
+            store_e<T, 4>(out, o);
+        } else {
+            const int64_t r = w.kvh * a.at.cap_recs + s.rec0 + w.it.chunk * s.nq + x;
+            *reinterpret_cast<pg_f32x4*>(a.rec + (r * 2 + which) * HDP + d) = c;
+            if (e == 0) *reinterpret_cast<float2*>(a.rec + a.rec_ml + 2 * r) = make_float2(m, l);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ matrix-core form
+// 16-bit types, HD 32 / 64 / 96 / 128.  Four waves stream 64 positions per step through
+// NS LDS stages that loads fill directly, one barrier per step; a 16-position quarter of
+// a tile lies in one page (pages hold a multiple of 16 positions), staged by one wave, so
+// its base and its bound are scalar: rows past the item's end land as zeros.  QW waves
+// side by side take 16 queries each, and the KW = 4 / QW groups of them a quarter, half
+// or all of the positions: one query block of 1 to 16, of 17 to 32 or of more, so that a
+// decode step's few queries use all waves too.  S^T = K Q^T, P from the score registers,
+// C = P V and Kctx = P K through the transposing LDS read.
+template <int HD> constexpr int pb_stages() { return HD <= 96 ? 3 : 2; }
+
+template <typename T, int HD, bool KCTX>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+paged_items_kernel(BatchArgs<T> a) {
+    constexpr int KK = HD / 32, DT = HD / 16, CPR = HD / 8, NS = pb_stages<HD>(), GPW = CPR / 4, R = kPbTile;
+    // a stage per array, so that a wait for one stage's loads never covers another's reads
+    __shared__ __align__(16) gqa_u4 K0[R * CPR], V0[R * CPR], K1[R * CPR], V1[R * CPR];
+    __shared__ __align__(16) gqa_u4 K2[NS == 3 ? R * CPR : 1], V2[NS == 3 ? R * CPR : 1];
+    __shared__ float2 ml[4][16];
+    using M = Mfma16<T>;
+    const PbWork w = pb_work(a);
+    if (!w.any) return;
+    const PbSeg& s = w.s;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int lr = lane & 15, lq = lane >> 4;
+    const int QW = s.nq <= 16 ? 1 : s.nq <= 32 ? 2 : 4;
+    const int qt = wave & (QW - 1), kg = wave / QW;
+    const TileLane<CPR> tl(lq, lr);
+    const int kend = min(s.key1, s.key0 + w.it.tile1 * R);
+    const int32_t* trow = a.table + (int64_t)s.row * a.table_ld;
+
+    // pages of this wave's quarter of the tiles jb .. jb + 63, one per lane
+    int jb = w.it.tile0, pgv;
+    auto pages = [&]() {
+        const int64_t t = (int64_t)s.key0 + (int64_t)(jb + lane) * R + 16 * wave;
+        pgv = trow[min(t, (int64_t)a.cap - 1) >> a.log_ps];
+    };
+    pages();
+    const int x = 16 * qt + lr, xq = min(x, s.nq - 1);
+    const bool odd_mine = pb_odd(a, s);
+    uint4 qf[KK];
+    {
+        const T* q = a.q_out + ((int64_t)pb_token(a, s, xq) * a.QH + w.kvh * a.G + (s.x0 + xq) % a.G) * HD + 8 * lq;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const uint4*>(q + 32 * kk);
+    }
+    const int sees = min(pb_sees(a, s, xq), kend);              // (lanes without a query: the last one's)
+    const int sees_first = __builtin_amdgcn_readfirstlane(min(pb_sees(a, s, min(16 * qt, s.nq - 1)), kend));
+    const int sees_last = __builtin_amdgcn_readfirstlane(min(pb_sees(a, s, min(16 * qt + 15, s.nq - 1)), kend));
+    const bool idle = 16 * qt >= s.nq;                          // no query in this wave
+    uint32_t voff[GPW];
+#pragma unroll
+    for (int j = 0; j < GPW; ++j) {
+        const int p = 64 * j + lane, row = p / CPR, c = p - row * CPR;
+        voff[j] = (uint32_t)(row * (int)a.ps_tok * (int)sizeof(T)) + (uint32_t)(c ^ kv_swz(row)) * 16u;
+    }
+    auto kst = [&](auto s_) -> gqa_u4* {
+        constexpr int I = decltype(s_)::value;
+        return I == 0 ? K0 : I == 1 ? K1 : K2;
+    };
+    auto vst = [&](auto s_) -> gqa_u4* {
+        constexpr int I = decltype(s_)::value;
+        return I == 0 ? V0 : I == 1 ? V1 : V2;
+    };
+    // this wave's quarter of tile j, 2 GPW loads (past the item's end: zeros)
+    auto load_tile = [&](auto s_, int j) {
+        const int t = s.key0 + j * R + 16 * wave;
+        const int rows = j < w.it.tile1 ? min(16, kend - t) : 0;
+        int bytes = 0;
+        int64_t off = 0;
+        if (rows > 0) {
+            if (j - jb >= 64) {
+                jb += 64;
+                pages();
+            }
+            const int page = __builtin_amdgcn_readlane(pgv, j - jb);
+            if ((unsigned)page < (unsigned)a.n_pages) {          // (all are, unless the table changed since the plan)
+                bytes = ((rows - 1) * (int)a.ps_tok + HD) * (int)sizeof(T);
+                off = (int64_t)page * a.ps_page + (int64_t)(t & ((1 << a.log_ps) - 1)) * a.ps_tok + w.kvh * a.ps_head;
+            }
+        }
+        const auto rk = __builtin_amdgcn_make_buffer_rsrc((void*)(a.kp + off), (short)0, bytes, kBufferDword3);
+        const auto rv = __builtin_amdgcn_make_buffer_rsrc((void*)(a.vp + off), (short)0, bytes, kBufferDword3);
+#pragma unroll
+        for (int i = 0; i < GPW; ++i) {
+            dma16(rk, kst(s_) + 64 * (wave * GPW + i), voff[i], 0);
+            dma16(rv, vst(s_) + 64 * (wave * GPW + i), voff[i], 0);
+        }
+    };
+    using S0 = std::integral_constant<int, 0>;
+    using S1 = std::integral_constant<int, 1>;
+    using S2 = std::integral_constant<int, 2>;
+    const bool odd = __syncthreads_or(odd_mine);
+
+    float mh = -INFINITY, lh = 0.0f;
+    pg_f32x4 accC[DT], accK[KCTX ? DT : 1];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) accC[dt] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int dt = 0; dt < (KCTX ? DT : 1); ++dt) accK[dt] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
+
+    auto body = [&](auto kw_) {
+        constexpr int KW = decltype(kw_)::value, NHF = 4 / KW;   // 16-row parts of a tile per wave
+        auto fold = [&](const gqa_u4* tk, const gqa_u4* tv, int r0) __attribute__((always_inline)) {
+            pg_f32x4 sc[NHF];
+#pragma unroll
+            for (int hf = 0; hf < NHF; ++hf) {
+                sc[hf] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk)
+                    sc[hf] = M::dot(__builtin_bit_cast(uint4, tile_s_frag<CPR>(tk + (hf >> 1) * 32 * CPR, tl, hf & 1, kk)),
+                                    qf[kk], sc[hf]);
+            }
+            const bool mask = r0 + 16 * NHF > sees_first;        // wave-uniform
+            float mx = -INFINITY;
+            if (mask) {
+#pragma unroll
+                for (int hf = 0; hf < NHF; ++hf)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (r0 + 16 * hf + 4 * lq + r >= sees) sc[hf][r] = -INFINITY;
+            }
+#pragma unroll
+            for (int hf = 0; hf < NHF; ++hf)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[hf][r]);
+            mx = max_16_32(mx) * a.qscale;
+            const float mnew = raised(mh, mx - M::kShift, M::kLag);
+            const float corr = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mh - mnew);
+            const float off = mnew == -INFINITY ? 0.0f : -mnew;  // (nothing seen yet: e^-inf, not e^NaN)
+            float ls = 0.0f, pv[NHF][4];
+#pragma unroll
+            for (int hf = 0; hf < NHF; ++hf)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    pv[hf][r] = __builtin_amdgcn_exp2f(fmaf(sc[hf][r], a.qscale, off));
+                    ls += pv[hf][r];
+                }
+            lh = fmaf(lh, corr, sum_16_32(ls));
+            const bool rescale = corr != 1.0f && mh != -INFINITY;     // (before, the sums are zero)
+            mh = mnew;
+            if (__any(rescale)) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float cf = __shfl(corr, 4 * lq + r, 64);
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        accC[dt][r] *= cf;
+                        if constexpr (KCTX) accK[dt][r] *= cf;
+                    }
+                }
+            }
+            if (odd && mask) {
+                // one position at a time, with only the queries that see it
+#pragma unroll 1
+                for (int row = 0; row < 16 * NHF; ++row) {
+                    float mine = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 4 * NHF; ++i) mine = (row >> 4) * 4 + (row & 3) == i ? pv[i / 4][i % 4] : mine;
+                    const int g = (row >> 2) & 3;
+                    float p[4];
+                    bool seen[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        p[i] = __shfl(mine, 16 * g + 4 * lq + i, 64);
+                        seen[i] = r0 + row < __shfl(sees, 4 * lq + i, 64);
+                    }
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        const int d = 16 * dt + lr, at = row * CPR + ((d >> 3) ^ kv_swz(row));
+                        const float v = ld(reinterpret_cast<const T*>(tv + at) + (d & 7));
+                        const float k = KCTX ? ld(reinterpret_cast<const T*>(tk + at) + (d & 7)) : 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            accC[dt][i] = seen[i] ? fmaf(p[i], v, accC[dt][i]) : accC[dt][i];
+                            if constexpr (KCTX) accK[dt][i] = seen[i] ? fmaf(p[i], k, accK[dt][i]) : accK[dt][i];
+                        }
+                    }
+                }
+                return;
+            }
+            // the weights enter the products rounded to the storage type (half a step of
+            // it, relative, per weight, down to Mfma16's smallest: below the rounding of
+            // the outputs); their sum l is that of the unrounded ones
+#pragma unroll
+            for (int u = 0; u < (NHF + 1) / 2; ++u) {
+                uint4 pa = make_uint4(M::pack(pv[2 * u][0], pv[2 * u][1]), M::pack(pv[2 * u][2], pv[2 * u][3]), 0, 0);
+                if constexpr (NHF > 1) {
+                    pa.z = M::pack(pv[2 * u + 1][0], pv[2 * u + 1][1]);
+                    pa.w = M::pack(pv[2 * u + 1][2], pv[2 * u + 1][3]);
+                }
+                auto frag = [&](const gqa_u4* tile, int dt) __attribute__((always_inline)) {
+                    if constexpr (NHF > 1) {
+                        return tile_tr_frag<CPR>(tile + u * 32 * CPR, tl, dt);
+                    } else {                         // 16 rows: the other half meets zero weights
+                        const char* p = reinterpret_cast<const char*>(tile) + tl.t_off[dt & 1][0] + 64 * (dt >> 1);
+                        const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                                       (__attribute__((address_space(3))) gqa_v4s*)(p)));
+                        return make_uint4(lo.x, lo.y, 0, 0);
+                    }
+                };
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    accC[dt] = M::dot(pa, frag(tv, dt), accC[dt]);
+                    if constexpr (KCTX) accK[dt] = M::dot(pa, frag(tk, dt), accK[dt]);
+                }
+            }
+        };
+        // step j computes tile j from stage j % NS, requests tile j + NS - 1 into the stage
+        // that every wave is done with, waits for tile j + 1 and passes one barrier
+        auto step = [&](auto s_, int j) {
+            constexpr int cur = decltype(s_)::value;
+            load_tile(std::integral_constant<int, (cur + NS - 1) % NS>{}, j + NS - 1);
+            const int r0 = s.key0 + j * R + kg * (R / KW);
+            if (j < w.it.tile1 && !idle && r0 < sees_last)
+                fold(kst(s_) + kg * (R / KW) * CPR, vst(s_) + kg * (R / KW) * CPR, r0);
+            wait_vmcnt<2 * GPW * (NS - 2)>();
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        };
+        load_tile(S0{}, w.it.tile0);
+        if constexpr (NS == 3) load_tile(S1{}, w.it.tile0 + 1);
+        wait_vmcnt<2 * GPW * (NS - 2)>();
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+            asm volatile("" : "+v"(qf[kk].x), "+v"(qf[kk].y), "+v"(qf[kk].z), "+v"(qf[kk].w));
+        for (int j = w.it.tile0; j < w.it.tile1; j += NS) {
+            step(S0{}, j);
+            step(S1{}, j + 1);
+            if constexpr (NS == 3) step(S2{}, j + 2);
+        }
+    };
+    if (QW == 4) body(std::integral_constant<int, 1>{});
+    else if (QW == 2) body(std::integral_constant<int, 2>{});
+    else body(std::integral_constant<int, 4>{});
+    wait_vmcnt<0>();                                 // no load into LDS outlives the loop
+    __syncthreads();
+    // wave w's sums in the w-th of four stage arrays, whose size they have
+    static_assert(16 * 2 * HD * sizeof(float) == sizeof(K0), "a wave's sums fill a stage");
+    auto part = [&](int i) { return reinterpret_cast<float*>(i == 0 ? K0 : i == 1 ? V0 : i == 2 ? K1 : V1); };
+    if (lq == 0) ml[wave][lr] = make_float2(mh, lh);
+    pg_f32x4* mine = reinterpret_cast<pg_f32x4*>(part(wave)) + lane;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+        mine[64 * dt] = accC[dt];
+        if constexpr (KCTX) mine[64 * (DT + dt)] = accK[dt];
+    }
+    __syncthreads();
+    pb_finish<HD, KCTX>(a, w, QW, ml, part);
+}
+
+// ------------------------------------------------------------------ fp32 form
+// fp32 (whose products stay in fp32, on v_mfma_f32_16x16x4) and the head sizes the form
+// above does not take, converted to fp32 as they are staged.  The same waves and query
+// blocks; RT positions per step in one LDS buffer, the next ones in flight in registers.
+// The products' operands may take the dimensions in any order that both share: lane
+// group lq takes HD / 4 neighbouring ones of them, so that a lane's are 16-byte reads.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256)
+paged_items_f32_kernel(BatchArgs<T> a) {
+    constexpr int HDP = HD < 16 ? 16 : HD;           // heads of 8 are filled up with zeros
+    constexpr int RT = HDP <= 128 ? 64 : 32, PITCH = HDP + 4, Q4 = HDP / 16, DT = HDP / 16;
+    constexpr int EP = 16 / sizeof(T), PR = HD / EP; // elements of a 16-byte piece, pieces of a row
+    constexpr int NP = (RT * PR + 255) / 256;        // pieces per thread and tensor
+    constexpr int kTile = 2 * RT * PITCH, kRed = 4 * 16 * 2 * HDP;
+    __shared__ __align__(16) float lds[kTile > kRed ? kTile : kRed];
+    __shared__ float2 ml[4][16];
+    const PbWork w = pb_work(a);
+    if (!w.any) return;
+    const PbSeg& s = w.s;
+    const bool kctx = a.k_out != nullptr;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int lr = lane & 15, lq = lane >> 4;
+    const int QW = s.nq <= 16 ? 1 : s.nq <= 32 ? 2 : 4, KW = 4 / QW;
+    const int qt = wave & (QW - 1), kg = wave / QW;
+    const int k0 = s.key0 + w.it.tile0 * kPbTile, kend = min(s.key1, s.key0 + w.it.tile1 * kPbTile);
+    const int32_t* trow = a.table + (int64_t)s.row * a.table_ld;
+    const int ps_mask = (1 << a.log_ps) - 1;
+    float* const tk = lds;
+    float* const tv = lds + RT * PITCH;
+    if constexpr (HDP > HD) {
+        for (int i = tid; i < kTile; i += 256) lds[i] = 0.0f;
+        __syncthreads();
+    }
+    // pages of 64 runs of 16 positions from jb on, one per lane
+    int jb = k0, pgv;
+    auto pages = [&]() { pgv = trow[min((int64_t)jb + 16 * lane, (int64_t)a.cap - 1) >> a.log_ps]; };
+    pages();
+    const int x = 16 * qt + lr, xq = min(x, s.nq - 1);
+    const bool odd_mine = pb_odd(a, s);
+    // q of column lr, dimensions lq HDP / 4 ..
+    float qf[HDP / 4];
+    {
+        const T* q = a.q_out + ((int64_t)pb_token(a, s, xq) * a.QH + w.kvh * a.G + (s.x0 + xq) % a.G) * HD;
+#pragma unroll
+        for (int i = 0; i < HDP / 4; ++i) {
+            const int d = lq * (HDP / 4) + i;
+            qf[i] = d < HD ? ld(q + d) : 0.0f;
+        }
+    }
+    const int sees = min(pb_sees(a, s, xq), kend);
+    const int sees_first = __builtin_amdgcn_readfirstlane(min(pb_sees(a, s, min(16 * qt, s.nq - 1)), kend));
+    const int sees_last = __builtin_amdgcn_readfirstlane(min(pb_sees(a, s, min(16 * qt + 15, s.nq - 1)), kend));
+    const bool idle = 16 * qt >= s.nq;
+    u32x4 kr[NP], vr[NP];
+    auto load = [&](int t0) {                        // positions t0 .. t0 + RT - 1
+        if (t0 < kend && t0 - jb >= 16 * 64) {
+            jb += 16 * 64;
+            pages();
+        }
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int p = i * 256 + tid, row = p / PR, c = p - row * PR, t = t0 + row;
+            const int page = __shfl(pgv, ((t - jb) >> 4) & 63, 64);
+            kr[i] = vr[i] = u32x4{0, 0, 0, 0};
+            if (row < RT && t < kend && (unsigned)page < (unsigned)a.n_pages) {
+                const int64_t off = (int64_t)page * a.ps_page + (int64_t)(t & ps_mask) * a.ps_tok + w.kvh * a.ps_head + c * EP;
+                kr[i] = *reinterpret_cast<const u32x4*>(a.kp + off);
+                vr[i] = *reinterpret_cast<const u32x4*>(a.vp + off);
+            }
+        }
+    };
+    auto put = [&](float* at, u32x4 v) {
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<u32x4*>(at) = v;
+        } else {
+            float f[8];
+            Vec8<T>::load(reinterpret_cast<const T*>(&v), f);
+            Vec8<float>::store(at, f);
+        }
+    };
+    const bool odd = __syncthreads_or(odd_mine);
+    float mh = -INFINITY, lh = 0.0f;
+    pg_f32x4 accC[DT], accK[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) accC[dt] = accK[dt] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
+    load(k0);
+    for (int t0 = k0; t0 < kend; t0 += RT) {
+        __syncthreads();                             // the tile's last reads
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int p = i * 256 + tid, row = p / PR, c = p - row * PR;
+            if (row < RT) {
+                put(tk + row * PITCH + c * EP, kr[i]);
+                put(tv + row * PITCH + c * EP, vr[i]);
+            }
+        }
+        load(t0 + RT);
+        lds_barrier();
+        if (idle) continue;
+        for (int hf = kg; hf < RT / 16; hf += KW) {
+            const int r0 = t0 + 16 * hf;
+            if (r0 >= sees_last) break;              // (a wave's: uniform)
+            pg_f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+            const float* kq = tk + (16 * hf + lr) * PITCH + lq * (HDP / 4);
+#pragma unroll
+            for (int i = 0; i < Q4; ++i) {
+                const pg_f32x4 kx = *reinterpret_cast<const pg_f32x4*>(kq + 4 * i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[e], qf[4 * i + e], sc, 0, 0, 0);
+            }
+            const bool mask = r0 + 16 > sees_first;
+            float mx = -INFINITY, pv[4], ls = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (mask && r0 + 4 * lq + r >= sees) sc[r] = -INFINITY;
+                mx = fmaxf(mx, sc[r]);
+            }
+            mx = max_16_32(mx) * a.qscale;
+            const float mnew = raised(mh, mx);
+            const float corr = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mh - mnew);
+            const float off = mnew == -INFINITY ? 0.0f : -mnew;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                pv[r] = __builtin_amdgcn_exp2f(fmaf(sc[r], a.qscale, off));
+                ls += pv[r];
+            }
+            lh = fmaf(lh, corr, sum_16_32(ls));
+            const bool rescale = corr != 1.0f && mh != -INFINITY;
+            mh = mnew;
+            if (__any(rescale)) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float cf = __shfl(corr, 4 * lq + r, 64);
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        accC[dt][r] *= cf;
+                        accK[dt][r] *= cf;
+                    }
+                }
+            }
+            if (odd && mask) {
+                // one position at a time, with only the queries that see it
+#pragma unroll 1
+                for (int n = 0; n < 16; ++n) {
+                    const int row = 16 * hf + n;
+                    const float own = (n & 3) == 0 ? pv[0] : (n & 3) == 1 ? pv[1] : (n & 3) == 2 ? pv[2] : pv[3];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float p = __shfl(own, 16 * (n >> 2) + 4 * lq + i, 64);
+                        const bool seen = t0 + row < __shfl(sees, 4 * lq + i, 64);
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt) {
+                            const float v = tv[row * PITCH + 16 * dt + lr], k = tk[row * PITCH + 16 * dt + lr];
+                            accC[dt][i] = seen ? fmaf(p, v, accC[dt][i]) : accC[dt][i];
+                            accK[dt][i] = seen ? fmaf(p, k, accK[dt][i]) : accK[dt][i];
+                        }
+                    }
+                }
+                continue;
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float* vq = tv + (16 * hf + 4 * lq + r) * PITCH + lr;
+                const float* kx = tk + (16 * hf + 4 * lq + r) * PITCH + lr;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    accC[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[r], vq[16 * dt], accC[dt], 0, 0, 0);
+                    if (kctx) accK[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[r], kx[16 * dt], accK[dt], 0, 0, 0);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    auto part = [&](int i) { return lds + i * 16 * 2 * HDP; };
+    if (lq == 0) ml[wave][lr] = make_float2(mh, lh);
+    pg_f32x4* mine = reinterpret_cast<pg_f32x4*>(part(wave)) + lane;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+        mine[64 * dt] = accC[dt];
+        mine[64 * (DT + dt)] = accK[dt];
+    }
+    __syncthreads();
+    if (kctx) pb_finish<HDP, true>(a, w, QW, ml, part);
+    else pb_finish<HDP, false>(a, w, QW, ml, part);
+}
+
+// ------------------------------------------------------------------ the join
+// Four queries of an own segment per task: their records are the chunks of the segment
+// itself and of the group's segment that holds them.  Wave w takes records w, w + 4, ..
+// of all four queries, 2 kPbJoin in flight each; the waves meet in LDS.
+constexpr int kPbJoin = 2;
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(256)
+paged_batch_join_kernel(BatchArgs<T> a) {
+    constexpr int HDP = HD < 16 ? 16 : HD;
+    constexpr int NV = HDP > 128 ? 2 : 1, NL = HDP / 2 / NV;   // lanes of four sums
+    __shared__ float2 ml[4][4];
+    __shared__ __align__(16) float sums[4][4][2 * HDP];
+    if (!plan_fits(a)) return;
+    const int n_tasks = min(a.plan[2], a.at.cap_joins) * a.KVH, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int n_joins = n_tasks / a.KVH;
+    const bool kctx = a.k_out != nullptr;
+    for (int task = blockIdx.x; task < n_tasks; task += gridDim.x) {
+        const int kvh = task / n_joins;
+        const int2 jt = reinterpret_cast<const int2*>(a.plan + a.at.joins)[task - kvh * n_joins];
+        const PbSeg s = reinterpret_cast<const PbSeg*>(a.plan + a.at.segs)[jt.x];
+        const int x0 = jt.y, nx = min(4, s.nq - x0);
+        // the group's records of each query: (first, distance), and how many
+        int64_t common[4];
+        int step[4], nc = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            common[i] = 0;
+            step[i] = 0;
+            if (s.pseg0 < 0) continue;
+            const int gx = s.gx0 + s.x0 + x0 + min(i, nx - 1);
+            const PbSeg& p = reinterpret_cast<const PbSeg*>(a.plan + a.at.segs)[s.pseg0 + gx / kPbQ];
+            common[i] = p.rec0 + gx % kPbQ;
+            step[i] = p.nq;
+            nc = max(nc, p.nchunk);                  // (segments of a group have the same positions, so as many)
+        }
+        const int n = nc + s.nchunk;
+        float M[4], L[4];
+        pg_f32x4 acc[4][NV];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            M[i] = -INFINITY;
+            L[i] = 0.0f;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) acc[i][v] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        for (int c0 = wave; c0 < n; c0 += 4 * kPbJoin) {
+            float2 e[kPbJoin][4];
+            pg_f32x4 y[kPbJoin][4][NV];
+#pragma unroll
+            for (int u = 0; u < kPbJoin; ++u) {
+                const int c = min(c0 + 4 * u, n - 1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int64_t r = kvh * a.at.cap_recs +
+                                      (c < nc ? common[i] + (int64_t)c * step[i] : s.rec0 + (int64_t)(c - nc) * s.nq + x0 + min(i, nx - 1));
+                    e[u][i] = *reinterpret_cast<const float2*>(a.rec + a.rec_ml + 2 * r);
+#pragma unroll
+                    for (int v = 0; v < NV; ++v)
+                        if (lane < NL) y[u][i][v] = *reinterpret_cast<const pg_f32x4*>(a.rec + r * 2 * HDP + 4 * (lane + NL * v));
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kPbJoin; ++u) {
+                if (c0 + 4 * u >= n) continue;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float m = fmaxf(M[i], e[u][i].x);
+                    const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M[i] - m);
+                    const float g = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(e[u][i].x - m);
+                    L[i] = fmaf(L[i], f, e[u][i].y * g);
+#pragma unroll
+                    for (int v = 0; v < NV; ++v)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) acc[i][v][k] = fmaf(acc[i][v][k], f, y[u][i][v][k] * g);
+                    M[i] = m;
+                }
+            }
+        }
+        __syncthreads();                             // the last task's sums are read
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (lane == 0) ml[i][wave] = make_float2(M[i], L[i]);
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                if (lane < NL) *reinterpret_cast<pg_f32x4*>(&sums[i][wave][4 * (lane + NL * v)]) = acc[i][v];
+        }
+        __syncthreads();
+        constexpr int quads = HDP / 4;
+        const int per = kctx ? 2 * quads : quads;
+        for (int k = threadIdx.x; k < nx * per; k += 256) {
+            const int i = k / per, d2 = 4 * (k - i * per), which = d2 >= HDP, d = d2 - which * HDP;
+            if (HDP > HD && d >= HD) continue;
+            float m = -INFINITY, l = 0.0f;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) m = fmaxf(m, ml[i][v].x);
+            float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml[i][v].x - m);
+                l = fmaf(ml[i][v].y, f, l);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) o[q] = fmaf(sums[i][v][d2 + q], f, o[q]);
+            }
+            const float inv = 1.0f / l;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) o[q] *= inv;
+            const int x = s.x0 + x0 + i, h = kvh * a.G + x % a.G;
+            store_e<T, 4>((which ? a.k_out : a.c_out) + (int64_t)(s.base + x / a.G) * a.out_ld + (int64_t)h * HD + d, o);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ host side
+
+static int batch_sizes(const char* who, int64_t R, int64_t N, int64_t QH, int64_t KVH, int64_t NP, int64_t PS, int64_t MP,
+                       int64_t table_ld) {
+    LOOM_CHECK(R >= 0 && R <= kPbMaxRows, "%s: 0 to %d rows, got %lld", who, kPbMaxRows, (long long)R);
+    LOOM_CHECK(N >= 0 && N <= kPbMaxTokens, "%s: 0 to %lld tokens, got %lld", who, (long long)kPbMaxTokens, (long long)N);
+    LOOM_CHECK(KVH >= 1 && QH >= KVH && QH <= 1024 && QH % KVH == 0, "%s: bad heads QH=%lld KVH=%lld", who,
+               (long long)QH, (long long)KVH);
+    LOOM_CHECK(PS >= 16 && PS <= 1024 && (PS & (PS - 1)) == 0, "%s: page_size must be a power of two from 16 to 1024, got %lld",
+               who, (long long)PS);
+    LOOM_CHECK(NP >= 1 && NP < ((int64_t)1 << 30), "%s: bad n_pages %lld", who, (long long)NP);
+    LOOM_CHECK(MP >= 1 && MP <= ((int64_t)1 << 24) / PS && table_ld >= MP,
+               "%s: the table must hold 1 page to 2^24 tokens per row (max_pages=%lld, row stride %lld)", who,
+               (long long)MP, (long long)table_ld);
+    return LOOM_OK;
+}
+
+struct BatchCall {
+    const void* qkv;
+    int64_t qkv_ld;
+    void *kp, *vp;
+    int64_t page_stride, token_stride, head_stride, n_pages, page_size;
+    const int32_t* table;
+    int64_t table_ld, max_pages, rows;
+    const int32_t *rows_of, *positions;
+    const int64_t* slots;
+    const void* plan;
+    int64_t plan_bytes;
+    const float *cosv, *sinv;
+    int64_t n_pos;
+    void *q_out, *c_out, *k_out;
+    int64_t out_ld;
+    void* ws;
+    int64_t ws_bytes, N, QH, KVH, HD;
+};
+
+static int64_t pb_rec_floats(const PbLayout& at, int64_t KVH, int64_t HD) {
+    const int64_t HDP = HD < 16 ? 16 : HD;
+    return KVH * at.cap_recs * (2 * HDP + 2);
+}
+
+template <typename T>
+static int batch_launch(const BatchCall& c, hipStream_t st) {
+    BatchArgs<T> a{};
+    a.qkv = (const T*)c.qkv;
+    a.qkv_ld = c.qkv_ld;
+    a.kp = (T*)c.kp;
+    a.vp = (T*)c.vp;
+    a.ps_page = c.page_stride;
+    a.ps_tok = c.token_stride;
+    a.ps_head = c.head_stride;
+    a.table = c.table;
+    a.table_ld = c.table_ld;
+    a.positions = c.positions;
+    a.rows_of = c.rows_of;
+    a.slots_of = c.slots;
+    a.cosv = c.cosv;
+    a.sinv = c.sinv;
+    a.q_out = (T*)c.q_out;
+    a.c_out = (T*)c.c_out;
+    a.k_out = (T*)c.k_out;
+    a.out_ld = c.out_ld;
+    a.plan = (const int32_t*)c.plan;
+    a.at = pb_layout(c.rows, c.N, c.QH, c.KVH);
+    a.rec = (float*)c.ws;
+    const int64_t HDP = c.HD < 16 ? 16 : c.HD;
+    a.rec_ml = c.KVH * a.at.cap_recs * 2 * HDP;
+    a.odd = (uint8_t*)((float*)c.ws + pb_rec_floats(a.at, c.KVH, c.HD));
+    a.R = (int)c.rows;
+    a.N = (int)c.N;
+    a.QH = (int)c.QH;
+    a.KVH = (int)c.KVH;
+    a.G = (int)(c.QH / c.KVH);
+    a.HD = (int)c.HD;
+    a.log_ps = __builtin_ctzll((unsigned long long)c.page_size);
+    a.cap = (int)(c.max_pages * c.page_size);
+    a.n_pages = (int)c.n_pages;
+    a.n_pos = (int)min(c.n_pos, (int64_t)1 << 30);
+    a.qscale = kLog2e / sqrtf((float)c.HD);
+    const dim3 appends((unsigned)ceil_div(c.N, 4));
+    if (c.HD >= 16) hipLaunchKernelGGL((paged_append_kernel<T, 8>), appends, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((paged_append_kernel<T, 4>), appends, dim3(256), 0, st, a);
+    if (int rc = launch_status("loom_paged_batch_step(append)")) return rc;
+    const dim3 grid((unsigned)(a.at.cap_items * c.KVH));
+    bool done = false;
+    if constexpr (sizeof(T) == 2) {
+#define LOOM_PB_M(HDV)                                                                              \
+        if (c.HD == HDV) {                                                                          \
+            if (c.k_out) hipLaunchKernelGGL((paged_items_kernel<T, HDV, true>), grid, dim3(256), 0, st, a); \
+            else hipLaunchKernelGGL((paged_items_kernel<T, HDV, false>), grid, dim3(256), 0, st, a); \
+            done = true;                                                                            \
+        }
+        LOOM_PB_M(96) LOOM_PB_M(128) LOOM_PB_M(64) LOOM_PB_M(32)
+#undef LOOM_PB_M
+#define LOOM_PB_F(HDV)                                                                              \
+        if (c.HD == HDV) {                                                                          \
+            hipLaunchKernelGGL((paged_items_f32_kernel<T, HDV>), grid, dim3(256), 0, st, a);        \
+            done = true;                                                                            \
+        }
+        LOOM_PB_F(8) LOOM_PB_F(16) LOOM_PB_F(256)
+    } else {
+        LOOM_PB_F(96) LOOM_PB_F(128) LOOM_PB_F(64) LOOM_PB_F(32) LOOM_PB_F(16) LOOM_PB_F(8) LOOM_PB_F(256)
+#undef LOOM_PB_F
+    }
+    LOOM_CHECK(done, "paged_batch_step: unsupported head_dim %lld (8, 16, 32, 64, 96, 128 or 256)", (long long)c.HD);
+    if (int rc = launch_status("loom_paged_batch_step(items)")) return rc;
+    const int64_t joins = (int64_t)a.at.cap_joins * c.KVH;
+    const dim3 jgrid((unsigned)(joins < 2048 ? joins : 2048));
+#define LOOM_PB_J(HDV)                                                                              \
+    if (c.HD == HDV) hipLaunchKernelGGL((paged_batch_join_kernel<T, HDV>), jgrid, dim3(256), 0, st, a);
+    LOOM_PB_J(96) LOOM_PB_J(128) LOOM_PB_J(64) LOOM_PB_J(32) LOOM_PB_J(16) LOOM_PB_J(8) LOOM_PB_J(256)
+#undef LOOM_PB_J
+    return launch_status("loom_paged_batch_step(join)");
+}
+
+}  // namespace loom
+
+using namespace loom;
+
+extern "C" int64_t loom_paged_plan_bytes(int64_t rows, int64_t n_tokens, int64_t QH, int64_t KVH) {
+    if (rows < 0 || rows > kPbMaxRows || n_tokens < 0 || n_tokens > kPbMaxTokens || KVH < 1 || QH < KVH || QH > 1024 || QH % KVH != 0)
+        return 0;
+    return pb_layout(rows, n_tokens, QH, KVH).total * (int64_t)sizeof(int32_t);
+}
+
+extern "C" int loom_paged_plan(const int32_t* table, int64_t table_ld, int64_t max_pages, int64_t n_pages, int64_t page_size,
+                               const int32_t* lens, const int32_t* new_tokens, int64_t rows, int64_t n_tokens, int64_t QH,
+                               int64_t KVH, int32_t* starts, int32_t* rows_of, int32_t* positions, int64_t* slots,
+                               int32_t* shared, void* plan, int64_t plan_bytes, void* stream) {
+    clear_error();
+    const char* who = "paged_plan";
+    if (int rc = batch_sizes(who, rows, n_tokens, QH, KVH, n_pages, page_size, max_pages, table_ld)) return rc;
+    LOOM_CHECK(((table && lens && new_tokens && shared) || rows == 0) && starts && ((rows_of && positions && slots) || n_tokens == 0),
+               "%s: a required pointer is NULL", who);
+    const int64_t need = loom_paged_plan_bytes(rows, n_tokens, QH, KVH);
+    LOOM_CHECK(plan != nullptr && plan_bytes >= need && ((uintptr_t)plan % 64) == 0,
+               "%s: a 64-byte aligned plan of %lld bytes is needed, got %lld", who, (long long)need, (long long)plan_bytes);
+    PlanArgs a{};
+    a.table = table;
+    a.table_ld = table_ld;
+    a.lens = lens;
+    a.fresh = new_tokens;
+    a.starts = starts;
+    a.rows_of = rows_of;
+    a.positions = positions;
+    a.shared = shared;
+    a.slots_of = slots;
+    a.plan = (int32_t*)plan;
+    a.at = pb_layout(rows, n_tokens, QH, KVH);
+    a.R = (int)rows;
+    a.N = (int)n_tokens;
+    a.QH = (int)QH;
+    a.KVH = (int)KVH;
+    a.G = (int)(QH / KVH);
+    a.log_ps = __builtin_ctzll((unsigned long long)page_size);
+    a.cap = (int)(max_pages * page_size);
+    a.n_pages = (int)n_pages;
+    hipStream_t st = (hipStream_t)stream;
+    if (rows > 0) {
+        hipLaunchKernelGGL(paged_rows_kernel, dim3((unsigned)ceil_div(rows, 16)), dim3(1024), 0, st, a);
+        if (int rc = launch_status("loom_paged_plan(rows)")) return rc;
+    }
+    hipLaunchKernelGGL(paged_plan_kernel, dim3((unsigned)(1 + ceil_div(n_tokens, 1024))), dim3(1024), 0, st, a);
+    return launch_status("loom_paged_plan(plan)");
+}
+
+extern "C" int64_t loom_paged_batch_workspace_bytes(int64_t rows, int64_t n_tokens, int64_t QH, int64_t KVH, int64_t HD) {
+    if (loom_paged_plan_bytes(rows, n_tokens, QH, KVH) == 0 || HD < 1 || HD > 256) return 0;
+    return pb_rec_floats(pb_layout(rows, n_tokens, QH, KVH), KVH, HD) * (int64_t)sizeof(float) + (n_tokens + 15) / 16 * 16;
+}
+
+extern "C" int loom_paged_batch_step(int dtype, const void* qkv, int64_t qkv_ld, void* k_pages, void* v_pages,
+                                     int64_t page_stride, int64_t token_stride, int64_t head_stride, int64_t n_pages,
+                                     int64_t page_size, const int32_t* table, int64_t table_ld, int64_t max_pages,
+                                     int64_t rows, const int32_t* rows_of, const int32_t* positions, const int64_t* slots,
+                                     const void* plan, int64_t plan_bytes, const float* cos_table, const float* sin_table,
+                                     int64_t n_pos, void* q_out, void* c_out, void* kctx_out, int64_t out_ld,
+                                     void* workspace, int64_t workspace_bytes, int64_t n_tokens, int64_t QH, int64_t KVH,
+                                     int64_t HD, void* stream) {
+    clear_error();
+    const char* who = "paged_batch_step";
+    const BatchCall c{qkv, qkv_ld, k_pages, v_pages, page_stride, token_stride, head_stride, n_pages, page_size, table,
+                      table_ld, max_pages, rows, rows_of, positions, slots, plan, plan_bytes, cos_table, sin_table, n_pos,
+                      q_out, c_out, kctx_out, out_ld, workspace, workspace_bytes, n_tokens, QH, KVH, HD};
+    const int64_t es = dtype == LOOM_F32 ? 4 : 2;
+    LOOM_CHECK(dtype == LOOM_F32 || dtype == LOOM_BF16 || dtype == LOOM_F16, "%s: unsupported dtype %d", who, dtype);
+    if (int rc = batch_sizes(who, rows, n_tokens, QH, KVH, n_pages, page_size, max_pages, table_ld)) return rc;
+    LOOM_CHECK(HD == 8 || HD == 16 || HD == 32 || HD == 64 || HD == 96 || HD == 128 || HD == 256,
+               "%s: unsupported head_dim %lld (8, 16, 32, 64, 96, 128 or 256)", who, (long long)HD);
+    LOOM_CHECK(token_stride >= HD && token_stride < ((int64_t)1 << 31) / (16 * es) && page_stride >= 0 && head_stride >= 0,
+               "%s: bad page strides", who);
+    if (n_tokens == 0) return LOOM_OK;
+    LOOM_CHECK(qkv && k_pages && v_pages && (table || rows == 0) && rows_of && positions && slots && plan && cos_table &&
+                   sin_table && q_out && c_out,
+               "%s: a required pointer is NULL", who);
+    LOOM_CHECK((token_stride * es) % 16 == 0 && (page_stride * es) % 16 == 0 && (head_stride * es) % 16 == 0 &&
+                   (((uintptr_t)k_pages | (uintptr_t)v_pages) % 16) == 0,
+               "%s: the pools and their strides must be multiples of 16 bytes", who);
+    const int64_t width = (QH + 2 * KVH) * HD;
+    LOOM_CHECK(qkv_ld >= width && (qkv_ld * es) % 16 == 0 && ((uintptr_t)qkv % 16) == 0,
+               "%s: the rows of qkv must be 16-byte aligned and hold %lld elements (row stride %lld)", who,
+               (long long)width, (long long)qkv_ld);
+    LOOM_CHECK(out_ld >= QH * HD && (out_ld * es) % 16 == 0, "%s: the output rows are %lld elements apart: %lld at least, and 16-byte aligned",
+               who, (long long)out_ld, (long long)(QH * HD));
+    LOOM_CHECK((((uintptr_t)q_out | (uintptr_t)c_out | (uintptr_t)kctx_out | (uintptr_t)cos_table | (uintptr_t)sin_table) % 16) == 0,
+               "%s: the outputs and the rotary tables must be 16-byte aligned", who);
+    LOOM_CHECK(n_pos >= 1, "%s: the rotary tables are empty", who);
+    const int64_t pn = loom_paged_plan_bytes(rows, n_tokens, QH, KVH);
+    LOOM_CHECK(plan_bytes >= pn && ((uintptr_t)plan % 64) == 0, "%s: a 64-byte aligned plan of %lld bytes is needed, got %lld", who,
+               (long long)pn, (long long)plan_bytes);
+    const int64_t need = loom_paged_batch_workspace_bytes(rows, n_tokens, QH, KVH, HD);
+    LOOM_CHECK(workspace != nullptr && workspace_bytes >= need && ((uintptr_t)workspace % 16) == 0,
+               "%s: a 16-byte aligned workspace of %lld bytes is needed, got %lld", who, (long long)need,
+               (long long)workspace_bytes);
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == LOOM_F32) return batch_launch<float>(c, s);
+    if (dtype == LOOM_BF16) return batch_launch<bf16_t>(c, s);
+    return batch_launch<f16_t>(c, s);
+}

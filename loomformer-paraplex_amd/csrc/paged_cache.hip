@@ -100,7 +100,7 @@ __device__ __forceinline__ void block_scan(const int (&v)[N], int (*waves)[N], i
 constexpr int kScanIds = 4;         // groups of four page ids per thread and round
 
 // One block.  lens[r] = lens[parent[r]] + advance, then the tokens lens[r] ..
-// lens[r] + n_new - 1 get pages of their own: where the row's last page is
+// lens[r] + n_new - 1 (n_new: n_each[r], or n_all for every row) get pages of their own: where the row's last page is
 // partly filled and held more than once, row order decides who copies it (each
 // row in turn copies while others hold it), and pages that are missing are
 // appended.  A row lets go of pages in their places that others hold too (they hold
@@ -116,7 +116,8 @@ template <bool FORK>
 __global__ void __launch_bounds__(1024)
 paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* __restrict__ lens,
                      int32_t* refs, int NP, int log_ps, const int32_t* __restrict__ parent, int R,
-                     int n_new, int advance, PageCopy* __restrict__ copies, int32_t* __restrict__ status) {
+                     int n_all, const int32_t* __restrict__ n_each, int advance, PageCopy* __restrict__ copies,
+                     int32_t* __restrict__ status) {
     extern __shared__ int32_t old[];                 // FORK: [R][MP]
     __shared__ __align__(16) int32_t tail[kPcMaxRows];
     __shared__ int32_t base[kPcMaxRows], slot0[kPcMaxRows], len_of[kPcMaxRows];
@@ -204,6 +205,7 @@ paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* _
     int page = -1, short_of = 0;
     bool copy = false;
     const int cap = MP * PS;
+    const int n_new = n_each != nullptr ? (r < R ? max(n_each[r], 0) : 0) : n_all;
     const int n = len >= 0 ? max(min(n_new, cap - len), 0) : 0;
     if (len >= 0 && n < n_new) short_of = 1;
     int miss0 = 0, last = -1;
@@ -513,6 +515,15 @@ static int table_checks(const char* who, const int32_t* table, int64_t ld, int64
     return LOOM_OK;
 }
 
+// The copies that a reservation listed
+static int cow_launch(const char* who, const PoolArgs& a, int64_t rows, const void* copies, hipStream_t st) {
+    // (about 2048 blocks, and no more than a block per page)
+    const int64_t y = ceil_div((int64_t)2048, rows), pages = 2 * (int64_t)a.layers;
+    hipLaunchKernelGGL(paged_cow_kernel, dim3((unsigned)rows, (unsigned)(y < pages ? y : pages)), dim3(256), 0, st, a,
+                       (const PageCopy*)copies);
+    return launch_status(who);
+}
+
 }  // namespace loom
 
 using namespace loom;
@@ -556,18 +567,41 @@ extern "C" int loom_paged_update(int dtype, void* k_pages, void* v_pages, int64_
     if (one)
         hipLaunchKernelGGL((paged_reserve_kernel<true>), dim3(1), dim3(1024), (unsigned)(rows * max_pages * sizeof(int32_t)),
                            st, table, table_ld, (int)max_pages, lens, refs, (int)n_pages, log_ps, parent, (int)rows,
-                           (int)n_new, (int)advance, (PageCopy*)workspace, status);
+                           (int)n_new, (const int32_t*)nullptr, (int)advance, (PageCopy*)workspace, status);
     else
         hipLaunchKernelGGL((paged_reserve_kernel<false>), dim3(1), dim3(1024), 0, st, table, table_ld, (int)max_pages,
-                           lens, refs, (int)n_pages, log_ps, parent, (int)rows, (int)n_new, (int)advance,
+                           lens, refs, (int)n_pages, log_ps, parent, (int)rows, (int)n_new, (const int32_t*)nullptr, (int)advance,
                            (PageCopy*)workspace, status);
     if (int rc = launch_status("loom_paged_update(reserve)")) return rc;
     if (n_new == 0) return LOOM_OK;
-    // (about 2048 blocks, and no more than a block per page)
-    const int64_t y = ceil_div((int64_t)2048, rows);
-    hipLaunchKernelGGL(paged_cow_kernel, dim3((unsigned)rows, (unsigned)(y < 2 * layers ? y : 2 * layers)), dim3(256), 0, st, a,
-                       (const PageCopy*)workspace);
-    return launch_status("loom_paged_update(copy)");
+    return cow_launch("loom_paged_update(copy)", a, rows, workspace, st);
+}
+
+extern "C" int loom_paged_reserve(int dtype, void* k_pages, void* v_pages, int64_t layers, int64_t layer_stride,
+                                  int64_t page_stride, int64_t token_stride, int64_t head_stride, int64_t n_pages,
+                                  int64_t page_size, int64_t KVH, int64_t HD, int32_t* table, int64_t table_ld,
+                                  int64_t max_pages, int32_t* lens, int32_t* refs, int32_t* status,
+                                  const int32_t* new_tokens, void* workspace, int64_t workspace_bytes, int64_t rows,
+                                  void* stream) {
+    clear_error();
+    const char* who = "paged_reserve";
+    PoolArgs a;
+    if (int rc = pool_checks(who, dtype, k_pages, v_pages, layers, layer_stride, page_stride, token_stride,
+                             head_stride, n_pages, page_size, KVH, HD, &a))
+        return rc;
+    if (int rc = table_checks(who, table, table_ld, max_pages, page_size, rows)) return rc;
+    LOOM_CHECK((lens && refs && status && new_tokens) || rows == 0, "%s: a required pointer is NULL", who);
+    LOOM_CHECK(workspace_bytes >= loom_paged_update_workspace_bytes(rows) && (workspace != nullptr || rows == 0) &&
+                   ((uintptr_t)workspace % 16) == 0,
+               "%s: a 16-byte aligned workspace of %lld bytes is needed, got %lld", who,
+               (long long)loom_paged_update_workspace_bytes(rows), (long long)workspace_bytes);
+    if (rows == 0) return LOOM_OK;
+    hipStream_t st = (hipStream_t)stream;
+    hipLaunchKernelGGL((paged_reserve_kernel<false>), dim3(1), dim3(1024), 0, st, table, table_ld, (int)max_pages,
+                       lens, refs, (int)n_pages, __builtin_ctzll((unsigned long long)page_size), (const int32_t*)nullptr,
+                       (int)rows, 0, new_tokens, 0, (PageCopy*)workspace, status);
+    if (int rc = launch_status("loom_paged_reserve(reserve)")) return rc;
+    return cow_launch("loom_paged_reserve(copy)", a, rows, workspace, st);
 }
 
 extern "C" int loom_paged_write(int dtype, void* k_pages, void* v_pages, int64_t layers, int64_t layer_stride,

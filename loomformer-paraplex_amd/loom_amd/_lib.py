@@ -129,6 +129,12 @@ SIGNATURES = {
                                     c_int64, c_int64, c_int64, c_int64, _P],
     "loom_paged_update": [*_POOL, _P, c_int64, c_int64, _P, _P, _P, _P, c_int64, c_int64, _P, c_int64,
                           c_int64, _P],
+    "loom_paged_reserve": [*_POOL, _P, c_int64, c_int64, _P, _P, _P, _P, _P, c_int64, c_int64, _P],
+    "loom_paged_plan": [_P, c_int64, c_int64, c_int64, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int64, _P, _P, _P,
+                        _P, _P, _P, c_int64, _P],
+    "loom_paged_batch_step": [c_int, _P, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, _P, c_int64,
+                              c_int64, c_int64, _P, _P, _P, _P, c_int64, _P, _P, c_int64, _P, _P, _P, c_int64, _P,
+                              c_int64, c_int64, c_int64, c_int64, c_int64, _P],
     "loom_paged_write": [*_POOL, _P, c_int64, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int64,
                          c_int64, _P, _P, c_int64, _P],
     "loom_paged_compact": [*_POOL, _P, c_int64, c_int64, _P, _P, _P, c_int64, c_int64, _P],
@@ -146,6 +152,8 @@ QUERIES = {"loom_gqa_workspace_bytes": ([c_int64] * 5, c_int64),
            "loom_tria_chunked_workspace_bytes": ([c_int64] * 4, c_int64),
            "loom_paged_decode_workspace_bytes": ([c_int64] * 5, c_int64),
            "loom_paged_update_workspace_bytes": ([c_int64], c_int64),
+           "loom_paged_plan_bytes": ([c_int64] * 4, c_int64),
+           "loom_paged_batch_workspace_bytes": ([c_int64] * 5, c_int64),
            "loom_paged_compact_workspace_bytes": ([c_int64], c_int64),
            "loom_beam_select_workspace_bytes": ([c_int64] * 4, c_int64),
            "loom_tria_chunked_fires_workspace_bytes": ([c_int64, c_int64, c_int64, _P, c_int64],

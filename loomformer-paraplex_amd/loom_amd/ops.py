@@ -11,7 +11,7 @@ from __future__ import annotations
 import ctypes
 
 import math
-from typing import List, Optional, Sequence, Tuple
+from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -611,6 +611,52 @@ def paged_update(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tens
     the holders of each page; status [1] is raised where pages ran out.  All
     bookkeeping is on the device."""
     (_host_module or _host()).paged_update(k_pages, v_pages, table, lens, refs, status, parent, n_new, advance)
+
+
+def paged_reserve(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                  refs: torch.Tensor, status: torch.Tensor, new: torch.Tensor) -> None:
+    """paged_update's reservation with a count per row: the next new[r] tokens (int32
+    [rows], negative: none) of every row that holds a sequence are made writable.  lens is not
+    changed."""
+    (_host_module or _host()).paged_reserve(k_pages, v_pages, table, lens, refs, status, new)
+
+
+class PagedPlan(NamedTuple):
+    """A step of a ragged batch (paged_plan).  The new tokens of all rows lie one row
+    behind the other in n_tokens flat places; those behind the last are padding."""
+    starts: torch.Tensor      # [rows + 1] int32: the place of each row's first new token, then their number
+    rows: torch.Tensor        # [n_tokens] int32: each place's row (-1: padding)
+    positions: torch.Tensor   # [n_tokens] int32: its position in the row (-1: padding)
+    slots: torch.Tensor       # [n_tokens] int64: page * page_size + place in the page (-1: none)
+    shared: torch.Tensor      # [rows] int32: first tokens of the row that are read once with other rows
+    work: torch.Tensor        # the step's work in equal shares, for paged_batch_step
+    sizes: Tuple[int, ...]    # what it was made for: pages, kv heads, page size, table columns, q heads
+
+
+def paged_plan(k_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, new: torch.Tensor, n_tokens: int,
+               q_heads: int) -> PagedPlan:
+    """Slot maps and work of a step in which row r brings new[r] tokens (int32 [rows];
+    none, one, a prompt), from the tables and lengths on the device.  n_tokens: places of
+    the flat batch, at least the sum of new.  k_pages: a layer's or all layers' pool
+    (its sizes alone count).  Rows whose first whole pages are the same are
+    found, and paged_batch_step reads those once for all of them.  The plan holds
+    for all layers, until table, lens or new change.  A row that lacks a page for
+    one of its tokens (paged_reserve, paged_update), or whose tokens do not all fit into the
+    batch, has no slots."""
+    return PagedPlan(*(_host_module or _host()).paged_plan(k_pages, table, lens, new, n_tokens, q_heads))
+
+
+def paged_batch_step(plan: PagedPlan, qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                     table: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                     want_kctx: bool = True) -> List[Optional[torch.Tensor]]:
+    """One layer of a planned step (GroupedQueryCausalSelfAttention over a ragged
+    batch, loomformer.py:3215-3332): qkv [n_tokens, (q_heads + 2 kv_heads) *
+    head_dim] projection rows, k_pages / v_pages, table, cos and sin as for
+    paged_decode_step.  Writes every token's roped k and its v to its slot and
+    returns [c, kctx or None, q], each [n_tokens, q_heads, head_dim]: A.V, A.K_roped
+    over the row's tokens up to itself, and the roped q.  Padding gives zeros; tokens
+    of rows without slots, or past the rotary tables, give NaN and are not written."""
+    return (_host_module or _host()).paged_batch_step(*plan, qkv, k_pages, v_pages, table, cos, sin, want_kctx)
 
 
 def paged_write(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, k_rows: torch.Tensor,

@@ -70,6 +70,23 @@ class PagedKVCache:
         ops.paged_update(self.k_pages, self.v_pages, self.table, self.lens, self.refs, self.status, parent, n_new,
                          advance)
 
+    def reserve(self, new: torch.Tensor) -> None:
+        """ops.paged_reserve on this cache: make the next new[r] tokens of each row writable."""
+        ops.paged_reserve(self.k_pages, self.v_pages, self.table, self.lens, self.refs, self.status, new)
+
+    def plan(self, new: torch.Tensor, n_tokens: int, q_heads: int) -> ops.PagedPlan:
+        """ops.paged_plan of a step in which each row brings new[r] tokens (reserved before)."""
+        return ops.paged_plan(self.k_pages, self.table, self.lens, new, n_tokens, q_heads)
+
+    def attend_batch(self, layer: int, plan: ops.PagedPlan, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                     want_kctx: bool = True) -> List[Optional[torch.Tensor]]:
+        """ops.paged_batch_step of one layer."""
+        return ops.paged_batch_step(plan, qkv, self.k_pages[layer], self.v_pages[layer], self.table, cos, sin, want_kctx)
+
+    def advance(self, new: torch.Tensor) -> None:
+        """Each row holds its new[r] tokens from now on (after the last layer of their step)."""
+        self.lens.add_(torch.where(self.lens >= 0, new.clamp(min=0), 0))
+
     def free(self, rows: torch.Tensor) -> None:
         """Rows of a bool mask [rows] let go of their pages and hold no sequence."""
         at = torch.arange(self.rows, dtype=torch.int32, device=self.lens.device)

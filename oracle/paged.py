@@ -167,3 +167,101 @@ def reorder_rows(t: torch.Tensor, parent, dim: int = 0) -> torch.Tensor:
     R = t.shape[dim]
     at = [p if 0 <= p < R else r for r, p in enumerate(parent.tolist())]
     return t.index_select(dim, torch.tensor(at, device=t.device))
+
+
+def reserve(k_pages, v_pages, table, lens, refs, new):
+    """paged_reserve on copies: (k_pages, v_pages, table, refs, status), row by row."""
+    kp, vp, rows, rf, status = k_pages.clone(), v_pages.clone(), table.tolist(), refs.tolist(), 0
+    NP, PS, MP = kp.shape[1], kp.shape[3], table.shape[1]
+    valid = lambda p: 0 <= p < NP  # noqa: E731
+    want = [min(max(int(m), 0), MP * PS - n) if n >= 0 else 0 for n, m in zip(lens.tolist(), new.tolist())]
+    status += sum(n >= 0 and w < int(m) for n, m, w in zip(lens.tolist(), new.tolist(), want))
+    held, gone = list(rf), []
+    for r, n in enumerate(lens.tolist()):             # pages behind the tokens that are not the row's alone
+        kept = True
+        for s in range(-(-n // PS), (n + want[r] - 1) // PS + 1) if want[r] > 0 else ():
+            kept = kept and valid(rows[r][s]) and held[rows[r][s]] <= 1
+            if not kept and valid(rows[r][s]):
+                gone.append(rows[r][s])
+                rows[r][s] = -1
+    for p in gone:
+        rf[p] -= 1
+    free = [p for p in range(NP) if rf[p] <= 0]
+    take = lambda: free.pop(0) if free else -1  # noqa: E731
+    for r, n in enumerate(lens.tolist()):
+        if want[r] <= 0:
+            continue
+        s = n // PS
+        if n % PS and valid(rows[r][s]) and rf[rows[r][s]] > 1:
+            p, q = rows[r][s], take()
+            rf[p] -= 1
+            rows[r][s] = q
+            if q >= 0:
+                rf[q] = 1
+                kp[:, q, :, :n % PS] = kp[:, p, :, :n % PS]
+                vp[:, q, :, :n % PS] = vp[:, p, :, :n % PS]
+            else:
+                status += 1
+        for s in range(-(-n // PS), (n + want[r] - 1) // PS + 1):
+            if not valid(rows[r][s]):
+                rows[r][s] = take()
+                if rows[r][s] >= 0:
+                    rf[rows[r][s]] = 1
+                else:
+                    status += 1
+    return kp, vp, torch.tensor(rows, dtype=torch.int32), torch.tensor(rf, dtype=torch.int32), status
+
+
+def maps(table, lens, new, n_tokens, n_pages, page_size):
+    """paged_plan's maps: starts, rows, positions, slots; and which rows have slots."""
+    tab, ln = table.tolist(), lens.tolist()
+    count = [min(max(int(m), 0), n_tokens + 1) if n >= 0 else 0 for n, m in zip(ln, new.tolist())]
+    starts, rows, pos, slots, ok = [0], [-1] * n_tokens, [-1] * n_tokens, [-1] * n_tokens, []
+    for r, m in enumerate(count):
+        a, n = starts[-1], ln[r]
+        starts.append(a + m)
+        cap = len(tab[r]) * page_size
+        ok.append(m > 0 and a + m <= n_tokens and n + m <= cap and
+                  all(0 <= p < n_pages for p in tab[r][:-(-(n + m) // page_size)]))
+        for t in range(a, min(a + m, n_tokens)):
+            rows[t], pos[t] = r, n + t - a
+            if ok[r]:
+                slots[t] = tab[r][pos[t] // page_size] * page_size + pos[t] % page_size
+    return starts, rows, pos, slots, ok
+
+
+def batch_attention(q, k_pages, v_pages, table, lens, starts, ok):
+    """attention of a ragged batch (causal within each row's new tokens), and what the
+    bounds of a computed result go by, as attention() gives them."""
+    q, kp, vp = q.cpu().double(), k_pages.cpu(), v_pages.cpu()
+    N, QH, HD = q.shape
+    KVH = kp.shape[1]
+    G = QH // KVH
+    out = {n: torch.zeros(N, QH, HD, dtype=torch.float64) for n in ("c", "kctx", "c_abs", "kctx_abs")}
+    out.update(s_max=torch.zeros(N, QH, dtype=torch.float64), qk_abs=torch.zeros(N, QH, dtype=torch.float64),
+               n=torch.ones(N, dtype=torch.float64))
+    for r, good in enumerate(ok):
+        if not good:
+            continue
+        a, e, n = starts[r], starts[r + 1], int(lens[r])
+        k, v = rows_of(kp, table[r], n + e - a), rows_of(vp, table[r], n + e - a)
+        unseen = torch.arange(n + e - a)[None] > torch.arange(n, n + e - a)[:, None]
+        out["n"][a:e] = torch.arange(n + 1, n + e - a + 1, dtype=torch.float64)
+        for h in range(QH):
+            kk, vv, x = k[h // G], v[h // G], q[a:e, h]
+            # positions behind a token have no weight, whatever they hold
+            s = (x @ torch.nan_to_num(kk, 0.0, 0.0, 0.0).t() / math.sqrt(HD)).masked_fill(unseen, -math.inf)
+            s = torch.where(~unseen & ~torch.isfinite(kk).all(1)[None], (x @ kk.t()) / math.sqrt(HD), s)
+            w = torch.exp(s - s.amax(1, keepdim=True))
+            w = w / w.sum(1, keepdim=True)
+            for name, m in (("c", vv), ("kctx", kk)):
+                clean = torch.isfinite(m).all(1)
+                if bool(clean.all()):
+                    out[name][a:e, h], out[name + "_abs"][a:e, h] = w @ m, w @ m.abs()
+                else:                                 # token by token, over what it sees
+                    for i in range(e - a):
+                        out[name][a + i, h] = w[i, :n + i + 1] @ m[:n + i + 1]
+                        out[name + "_abs"][a + i, h] = w[i, :n + i + 1] @ m[:n + i + 1].abs()
+            out["s_max"][a:e, h] = s.masked_fill(unseen, 0.0).abs().amax(1)
+            out["qk_abs"][a:e, h] = (x.abs() @ torch.nan_to_num(kk, 0.0, 0.0, 0.0).abs().t()).masked_fill(unseen, 0.0).amax(1) / math.sqrt(HD)
+    return out
