@@ -13,7 +13,7 @@
 // Which rows share what only the device knows, so a step is planned there, once for
 // all layers:
 //   rows     which rows begin with the same pages, and how many (paged_rows_kernel)
-//   plan     segments (a block of up to 64 queries and the positions they read), cut
+//   plan     segments (a block of up to 128 queries and the positions they read), cut
 //            into items of about equal work, one block each (paged_plan_kernel)
 // and a layer is three launches: rope and append, the items, the join.
 #include "attn_tile.h"
@@ -24,10 +24,10 @@
 namespace loom {
 
 constexpr int kPbMaxRows = 1024;
-constexpr int kPbQ = 64;            // queries (a token's heads of one kv head) of a block
+constexpr int kPbQ = 128;           // queries (a token's heads of one kv head) of a block
 constexpr int kPbTile = 64;         // positions of a step of a block
 constexpr int kPbLeast = 2;         // an item has so many tiles at least
-constexpr int kPbAlone = 32;        // rows with more queries fill a block by themselves and share nothing
+constexpr int kPbAlone = 64;        // rows with more queries fill a block by themselves and share nothing
 constexpr int kPbShare = 64;        // common positions from which reading them once pays
 constexpr int kPbMagic = 0x4c50424c;
 constexpr int64_t kPbMaxTokens = (int64_t)1 << 20;
@@ -556,18 +556,21 @@ __device__ __forceinline__ bool pb_odd(const BatchArgs<T>& a, const PbSeg& s) {
     return odd;
 }
 
-// The end of an item: the waves' (m, l, C, Kctx) from LDS joined into records, or into
-// the outputs where the queries have no other part.  part(w): the sums of wave w's 16
-// queries as its lanes hold them, C then Kctx, four queries' of one dimension side by
-// side; ml[w][16]: (m, l).  Query x is in the waves x / 16 + QW k.
+// The end of an item, for 16 queries of each wave: the waves' (m, l, C, Kctx) from LDS
+// joined into records, or into the outputs where the queries have no other part.
+// part(w): the sums of wave w's queries as its lanes hold them, C then Kctx, four queries'
+// of one dimension side by side; ml[w][16]: (m, l).  QW waves stand side by side: wave w's
+// queries begin at first + (w % QW) apart, and waves w, w + QW, .. have the same.
 template <int HDP, bool KCTX, typename T, typename P>
-__device__ __forceinline__ void pb_finish(const BatchArgs<T>& a, const PbWork& w, int QW, const float2 (*ml)[16], P part) {
+__device__ __forceinline__ void pb_finish(const BatchArgs<T>& a, const PbWork& w, int QW, int first, int apart,
+                                          const float2 (*ml)[16], P part) {
     const PbSeg& s = w.s;
     constexpr int quads = HDP / 4, per = KCTX ? 2 * quads : quads;
     const int KW = 4 / QW;
-    for (int k = threadIdx.x; k < s.nq * per; k += 256) {
-        const int x = k / per, e = k - x * per, which = e >= quads, d = 4 * (e - which * quads);
-        const int w0 = x >> 4, j = x & 15;
+    for (int k = threadIdx.x; k < QW * 16 * per; k += 256) {
+        const int y = k / per, e = k - y * per, which = e >= quads, d = 4 * (e - which * quads);
+        const int w0 = y >> 4, j = y & 15, x = first + w0 * apart + j;
+        if (x >= s.nq) continue;
         float m = -INFINITY, l = 0.0f;
         for (int g = 0; g < KW; ++g) m = fmaxf(m, ml[w0 + QW * g][j].x);
         pg_f32x4 c = {0.f, 0.f, 0.f, 0.f};
@@ -600,10 +603,17 @@ __device__ __forceinline__ void pb_finish(const BatchArgs<T>& a, const PbWork& w
 // NS LDS stages that loads fill directly, one barrier per step; a 16-position quarter of
 // a tile lies in one page (pages hold a multiple of 16 positions), staged by one wave, so
 // its base and its bound are scalar: rows past the item's end land as zeros.  QW waves
-// side by side take 16 queries each, and the KW = 4 / QW groups of them a quarter, half
-// or all of the positions: one query block of 1 to 16, of 17 to 32 or of more, so that a
-// decode step's few queries use all waves too.  S^T = K Q^T, P from the score registers,
-// C = P V and Kctx = P K through the transposing LDS read.
+// side by side take NQ times 16 queries each, and the KW = 4 / QW groups of them a quarter,
+// half or all of the positions, so that a decode step's few queries use all waves too:
+//   queries      QW NQ KW
+//   1 .. 16       1  1  4
+//   17 .. 32      2  1  2
+//   33 .. 64      2  2  2
+//   65 .. 128     4  2  1
+// Two query blocks per wave share every K and V fragment's LDS read.  S^T = K Q^T, P from
+// the score registers, C = P V and Kctx = P K through the transposing LDS read.  A lane's
+// sum of weights is its own until the end, and the reference of the exponents is looked at
+// lane by lane: the lanes of a column meet only where it has to rise.
 template <int HD> constexpr int pb_stages() { return HD <= 96 ? 3 : 2; }
 
 template <typename T, int HD, bool KCTX>
@@ -620,8 +630,6 @@ paged_items_kernel(BatchArgs<T> a) {
     const PbSeg& s = w.s;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int lr = lane & 15, lq = lane >> 4;
-    const int QW = s.nq <= 16 ? 1 : s.nq <= 32 ? 2 : 4;
-    const int qt = wave & (QW - 1), kg = wave / QW;
     const TileLane<CPR> tl(lq, lr);
     const int kend = min(s.key1, s.key0 + w.it.tile1 * R);
     const int32_t* trow = a.table + (int64_t)s.row * a.table_ld;
@@ -633,18 +641,7 @@ paged_items_kernel(BatchArgs<T> a) {
         pgv = trow[min(t, (int64_t)a.cap - 1) >> a.log_ps];
     };
     pages();
-    const int x = 16 * qt + lr, xq = min(x, s.nq - 1);
     const bool odd_mine = pb_odd(a, s);
-    uint4 qf[KK];
-    {
-        const T* q = a.q_out + ((int64_t)pb_token(a, s, xq) * a.QH + w.kvh * a.G + (s.x0 + xq) % a.G) * HD + 8 * lq;
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) qf[kk] = *reinterpret_cast<const uint4*>(q + 32 * kk);
-    }
-    const int sees = min(pb_sees(a, s, xq), kend);              // (lanes without a query: the last one's)
-    const int sees_first = __builtin_amdgcn_readfirstlane(min(pb_sees(a, s, min(16 * qt, s.nq - 1)), kend));
-    const int sees_last = __builtin_amdgcn_readfirstlane(min(pb_sees(a, s, min(16 * qt + 15, s.nq - 1)), kend));
-    const bool idle = 16 * qt >= s.nq;                          // no query in this wave
     uint32_t voff[GPW];
 #pragma unroll
     for (int j = 0; j < GPW; ++j) {
@@ -684,93 +681,134 @@ paged_items_kernel(BatchArgs<T> a) {
             dma16(rv, vst(s_) + 64 * (wave * GPW + i), voff[i], 0);
         }
     };
-    using S0 = std::integral_constant<int, 0>;
-    using S1 = std::integral_constant<int, 1>;
-    using S2 = std::integral_constant<int, 2>;
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    using I4 = std::integral_constant<int, 4>;
     const bool odd = __syncthreads_or(odd_mine);
 
-    float mh = -INFINITY, lh = 0.0f;
-    pg_f32x4 accC[DT], accK[KCTX ? DT : 1];
+    auto body = [&](auto kw_, auto nq_, auto odd_, int xb) __attribute__((always_inline)) {   // queries from xb on
+        constexpr int KW = decltype(kw_)::value, NQ = decltype(nq_)::value, QW = 4 / KW;
+        constexpr bool ODD = decltype(odd_)::value;
+        constexpr int NHF = KW == 4 ? 1 : 2;                 // 16-row parts of a fold
+        constexpr int FOLDS = 4 / (KW * NHF);                // folds of a wave per tile
+        const int kg = wave / QW, x0 = xb + (wave & (QW - 1)) * 16 * NQ;
+        // q of column lr, positions that the column sees; (columns without a query: the last one's)
+        uint4 qf[NQ][KK];
+        int sees[NQ];
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) accC[dt] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < NQ; ++n) {
+            const int x = min(x0 + 16 * n + lr, s.nq - 1);
+            const T* q = a.q_out + ((int64_t)pb_token(a, s, x) * a.QH + w.kvh * a.G + (s.x0 + x) % a.G) * HD + 8 * lq;
 #pragma unroll
-    for (int dt = 0; dt < (KCTX ? DT : 1); ++dt) accK[dt] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
-
-    auto body = [&](auto kw_) {
-        constexpr int KW = decltype(kw_)::value, NHF = 4 / KW;   // 16-row parts of a tile per wave
+            for (int kk = 0; kk < KK; ++kk) qf[n][kk] = *reinterpret_cast<const uint4*>(q + 32 * kk);
+            sees[n] = min(pb_sees(a, s, x), kend);
+        }
+        const int sees_first = __builtin_amdgcn_readfirstlane(min(pb_sees(a, s, min(x0, s.nq - 1)), kend));
+        float mh[NQ], off[NQ], lh[NQ];                       // the reference, minus it (0 before there is one), the sum
+        pg_f32x4 accC[NQ][DT], accK[NQ][KCTX ? DT : 1];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            mh[n] = -INFINITY;
+            off[n] = lh[n] = 0.0f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) accC[n][dt] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int dt = 0; dt < (KCTX ? DT : 1); ++dt) accK[n][dt] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
+        }
         auto fold = [&](const gqa_u4* tk, const gqa_u4* tv, int r0) __attribute__((always_inline)) {
-            pg_f32x4 sc[NHF];
+            pg_f32x4 sc[NQ][NHF];
 #pragma unroll
             for (int hf = 0; hf < NHF; ++hf) {
-                sc[hf] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int kk = 0; kk < KK; ++kk)
-                    sc[hf] = M::dot(__builtin_bit_cast(uint4, tile_s_frag<CPR>(tk + (hf >> 1) * 32 * CPR, tl, hf & 1, kk)),
-                                    qf[kk], sc[hf]);
+                for (int n = 0; n < NQ; ++n) sc[n][hf] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) {
+                    const uint4 f = __builtin_bit_cast(uint4, tile_s_frag<CPR>(tk, tl, hf, kk));
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) sc[n][hf] = M::dot(f, qf[n][kk], sc[n][hf]);
+                }
             }
             const bool mask = r0 + 16 * NHF > sees_first;        // wave-uniform
-            float mx = -INFINITY;
             if (mask) {
+#pragma unroll
+                for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                    for (int hf = 0; hf < NHF; ++hf)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (r0 + 16 * hf + 4 * lq + r >= sees[n]) sc[n][hf][r] = -INFINITY;
+            }
+            float mx[NQ];
+            bool rise = false;
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                mx[n] = -INFINITY;
 #pragma unroll
                 for (int hf = 0; hf < NHF; ++hf)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (r0 + 16 * hf + 4 * lq + r >= sees) sc[hf][r] = -INFINITY;
+                    for (int r = 0; r < 4; ++r) mx[n] = fmaxf(mx[n], sc[n][hf][r]);
+                mx[n] = fmaf(mx[n], a.qscale, -M::kShift);
+                rise |= mx[n] > mh[n] + M::kLag;
             }
+            if (__any(rise)) {
 #pragma unroll
-            for (int hf = 0; hf < NHF; ++hf)
+                for (int n = 0; n < NQ; ++n) {
+                    const float mnew = raised(mh[n], max_16_32(mx[n]), M::kLag);
+                    const float corr = mnew == mh[n] ? 1.0f : __builtin_amdgcn_exp2f(mh[n] - mnew);
+                    const bool first = mh[n] == -INFINITY;       // the sums are zero
+                    mh[n] = mnew;
+                    off[n] = mnew == -INFINITY ? 0.0f : -mnew;   // (nothing seen yet: e^-inf, not e^NaN)
+                    lh[n] *= corr;
+                    if (__any(!first && corr != 1.0f)) {
+                        pg_f32x4 cf;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[hf][r]);
-            mx = max_16_32(mx) * a.qscale;
-            const float mnew = raised(mh, mx - M::kShift, M::kLag);
-            const float corr = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mh - mnew);
-            const float off = mnew == -INFINITY ? 0.0f : -mnew;  // (nothing seen yet: e^-inf, not e^NaN)
-            float ls = 0.0f, pv[NHF][4];
+                        for (int r = 0; r < 4; ++r) cf[r] = __shfl(first ? 1.0f : corr, 4 * lq + r, 64);
 #pragma unroll
-            for (int hf = 0; hf < NHF; ++hf)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    pv[hf][r] = __builtin_amdgcn_exp2f(fmaf(sc[hf][r], a.qscale, off));
-                    ls += pv[hf][r];
-                }
-            lh = fmaf(lh, corr, sum_16_32(ls));
-            const bool rescale = corr != 1.0f && mh != -INFINITY;     // (before, the sums are zero)
-            mh = mnew;
-            if (__any(rescale)) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float cf = __shfl(corr, 4 * lq + r, 64);
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        accC[dt][r] *= cf;
-                        if constexpr (KCTX) accK[dt][r] *= cf;
+                        for (int dt = 0; dt < DT; ++dt) {
+                            accC[n][dt] *= cf;
+                            if constexpr (KCTX) accK[n][dt] *= cf;
+                        }
                     }
                 }
             }
-            if (odd && mask) {
+            float pv[NQ][NHF][4];
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+                for (int hf = 0; hf < NHF; ++hf)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        pv[n][hf][r] = __builtin_amdgcn_exp2f(fmaf(sc[n][hf][r], a.qscale, off[n]));
+                        lh[n] += pv[n][hf][r];
+                    }
+            }
+            if (ODD && mask) {
                 // one position at a time, with only the queries that see it
 #pragma unroll 1
                 for (int row = 0; row < 16 * NHF; ++row) {
-                    float mine = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 4 * NHF; ++i) mine = (row >> 4) * 4 + (row & 3) == i ? pv[i / 4][i % 4] : mine;
                     const int g = (row >> 2) & 3;
-                    float p[4];
-                    bool seen[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        p[i] = __shfl(mine, 16 * g + 4 * lq + i, 64);
-                        seen[i] = r0 + row < __shfl(sees, 4 * lq + i, 64);
-                    }
+                    for (int n = 0; n < NQ; ++n) {
+                        float mine = 0.0f;
 #pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        const int d = 16 * dt + lr, at = row * CPR + ((d >> 3) ^ kv_swz(row));
-                        const float v = ld(reinterpret_cast<const T*>(tv + at) + (d & 7));
-                        const float k = KCTX ? ld(reinterpret_cast<const T*>(tk + at) + (d & 7)) : 0.0f;
+                        for (int i = 0; i < 4 * NHF; ++i) mine = (row >> 4) * 4 + (row & 3) == i ? pv[n][i / 4][i % 4] : mine;
+                        float p[4];
+                        bool seen[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            accC[dt][i] = seen[i] ? fmaf(p[i], v, accC[dt][i]) : accC[dt][i];
-                            if constexpr (KCTX) accK[dt][i] = seen[i] ? fmaf(p[i], k, accK[dt][i]) : accK[dt][i];
+                            p[i] = __shfl(mine, 16 * g + 4 * lq + i, 64);
+                            seen[i] = r0 + row < __shfl(sees[n], 4 * lq + i, 64);
+                        }
+#pragma unroll
+                        for (int dt = 0; dt < DT; ++dt) {
+                            const int d = 16 * dt + lr, at = row * CPR + ((d >> 3) ^ kv_swz(row));
+                            const float v = ld(reinterpret_cast<const T*>(tv + at) + (d & 7));
+                            const float k = KCTX ? ld(reinterpret_cast<const T*>(tk + at) + (d & 7)) : 0.0f;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                accC[n][dt][i] = seen[i] ? fmaf(p[i], v, accC[n][dt][i]) : accC[n][dt][i];
+                                if constexpr (KCTX) accK[n][dt][i] = seen[i] ? fmaf(p[i], k, accK[n][dt][i]) : accK[n][dt][i];
+                            }
                         }
                     }
                 }
@@ -779,71 +817,109 @@ paged_items_kernel(BatchArgs<T> a) {
             // the weights enter the products rounded to the storage type (half a step of
             // it, relative, per weight, down to Mfma16's smallest: below the rounding of
             // the outputs); their sum l is that of the unrounded ones
+            uint4 pa[NQ];
 #pragma unroll
-            for (int u = 0; u < (NHF + 1) / 2; ++u) {
-                uint4 pa = make_uint4(M::pack(pv[2 * u][0], pv[2 * u][1]), M::pack(pv[2 * u][2], pv[2 * u][3]), 0, 0);
+            for (int n = 0; n < NQ; ++n) {
+                pa[n] = make_uint4(M::pack(pv[n][0][0], pv[n][0][1]), M::pack(pv[n][0][2], pv[n][0][3]), 0, 0);
                 if constexpr (NHF > 1) {
-                    pa.z = M::pack(pv[2 * u + 1][0], pv[2 * u + 1][1]);
-                    pa.w = M::pack(pv[2 * u + 1][2], pv[2 * u + 1][3]);
+                    pa[n].z = M::pack(pv[n][1][0], pv[n][1][1]);
+                    pa[n].w = M::pack(pv[n][1][2], pv[n][1][3]);
                 }
-                auto frag = [&](const gqa_u4* tile, int dt) __attribute__((always_inline)) {
-                    if constexpr (NHF > 1) {
-                        return tile_tr_frag<CPR>(tile + u * 32 * CPR, tl, dt);
-                    } else {                         // 16 rows: the other half meets zero weights
-                        const char* p = reinterpret_cast<const char*>(tile) + tl.t_off[dt & 1][0] + 64 * (dt >> 1);
-                        const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                                       (__attribute__((address_space(3))) gqa_v4s*)(p)));
-                        return make_uint4(lo.x, lo.y, 0, 0);
-                    }
-                };
+            }
+            auto frag = [&](const gqa_u4* tile, int dt) __attribute__((always_inline)) {
+                if constexpr (NHF > 1) {
+                    return tile_tr_frag<CPR>(tile, tl, dt);
+                } else {                             // 16 rows: the other half meets zero weights
+                    const char* p = reinterpret_cast<const char*>(tile) + tl.t_off[dt & 1][0] + 64 * (dt >> 1);
+                    const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                                   (__attribute__((address_space(3))) gqa_v4s*)(p)));
+                    return make_uint4(lo.x, lo.y, 0, 0);
+                }
+            };
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    accC[dt] = M::dot(pa, frag(tv, dt), accC[dt]);
-                    if constexpr (KCTX) accK[dt] = M::dot(pa, frag(tk, dt), accK[dt]);
+            for (int dt = 0; dt < DT; ++dt) {
+                const uint4 fv = frag(tv, dt);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) accC[n][dt] = M::dot(pa[n], fv, accC[n][dt]);
+                if constexpr (KCTX) {
+                    const uint4 fk = frag(tk, dt);
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) accK[n][dt] = M::dot(pa[n], fk, accK[n][dt]);
                 }
             }
         };
         // step j computes tile j from stage j % NS, requests tile j + NS - 1 into the stage
         // that every wave is done with, waits for tile j + 1 and passes one barrier
-        auto step = [&](auto s_, int j) {
+        auto step = [&](auto s_, int j) __attribute__((always_inline)) {
             constexpr int cur = decltype(s_)::value;
             load_tile(std::integral_constant<int, (cur + NS - 1) % NS>{}, j + NS - 1);
-            const int r0 = s.key0 + j * R + kg * (R / KW);
-            if (j < w.it.tile1 && !idle && r0 < sees_last)
-                fold(kst(s_) + kg * (R / KW) * CPR, vst(s_) + kg * (R / KW) * CPR, r0);
+#pragma unroll
+            for (int u = 0; u < FOLDS; ++u) {
+                const int row = kg * (R / KW) + u * 16 * NHF, r0 = s.key0 + j * R + row;
+                // (unconditionally: a branch around it costs the loop's registers more than what a wave
+                // without a query, or that sees nothing here yet, could save)
+                fold(kst(s_) + row * CPR, vst(s_) + row * CPR, r0);
+            }
             wait_vmcnt<2 * GPW * (NS - 2)>();
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         };
-        load_tile(S0{}, w.it.tile0);
-        if constexpr (NS == 3) load_tile(S1{}, w.it.tile0 + 1);
+        load_tile(std::integral_constant<int, 0>{}, w.it.tile0);
+        if constexpr (NS == 3) load_tile(I1{}, w.it.tile0 + 1);
         wait_vmcnt<2 * GPW * (NS - 2)>();
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk)
-            asm volatile("" : "+v"(qf[kk].x), "+v"(qf[kk].y), "+v"(qf[kk].z), "+v"(qf[kk].w));
-        for (int j = w.it.tile0; j < w.it.tile1; j += NS) {
-            step(S0{}, j);
-            step(S1{}, j + 1);
-            if constexpr (NS == 3) step(S2{}, j + 2);
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk)
+                asm volatile("" : "+v"(qf[n][kk].x), "+v"(qf[n][kk].y), "+v"(qf[n][kk].z), "+v"(qf[n][kk].w));
+        for (int j = w.it.tile0;; j += NS) {         // (an item has a tile)
+            step(std::integral_constant<int, 0>{}, j);
+            if (j + 1 >= w.it.tile1) break;
+            step(I1{}, j + 1);
+            if (j + 2 >= w.it.tile1) break;
+            if constexpr (NS == 3) {
+                step(I2{}, j + 2);
+                if (j + 3 >= w.it.tile1) break;
+            }
+        }
+        wait_vmcnt<0>();                             // no load into LDS outlives the loop
+        // wave w's sums in the w-th of four stage arrays, whose size they have
+        static_assert(16 * 2 * HD * sizeof(float) == sizeof(K0), "a wave's sums of 16 queries fill a stage");
+        auto part = [&](int i) { return reinterpret_cast<float*>(i == 0 ? K0 : i == 1 ? V0 : i == 2 ? K1 : V1); };
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+            __syncthreads();
+            lh[n] = sum_16_32(lh[n]);
+            if (lq == 0) ml[wave][lr] = make_float2(mh[n], lh[n]);
+            pg_f32x4* mine = reinterpret_cast<pg_f32x4*>(part(wave)) + lane;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                mine[64 * dt] = accC[n][dt];
+                if constexpr (KCTX) mine[64 * (DT + dt)] = accK[n][dt];
+            }
+            __syncthreads();
+            pb_finish<HD, KCTX>(a, w, QW, xb + 16 * n, 16 * NQ, ml, part);
         }
     };
-    if (QW == 4) body(std::integral_constant<int, 1>{});
-    else if (QW == 2) body(std::integral_constant<int, 2>{});
-    else body(std::integral_constant<int, 4>{});
-    wait_vmcnt<0>();                                 // no load into LDS outlives the loop
-    __syncthreads();
-    // wave w's sums in the w-th of four stage arrays, whose size they have
-    static_assert(16 * 2 * HD * sizeof(float) == sizeof(K0), "a wave's sums fill a stage");
-    auto part = [&](int i) { return reinterpret_cast<float*>(i == 0 ? K0 : i == 1 ? V0 : i == 2 ? K1 : V1); };
-    if (lq == 0) ml[wave][lr] = make_float2(mh, lh);
-    pg_f32x4* mine = reinterpret_cast<pg_f32x4*>(part(wave)) + lane;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-        mine[64 * dt] = accC[dt];
-        if constexpr (KCTX) mine[64 * (DT + dt)] = accK[dt];
+    if (odd) {
+        // (code of its own, 64 queries at a time: its registers would be the others' loss)
+        for (int xb = 0; xb < s.nq; xb += 64) {
+            if (xb > 0) {
+                jb = w.it.tile0;
+                pages();
+                __syncthreads();                     // the last queries' sums are read
+            }
+            body(I1{}, I1{}, std::true_type{}, xb);
+        }
+    } else if (s.nq <= 16) {
+        body(I4{}, I1{}, std::false_type{}, 0);
+    } else if (s.nq <= 32) {
+        body(I2{}, I1{}, std::false_type{}, 0);
+    } else if (s.nq <= 64) {
+        body(I2{}, I2{}, std::false_type{}, 0);
+    } else {
+        body(I1{}, I2{}, std::false_type{}, 0);
     }
-    __syncthreads();
-    pb_finish<HD, KCTX>(a, w, QW, ml, part);
 }
 
 // ------------------------------------------------------------------ fp32 form
@@ -865,11 +941,14 @@ paged_items_f32_kernel(BatchArgs<T> a) {
     const PbWork w = pb_work(a);
     if (!w.any) return;
     const PbSeg& s = w.s;
+    // 64 of the segment's queries: blocks of y = 1 take the others
+    const int xb = 64 * blockIdx.y, nq = min(s.nq - xb, 64);
+    if (nq <= 0) return;
     const bool kctx = a.k_out != nullptr;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int lr = lane & 15, lq = lane >> 4;
-    const int QW = s.nq <= 16 ? 1 : s.nq <= 32 ? 2 : 4, KW = 4 / QW;
-    const int qt = wave & (QW - 1), kg = wave / QW;
+    const int QW = nq <= 16 ? 1 : nq <= 32 ? 2 : 4, KW = 4 / QW;
+    const int x0 = xb + 16 * (wave & (QW - 1)), kg = wave / QW;
     const int k0 = s.key0 + w.it.tile0 * kPbTile, kend = min(s.key1, s.key0 + w.it.tile1 * kPbTile);
     const int32_t* trow = a.table + (int64_t)s.row * a.table_ld;
     const int ps_mask = (1 << a.log_ps) - 1;
@@ -883,7 +962,7 @@ paged_items_f32_kernel(BatchArgs<T> a) {
     int jb = k0, pgv;
     auto pages = [&]() { pgv = trow[min((int64_t)jb + 16 * lane, (int64_t)a.cap - 1) >> a.log_ps]; };
     pages();
-    const int x = 16 * qt + lr, xq = min(x, s.nq - 1);
+    const int xq = min(x0 + lr, s.nq - 1);
     const bool odd_mine = pb_odd(a, s);
     // q of column lr, dimensions lq HDP / 4 ..
     float qf[HDP / 4];
@@ -896,9 +975,9 @@ paged_items_f32_kernel(BatchArgs<T> a) {
         }
     }
     const int sees = min(pb_sees(a, s, xq), kend);
-    const int sees_first = __builtin_amdgcn_readfirstlane(min(pb_sees(a, s, min(16 * qt, s.nq - 1)), kend));
-    const int sees_last = __builtin_amdgcn_readfirstlane(min(pb_sees(a, s, min(16 * qt + 15, s.nq - 1)), kend));
-    const bool idle = 16 * qt >= s.nq;
+    const int sees_first = __builtin_amdgcn_readfirstlane(min(pb_sees(a, s, min(x0, s.nq - 1)), kend));
+    const int sees_last = __builtin_amdgcn_readfirstlane(min(pb_sees(a, s, min(x0 + 15, s.nq - 1)), kend));
+    const bool idle = x0 >= s.nq;
     u32x4 kr[NP], vr[NP];
     auto load = [&](int t0) {                        // positions t0 .. t0 + RT - 1
         if (t0 < kend && t0 - jb >= 16 * 64) {
@@ -1028,8 +1107,8 @@ paged_items_f32_kernel(BatchArgs<T> a) {
         mine[64 * (DT + dt)] = accK[dt];
     }
     __syncthreads();
-    if (kctx) pb_finish<HDP, true>(a, w, QW, ml, part);
-    else pb_finish<HDP, false>(a, w, QW, ml, part);
+    if (kctx) pb_finish<HDP, true>(a, w, QW, xb, 16, ml, part);
+    else pb_finish<HDP, false>(a, w, QW, xb, 16, ml, part);
 }
 
 // ------------------------------------------------------------------ the join
@@ -1241,7 +1320,7 @@ static int batch_launch(const BatchCall& c, hipStream_t st) {
 #undef LOOM_PB_M
 #define LOOM_PB_F(HDV)                                                                              \
         if (c.HD == HDV) {                                                                          \
-            hipLaunchKernelGGL((paged_items_f32_kernel<T, HDV>), grid, dim3(256), 0, st, a);        \
+            hipLaunchKernelGGL((paged_items_f32_kernel<T, HDV>), dim3(grid.x, kPbQ / 64), dim3(256), 0, st, a);        \
             done = true;                                                                            \
         }
         LOOM_PB_F(8) LOOM_PB_F(16) LOOM_PB_F(256)
