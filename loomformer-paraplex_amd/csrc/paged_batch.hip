@@ -27,6 +27,7 @@ constexpr int kPbMaxRows = 1024;
 constexpr int kPbQ = 128;           // queries (a token's heads of one kv head) of a block
 constexpr int kPbTile = 64;         // positions of a step of a block
 constexpr int kPbLeast = 2;         // an item has so many tiles at least
+constexpr float kPbRecord = 2.5e-4f;  // a query's record, in a block's time for a tile of its queries
 constexpr int kPbAlone = 64;        // rows with more queries fill a block by themselves and share nothing
 constexpr int kPbShare = 64;        // common positions from which reading them once pays
 constexpr int kPbMagic = 0x4c50424c;
@@ -44,27 +45,31 @@ struct alignas(64) PbSeg {
     int common;                     // the positions that a group of rows shares
     int nchunk, rec0;               // items; record of (chunk, x) is rec0 + chunk nq + x (rec0 < 0: none)
     int tiles;
-    int pseg0, gx0;                 // own, of a group: the group's first segment, x = 0's place in its list
-    int pad[3];
+    int pad[5];
 };
 struct alignas(16) PbItem {
     int seg, chunk, tile0, tile1;
 };
+// An own segment whose queries' sums are in records: of query x, records own + x and every
+// nq-th behind it, own_n in all, and, where the row shares positions, common_n of the group's segment
+// that holds the query, which is the g0 + x-th of the group's group_q.
+struct alignas(64) PbJoin {
+    int base, x0, nq;               // the list's first token, the first query's place in it
+    int own, own_n;
+    int common_n, common0, g0, group_q;
+    int pad[7];
+};
 
 // The plan's parts, in ints from its start
 struct PbLayout {
-    int64_t rows, segs, items, joins, toks, total;      // rows: 4 ints each
-    int cap_segs, cap_items, cap_joins, cap_toks;
+    int64_t rows, segs, items, joins, tasks, toks, total;    // rows: 4 ints each
+    int cap_segs, cap_items, cap_joins, cap_tasks, cap_toks;
     int64_t cap_recs;               // records of a kv head
-    int slots;
+    int slots;                      // blocks per kv head that the device holds at once
 };
-// header: 0 magic, 1 items, 2 joins, 3.. the sizes it was made for
+// header: 0 magic, 1 items, 2 tasks of the join (join * kPbParts + which four queries), 3.. the sizes it was made for
+constexpr int kPbParts = kPbQ / 4;
 constexpr int kPbHeader = 16;
-
-static int pb_slots(int64_t KVH) {
-    const int64_t n = 2 * (int64_t)device_cus() / KVH;
-    return n < 1 ? 1 : (int)n;
-}
 
 // What a plan can need at most.  Own segments: a row's last may be partly filled;
 // common ones: of the rows that share, at least two to a group.  An item is
@@ -72,19 +77,22 @@ static int pb_slots(int64_t KVH) {
 // slots + segments, and segments of more than one item have at most 2 slots of them.
 static PbLayout pb_layout(int64_t R, int64_t N, int64_t QH, int64_t KVH) {
     PbLayout p{};
-    const int64_t G = QH / KVH, NG = N * G, some = NG < kPbAlone * R ? NG : kPbAlone * R;
-    p.slots = pb_slots(KVH);
-    p.cap_segs = (int)(R + NG / kPbQ + R / 2 + some / kPbQ + 2);
+    const int64_t G = QH / KVH, NG = N * G, some = NG < kPbAlone * R ? NG : kPbAlone * R, cus = device_cus();
+    const int64_t slots = 2 * cus / KVH;
+    p.slots = slots < 1 ? 1 : (int)slots;
+    p.cap_segs = (int)(R + NG / 64 + R / 2 + some / kPbQ + 2);
     p.cap_items = p.cap_segs + p.slots;
     const int64_t split = kPbQ < NG ? kPbQ : NG;          // queries of a split segment
-    p.cap_joins = (int)(p.slots * ((split + 3) / 4) + some / 4 + R + 1);
+    p.cap_joins = (int)(p.slots + R + 1);
+    p.cap_tasks = (int)(p.slots * ((split + 3) / 4) + some / 4 + R + 1);
     p.cap_toks = (int)some + 1;
     p.cap_recs = 2 * p.slots * split + 2 * some;
     p.rows = kPbHeader;
     p.segs = (p.rows + 4 * R + 15) / 16 * 16;
-    p.items = p.segs + (int64_t)p.cap_segs * (sizeof(PbSeg) / 4);
-    p.joins = p.items + (int64_t)p.cap_items * (sizeof(PbItem) / 4);
-    p.toks = p.joins + 2 * (int64_t)p.cap_joins;
+    p.joins = p.segs + (int64_t)p.cap_segs * (sizeof(PbSeg) / 4);
+    p.items = p.joins + (int64_t)p.cap_joins * (sizeof(PbJoin) / 4);
+    p.tasks = p.items + (int64_t)p.cap_items * (sizeof(PbItem) / 4);
+    p.toks = p.tasks + p.cap_tasks;
     p.total = (p.toks + p.cap_toks + 3) / 4 * 4;
     return p;
 }
@@ -112,48 +120,58 @@ __device__ __forceinline__ int pb_fresh(const PlanArgs& a, int r) {
 // A wave per row: whether the row has a page for each of its tokens, the ones to come
 // included, and with which other row it shares how many leading pages.  Rows that
 // start with the same page belong together; the lowest of them leads, found in a hash
-// table in LDS that every block fills from all rows' first entries.  rows[r] = (the
+// table in LDS that every block fills from all rows' first entries.  A row's state: (the
 // leader or -1, whole pages in common with it, pages all there, 0).  Bound by the chain
 // first entries, hash, the two rows' entries, 256 of each in flight per wave.
 constexpr int kPbHash = 2048;
 
-__global__ void __launch_bounds__(1024)
-paged_rows_kernel(PlanArgs a) {
-    __shared__ int key[kPbHash], low[kPbHash];
-    const int tid = threadIdx.x, lane = tid & 63, PS = 1 << a.log_ps;
-    for (int i = tid; i < kPbHash; i += 1024) {
-        key[i] = -1;
-        low[i] = kPbMaxRows;
-    }
-    auto candidate = [&](int r, int m, int n, int page) {
-        return m > 0 && (int64_t)m * a.G <= kPbAlone && n >= PS && (unsigned)page < (unsigned)a.n_pages;
-    };
-    // (at most 1024 different keys in 2048 places: every search ends)
-    auto place = [&](int page) { return (int)(((uint32_t)page * 2654435761u) >> 21); };
-    __syncthreads();
+struct PbHash {
+    int key[kPbHash], low[kPbHash];
+};
+
+// (at most 1024 different keys in 2048 places: every search ends)
+__device__ __forceinline__ int pb_place(int page) { return (int)(((uint32_t)page * 2654435761u) >> 21); }
+
+__device__ __forceinline__ bool pb_candidate(const PlanArgs& a, int m, int n, int page) {
+    return m > 0 && (int64_t)m * a.G <= kPbAlone && n >= 1 << a.log_ps && (unsigned)page < (unsigned)a.n_pages;
+}
+
+// The table of all rows' first pages (1024 threads)
+__device__ __forceinline__ void pb_hash(const PlanArgs& a, PbHash& hash) {
+    const int tid = threadIdx.x;
+    int page = -1, m = 0, n = -1;
     if (tid < a.R) {
-        const int page = a.table[(int64_t)tid * a.table_ld];
-        if (candidate(tid, pb_fresh(a, tid), a.lens[tid], page)) {
-            for (int h = place(page);; h = (h + 1) & (kPbHash - 1)) {
-                const int was = atomicCAS(&key[h], -1, page);
-                if (was == -1 || was == page) {
-                    atomicMin(&low[h], tid);
-                    break;
-                }
+        page = a.table[(int64_t)tid * a.table_ld];
+        m = pb_fresh(a, tid);
+        n = a.lens[tid];
+    }
+    for (int i = tid; i < kPbHash; i += 1024) {
+        hash.key[i] = -1;
+        hash.low[i] = kPbMaxRows;
+    }
+    __syncthreads();
+    if (pb_candidate(a, m, n, page)) {
+        for (int h = pb_place(page);; h = (h + 1) & (kPbHash - 1)) {
+            const int was = atomicCAS(&hash.key[h], -1, page);
+            if (was == -1 || was == page) {
+                atomicMin(&hash.low[h], tid);
+                break;
             }
         }
     }
     __syncthreads();
-    const int r = blockIdx.x * 16 + __builtin_amdgcn_readfirstlane(tid >> 6);
-    if (r >= a.R) return;
-    const int n = a.lens[r], m = pb_fresh(a, r);
+}
+
+// Row r's state, by a wave
+__device__ __forceinline__ int4 pb_row(const PlanArgs& a, const PbHash& hash, int r) {
+    const int lane = threadIdx.x & 63, PS = 1 << a.log_ps, n = a.lens[r], m = pb_fresh(a, r);
     const int32_t* row = a.table + (int64_t)r * a.table_ld;
     const int first = row[0];
     int lead = -1;
-    if (candidate(r, m, n, first)) {
-        int h = place(first);
-        while (key[h] != first) h = (h + 1) & (kPbHash - 1);
-        lead = low[h];
+    if (pb_candidate(a, m, n, first)) {
+        int h = pb_place(first);
+        while (hash.key[h] != first) h = (h + 1) & (kPbHash - 1);
+        lead = hash.low[h];
     }
     lead = __builtin_amdgcn_readfirstlane(lead);
     const bool fits = n >= 0 && n <= a.cap && m <= a.cap - n;
@@ -176,26 +194,36 @@ paged_rows_kernel(PlanArgs a) {
             if (differ) same = min(same, c0 + 64 * u + (int)__ffsll(differ) - 1);
         }
     }
-    if (lane == 0) *reinterpret_cast<int4*>(a.plan + a.at.rows + 4 * r) = make_int4(lead, same, there, 0);
+    return make_int4(lead, same, there, 0);
+}
+
+__global__ void __launch_bounds__(1024)
+paged_rows_kernel(PlanArgs a) {
+    __shared__ PbHash hash;
+    pb_hash(a, hash);
+    const int r = blockIdx.x * 16 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (r >= a.R) return;
+    const int4 s = pb_row(a, hash, r);
+    if ((threadIdx.x & 63) == 0) *reinterpret_cast<int4*>(a.plan + a.at.rows + 4 * r) = s;
 }
 
 // ------------------------------------------------------------------ plan
 
 // Exclusive scan of N counts over the 1024 threads of a block; total: their sums.
 template <int N>
-__device__ __forceinline__ void pb_scan(const int (&v)[N], int (*waves)[N], int (&before)[N], int (&total)[N]) {
+__device__ __forceinline__ void pb_scan(const int (&v)[N], int* waves, int (&before)[N], int (&total)[N]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int incl[N];
     __syncthreads();                                 // the previous use of `waves` is over
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         incl[k] = wave_scan_int(v[k]);
-        if (lane == 63) waves[wave][k] = incl[k];
+        if (lane == 63) waves[wave * N + k] = incl[k];
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-        const int mine = lane < 16 ? waves[lane][k] : 0;
+        const int mine = lane < 16 ? waves[lane * N + k] : 0;
         const int upto = wave_scan_int(mine);
         total[k] = __builtin_amdgcn_readlane(upto, 15);
         before[k] = __builtin_amdgcn_readlane(upto - mine, __builtin_amdgcn_readfirstlane(wave)) + incl[k] - v[k];
@@ -216,21 +244,36 @@ __device__ __forceinline__ int pb_find(const int* values, int n, int x) {
 // tokens' rows, positions and slots.  Both begin with a scan over the rows' counts.
 // Block 0 is one block because each stage needs the whole of the one before; it is
 // bound by their latency, a pass over the rows or the segments with a block scan each.
+// ALONE: of few rows every block finds the states itself, and the launch before is saved.
+constexpr int kPbFewRows = 32;
+
+template <bool ALONE>
 __global__ void __launch_bounds__(1024)
 paged_plan_kernel(PlanArgs a) {
-    __shared__ int first[kPbMaxRows], m_of[kPbMaxRows], lead_of[kPbMaxRows];
+    __shared__ __align__(16) int first[kPbMaxRows], m_of[kPbMaxRows], lead_of[kPbMaxRows];
     __shared__ int gpages[kPbMaxRows], gtoks[kPbMaxRows], gbase[kPbMaxRows], pbase[kPbMaxRows], sbase[kPbMaxRows];
-    __shared__ int rowx[kPbMaxRows];
-    __shared__ int waves[16][3];
+    __shared__ int rowx[kPbMaxRows], grec[kPbMaxRows];
+    __shared__ int waves[16 * 4];
     const int tid = threadIdx.x, r = tid, PS = 1 << a.log_ps;
     int m = 0;
     int4 info = make_int4(-1, 0, 0, 0);
-    if (r < a.R) {
+    if constexpr (ALONE) {
+        __shared__ PbHash hash;
+        __shared__ int4 state[kPbFewRows];
+        if (r < a.R) m = pb_fresh(a, r);
+        pb_hash(a, hash);
+        for (int i = __builtin_amdgcn_readfirstlane(tid >> 6); i < a.R; i += 16) {
+            const int4 s = pb_row(a, hash, i);
+            if ((tid & 63) == 0) state[i] = s;
+        }
+        __syncthreads();
+        if (r < a.R) info = state[r];
+    } else if (r < a.R) {
         m = pb_fresh(a, r);
         info = *reinterpret_cast<const int4*>(a.plan + a.at.rows + 4 * r);
     }
     int m1[1] = {m}, start1[1], all1[1];
-    pb_scan<1>(m1, reinterpret_cast<int(*)[1]>(waves), start1, all1);
+    pb_scan<1>(m1, waves, start1, all1);
     const int start = start1[0];
     const bool ok = m > 0 && info.z != 0 && start + m <= a.N;
     first[r] = r < a.R ? start : 0x7fffffff;
@@ -272,35 +315,43 @@ paged_plan_kernel(PlanArgs a) {
     // common positions of the group that row r leads
     const bool pays = gbase[r] >= 2 && gpages[r] << a.log_ps >= kPbShare;
     const int npre = pays ? (gtoks[r] * a.G + kPbQ - 1) / kPbQ : 0;
-    const int nown = ok ? (int)(((int64_t)m * a.G + kPbQ - 1) / kPbQ) : 0;
+    const int64_t queries = ok ? (int64_t)m * a.G : 0;
     __syncthreads();
     if (!pays) gpages[r] = 0;
-    int three[3] = {pays ? gtoks[r] : 0, npre, nown}, before[3], total[3];
-    pb_scan<3>(three, waves, before, total);
+    int four[4] = {pays ? gtoks[r] : 0, npre, (int)((queries + kPbQ - 1) / kPbQ), (int)((queries + 63) / 64)}, before[4], total[4];
+    pb_scan<4>(four, waves, before, total);
+    // own segments of 64 queries where those fill the device whole and ones of 128 would have to be split
+    const bool small = total[2] < a.at.slots && total[3] >= a.at.slots;
+    const int own_q = small ? 64 : kPbQ, n_own = small ? total[3] : total[2];
     gbase[r] = before[0];
     pbase[r] = before[1];
-    sbase[r] = total[1] + before[2];
+    sbase[r] = total[1] + (small ? before[3] : before[2]);
     __syncthreads();
     const int shared = lead >= 0 ? gpages[lead] << a.log_ps : 0;
     int ahead = 0;                                   // tokens of the group's rows before this one
     if (shared > 0) {
-        for (int i = lead; i < r; ++i) ahead += lead_of[i] == lead ? m_of[i] : 0;
+#pragma unroll 4
+        for (int i = lead & ~3; i < r; i += 4) {     // (rows in front of the leader have others)
+            const int4 l = *reinterpret_cast<const int4*>(lead_of + i), n = *reinterpret_cast<const int4*>(m_of + i);
+            ahead += (l.x == lead ? n.x : 0) + (l.y == lead && i + 1 < r ? n.y : 0) + (l.z == lead && i + 2 < r ? n.z : 0) +
+                     (l.w == lead && i + 3 < r ? n.w : 0);
+        }
         for (int i = 0; i < m; ++i) a.plan[a.at.toks + gbase[lead] + ahead + i] = start + i;
     }
     rowx[r] = ahead;
     if (r < a.R) a.shared[r] = shared;
     __syncthreads();
 
-    const int nseg = total[1] + total[2];
-    // a segment without its share of the work
-    auto segment = [&](int i) __attribute__((always_inline)) {
+    const int nseg = total[1] + n_own;
+    // a segment without its share of the work; *of: its row or its group's leader
+    auto segment = [&](int i, int* of) __attribute__((always_inline)) {
         PbSeg s;
         s.common = i < total[1];
-        const int row = pb_find(s.common ? pbase : sbase, a.R, i), x0 = (i - (s.common ? pbase : sbase)[row]) * kPbQ;
+        const int row = pb_find(s.common ? pbase : sbase, a.R, i);
+        const int x0 = s.common ? (i - pbase[row]) * kPbQ : (i - sbase[row]) * own_q;
+        *of = row;
         s.row = row;
         s.x0 = x0;
-        s.pseg0 = -1;
-        s.gx0 = 0;
         if (s.common) {
             s.nq = min(kPbQ, gtoks[row] * a.G - x0);
             s.base = gbase[row];
@@ -308,59 +359,98 @@ paged_plan_kernel(PlanArgs a) {
             s.key1 = gpages[row] << a.log_ps;
             s.lens = s.key1;
         } else {
-            s.nq = (int)min((int64_t)kPbQ, (int64_t)m_of[row] * a.G - x0);
+            s.nq = (int)min((int64_t)own_q, (int64_t)m_of[row] * a.G - x0);
             s.base = first[row];
             s.lens = a.lens[row];
             const int l = lead_of[row];
             s.key0 = l >= 0 ? gpages[l] << a.log_ps : 0;
             s.key1 = s.lens + (x0 + s.nq - 1) / a.G + 1;
-            if (s.key0 > 0) {
-                s.pseg0 = pbase[l];
-                s.gx0 = rowx[row] * a.G;
-            }
         }
         s.tiles = (s.key1 - s.key0 + kPbTile - 1) / kPbTile;
         return s;
     };
+    auto chunks = [&](int n, int chunk) { return (n + chunk - 1) / chunk; };
     // (up to 2^24 segments of 2^18 tiles: the sum's upper and lower 20 bits apart)
-    int64_t mine = 0;
-    for (int i = tid; i < nseg; i += 1024) mine += segment(i).tiles;
-    int sum[2] = {(int)(mine >> 20), (int)(mine & 0xfffff)}, none[2], tiles[2];
-    pb_scan<2>(sum, reinterpret_cast<int(*)[2]>(waves), none, tiles);
+    int64_t mine = 0, sixteens = 0;                  // tiles; tiles times blocks of 16 queries
+    int of = 0;
+    PbSeg s{};                                       // the thread's first segment, often its only one
+    for (int i = tid; i < nseg; i += 1024) {
+        const PbSeg g = segment(i, &of);
+        if (i == tid) s = g;
+        mine += g.tiles;
+        sixteens += (int64_t)g.tiles * ((g.nq + 15) / 16);
+    }
+    const int of0 = nseg <= 1024 ? of : 0;
+    // the common segments' records come first: a group's begin behind those of the groups before it
+    int sum[4] = {(int)(mine >> 20), (int)(mine & 0xfffff), (int)(sixteens >> 20), (int)(sixteens & 0xfffff)}, none[4], tiles[4];
+    pb_scan<4>(sum, waves, none, tiles);
     const int64_t all_tiles = ((int64_t)tiles[0] << 20) + tiles[1];
-    const int chunk = max(kPbLeast, (int)min((all_tiles + a.at.slots - 1) / a.at.slots, (int64_t)1 << 30));
-    int item0 = 0, rec0 = 0, join0 = 0;
+    // An item has at least the tiles that fill the device.  It leaves a record per query, which
+    // is written and read at the copy's rate by all blocks together, while a tile is
+    // one block's time: c tiles and work / c records take least where c^2 is their ratio.
+    const float ratio = kPbRecord * (float)a.KVH * 16.0f * ((float)tiles[2] * 1048576.0f + (float)tiles[3]);
+    const int64_t fill = (all_tiles + a.at.slots - 1) / a.at.slots;
+    const int chunk = max(max(kPbLeast, (int)sqrtf(ratio)), (int)min(fill, (int64_t)1 << 30));
+    if (total[1] > 0) {
+        const int positions = gpages[r] << a.log_ps;
+        int recs[1] = {pays ? gtoks[r] * a.G * chunks((positions + kPbTile - 1) / kPbTile, chunk) : 0}, at1[1], all_r[1];
+        pb_scan<1>(recs, waves, at1, all_r);
+        grec[r] = at1[0];
+        __syncthreads();
+    }
+    int item0 = 0, rec0 = 0, join0 = 0, task0 = 0;
     for (int i0 = 0; i0 < nseg; i0 += 1024) {
         const int i = i0 + tid;
-        PbSeg s{};
-        int want[3] = {0, 0, 0}, at[3], all[3];
-        bool rec = false;
-        if (i < nseg) {
-            s = segment(i);
-            s.nchunk = (s.tiles + chunk - 1) / chunk;
-            rec = s.nchunk > 1 || s.common || s.pseg0 >= 0;
-            want[0] = s.nchunk;
-            want[1] = rec ? s.nchunk * s.nq : 0;
-            want[2] = rec && !s.common ? (s.nq + 3) / 4 : 0;
+        const bool in = i < nseg;
+        of = of0;
+        if (nseg > 1024 && in) s = segment(i, &of);
+        int want[4] = {0, 0, 0, 0}, at[4], sums[4];
+        bool rec = false, shares = false;
+        if (in) {
+            s.nchunk = chunks(s.tiles, chunk);
+            shares = !s.common && s.key0 > 0;
+            rec = s.nchunk > 1 || s.common || shares;
+            want[0] = rec ? s.nchunk * s.nq : 0;
+            want[1] = rec && !s.common;
+            want[2] = s.nchunk;
+            want[3] = want[1] ? (s.nq + 3) / 4 : 0;
         }
-        pb_scan<3>(want, waves, at, all);
-        if (i < nseg) {
-            s.rec0 = rec ? rec0 + at[1] : -1;
+        pb_scan<4>(want, waves, at, sums);
+        if (in) {
+            s.rec0 = rec ? rec0 + at[0] : -1;
             reinterpret_cast<PbSeg*>(a.plan + a.at.segs)[i] = s;
-            PbItem* items = reinterpret_cast<PbItem*>(a.plan + a.at.items) + item0 + at[0];
+            PbItem* items = reinterpret_cast<PbItem*>(a.plan + a.at.items) + item0 + at[2];
+            const int q = s.tiles / s.nchunk, more = s.tiles - q * s.nchunk;
             for (int k = 0; k < s.nchunk; ++k)
-                items[k] = PbItem{i, k, (int)((int64_t)k * s.tiles / s.nchunk), (int)((int64_t)(k + 1) * s.tiles / s.nchunk)};
-            int2* joins = reinterpret_cast<int2*>(a.plan + a.at.joins) + join0 + at[2];
-            for (int k = 0; k < want[2]; ++k) joins[k] = make_int2(i, 4 * k);
+                items[k] = PbItem{i, k, k * q + min(k, more), (k + 1) * q + min(k + 1, more)};
+            if (want[1]) {
+                PbJoin t{};
+                t.base = s.base;
+                t.x0 = s.x0;
+                t.nq = s.nq;
+                t.own = s.rec0;
+                t.own_n = s.nchunk;
+                if (shares) {
+                    const int l = lead_of[of];
+                    t.common_n = chunks(((gpages[l] << a.log_ps) + kPbTile - 1) / kPbTile, chunk);
+                    t.common0 = grec[l];
+                    t.g0 = rowx[of] * a.G + s.x0;
+                    t.group_q = gtoks[l] * a.G;
+                }
+                reinterpret_cast<PbJoin*>(a.plan + a.at.joins)[join0 + at[1]] = t;
+                int32_t* tasks = a.plan + a.at.tasks + task0 + at[3];
+                for (int k = 0; k < want[3]; ++k) tasks[k] = (join0 + at[1]) * kPbParts + k;
+            }
         }
-        item0 += all[0];
-        rec0 += all[1];
-        join0 += all[2];
+        rec0 += sums[0];
+        join0 += sums[1];
+        item0 += sums[2];
+        task0 += sums[3];
     }
     if (tid == 0) {
         a.plan[0] = kPbMagic;
         a.plan[1] = item0;
-        a.plan[2] = join0;
+        a.plan[2] = task0;
         a.plan[3] = a.R;
         a.plan[4] = a.N;
         a.plan[5] = a.QH;
@@ -431,16 +521,15 @@ __device__ __forceinline__ void store_e(T* p, const float (&v)[E]) {
     }
 }
 
-// A wave per token: q and k roped and rounded, q to q_out, k and v into the token's
-// slot.  A lane takes E elements of a head and their partners half a head on, so that
+// A block per token: q and k roped and rounded, q to q_out, k and v into the token's
+// slot.  A thread takes E elements of a head and their partners half a head on, so that
 // each is loaded once.  Tokens behind the last give zeros, tokens of a row without room
 // or a page NaN; both are done here.  A copy with a little arithmetic: bound by the
-// bytes in and out.
+// bytes in and out, or, of few tokens, by one load after the other.
 template <typename T, int E>
 __global__ void __launch_bounds__(256)
 paged_append_kernel(BatchArgs<T> a) {
-    const int t = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (t >= a.N) return;
+    const int t = blockIdx.x, tid = threadIdx.x;
     const int row = a.rows_of[t], pos = a.positions[t], half = a.HD / 2;
     const int64_t slot = a.slots_of[t], page = slot >> a.log_ps;
     const bool fits = plan_fits(a);
@@ -450,7 +539,7 @@ paged_append_kernel(BatchArgs<T> a) {
         float v[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] = fill;
-        for (int i = lane; i < a.QH * a.HD / E; i += 64) {
+        for (int i = tid; i < a.QH * a.HD / E; i += 256) {
             const int h = i * E / a.HD, d = i * E - h * a.HD;
             store_e<T, E>(a.q_out + ((int64_t)t * a.QH + h) * a.HD + d, v);
             // (the items write those of tokens that the plan has)
@@ -458,48 +547,48 @@ paged_append_kernel(BatchArgs<T> a) {
             store_e<T, E>(a.c_out + t * a.out_ld + i * E, v);
             if (a.k_out != nullptr) store_e<T, E>(a.k_out + t * a.out_ld + i * E, v);
         }
-        if (lane == 0) a.odd[t] = 1;
+        if (tid == 0) a.odd[t] = 1;
         return;
     }
     const T* x = a.qkv + t * a.qkv_ld;
     const float *cr = a.cosv + (int64_t)pos * a.HD, *sr = a.sinv + (int64_t)pos * a.HD;
     const int64_t at = page * a.ps_page + (slot & ((1 << a.log_ps) - 1)) * a.ps_tok;
-    const int per = half / E;
+    const int per = half / E, turns = (a.QH + a.KVH) * per, vper = a.HD / E;
     bool odd = false;
-    for (int i = lane; i < (a.QH + a.KVH) * per; i += 64) {
-        const int h = i / per, d = (i - h * per) * E;
-        float u[E], w[E], c0[E], s0[E], c1[E], s1[E], lo[E], hi[E];
-        load_e<T, E>(x + h * a.HD + d, u);
-        load_e<T, E>(x + h * a.HD + d + half, w);
-        load_e<float, E>(cr + d, c0);
-        load_e<float, E>(sr + d, s0);
-        load_e<float, E>(cr + d + half, c1);
-        load_e<float, E>(sr + d + half, s1);
+    for (int i = tid; i < turns + a.KVH * vper; i += 256) {
+        if (i < turns) {
+            const int h = i / per, d = (i - h * per) * E;
+            float u[E], w[E], c0[E], s0[E], c1[E], s1[E], lo[E], hi[E];
+            load_e<T, E>(x + h * a.HD + d, u);
+            load_e<T, E>(x + h * a.HD + d + half, w);
+            load_e<float, E>(cr + d, c0);
+            load_e<float, E>(sr + d, s0);
+            load_e<float, E>(cr + d + half, c1);
+            load_e<float, E>(sr + d + half, s1);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            lo[e] = turn<T>(u[e], c0[e], -w[e], s0[e]);
-            hi[e] = turn<T>(w[e], c1[e], u[e], s1[e]);
-        }
-        T* out = h < a.QH ? a.q_out + ((int64_t)t * a.QH + h) * a.HD : a.kp + at + (h - a.QH) * a.ps_head;
-        store_e<T, E>(out + d, lo);
-        store_e<T, E>(out + d + half, hi);
-        if (h >= a.QH) {
+            for (int e = 0; e < E; ++e) {
+                lo[e] = turn<T>(u[e], c0[e], -w[e], s0[e]);
+                hi[e] = turn<T>(w[e], c1[e], u[e], s1[e]);
+            }
+            T* out = h < a.QH ? a.q_out + ((int64_t)t * a.QH + h) * a.HD : a.kp + at + (h - a.QH) * a.ps_head;
+            store_e<T, E>(out + d, lo);
+            store_e<T, E>(out + d + half, hi);
+            if (h >= a.QH) {
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                odd |= !(fabsf(round_to<T>(lo[e])) < INFINITY) || !(fabsf(round_to<T>(hi[e])) < INFINITY);
+                for (int e = 0; e < E; ++e)
+                    odd |= !(fabsf(round_to<T>(lo[e])) < INFINITY) || !(fabsf(round_to<T>(hi[e])) < INFINITY);
+            }
+        } else {
+            const int h = (i - turns) / vper, d = (i - turns - h * vper) * E;
+            float u[E];
+            load_e<T, E>(x + (a.QH + a.KVH + h) * a.HD + d, u);
+            store_e<T, E>(a.vp + at + h * a.ps_head + d, u);
+#pragma unroll
+            for (int e = 0; e < E; ++e) odd |= !(fabsf(u[e]) < INFINITY);
         }
     }
-    const int vper = a.HD / E;
-    for (int i = lane; i < a.KVH * vper; i += 64) {
-        const int h = i / vper, d = (i - h * vper) * E;
-        float u[E];
-        load_e<T, E>(x + (a.QH + a.KVH + h) * a.HD + d, u);
-        store_e<T, E>(a.vp + at + h * a.ps_head + d, u);
-#pragma unroll
-        for (int e = 0; e < E; ++e) odd |= !(fabsf(u[e]) < INFINITY);
-    }
-    odd = __any(odd);
-    if (lane == 0) a.odd[t] = odd;
+    odd = __syncthreads_or(odd);
+    if (tid == 0) a.odd[t] = odd;
 }
 
 // What a block works on: its item, or nothing (seg < 0)
@@ -510,22 +599,24 @@ struct PbWork {
     bool any;
 };
 
+// Item blockIdx.x / KVH of kv head blockIdx.x % KVH: blocks go to the XCDs in turn, so that 8 kv
+// heads have an XCD's L2 each for their keys, and fewer share them among several.
 template <typename T>
 __device__ __forceinline__ PbWork pb_work(const BatchArgs<T>& a) {
     PbWork w;
-    const int n_items = min(a.plan[1], a.at.cap_items);
-    const int n = n_items * a.KVH, L = (int)blockIdx.x;
-    w.any = L < n && plan_fits(a);
-    if (!w.any) return w;
-    const int k = xcd_contiguous(L, n);
-    w.kvh = k / n_items;
+    const int item = blockIdx.x / a.KVH;
     auto uniform = [](auto v) {                      // the same in all lanes, which the compiler may not see
         int* p = reinterpret_cast<int*>(&v);
 #pragma unroll
         for (int i = 0; i < (int)(sizeof(v) / sizeof(int)); ++i) p[i] = __builtin_amdgcn_readfirstlane(p[i]);
         return v;
     };
-    w.it = uniform(reinterpret_cast<const PbItem*>(a.plan + a.at.items)[k - w.kvh * n_items]);
+    // (the item is loaded with the count that says whether it is one)
+    const PbItem it = reinterpret_cast<const PbItem*>(a.plan + a.at.items)[item];
+    w.any = item < a.plan[1] && plan_fits(a);
+    if (!w.any) return w;
+    w.kvh = blockIdx.x - item * a.KVH;
+    w.it = uniform(it);
     w.s = uniform(reinterpret_cast<const PbSeg*>(a.plan + a.at.segs)[w.it.seg]);
     return w;
 }
@@ -543,9 +634,12 @@ __device__ __forceinline__ int pb_sees(const BatchArgs<T>& a, const PbSeg& s, in
     return s.common ? s.key1 : s.lens + (s.x0 + x) / a.G + 1;
 }
 
-// Whether a new token that some query of the block must not see, but others read with
-// it in one tile, holds an infinity or NaN: zero weights do not silence those in a
-// matrix product.  Such tokens lie from the first query's position on.
+// Infinities and NaN.  A weight of zero does not silence them in a matrix product, so a
+// new token that holds one must not enter the products of queries that do not see it.
+// Where a block has such a token (pb_odd), the products leave out what is not finite in
+// rows that not every query sees, and the item's end adds it to the sums of the
+// queries that do (pb_poison): an infinity of v is the sum's, one of k (whose score is NaN
+// or an infinity, and 0 times an infinity) is NaN.  Such tokens lie behind the first query's.
 template <typename T>
 __device__ __forceinline__ bool pb_odd(const BatchArgs<T>& a, const PbSeg& s) {
     bool odd = false;
@@ -556,13 +650,43 @@ __device__ __forceinline__ bool pb_odd(const BatchArgs<T>& a, const PbSeg& s) {
     return odd;
 }
 
+template <typename T>
+__device__ __noinline__ pg_f32x4 pb_poison(const T* pool, const uint8_t* odd, const int32_t* row, int64_t ps_page, int64_t ps_tok,
+                                           int lens, int log_ps, int n_pages, int first, int last, bool nan) {
+    pg_f32x4 c = {0.f, 0.f, 0.f, 0.f};
+    for (int i = first; i <= last; ++i) {
+        if (odd[i] == 0) continue;
+        const int t = lens + i, page = row[t >> log_ps];
+        if ((unsigned)page >= (unsigned)n_pages) continue;
+        const T* p = pool + (int64_t)page * ps_page + (int64_t)(t & ((1 << log_ps) - 1)) * ps_tok;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float v = ld(p + e);
+            if (!(fabsf(v) < INFINITY)) c[e] += nan ? NAN : v;
+        }
+    }
+    return c;
+}
+
+// 16-bit elements that are not finite as zeros
+template <typename T>
+__device__ __forceinline__ gqa_u4 pb_finite(gqa_u4 w) {
+    constexpr uint32_t E = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if ((w[i] & E) == E) w[i] &= 0xffff0000u;
+        if ((w[i] & (E << 16)) == E << 16) w[i] &= 0xffffu;
+    }
+    return w;
+}
+
 // The end of an item, for 16 queries of each wave: the waves' (m, l, C, Kctx) from LDS
 // joined into records, or into the outputs where the queries have no other part.
 // part(w): the sums of wave w's queries as its lanes hold them, C then Kctx, four queries'
 // of one dimension side by side; ml[w][16]: (m, l).  QW waves stand side by side: wave w's
 // queries begin at first + (w % QW) apart, and waves w, w + QW, .. have the same.
 template <int HDP, bool KCTX, typename T, typename P>
-__device__ __forceinline__ void pb_finish(const BatchArgs<T>& a, const PbWork& w, int QW, int first, int apart,
+__device__ __forceinline__ void pb_finish(const BatchArgs<T>& a, const PbWork& w, int QW, int first, int apart, bool odd,
                                           const float2 (*ml)[16], P part) {
     const PbSeg& s = w.s;
     constexpr int quads = HDP / 4, per = KCTX ? 2 * quads : quads;
@@ -583,6 +707,9 @@ __device__ __forceinline__ void pb_finish(const BatchArgs<T>& a, const PbWork& w
 #pragma unroll
             for (int i = 0; i < 4; ++i) c[i] = fmaf(v[4 * i], f, c[i]);
         }
+        if (odd && !(HDP > a.HD && d >= a.HD))
+            c += pb_poison((which ? a.kp : a.vp) + w.kvh * a.ps_head + d, a.odd + s.base, a.table + (int64_t)s.row * a.table_ld, a.ps_page,
+                           a.ps_tok, s.lens, a.log_ps, a.n_pages, s.x0 / a.G + 1, (s.x0 + x) / a.G, which);
         if (s.rec0 < 0) {
             if (HDP > a.HD && d >= a.HD) continue;
             const int h = w.kvh * a.G + (s.x0 + x) % a.G;
@@ -616,6 +743,41 @@ __device__ __forceinline__ void pb_finish(const BatchArgs<T>& a, const PbWork& w
 // lane by lane: the lanes of a column meet only where it has to rise.
 template <int HD> constexpr int pb_stages() { return HD <= 96 ? 3 : 2; }
 
+// Where a row's 16-byte pieces lie in a stage: piece c of row r at c ^ swz(r), so that both
+// fragment reads spread over the banks.  Rows of 4 or 12 pieces go by attn_tile.h's two bits;
+// of 8 and 16, where rows begin on the same banks, by three and four.  LDS cycles of a 16-byte
+// read and of a transposing one, timed over such maps with 16 waves: 3.7 and 2.05 at best
+// (the two bits in rows of 16 pieces: 10.9 and 4.9; no swizzle: 19.3 and 9.0).
+template <int CPR>
+struct PbLane {
+    static constexpr bool kXor = CPR == 8 || CPR == 16;
+    // nibble r: bits (r2, r1, r1^r2, r0^r3) of rows of 16 pieces, (r0^r1, r1, r1^r2) of 8
+    static constexpr uint64_t kMap = CPR == 16 ? 0x3b5d6e08b3d5e680ull : 0x2354671023546710ull;
+    const TileLane<CPR> lane;
+    uint32_t s_at, t_at;
+    __device__ __forceinline__ static int swz(int r) {
+        if constexpr (kXor) return (int)(kMap >> (4 * (r & 15))) & 15;
+        else return kv_swz(r);
+    }
+    __device__ __forceinline__ PbLane(int lq, int lr) : lane(lq, lr) {
+        const int row = 4 * lq + (lr >> 2);
+        s_at = (uint32_t)(lr * CPR + (lq ^ swz(lr))) * 16;
+        t_at = (uint32_t)(row * CPR + (((lr & 3) >> 1) ^ swz(row))) * 16 + 8 * (lr & 1);
+    }
+    // the A operand of S^T: row 16 hf + l % 16, dims 32 kk + 8 (l / 16) ..
+    __device__ __forceinline__ gqa_u4 s_frag(const gqa_u4* tile, int hf, int kk) const {
+        if constexpr (kXor)
+            return *reinterpret_cast<const gqa_u4*>(reinterpret_cast<const char*>(tile + 16 * hf * CPR) + (s_at ^ (kk << 6)));
+        else return tile_s_frag<CPR>(tile, lane, hf, kk);
+    }
+    // rows 16 h + 4 (l / 16) .. + 3 of dim 16 dt + l % 16
+    __device__ __forceinline__ uint2 tr_half(const gqa_u4* tile, int h, int dt) const {
+        const char* p = reinterpret_cast<const char*>(tile + 16 * h * CPR) +
+                        (kXor ? t_at ^ (dt << 5) : lane.t_off[dt & 1][0] + 64 * (dt >> 1));
+        return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) gqa_v4s*)(p)));
+    }
+};
+
 template <typename T, int HD, bool KCTX>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
 paged_items_kernel(BatchArgs<T> a) {
@@ -630,7 +792,7 @@ paged_items_kernel(BatchArgs<T> a) {
     const PbSeg& s = w.s;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int lr = lane & 15, lq = lane >> 4;
-    const TileLane<CPR> tl(lq, lr);
+    const PbLane<CPR> tl(lq, lr);
     const int kend = min(s.key1, s.key0 + w.it.tile1 * R);
     const int32_t* trow = a.table + (int64_t)s.row * a.table_ld;
 
@@ -646,7 +808,7 @@ paged_items_kernel(BatchArgs<T> a) {
 #pragma unroll
     for (int j = 0; j < GPW; ++j) {
         const int p = 64 * j + lane, row = p / CPR, c = p - row * CPR;
-        voff[j] = (uint32_t)(row * (int)a.ps_tok * (int)sizeof(T)) + (uint32_t)(c ^ kv_swz(row)) * 16u;
+        voff[j] = (uint32_t)(row * (int)a.ps_tok * (int)sizeof(T)) + (uint32_t)(c ^ tl.swz(row)) * 16u;
     }
     auto kst = [&](auto s_) -> gqa_u4* {
         constexpr int I = decltype(s_)::value;
@@ -686,12 +848,11 @@ paged_items_kernel(BatchArgs<T> a) {
     using I4 = std::integral_constant<int, 4>;
     const bool odd = __syncthreads_or(odd_mine);
 
-    auto body = [&](auto kw_, auto nq_, auto odd_, int xb) __attribute__((always_inline)) {   // queries from xb on
+    auto body = [&](auto kw_, auto nq_) __attribute__((always_inline)) {
         constexpr int KW = decltype(kw_)::value, NQ = decltype(nq_)::value, QW = 4 / KW;
-        constexpr bool ODD = decltype(odd_)::value;
         constexpr int NHF = KW == 4 ? 1 : 2;                 // 16-row parts of a fold
         constexpr int FOLDS = 4 / (KW * NHF);                // folds of a wave per tile
-        const int kg = wave / QW, x0 = xb + (wave & (QW - 1)) * 16 * NQ;
+        const int kg = wave / QW, x0 = (wave & (QW - 1)) * 16 * NQ;
         // q of column lr, positions that the column sees; (columns without a query: the last one's)
         uint4 qf[NQ][KK];
         int sees[NQ];
@@ -704,6 +865,7 @@ paged_items_kernel(BatchArgs<T> a) {
             sees[n] = min(pb_sees(a, s, x), kend);
         }
         const int sees_first = __builtin_amdgcn_readfirstlane(min(pb_sees(a, s, min(x0, s.nq - 1)), kend));
+        const int seen_by_all = pb_sees(a, s, 0);            // positions that every query of the block sees
         float mh[NQ], off[NQ], lh[NQ];                       // the reference, minus it (0 before there is one), the sum
         pg_f32x4 accC[NQ][DT], accK[NQ][KCTX ? DT : 1];
 #pragma unroll
@@ -715,7 +877,8 @@ paged_items_kernel(BatchArgs<T> a) {
 #pragma unroll
             for (int dt = 0; dt < (KCTX ? DT : 1); ++dt) accK[n][dt] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        auto fold = [&](const gqa_u4* tk, const gqa_u4* tv, int r0) __attribute__((always_inline)) {
+        // rows r0 .. of the stage at tk, tv; the last `dirty` of the block's rows here are not seen by all its queries
+        auto fold = [&](const gqa_u4* tk, const gqa_u4* tv, int r0, int dirty) __attribute__((always_inline)) {
             pg_f32x4 sc[NQ][NHF];
 #pragma unroll
             for (int hf = 0; hf < NHF; ++hf) {
@@ -723,10 +886,21 @@ paged_items_kernel(BatchArgs<T> a) {
                 for (int n = 0; n < NQ; ++n) sc[n][hf] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int kk = 0; kk < KK; ++kk) {
-                    const uint4 f = __builtin_bit_cast(uint4, tile_s_frag<CPR>(tk, tl, hf, kk));
+                    const uint4 f = __builtin_bit_cast(uint4, tl.s_frag(tk, hf, kk));
 #pragma unroll
                     for (int n = 0; n < NQ; ++n) sc[n][hf] = M::dot(f, qf[n][kk], sc[n][hf]);
                 }
+            }
+            if (dirty > 0) {                         // the block's rows of this fold, now that all waves have their scores
+                lds_barrier();
+                gqa_u4* const k = const_cast<gqa_u4*>(tk - (KW == 1 ? 0 : kg * (R / KW) * CPR));
+                gqa_u4* const v = const_cast<gqa_u4*>(tv - (KW == 1 ? 0 : kg * (R / KW) * CPR));
+                constexpr int rows = KW == 1 ? 16 * NHF : R;
+                for (int i = max(rows - dirty, 0) * CPR + tid; i < rows * CPR; i += 256) {
+                    k[i] = pb_finite<T>(k[i]);
+                    v[i] = pb_finite<T>(v[i]);
+                }
+                lds_barrier();
             }
             const bool mask = r0 + 16 * NHF > sees_first;        // wave-uniform
             if (mask) {
@@ -782,38 +956,6 @@ paged_items_kernel(BatchArgs<T> a) {
                         lh[n] += pv[n][hf][r];
                     }
             }
-            if (ODD && mask) {
-                // one position at a time, with only the queries that see it
-#pragma unroll 1
-                for (int row = 0; row < 16 * NHF; ++row) {
-                    const int g = (row >> 2) & 3;
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n) {
-                        float mine = 0.0f;
-#pragma unroll
-                        for (int i = 0; i < 4 * NHF; ++i) mine = (row >> 4) * 4 + (row & 3) == i ? pv[n][i / 4][i % 4] : mine;
-                        float p[4];
-                        bool seen[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            p[i] = __shfl(mine, 16 * g + 4 * lq + i, 64);
-                            seen[i] = r0 + row < __shfl(sees[n], 4 * lq + i, 64);
-                        }
-#pragma unroll
-                        for (int dt = 0; dt < DT; ++dt) {
-                            const int d = 16 * dt + lr, at = row * CPR + ((d >> 3) ^ kv_swz(row));
-                            const float v = ld(reinterpret_cast<const T*>(tv + at) + (d & 7));
-                            const float k = KCTX ? ld(reinterpret_cast<const T*>(tk + at) + (d & 7)) : 0.0f;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                accC[n][dt][i] = seen[i] ? fmaf(p[i], v, accC[n][dt][i]) : accC[n][dt][i];
-                                if constexpr (KCTX) accK[n][dt][i] = seen[i] ? fmaf(p[i], k, accK[n][dt][i]) : accK[n][dt][i];
-                            }
-                        }
-                    }
-                }
-                return;
-            }
             // the weights enter the products rounded to the storage type (half a step of
             // it, relative, per weight, down to Mfma16's smallest: below the rounding of
             // the outputs); their sum l is that of the unrounded ones
@@ -827,15 +969,12 @@ paged_items_kernel(BatchArgs<T> a) {
                 }
             }
             auto frag = [&](const gqa_u4* tile, int dt) __attribute__((always_inline)) {
-                if constexpr (NHF > 1) {
-                    return tile_tr_frag<CPR>(tile, tl, dt);
-                } else {                             // 16 rows: the other half meets zero weights
-                    const char* p = reinterpret_cast<const char*>(tile) + tl.t_off[dt & 1][0] + 64 * (dt >> 1);
-                    const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                                   (__attribute__((address_space(3))) gqa_v4s*)(p)));
-                    return make_uint4(lo.x, lo.y, 0, 0);
-                }
+                const uint2 lo = tl.tr_half(tile, 0, dt);
+                uint2 hi = make_uint2(0, 0);         // (of 16 rows the other half meets zero weights)
+                if constexpr (NHF > 1) hi = tl.tr_half(tile, 1, dt);
+                return make_uint4(lo.x, lo.y, hi.x, hi.y);
             };
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 const uint4 fv = frag(tv, dt);
@@ -847,9 +986,10 @@ paged_items_kernel(BatchArgs<T> a) {
                     for (int n = 0; n < NQ; ++n) accK[n][dt] = M::dot(pa[n], fk, accK[n][dt]);
                 }
             }
+            __builtin_amdgcn_s_setprio(0);
         };
-        // step j computes tile j from stage j % NS, requests tile j + NS - 1 into the stage
-        // that every wave is done with, waits for tile j + 1 and passes one barrier
+        // a step computes tile j from its stage, requests tile j + NS - 1 into the stage that every
+        // wave is done with, waits for tile j + 1 and passes one barrier
         auto step = [&](auto s_, int j) __attribute__((always_inline)) {
             constexpr int cur = decltype(s_)::value;
             load_tile(std::integral_constant<int, (cur + NS - 1) % NS>{}, j + NS - 1);
@@ -858,7 +998,9 @@ paged_items_kernel(BatchArgs<T> a) {
                 const int row = kg * (R / KW) + u * 16 * NHF, r0 = s.key0 + j * R + row;
                 // (unconditionally: a branch around it costs the loop's registers more than what a wave
                 // without a query, or that sees nothing here yet, could save)
-                fold(kst(s_) + row * CPR, vst(s_) + row * CPR, r0);
+                // (the block's: rows of the fold where all waves have the same, else of the tile)
+                const int end = KW == 1 ? r0 + 16 * NHF : s.key0 + (j + 1) * R;
+                fold(kst(s_) + row * CPR, vst(s_) + row * CPR, r0, odd ? end - seen_by_all : 0);
             }
             wait_vmcnt<2 * GPW * (NS - 2)>();
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -898,28 +1040,13 @@ paged_items_kernel(BatchArgs<T> a) {
                 if constexpr (KCTX) mine[64 * (DT + dt)] = accK[n][dt];
             }
             __syncthreads();
-            pb_finish<HD, KCTX>(a, w, QW, xb + 16 * n, 16 * NQ, ml, part);
+            pb_finish<HD, KCTX>(a, w, QW, 16 * n, 16 * NQ, odd, ml, part);
         }
     };
-    if (odd) {
-        // (code of its own, 64 queries at a time: its registers would be the others' loss)
-        for (int xb = 0; xb < s.nq; xb += 64) {
-            if (xb > 0) {
-                jb = w.it.tile0;
-                pages();
-                __syncthreads();                     // the last queries' sums are read
-            }
-            body(I1{}, I1{}, std::true_type{}, xb);
-        }
-    } else if (s.nq <= 16) {
-        body(I4{}, I1{}, std::false_type{}, 0);
-    } else if (s.nq <= 32) {
-        body(I2{}, I1{}, std::false_type{}, 0);
-    } else if (s.nq <= 64) {
-        body(I2{}, I2{}, std::false_type{}, 0);
-    } else {
-        body(I1{}, I2{}, std::false_type{}, 0);
-    }
+    if (s.nq <= 16) body(I4{}, I1{});
+    else if (s.nq <= 32) body(I2{}, I1{});
+    else if (s.nq <= 64) body(I2{}, I2{});
+    else body(I1{}, I2{});
 }
 
 // ------------------------------------------------------------------ fp32 form
@@ -1065,34 +1192,17 @@ paged_items_f32_kernel(BatchArgs<T> a) {
                     }
                 }
             }
-            if (odd && mask) {
-                // one position at a time, with only the queries that see it
-#pragma unroll 1
-                for (int n = 0; n < 16; ++n) {
-                    const int row = 16 * hf + n;
-                    const float own = (n & 3) == 0 ? pv[0] : (n & 3) == 1 ? pv[1] : (n & 3) == 2 ? pv[2] : pv[3];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float p = __shfl(own, 16 * (n >> 2) + 4 * lq + i, 64);
-                        const bool seen = t0 + row < __shfl(sees, 4 * lq + i, 64);
-#pragma unroll
-                        for (int dt = 0; dt < DT; ++dt) {
-                            const float v = tv[row * PITCH + 16 * dt + lr], k = tk[row * PITCH + 16 * dt + lr];
-                            accC[dt][i] = seen ? fmaf(p, v, accC[dt][i]) : accC[dt][i];
-                            accK[dt][i] = seen ? fmaf(p, k, accK[dt][i]) : accK[dt][i];
-                        }
-                    }
-                }
-                continue;
-            }
+            // (rows that not all columns see: see pb_odd)
+            const int partly = odd ? sees_first - r0 - 4 * lq : 4;
+            auto finite = [&](float v, int r) __attribute__((always_inline)) { return r >= partly && !(fabsf(v) < INFINITY) ? 0.0f : v; };
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float* vq = tv + (16 * hf + 4 * lq + r) * PITCH + lr;
                 const float* kx = tk + (16 * hf + 4 * lq + r) * PITCH + lr;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
-                    accC[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[r], vq[16 * dt], accC[dt], 0, 0, 0);
-                    if (kctx) accK[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[r], kx[16 * dt], accK[dt], 0, 0, 0);
+                    accC[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[r], finite(vq[16 * dt], r), accC[dt], 0, 0, 0);
+                    if (kctx) accK[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[r], finite(kx[16 * dt], r), accK[dt], 0, 0, 0);
                 }
             }
         }
@@ -1107,15 +1217,29 @@ paged_items_f32_kernel(BatchArgs<T> a) {
         mine[64 * (DT + dt)] = accK[dt];
     }
     __syncthreads();
-    if (kctx) pb_finish<HDP, true>(a, w, QW, xb, 16, ml, part);
-    else pb_finish<HDP, false>(a, w, QW, xb, 16, ml, part);
+    if (kctx) pb_finish<HDP, true>(a, w, QW, xb, 16, odd, ml, part);
+    else pb_finish<HDP, false>(a, w, QW, xb, 16, odd, ml, part);
 }
 
 // ------------------------------------------------------------------ the join
 // Four queries of an own segment per task: their records are the chunks of the segment
-// itself and of the group's segment that holds them.  Wave w takes records w, w + 4, ..
-// of all four queries, 2 kPbJoin in flight each; the waves meet in LDS.
+// itself and of the group's segments that hold them.  Where a query has few, a
+// wave does one, all its records in flight; else wave w takes records w, w + 4, .. of all
+// four, kPbJoin of each in flight, and the waves meet in LDS.  Bound by the records' bytes.
 constexpr int kPbJoin = 2;
+constexpr int kPbFew = 8;
+
+// (m, l, v) and a record's (e, y) as one
+template <int NV>
+__device__ __forceinline__ void pb_add(float& m, float& l, pg_f32x4 (&v)[NV], float2 e, const pg_f32x4 (&y)[NV]) {
+    const float most = fmaxf(m, e.x);
+    const float f = most == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - most);
+    const float g = most == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(e.x - most);
+    l = fmaf(l, f, e.y * g);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) v[k] = v[k] * f + y[k] * g;
+    m = most;
+}
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(256)
@@ -1124,86 +1248,96 @@ paged_batch_join_kernel(BatchArgs<T> a) {
     constexpr int NV = HDP > 128 ? 2 : 1, NL = HDP / 2 / NV;   // lanes of four sums
     __shared__ float2 ml[4][4];
     __shared__ __align__(16) float sums[4][4][2 * HDP];
-    if (!plan_fits(a)) return;
-    const int n_tasks = min(a.plan[2], a.at.cap_joins) * a.KVH, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int n_joins = n_tasks / a.KVH;
+    const int kvh = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int at = min(lane, NL - 1);
     const bool kctx = a.k_out != nullptr;
+    const PbJoin* joins = reinterpret_cast<const PbJoin*>(a.plan + a.at.joins);
+    int next = a.plan[a.at.tasks + min((int)blockIdx.x, a.at.cap_tasks - 1)];    // with the count that says whether it is one
+    const int n_tasks = min(a.plan[2], a.at.cap_tasks);
+    if (!plan_fits(a)) return;
+    const float* rec = a.rec + kvh * a.at.cap_recs * 2 * HDP;
+    const float* rml = a.rec + a.rec_ml + kvh * a.at.cap_recs * 2;
     for (int task = blockIdx.x; task < n_tasks; task += gridDim.x) {
-        const int kvh = task / n_joins;
-        const int2 jt = reinterpret_cast<const int2*>(a.plan + a.at.joins)[task - kvh * n_joins];
-        const PbSeg s = reinterpret_cast<const PbSeg*>(a.plan + a.at.segs)[jt.x];
-        const int x0 = jt.y, nx = min(4, s.nq - x0);
-        // the group's records of each query: (first, distance), and how many
-        int64_t common[4];
-        int step[4], nc = 0;
+        if (task != (int)blockIdx.x) next = a.plan[a.at.tasks + task];
+        const PbJoin t = joins[next / kPbParts];
+        const int y = 4 * (next % kPbParts), nx = min(4, t.nq - y);
+        const int base = t.base, x0 = t.x0 + y, own = t.own + y, own_step = t.nq, nc = t.common_n, n = nc + t.own_n;
+        // the group's segments: 128 queries each but the last, all of the same chunks; query
+        // `cut` of the four is the first of the next one
+        const int g = t.g0 + y, seg = g / kPbQ, r0 = t.common0 + seg * kPbQ * nc, cut = (seg + 1) * kPbQ - g;
+        const int step0 = min(kPbQ, t.group_q - seg * kPbQ), common0 = r0 + g - seg * kPbQ;
+        const int step1 = min(kPbQ, t.group_q - (seg + 1) * kPbQ), common1 = r0 + kPbQ * nc + g - (seg + 1) * kPbQ;
+        // record c of query i
+        auto place = [=](int i, int c) __attribute__((always_inline)) -> int64_t {
+            const int c0 = common0 + c * step0, c1 = common1 + c * step1, c2 = own + (c - nc) * own_step;
+            return (c >= nc ? c2 : i < cut ? c0 : c1) + i;
+        };
+        auto out = [=](int i, int d2, const float (&o)[4]) __attribute__((always_inline)) {   // four sums of query i from d2 on
+            const int which = d2 >= HDP, d = d2 - which * HDP;
+            if ((which && !kctx) || (HDP > HD && d >= HD)) return;
+            const int x = x0 + i, h = kvh * a.G + x % a.G;
+            store_e<T, 4>((which ? a.k_out : a.c_out) + (int64_t)(base + x / a.G) * a.out_ld + (int64_t)h * HD + d, o);
+        };
+        if (n <= kPbFew) {
+            const int i = wave;
+            if (i >= nx) continue;
+            float2 e[kPbFew];
+            pg_f32x4 y[kPbFew][NV];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            common[i] = 0;
-            step[i] = 0;
-            if (s.pseg0 < 0) continue;
-            const int gx = s.gx0 + s.x0 + x0 + min(i, nx - 1);
-            const PbSeg& p = reinterpret_cast<const PbSeg*>(a.plan + a.at.segs)[s.pseg0 + gx / kPbQ];
-            common[i] = p.rec0 + gx % kPbQ;
-            step[i] = p.nq;
-            nc = max(nc, p.nchunk);                  // (segments of a group have the same positions, so as many)
+            for (int c = 0; c < kPbFew; ++c) {
+                const int64_t r = place(i, min(c, n - 1));
+                e[c] = *reinterpret_cast<const float2*>(rml + 2 * r);
+#pragma unroll
+                for (int v = 0; v < NV; ++v)
+                    y[c][v] = *reinterpret_cast<const pg_f32x4*>(rec + r * 2 * HDP + 4 * (at + NL * v));
+            }
+            float m = e[0].x, l = e[0].y;
+#pragma unroll
+            for (int c = 1; c < kPbFew; ++c)
+                if (c < n) pb_add<NV>(m, l, y[0], e[c], y[c]);
+            const float inv = 1.0f / l;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const float o[4] = {y[0][v][0] * inv, y[0][v][1] * inv, y[0][v][2] * inv, y[0][v][3] * inv};
+                if (lane < NL) out(i, 4 * (lane + NL * v), o);
+            }
+            continue;
         }
-        const int n = nc + s.nchunk;
-        float M[4], L[4];
-        pg_f32x4 acc[4][NV];
+        float m[4], l[4];
+        pg_f32x4 sum[4][NV];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            M[i] = -INFINITY;
-            L[i] = 0.0f;
+            m[i] = -INFINITY;
+            l[i] = 0.0f;
 #pragma unroll
-            for (int v = 0; v < NV; ++v) acc[i][v] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int v = 0; v < NV; ++v) sum[i][v] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
         }
         for (int c0 = wave; c0 < n; c0 += 4 * kPbJoin) {
-            float2 e[kPbJoin][4];
-            pg_f32x4 y[kPbJoin][4][NV];
+            float2 e[4 * kPbJoin];
+            pg_f32x4 y[4 * kPbJoin][NV];
 #pragma unroll
-            for (int u = 0; u < kPbJoin; ++u) {
-                const int c = min(c0 + 4 * u, n - 1);
+            for (int k = 0; k < 4 * kPbJoin; ++k) {                  // query k / kPbJoin, the wave's next record k % kPbJoin
+                const int64_t r = place(min(k / kPbJoin, nx - 1), min(c0 + 4 * (k % kPbJoin), n - 1));
+                e[k] = *reinterpret_cast<const float2*>(rml + 2 * r);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int64_t r = kvh * a.at.cap_recs +
-                                      (c < nc ? common[i] + (int64_t)c * step[i] : s.rec0 + (int64_t)(c - nc) * s.nq + x0 + min(i, nx - 1));
-                    e[u][i] = *reinterpret_cast<const float2*>(a.rec + a.rec_ml + 2 * r);
-#pragma unroll
-                    for (int v = 0; v < NV; ++v)
-                        if (lane < NL) y[u][i][v] = *reinterpret_cast<const pg_f32x4*>(a.rec + r * 2 * HDP + 4 * (lane + NL * v));
-                }
+                for (int v = 0; v < NV; ++v)
+                    y[k][v] = *reinterpret_cast<const pg_f32x4*>(rec + r * 2 * HDP + 4 * (at + NL * v));
             }
 #pragma unroll
-            for (int u = 0; u < kPbJoin; ++u) {
-                if (c0 + 4 * u >= n) continue;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float m = fmaxf(M[i], e[u][i].x);
-                    const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M[i] - m);
-                    const float g = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(e[u][i].x - m);
-                    L[i] = fmaf(L[i], f, e[u][i].y * g);
-#pragma unroll
-                    for (int v = 0; v < NV; ++v)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) acc[i][v][k] = fmaf(acc[i][v][k], f, y[u][i][v][k] * g);
-                    M[i] = m;
-                }
-            }
+            for (int k = 0; k < 4 * kPbJoin; ++k)
+                if (c0 + 4 * (k % kPbJoin) < n) pb_add<NV>(m[k / kPbJoin], l[k / kPbJoin], sum[k / kPbJoin], e[k], y[k]);
         }
         __syncthreads();                             // the last task's sums are read
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (lane == 0) ml[i][wave] = make_float2(M[i], L[i]);
+            if (lane == 0) ml[i][wave] = make_float2(m[i], l[i]);
 #pragma unroll
             for (int v = 0; v < NV; ++v)
-                if (lane < NL) *reinterpret_cast<pg_f32x4*>(&sums[i][wave][4 * (lane + NL * v)]) = acc[i][v];
+                if (lane < NL) *reinterpret_cast<pg_f32x4*>(&sums[i][wave][4 * (lane + NL * v)]) = sum[i][v];
         }
         __syncthreads();
-        constexpr int quads = HDP / 4;
-        const int per = kctx ? 2 * quads : quads;
-        for (int k = threadIdx.x; k < nx * per; k += 256) {
-            const int i = k / per, d2 = 4 * (k - i * per), which = d2 >= HDP, d = d2 - which * HDP;
-            if (HDP > HD && d >= HD) continue;
+        for (int k = threadIdx.x; k < nx * (HDP / 4) * 2; k += 256) {
+            const int i = k / (HDP / 2), d2 = 4 * (k - i * (HDP / 2));
             float m = -INFINITY, l = 0.0f;
 #pragma unroll
             for (int v = 0; v < 4; ++v) m = fmaxf(m, ml[i][v].x);
@@ -1218,8 +1352,7 @@ paged_batch_join_kernel(BatchArgs<T> a) {
             const float inv = 1.0f / l;
 #pragma unroll
             for (int q = 0; q < 4; ++q) o[q] *= inv;
-            const int x = s.x0 + x0 + i, h = kvh * a.G + x % a.G;
-            store_e<T, 4>((which ? a.k_out : a.c_out) + (int64_t)(s.base + x / a.G) * a.out_ld + (int64_t)h * HD + d, o);
+            out(i, d2, o);
         }
     }
 }
@@ -1303,7 +1436,7 @@ static int batch_launch(const BatchCall& c, hipStream_t st) {
     a.n_pages = (int)c.n_pages;
     a.n_pos = (int)min(c.n_pos, (int64_t)1 << 30);
     a.qscale = kLog2e / sqrtf((float)c.HD);
-    const dim3 appends((unsigned)ceil_div(c.N, 4));
+    const dim3 appends((unsigned)c.N);
     if (c.HD >= 16) hipLaunchKernelGGL((paged_append_kernel<T, 8>), appends, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((paged_append_kernel<T, 4>), appends, dim3(256), 0, st, a);
     if (int rc = launch_status("loom_paged_batch_step(append)")) return rc;
@@ -1330,8 +1463,8 @@ static int batch_launch(const BatchCall& c, hipStream_t st) {
     }
     LOOM_CHECK(done, "paged_batch_step: unsupported head_dim %lld (8, 16, 32, 64, 96, 128 or 256)", (long long)c.HD);
     if (int rc = launch_status("loom_paged_batch_step(items)")) return rc;
-    const int64_t joins = (int64_t)a.at.cap_joins * c.KVH;
-    const dim3 jgrid((unsigned)(joins < 2048 ? joins : 2048));
+    const int64_t joins = ceil_div(4096, c.KVH);
+    const dim3 jgrid((unsigned)(joins < a.at.cap_tasks ? joins : a.at.cap_tasks), (unsigned)c.KVH);
 #define LOOM_PB_J(HDV)                                                                              \
     if (c.HD == HDV) hipLaunchKernelGGL((paged_batch_join_kernel<T, HDV>), jgrid, dim3(256), 0, st, a);
     LOOM_PB_J(96) LOOM_PB_J(128) LOOM_PB_J(64) LOOM_PB_J(32) LOOM_PB_J(16) LOOM_PB_J(8) LOOM_PB_J(256)
@@ -1382,11 +1515,14 @@ extern "C" int loom_paged_plan(const int32_t* table, int64_t table_ld, int64_t m
     a.cap = (int)(max_pages * page_size);
     a.n_pages = (int)n_pages;
     hipStream_t st = (hipStream_t)stream;
-    if (rows > 0) {
+    const dim3 blocks((unsigned)(1 + ceil_div(n_tokens, 1024)));
+    if (rows <= kPbFewRows) {
+        hipLaunchKernelGGL((paged_plan_kernel<true>), blocks, dim3(1024), 0, st, a);
+    } else {
         hipLaunchKernelGGL(paged_rows_kernel, dim3((unsigned)ceil_div(rows, 16)), dim3(1024), 0, st, a);
         if (int rc = launch_status("loom_paged_plan(rows)")) return rc;
+        hipLaunchKernelGGL((paged_plan_kernel<false>), blocks, dim3(1024), 0, st, a);
     }
-    hipLaunchKernelGGL(paged_plan_kernel, dim3((unsigned)(1 + ceil_div(n_tokens, 1024))), dim3(1024), 0, st, a);
     return launch_status("loom_paged_plan(plan)");
 }
 
