@@ -26,7 +26,7 @@ namespace loom {
 constexpr int kPbMaxRows = 1024;
 constexpr int kPbQ = 128;           // queries (a token's heads of one kv head) of a block
 constexpr int kPbTile = 64;         // positions of a step of a block
-constexpr int kPbLeast = 2;         // an item has so many tiles at least
+constexpr int kPbLeast = 1;         // an item has so many tiles at least
 constexpr float kPbRecord = 2.5e-4f;  // a query's record, in a block's time for a tile of its queries
 constexpr int kPbAlone = 64;        // rows with more queries fill a block by themselves and share nothing
 constexpr int kPbShare = 64;        // common positions from which reading them once pays
@@ -35,21 +35,21 @@ constexpr int64_t kPbMaxTokens = (int64_t)1 << 20;
 
 // A block of queries and the positions they read.  Query x (0 .. nq - 1) is query x0 +
 // x of a list of tokens times the kv head's G heads: token list entry (x0 + x) / G,
-// head (x0 + x) % G.
-struct alignas(64) PbSeg {
+// head (x0 + x) % G.  An item is a segment's tiles tile0 .. tile1 - 1, the work of a block.
+constexpr int kPbOwn = 0, kPbRun = 1, kPbList = 2;   // the list: a row's own tokens, a group's that
+                                                     // lie one behind the other, or a group's in toks
+struct alignas(64) PbItem {
     int row;                        // whose table entries name the pages
     int key0, key1;                 // positions key0 .. key1 - 1, key0 a multiple of 16
-    int base;                       // the list's first token (common: its place in toks)
+    int base;                       // the list's first token (or its place in toks)
     int x0, nq;
     int lens;                       // own: tokens the row held before the step
-    int common;                     // the positions that a group of rows shares
-    int nchunk, rec0;               // items; record of (chunk, x) is rec0 + chunk nq + x (rec0 < 0: none)
-    int tiles;
+    int kind;
+    int tile0, tile1;
+    int rec;                        // the item's record of query x is rec + x (< 0: none)
     int pad[5];
 };
-struct alignas(16) PbItem {
-    int seg, chunk, tile0, tile1;
-};
+
 // An own segment whose queries' sums are in records: of query x, records own + x and every
 // nq-th behind it, own_n in all, and, where the row shares positions, common_n of the group's segment
 // that holds the query, which is the g0 + x-th of the group's group_q.
@@ -62,8 +62,8 @@ struct alignas(64) PbJoin {
 
 // The plan's parts, in ints from its start
 struct PbLayout {
-    int64_t rows, segs, items, joins, tasks, toks, total;    // rows: 4 ints each
-    int cap_segs, cap_items, cap_joins, cap_tasks, cap_toks;
+    int64_t rows, items, joins, tasks, toks, total;    // rows: 4 ints each
+    int cap_items, cap_joins, cap_tasks, cap_toks;
     int64_t cap_recs;               // records of a kv head
     int slots;                      // blocks per kv head that the device holds at once
 };
@@ -80,18 +80,16 @@ static PbLayout pb_layout(int64_t R, int64_t N, int64_t QH, int64_t KVH) {
     const int64_t G = QH / KVH, NG = N * G, some = NG < kPbAlone * R ? NG : kPbAlone * R, cus = device_cus();
     const int64_t slots = 2 * cus / KVH;
     p.slots = slots < 1 ? 1 : (int)slots;
-    p.cap_segs = (int)(R + NG / 64 + R / 2 + some / kPbQ + 2);
-    p.cap_items = p.cap_segs + p.slots;
+    p.cap_items = (int)(R + NG / 64 + R / 2 + some / kPbQ + 2) + p.slots;
     const int64_t split = kPbQ < NG ? kPbQ : NG;          // queries of a split segment
     p.cap_joins = (int)(p.slots + R + 1);
     p.cap_tasks = (int)(p.slots * ((split + 3) / 4) + some / 4 + R + 1);
     p.cap_toks = (int)some + 1;
     p.cap_recs = 2 * p.slots * split + 2 * some;
     p.rows = kPbHeader;
-    p.segs = (p.rows + 4 * R + 15) / 16 * 16;
-    p.joins = p.segs + (int64_t)p.cap_segs * (sizeof(PbSeg) / 4);
-    p.items = p.joins + (int64_t)p.cap_joins * (sizeof(PbJoin) / 4);
-    p.tasks = p.items + (int64_t)p.cap_items * (sizeof(PbItem) / 4);
+    p.items = (p.rows + 4 * R + 15) / 16 * 16;
+    p.joins = p.items + (int64_t)p.cap_items * (sizeof(PbItem) / 4);
+    p.tasks = p.joins + (int64_t)p.cap_joins * (sizeof(PbJoin) / 4);
     p.toks = p.tasks + p.cap_tasks;
     p.total = (p.toks + p.cap_toks + 3) / 4 * 4;
     return p;
@@ -252,7 +250,7 @@ __global__ void __launch_bounds__(1024)
 paged_plan_kernel(PlanArgs a) {
     __shared__ __align__(16) int first[kPbMaxRows], m_of[kPbMaxRows], lead_of[kPbMaxRows];
     __shared__ int gpages[kPbMaxRows], gtoks[kPbMaxRows], gbase[kPbMaxRows], pbase[kPbMaxRows], sbase[kPbMaxRows];
-    __shared__ int rowx[kPbMaxRows], grec[kPbMaxRows];
+    __shared__ int rowx[kPbMaxRows], grec[kPbMaxRows], gend[kPbMaxRows];
     __shared__ int waves[16 * 4];
     const int tid = threadIdx.x, r = tid, PS = 1 << a.log_ps;
     int m = 0;
@@ -304,12 +302,14 @@ paged_plan_kernel(PlanArgs a) {
     lead_of[r] = lead;
     gpages[r] = 0x7fffffff;
     gtoks[r] = 0;
+    gend[r] = 0;
     gbase[r] = 0;                                    // rows of the group, for now
     __syncthreads();
     if (lead >= 0) {
         atomicMin(&gpages[lead], info.y);
         atomicAdd(&gtoks[lead], m);
         atomicAdd(&gbase[lead], 1);
+        atomicMax(&gend[lead], start + m);
     }
     __syncthreads();
     // common positions of the group that row r leads
@@ -343,22 +343,24 @@ paged_plan_kernel(PlanArgs a) {
     __syncthreads();
 
     const int nseg = total[1] + n_own;
-    // a segment without its share of the work; *of: its row or its group's leader
-    auto segment = [&](int i, int* of) __attribute__((always_inline)) {
-        PbSeg s;
-        s.common = i < total[1];
-        const int row = pb_find(s.common ? pbase : sbase, a.R, i);
-        const int x0 = s.common ? (i - pbase[row]) * kPbQ : (i - sbase[row]) * own_q;
+    // a segment as one item; *of: its row or its group's leader, *tiles_of: its tiles
+    auto segment = [&](int i, int* of, int* tiles_of) __attribute__((always_inline)) {
+        PbItem s{};
+        const bool common = i < total[1];
+        const int row = pb_find(common ? pbase : sbase, a.R, i);
+        const int x0 = common ? (i - pbase[row]) * kPbQ : (i - sbase[row]) * own_q;
         *of = row;
         s.row = row;
         s.x0 = x0;
-        if (s.common) {
+        if (common) {
             s.nq = min(kPbQ, gtoks[row] * a.G - x0);
-            s.base = gbase[row];
+            s.kind = gend[row] - first[row] == gtoks[row] ? kPbRun : kPbList;
+            s.base = s.kind == kPbRun ? first[row] : gbase[row];
             s.key0 = 0;
             s.key1 = gpages[row] << a.log_ps;
             s.lens = s.key1;
         } else {
+            s.kind = kPbOwn;
             s.nq = (int)min((int64_t)own_q, (int64_t)m_of[row] * a.G - x0);
             s.base = first[row];
             s.lens = a.lens[row];
@@ -366,19 +368,23 @@ paged_plan_kernel(PlanArgs a) {
             s.key0 = l >= 0 ? gpages[l] << a.log_ps : 0;
             s.key1 = s.lens + (x0 + s.nq - 1) / a.G + 1;
         }
-        s.tiles = (s.key1 - s.key0 + kPbTile - 1) / kPbTile;
+        *tiles_of = (s.key1 - s.key0 + kPbTile - 1) / kPbTile;
         return s;
     };
     auto chunks = [&](int n, int chunk) { return (n + chunk - 1) / chunk; };
     // (up to 2^24 segments of 2^18 tiles: the sum's upper and lower 20 bits apart)
     int64_t mine = 0, sixteens = 0;                  // tiles; tiles times blocks of 16 queries
-    int of = 0;
-    PbSeg s{};                                       // the thread's first segment, often its only one
+    int of = 0, s_tiles = 0;
+    PbItem s{};                                      // the thread's first segment, often its only one
     for (int i = tid; i < nseg; i += 1024) {
-        const PbSeg g = segment(i, &of);
-        if (i == tid) s = g;
-        mine += g.tiles;
-        sixteens += (int64_t)g.tiles * ((g.nq + 15) / 16);
+        int n;
+        const PbItem g = segment(i, &of, &n);
+        if (i == tid) {
+            s = g;
+            s_tiles = n;
+        }
+        mine += n;
+        sixteens += (int64_t)n * ((g.nq + 15) / 16);
     }
     const int of0 = nseg <= 1024 ? of : 0;
     // the common segments' records come first: a group's begin behind those of the groups before it
@@ -403,33 +409,34 @@ paged_plan_kernel(PlanArgs a) {
         const int i = i0 + tid;
         const bool in = i < nseg;
         of = of0;
-        if (nseg > 1024 && in) s = segment(i, &of);
+        if (nseg > 1024 && in) s = segment(i, &of, &s_tiles);
         int want[4] = {0, 0, 0, 0}, at[4], sums[4];
-        bool rec = false, shares = false;
+        const int n = chunks(s_tiles, chunk);
+        const bool shares = s.kind == kPbOwn && s.key0 > 0, rec = n > 1 || s.kind != kPbOwn || shares;
         if (in) {
-            s.nchunk = chunks(s.tiles, chunk);
-            shares = !s.common && s.key0 > 0;
-            rec = s.nchunk > 1 || s.common || shares;
-            want[0] = rec ? s.nchunk * s.nq : 0;
-            want[1] = rec && !s.common;
-            want[2] = s.nchunk;
+            want[0] = rec ? n * s.nq : 0;
+            want[1] = rec && s.kind == kPbOwn;
+            want[2] = n;
             want[3] = want[1] ? (s.nq + 3) / 4 : 0;
         }
         pb_scan<4>(want, waves, at, sums);
         if (in) {
-            s.rec0 = rec ? rec0 + at[0] : -1;
-            reinterpret_cast<PbSeg*>(a.plan + a.at.segs)[i] = s;
+            const int own = rec0 + at[0];
             PbItem* items = reinterpret_cast<PbItem*>(a.plan + a.at.items) + item0 + at[2];
-            const int q = s.tiles / s.nchunk, more = s.tiles - q * s.nchunk;
-            for (int k = 0; k < s.nchunk; ++k)
-                items[k] = PbItem{i, k, k * q + min(k, more), (k + 1) * q + min(k + 1, more)};
+            const int q = s_tiles / n, more = s_tiles - q * n;
+            for (int k = 0; k < n; ++k) {
+                s.tile0 = k * q + min(k, more);
+                s.tile1 = (k + 1) * q + min(k + 1, more);
+                s.rec = rec ? own + k * s.nq : -1;
+                items[k] = s;
+            }
             if (want[1]) {
                 PbJoin t{};
                 t.base = s.base;
                 t.x0 = s.x0;
                 t.nq = s.nq;
-                t.own = s.rec0;
-                t.own_n = s.nchunk;
+                t.own = own;
+                t.own_n = n;
                 if (shares) {
                     const int l = lead_of[of];
                     t.common_n = chunks(((gpages[l] << a.log_ps) + kPbTile - 1) / kPbTile, chunk);
@@ -591,47 +598,40 @@ paged_append_kernel(BatchArgs<T> a) {
     if (tid == 0) a.odd[t] = odd;
 }
 
-// What a block works on: its item, or nothing (seg < 0)
+// What a block works on: an item of a kv head, or nothing.  Item blockIdx.x / KVH of kv head
+// blockIdx.x % KVH: blocks go to the XCDs in turn, so that 8 kv heads have an XCD's L2 each
+// for their keys, and fewer share them among several.
 struct PbWork {
-    PbSeg s;
-    PbItem it;
+    PbItem s;
     int kvh;
     bool any;
 };
 
-// Item blockIdx.x / KVH of kv head blockIdx.x % KVH: blocks go to the XCDs in turn, so that 8 kv
-// heads have an XCD's L2 each for their keys, and fewer share them among several.
 template <typename T>
 __device__ __forceinline__ PbWork pb_work(const BatchArgs<T>& a) {
     PbWork w;
     const int item = blockIdx.x / a.KVH;
-    auto uniform = [](auto v) {                      // the same in all lanes, which the compiler may not see
-        int* p = reinterpret_cast<int*>(&v);
-#pragma unroll
-        for (int i = 0; i < (int)(sizeof(v) / sizeof(int)); ++i) p[i] = __builtin_amdgcn_readfirstlane(p[i]);
-        return v;
-    };
     // (the item is loaded with the count that says whether it is one)
-    const PbItem it = reinterpret_cast<const PbItem*>(a.plan + a.at.items)[item];
+    w.s = reinterpret_cast<const PbItem*>(a.plan + a.at.items)[item];
     w.any = item < a.plan[1] && plan_fits(a);
-    if (!w.any) return w;
     w.kvh = blockIdx.x - item * a.KVH;
-    w.it = uniform(it);
-    w.s = uniform(reinterpret_cast<const PbSeg*>(a.plan + a.at.segs)[w.it.seg]);
+    int* p = reinterpret_cast<int*>(&w.s);           // the same in all lanes, which the compiler may not see
+#pragma unroll
+    for (int i = 0; i < 11; ++i) p[i] = __builtin_amdgcn_readfirstlane(p[i]);
     return w;
 }
 
 // Flat token of query x of a segment
 template <typename T>
-__device__ __forceinline__ int pb_token(const BatchArgs<T>& a, const PbSeg& s, int x) {
-    const int i = (s.x0 + x) / a.G;
-    return s.common ? a.plan[a.at.toks + s.base + i] : s.base + i;
+__device__ __forceinline__ int pb_token(const BatchArgs<T>& a, const PbItem& s, int x) {
+    const int i = s.base + (s.x0 + x) / a.G;
+    return s.kind == kPbList ? a.plan[a.at.toks + i] : i;
 }
 
 // Positions that query x sees: all of a common segment, up to itself of its own row's
 template <typename T>
-__device__ __forceinline__ int pb_sees(const BatchArgs<T>& a, const PbSeg& s, int x) {
-    return s.common ? s.key1 : s.lens + (s.x0 + x) / a.G + 1;
+__device__ __forceinline__ int pb_sees(const BatchArgs<T>& a, const PbItem& s, int x) {
+    return s.kind != kPbOwn ? s.key1 : s.lens + (s.x0 + x) / a.G + 1;
 }
 
 // Infinities and NaN.  A weight of zero does not silence them in a matrix product, so a
@@ -641,9 +641,9 @@ __device__ __forceinline__ int pb_sees(const BatchArgs<T>& a, const PbSeg& s, in
 // queries that do (pb_poison): an infinity of v is the sum's, one of k (whose score is NaN
 // or an infinity, and 0 times an infinity) is NaN.  Such tokens lie behind the first query's.
 template <typename T>
-__device__ __forceinline__ bool pb_odd(const BatchArgs<T>& a, const PbSeg& s) {
+__device__ __forceinline__ bool pb_odd(const BatchArgs<T>& a, const PbItem& s) {
     bool odd = false;
-    if (!s.common) {
+    if (s.kind == kPbOwn) {
         const int last = (s.x0 + s.nq - 1) / a.G;
         for (int i = s.x0 / a.G + 1 + threadIdx.x; i <= last; i += 256) odd |= a.odd[s.base + i] != 0;
     }
@@ -688,7 +688,7 @@ __device__ __forceinline__ gqa_u4 pb_finite(gqa_u4 w) {
 template <int HDP, bool KCTX, typename T, typename P>
 __device__ __forceinline__ void pb_finish(const BatchArgs<T>& a, const PbWork& w, int QW, int first, int apart, bool odd,
                                           const float2 (*ml)[16], P part) {
-    const PbSeg& s = w.s;
+    const PbItem& s = w.s;
     constexpr int quads = HDP / 4, per = KCTX ? 2 * quads : quads;
     const int KW = 4 / QW;
     for (int k = threadIdx.x; k < QW * 16 * per; k += 256) {
@@ -710,7 +710,7 @@ __device__ __forceinline__ void pb_finish(const BatchArgs<T>& a, const PbWork& w
         if (odd && !(HDP > a.HD && d >= a.HD))
             c += pb_poison((which ? a.kp : a.vp) + w.kvh * a.ps_head + d, a.odd + s.base, a.table + (int64_t)s.row * a.table_ld, a.ps_page,
                            a.ps_tok, s.lens, a.log_ps, a.n_pages, s.x0 / a.G + 1, (s.x0 + x) / a.G, which);
-        if (s.rec0 < 0) {
+        if (s.rec < 0) {
             if (HDP > a.HD && d >= a.HD) continue;
             const int h = w.kvh * a.G + (s.x0 + x) % a.G;
             T* out = (which ? a.k_out : a.c_out) + (int64_t)pb_token(a, s, x) * a.out_ld + (int64_t)h * a.HD + d;
@@ -718,7 +718,7 @@ __device__ __forceinline__ void pb_finish(const BatchArgs<T>& a, const PbWork& w
             const float o[4] = {c[0] * inv, c[1] * inv, c[2] * inv, c[3] * inv};
             store_e<T, 4>(out, o);
         } else {
-            const int64_t r = w.kvh * a.at.cap_recs + s.rec0 + w.it.chunk * s.nq + x;
+            const int64_t r = w.kvh * a.at.cap_recs + s.rec + x;
             *reinterpret_cast<pg_f32x4*>(a.rec + (r * 2 + which) * HDP + d) = c;
             if (e == 0) *reinterpret_cast<float2*>(a.rec + a.rec_ml + 2 * r) = make_float2(m, l);
         }
@@ -789,15 +789,15 @@ paged_items_kernel(BatchArgs<T> a) {
     using M = Mfma16<T>;
     const PbWork w = pb_work(a);
     if (!w.any) return;
-    const PbSeg& s = w.s;
+    const PbItem& s = w.s;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int lr = lane & 15, lq = lane >> 4;
     const PbLane<CPR> tl(lq, lr);
-    const int kend = min(s.key1, s.key0 + w.it.tile1 * R);
+    const int kend = min(s.key1, s.key0 + s.tile1 * R);
     const int32_t* trow = a.table + (int64_t)s.row * a.table_ld;
 
     // pages of this wave's quarter of the tiles jb .. jb + 63, one per lane
-    int jb = w.it.tile0, pgv;
+    int jb = s.tile0, pgv;
     auto pages = [&]() {
         const int64_t t = (int64_t)s.key0 + (int64_t)(jb + lane) * R + 16 * wave;
         pgv = trow[min(t, (int64_t)a.cap - 1) >> a.log_ps];
@@ -821,7 +821,7 @@ paged_items_kernel(BatchArgs<T> a) {
     // this wave's quarter of tile j, 2 GPW loads (past the item's end: zeros)
     auto load_tile = [&](auto s_, int j) {
         const int t = s.key0 + j * R + 16 * wave;
-        const int rows = j < w.it.tile1 ? min(16, kend - t) : 0;
+        const int rows = j < s.tile1 ? min(16, kend - t) : 0;
         int bytes = 0;
         int64_t off = 0;
         if (rows > 0) {
@@ -1005,8 +1005,8 @@ paged_items_kernel(BatchArgs<T> a) {
             wait_vmcnt<2 * GPW * (NS - 2)>();
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         };
-        load_tile(std::integral_constant<int, 0>{}, w.it.tile0);
-        if constexpr (NS == 3) load_tile(I1{}, w.it.tile0 + 1);
+        load_tile(std::integral_constant<int, 0>{}, s.tile0);
+        if constexpr (NS == 3) load_tile(I1{}, s.tile0 + 1);
         wait_vmcnt<2 * GPW * (NS - 2)>();
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
@@ -1014,14 +1014,14 @@ paged_items_kernel(BatchArgs<T> a) {
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk)
                 asm volatile("" : "+v"(qf[n][kk].x), "+v"(qf[n][kk].y), "+v"(qf[n][kk].z), "+v"(qf[n][kk].w));
-        for (int j = w.it.tile0;; j += NS) {         // (an item has a tile)
+        for (int j = s.tile0;; j += NS) {         // (an item has a tile)
             step(std::integral_constant<int, 0>{}, j);
-            if (j + 1 >= w.it.tile1) break;
+            if (j + 1 >= s.tile1) break;
             step(I1{}, j + 1);
-            if (j + 2 >= w.it.tile1) break;
+            if (j + 2 >= s.tile1) break;
             if constexpr (NS == 3) {
                 step(I2{}, j + 2);
-                if (j + 3 >= w.it.tile1) break;
+                if (j + 3 >= s.tile1) break;
             }
         }
         wait_vmcnt<0>();                             // no load into LDS outlives the loop
@@ -1055,7 +1055,7 @@ paged_items_kernel(BatchArgs<T> a) {
 // blocks; RT positions per step in one LDS buffer, the next ones in flight in registers.
 // The products' operands may take the dimensions in any order that both share: lane
 // group lq takes HD / 4 neighbouring ones of them, so that a lane's are 16-byte reads.
-template <typename T, int HD>
+template <typename T, int HD, bool KCTX>
 __global__ void __launch_bounds__(256)
 paged_items_f32_kernel(BatchArgs<T> a) {
     constexpr int HDP = HD < 16 ? 16 : HD;           // heads of 8 are filled up with zeros
@@ -1067,16 +1067,15 @@ paged_items_f32_kernel(BatchArgs<T> a) {
     __shared__ float2 ml[4][16];
     const PbWork w = pb_work(a);
     if (!w.any) return;
-    const PbSeg& s = w.s;
-    // 64 of the segment's queries: blocks of y = 1 take the others
-    const int xb = 64 * blockIdx.y, nq = min(s.nq - xb, 64);
+    const PbItem& s = w.s;
+    // 32 of the segment's queries: blocks of other y take the others
+    const int xb = 32 * blockIdx.y, nq = min(s.nq - xb, 32);
     if (nq <= 0) return;
-    const bool kctx = a.k_out != nullptr;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int lr = lane & 15, lq = lane >> 4;
     const int QW = nq <= 16 ? 1 : nq <= 32 ? 2 : 4, KW = 4 / QW;
     const int x0 = xb + 16 * (wave & (QW - 1)), kg = wave / QW;
-    const int k0 = s.key0 + w.it.tile0 * kPbTile, kend = min(s.key1, s.key0 + w.it.tile1 * kPbTile);
+    const int k0 = s.key0 + s.tile0 * kPbTile, kend = min(s.key1, s.key0 + s.tile1 * kPbTile);
     const int32_t* trow = a.table + (int64_t)s.row * a.table_ld;
     const int ps_mask = (1 << a.log_ps) - 1;
     float* const tk = lds;
@@ -1103,8 +1102,7 @@ paged_items_f32_kernel(BatchArgs<T> a) {
     }
     const int sees = min(pb_sees(a, s, xq), kend);
     const int sees_first = __builtin_amdgcn_readfirstlane(min(pb_sees(a, s, min(x0, s.nq - 1)), kend));
-    const int sees_last = __builtin_amdgcn_readfirstlane(min(pb_sees(a, s, min(x0 + 15, s.nq - 1)), kend));
-    const bool idle = x0 >= s.nq;
+    const int sees_last = x0 >= s.nq ? 0 : __builtin_amdgcn_readfirstlane(min(pb_sees(a, s, min(x0 + 15, s.nq - 1)), kend));
     u32x4 kr[NP], vr[NP];
     auto load = [&](int t0) {                        // positions t0 .. t0 + RT - 1
         if (t0 < kend && t0 - jb >= 16 * 64) {
@@ -1133,10 +1131,12 @@ paged_items_f32_kernel(BatchArgs<T> a) {
         }
     };
     const bool odd = __syncthreads_or(odd_mine);
-    float mh = -INFINITY, lh = 0.0f;
-    pg_f32x4 accC[DT], accK[DT];
+    float mh = -INFINITY, off = 0.0f, lh = 0.0f;
+    pg_f32x4 accC[DT], accK[KCTX ? DT : 1];
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) accC[dt] = accK[dt] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int dt = 0; dt < DT; ++dt) accC[dt] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int dt = 0; dt < (KCTX ? DT : 1); ++dt) accK[dt] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
     load(k0);
     for (int t0 = k0; t0 < kend; t0 += RT) {
         __syncthreads();                             // the tile's last reads
@@ -1150,63 +1150,75 @@ paged_items_f32_kernel(BatchArgs<T> a) {
         }
         load(t0 + RT);
         lds_barrier();
-        if (idle) continue;
         for (int hf = kg; hf < RT / 16; hf += KW) {
             const int r0 = t0 + 16 * hf;
-            if (r0 >= sees_last) break;              // (a wave's: uniform)
-            pg_f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+            if (r0 >= sees_last) break;              // (a wave's: uniform; at once where it has no query)
+            // four sums side by side: a product waits for the one before it in its sum
+            pg_f32x4 part[4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
             const float* kq = tk + (16 * hf + lr) * PITCH + lq * (HDP / 4);
 #pragma unroll
             for (int i = 0; i < Q4; ++i) {
                 const pg_f32x4 kx = *reinterpret_cast<const pg_f32x4*>(kq + 4 * i);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sc = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[e], qf[4 * i + e], sc, 0, 0, 0);
+                for (int e = 0; e < 4; ++e) part[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(kx[e], qf[4 * i + e], part[e], 0, 0, 0);
             }
+            pg_f32x4 sc = (part[0] + part[1]) + (part[2] + part[3]);
             const bool mask = r0 + 16 > sees_first;
-            float mx = -INFINITY, pv[4], ls = 0.0f;
+            float mx = -INFINITY, pv[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 if (mask && r0 + 4 * lq + r >= sees) sc[r] = -INFINITY;
                 mx = fmaxf(mx, sc[r]);
             }
-            mx = max_16_32(mx) * a.qscale;
-            const float mnew = raised(mh, mx);
-            const float corr = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mh - mnew);
-            const float off = mnew == -INFINITY ? 0.0f : -mnew;
+            mx *= a.qscale;
+            if (__any(mx > mh + kPgLag)) {
+                const float mnew = raised(mh, max_16_32(mx));
+                const float corr = mnew == mh ? 1.0f : __builtin_amdgcn_exp2f(mh - mnew);
+                const bool first = mh == -INFINITY;              // the sums are zero
+                mh = mnew;
+                off = mnew == -INFINITY ? 0.0f : -mnew;
+                lh *= corr;
+                pg_f32x4 cf;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) cf[r] = __shfl(first ? 1.0f : corr, 4 * lq + r, 64);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    accC[dt] *= cf;
+                    if constexpr (KCTX) accK[dt] *= cf;
+                }
+            }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 pv[r] = __builtin_amdgcn_exp2f(fmaf(sc[r], a.qscale, off));
-                ls += pv[r];
+                lh += pv[r];
             }
-            lh = fmaf(lh, corr, sum_16_32(ls));
-            const bool rescale = corr != 1.0f && mh != -INFINITY;
-            mh = mnew;
-            if (__any(rescale)) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float cf = __shfl(corr, 4 * lq + r, 64);
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        accC[dt][r] *= cf;
-                        accK[dt][r] *= cf;
-                    }
-                }
-            }
-            // (rows that not all columns see: see pb_odd)
-            const int partly = odd ? sees_first - r0 - 4 * lq : 4;
-            auto finite = [&](float v, int r) __attribute__((always_inline)) { return r >= partly && !(fabsf(v) < INFINITY) ? 0.0f : v; };
+            const bool dirty = odd && mask;          // rows that not all columns see (pb_odd)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float* vq = tv + (16 * hf + 4 * lq + r) * PITCH + lr;
-                const float* kx = tk + (16 * hf + 4 * lq + r) * PITCH + lr;
+                const int row = 16 * hf + 4 * lq + r;
+                float v[DT], k[DT];
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
-                    accC[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[r], finite(vq[16 * dt], r), accC[dt], 0, 0, 0);
-                    if (kctx) accK[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[r], finite(kx[16 * dt], r), accK[dt], 0, 0, 0);
+                    v[dt] = tv[row * PITCH + lr + 16 * dt];
+                    if constexpr (KCTX) k[dt] = tk[row * PITCH + lr + 16 * dt];
+                }
+                if (dirty) {
+                    const bool partly = t0 + row >= sees_first;
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        if (partly && !(fabsf(v[dt]) < INFINITY)) v[dt] = 0.0f;
+                        if (KCTX && partly && !(fabsf(k[dt]) < INFINITY)) k[dt] = 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) {
+                    accC[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[r], v[dt], accC[dt], 0, 0, 0);
+                    if constexpr (KCTX) accK[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[r], k[dt], accK[dt], 0, 0, 0);
                 }
             }
         }
     }
+    lh = sum_16_32(lh);
     __syncthreads();
     auto part = [&](int i) { return lds + i * 16 * 2 * HDP; };
     if (lq == 0) ml[wave][lr] = make_float2(mh, lh);
@@ -1214,11 +1226,10 @@ paged_items_f32_kernel(BatchArgs<T> a) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
         mine[64 * dt] = accC[dt];
-        mine[64 * (DT + dt)] = accK[dt];
+        if constexpr (KCTX) mine[64 * (DT + dt)] = accK[dt];
     }
     __syncthreads();
-    if (kctx) pb_finish<HDP, true>(a, w, QW, xb, 16, odd, ml, part);
-    else pb_finish<HDP, false>(a, w, QW, xb, 16, odd, ml, part);
+    pb_finish<HDP, KCTX>(a, w, QW, xb, 16, odd, ml, part);
 }
 
 // ------------------------------------------------------------------ the join
@@ -1453,7 +1464,9 @@ static int batch_launch(const BatchCall& c, hipStream_t st) {
 #undef LOOM_PB_M
 #define LOOM_PB_F(HDV)                                                                              \
         if (c.HD == HDV) {                                                                          \
-            hipLaunchKernelGGL((paged_items_f32_kernel<T, HDV>), dim3(grid.x, kPbQ / 64), dim3(256), 0, st, a);        \
+            const dim3 halves(grid.x, kPbQ / 32);                                                   \
+            if (c.k_out) hipLaunchKernelGGL((paged_items_f32_kernel<T, HDV, true>), halves, dim3(256), 0, st, a); \
+            else hipLaunchKernelGGL((paged_items_f32_kernel<T, HDV, false>), halves, dim3(256), 0, st, a); \
             done = true;                                                                            \
         }
         LOOM_PB_F(8) LOOM_PB_F(16) LOOM_PB_F(256)
