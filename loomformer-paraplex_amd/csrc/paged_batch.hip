@@ -28,6 +28,7 @@ constexpr int kPbQ = 128;           // queries (a token's heads of one kv head) 
 constexpr int kPbTile = 64;         // positions of a step of a block
 constexpr int kPbLeast = 1;         // an item has so many tiles at least
 constexpr float kPbRecord = 2.5e-4f;  // a query's record, in a block's time for a tile of its queries
+constexpr int kPbFew = 8;           // records of a query that a wave of the join takes alone
 constexpr int kPbAlone = 64;        // rows with more queries fill a block by themselves and share nothing
 constexpr int kPbShare = 64;        // common positions from which reading them once pays
 constexpr int kPbMagic = 0x4c50424c;
@@ -67,8 +68,7 @@ struct PbLayout {
     int64_t cap_recs;               // records of a kv head
     int slots;                      // blocks per kv head that the device holds at once
 };
-// header: 0 magic, 1 items, 2 tasks of the join (join * kPbParts + which four queries), 3.. the sizes it was made for
-constexpr int kPbParts = kPbQ / 4;
+// header: 0 magic, 1 items, 2 tasks of the join (join * kPbQ + its first query), 3.. the sizes it was made for
 constexpr int kPbHeader = 16;
 
 // What a plan can need at most.  Own segments: a row's last may be partly filled;
@@ -83,7 +83,7 @@ static PbLayout pb_layout(int64_t R, int64_t N, int64_t QH, int64_t KVH) {
     p.cap_items = (int)(R + NG / 64 + R / 2 + some / kPbQ + 2) + p.slots;
     const int64_t split = kPbQ < NG ? kPbQ : NG;          // queries of a split segment
     p.cap_joins = (int)(p.slots + R + 1);
-    p.cap_tasks = (int)(p.slots * ((split + 3) / 4) + some / 4 + R + 1);
+    p.cap_tasks = (int)(p.slots * split + some + R + 1);
     p.cap_toks = (int)some + 1;
     p.cap_recs = 2 * p.slots * split + 2 * some;
     p.rows = kPbHeader;
@@ -207,24 +207,32 @@ paged_rows_kernel(PlanArgs a) {
 
 // ------------------------------------------------------------------ plan
 
-// Exclusive scan of N counts over the 1024 threads of a block; total: their sums.
-template <int N>
+// Exclusive scan of N counts over the NT threads of a block; total: their sums.
+template <int NT, int N>
 __device__ __forceinline__ void pb_scan(const int (&v)[N], int* waves, int (&before)[N], int (&total)[N]) {
+    constexpr int NW = NT / 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int incl[N];
     __syncthreads();                                 // the previous use of `waves` is over
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         incl[k] = wave_scan_int(v[k]);
-        if (lane == 63) waves[wave * N + k] = incl[k];
+        if constexpr (NW == 1) {
+            total[k] = __builtin_amdgcn_readlane(incl[k], 63);
+            before[k] = incl[k] - v[k];
+        } else if (lane == 63) {
+            waves[wave * N + k] = incl[k];
+        }
     }
-    __syncthreads();
+    if constexpr (NW > 1) {
+        __syncthreads();
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-        const int mine = lane < 16 ? waves[lane * N + k] : 0;
-        const int upto = wave_scan_int(mine);
-        total[k] = __builtin_amdgcn_readlane(upto, 15);
-        before[k] = __builtin_amdgcn_readlane(upto - mine, __builtin_amdgcn_readfirstlane(wave)) + incl[k] - v[k];
+        for (int k = 0; k < N; ++k) {
+            const int mine = lane < NW ? waves[lane * N + k] : 0;
+            const int upto = wave_scan_int(mine);
+            total[k] = __builtin_amdgcn_readlane(upto, NW - 1);
+            before[k] = __builtin_amdgcn_readlane(upto - mine, __builtin_amdgcn_readfirstlane(wave)) + incl[k] - v[k];
+        }
     }
 }
 
@@ -238,47 +246,91 @@ __device__ __forceinline__ int pb_find(const int* values, int n, int x) {
     return lo;
 }
 
-// Block 0: groups, segments, items, joins.  The others, 1024 flat tokens each: the
+// The rows' states as paged_rows_kernel finds them, by a block of NT threads at once: a
+// thread per row for the leaders, per table entry for the pages.
+template <int NT>
+__device__ __forceinline__ int4 pb_states(const PlanArgs& a, int m) {
+    __shared__ __align__(16) int page_of[NT], need_of[NT], whole_of[NT], same_of[NT], lacks[NT];
+    const int r = threadIdx.x, PS = 1 << a.log_ps;
+    int n = -1, page = -1 - r;                       // (no two rows that are no candidates have the same)
+    if (r < a.R) {
+        n = a.lens[r];
+        const int first = a.table[(int64_t)r * a.table_ld];
+        if (pb_candidate(a, m, n, first)) page = first;
+    }
+    const bool fits = n >= 0 && n <= a.cap && m <= a.cap - n;
+    page_of[r] = page;
+    need_of[r] = m > 0 && fits ? (n + m + PS - 1) >> a.log_ps : 0;
+    whole_of[r] = same_of[r] = page >= 0 ? n >> a.log_ps : 0;
+    lacks[r] = 0;
+    __syncthreads();
+    int lead = page >= 0 ? r : -1;
+    if (page >= 0) {
+#pragma unroll 4
+        for (int i = 0; i < r; i += 4) {
+            const int4 q = *reinterpret_cast<const int4*>(page_of + i);
+            if (q.w == page && i + 3 < lead) lead = i + 3;
+            if (q.z == page && i + 2 < lead) lead = i + 2;
+            if (q.y == page && i + 1 < lead) lead = i + 1;
+            if (q.x == page && i < lead) lead = i;
+        }
+    }
+    __syncthreads();
+    page_of[r] = lead;
+    __syncthreads();
+    const int MP = a.cap >> a.log_ps, entries = a.R * MP;
+    const float per = 1.0f / (float)MP;              // (entries are few: the quotient is off by one at most)
+    for (int i0 = r; i0 < entries; i0 += 4 * NT) {
+        int v[4], w[4], row[4], col[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = min(i0 + u * NT, entries - 1);
+            row[u] = (int)((float)i * per);
+            col[u] = i - row[u] * MP;
+            if (col[u] < 0) --row[u], col[u] += MP;
+            if (col[u] >= MP) ++row[u], col[u] -= MP;
+            const int l = page_of[row[u]];
+            v[u] = col[u] < need_of[row[u]] ? a.table[(int64_t)row[u] * a.table_ld + col[u]] : 0;
+            w[u] = col[u] < whole_of[row[u]] && l != row[u] ? a.table[(int64_t)max(l, 0) * a.table_ld + col[u]] : v[u];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if ((unsigned)v[u] >= (unsigned)a.n_pages) lacks[row[u]] = 1;
+            if (v[u] != w[u]) atomicMin(&same_of[row[u]], col[u]);
+        }
+    }
+    __syncthreads();
+    return make_int4(lead, same_of[r], fits && lacks[r] == 0, 0);
+}
+
+// Block 0: groups, segments, items, joins.  The others, NT flat tokens each: the
 // tokens' rows, positions and slots.  Both begin with a scan over the rows' counts.
 // Block 0 is one block because each stage needs the whole of the one before; it is
 // bound by their latency, a pass over the rows or the segments with a block scan each.
-// ALONE: of few rows every block finds the states itself, and the launch before is saved.
-constexpr int kPbFewRows = 32;
-
-template <bool ALONE>
-__global__ void __launch_bounds__(1024)
+// ALONE: of few table entries every block finds the states itself, and the launch before is
+// saved.  NT: at least as many threads as rows; a barrier of fewer waves is a shorter one.
+template <int NT, bool ALONE>
+__global__ void __launch_bounds__(NT)
 paged_plan_kernel(PlanArgs a) {
-    __shared__ __align__(16) int first[kPbMaxRows], m_of[kPbMaxRows], lead_of[kPbMaxRows];
-    __shared__ int gpages[kPbMaxRows], gtoks[kPbMaxRows], gbase[kPbMaxRows], pbase[kPbMaxRows], sbase[kPbMaxRows];
-    __shared__ int rowx[kPbMaxRows], grec[kPbMaxRows], gend[kPbMaxRows];
-    __shared__ int waves[16 * 4];
+    __shared__ __align__(16) int first[NT], m_of[NT], lead_of[NT];
+    __shared__ int gpages[NT], gtoks[NT], gbase[NT], pbase[NT], sbase[NT];
+    __shared__ int rowx[NT], grec[NT], gend[NT];
+    __shared__ int waves[NT / 64 * 4];
     const int tid = threadIdx.x, r = tid, PS = 1 << a.log_ps;
     int m = 0;
     int4 info = make_int4(-1, 0, 0, 0);
-    if constexpr (ALONE) {
-        __shared__ PbHash hash;
-        __shared__ int4 state[kPbFewRows];
-        if (r < a.R) m = pb_fresh(a, r);
-        pb_hash(a, hash);
-        for (int i = __builtin_amdgcn_readfirstlane(tid >> 6); i < a.R; i += 16) {
-            const int4 s = pb_row(a, hash, i);
-            if ((tid & 63) == 0) state[i] = s;
-        }
-        __syncthreads();
-        if (r < a.R) info = state[r];
-    } else if (r < a.R) {
-        m = pb_fresh(a, r);
-        info = *reinterpret_cast<const int4*>(a.plan + a.at.rows + 4 * r);
-    }
+    if (r < a.R) m = pb_fresh(a, r);
+    if constexpr (ALONE) info = pb_states<NT>(a, m);
+    else if (r < a.R) info = *reinterpret_cast<const int4*>(a.plan + a.at.rows + 4 * r);
     int m1[1] = {m}, start1[1], all1[1];
-    pb_scan<1>(m1, waves, start1, all1);
+    pb_scan<NT, 1>(m1, waves, start1, all1);
     const int start = start1[0];
     const bool ok = m > 0 && info.z != 0 && start + m <= a.N;
     first[r] = r < a.R ? start : 0x7fffffff;
     m_of[r] = ok ? m : 0;
     if (blockIdx.x > 0) {
         __syncthreads();
-        const int t = (blockIdx.x - 1) * 1024 + tid;
+        const int t = (blockIdx.x - 1) * NT + tid;
         if (t >= a.N) return;
         int row = -1, pos = -1;
         int64_t slot = -1;
@@ -319,7 +371,7 @@ paged_plan_kernel(PlanArgs a) {
     __syncthreads();
     if (!pays) gpages[r] = 0;
     int four[4] = {pays ? gtoks[r] : 0, npre, (int)((queries + kPbQ - 1) / kPbQ), (int)((queries + 63) / 64)}, before[4], total[4];
-    pb_scan<4>(four, waves, before, total);
+    pb_scan<NT, 4>(four, waves, before, total);
     // own segments of 64 queries where those fill the device whole and ones of 128 would have to be split
     const bool small = total[2] < a.at.slots && total[3] >= a.at.slots;
     const int own_q = small ? 64 : kPbQ, n_own = small ? total[3] : total[2];
@@ -376,7 +428,7 @@ paged_plan_kernel(PlanArgs a) {
     int64_t mine = 0, sixteens = 0;                  // tiles; tiles times blocks of 16 queries
     int of = 0, s_tiles = 0;
     PbItem s{};                                      // the thread's first segment, often its only one
-    for (int i = tid; i < nseg; i += 1024) {
+    for (int i = tid; i < nseg; i += NT) {
         int n;
         const PbItem g = segment(i, &of, &n);
         if (i == tid) {
@@ -386,10 +438,10 @@ paged_plan_kernel(PlanArgs a) {
         mine += n;
         sixteens += (int64_t)n * ((g.nq + 15) / 16);
     }
-    const int of0 = nseg <= 1024 ? of : 0;
+    const int of0 = nseg <= NT ? of : 0;
     // the common segments' records come first: a group's begin behind those of the groups before it
     int sum[4] = {(int)(mine >> 20), (int)(mine & 0xfffff), (int)(sixteens >> 20), (int)(sixteens & 0xfffff)}, none[4], tiles[4];
-    pb_scan<4>(sum, waves, none, tiles);
+    pb_scan<NT, 4>(sum, waves, none, tiles);
     const int64_t all_tiles = ((int64_t)tiles[0] << 20) + tiles[1];
     // An item has at least the tiles that fill the device.  It leaves a record per query, which
     // is written and read at the copy's rate by all blocks together, while a tile is
@@ -400,36 +452,29 @@ paged_plan_kernel(PlanArgs a) {
     if (total[1] > 0) {
         const int positions = gpages[r] << a.log_ps;
         int recs[1] = {pays ? gtoks[r] * a.G * chunks((positions + kPbTile - 1) / kPbTile, chunk) : 0}, at1[1], all_r[1];
-        pb_scan<1>(recs, waves, at1, all_r);
+        pb_scan<NT, 1>(recs, waves, at1, all_r);
         grec[r] = at1[0];
         __syncthreads();
     }
     int item0 = 0, rec0 = 0, join0 = 0, task0 = 0;
-    for (int i0 = 0; i0 < nseg; i0 += 1024) {
+    for (int i0 = 0; i0 < nseg; i0 += NT) {
         const int i = i0 + tid;
         const bool in = i < nseg;
         of = of0;
-        if (nseg > 1024 && in) s = segment(i, &of, &s_tiles);
+        if (nseg > NT && in) s = segment(i, &of, &s_tiles);
         int want[4] = {0, 0, 0, 0}, at[4], sums[4];
         const int n = chunks(s_tiles, chunk);
         const bool shares = s.kind == kPbOwn && s.key0 > 0, rec = n > 1 || s.kind != kPbOwn || shares;
+        const int common_n = shares ? chunks((s.key0 + kPbTile - 1) / kPbTile, chunk) : 0;
         if (in) {
             want[0] = rec ? n * s.nq : 0;
             want[1] = rec && s.kind == kPbOwn;
             want[2] = n;
-            want[3] = want[1] ? (s.nq + 3) / 4 : 0;
+            want[3] = !want[1] ? 0 : n + common_n <= kPbFew ? (s.nq + 3) / 4 : s.nq;
         }
-        pb_scan<4>(want, waves, at, sums);
+        pb_scan<NT, 4>(want, waves, at, sums);
         if (in) {
             const int own = rec0 + at[0];
-            PbItem* items = reinterpret_cast<PbItem*>(a.plan + a.at.items) + item0 + at[2];
-            const int q = s_tiles / n, more = s_tiles - q * n;
-            for (int k = 0; k < n; ++k) {
-                s.tile0 = k * q + min(k, more);
-                s.tile1 = (k + 1) * q + min(k + 1, more);
-                s.rec = rec ? own + k * s.nq : -1;
-                items[k] = s;
-            }
             if (want[1]) {
                 PbJoin t{};
                 t.base = s.base;
@@ -439,15 +484,53 @@ paged_plan_kernel(PlanArgs a) {
                 t.own_n = n;
                 if (shares) {
                     const int l = lead_of[of];
-                    t.common_n = chunks(((gpages[l] << a.log_ps) + kPbTile - 1) / kPbTile, chunk);
+                    t.common_n = common_n;
                     t.common0 = grec[l];
                     t.g0 = rowx[of] * a.G + s.x0;
                     t.group_q = gtoks[l] * a.G;
                 }
                 reinterpret_cast<PbJoin*>(a.plan + a.at.joins)[join0 + at[1]] = t;
-                int32_t* tasks = a.plan + a.at.tasks + task0 + at[3];
-                for (int k = 0; k < want[3]; ++k) tasks[k] = (join0 + at[1]) * kPbParts + k;
             }
+        }
+        // the items of a segment and the tasks of a join: by its thread, and by the wave where few
+        // of its threads have many (1 row of 16384: 10.1 -> 6.7 us)
+        auto put = [&](PbItem g, int k, int n, int own, int at_item) __attribute__((always_inline)) {
+            const int q = g.tile1 / n, more = g.tile1 - q * n;       // (tile1: all its tiles)
+            g.tile0 = k * q + min(k, more);
+            g.tile1 = (k + 1) * q + min(k + 1, more);
+            if (own >= 0) g.rec = own + k * g.nq;
+            reinterpret_cast<PbItem*>(a.plan + a.at.items)[at_item + k] = g;
+        };
+        s.tile1 = s_tiles;
+        s.rec = -1;
+        const int own = rec ? rec0 + at[0] : -1, item = item0 + at[2], task = task0 + at[3];
+        const int code = (join0 + at[1]) * kPbQ, step = n + common_n <= kPbFew ? 4 : 1, tasks = want[3];
+        constexpr int kMany = 8, kFewOf = 4;
+        const int lane = tid & 63;
+        unsigned long long big = __ballot(in && n > kMany);
+        if (__popcll(big) > kFewOf) big = 0;
+        if (in && !(big >> lane & 1))
+            for (int k = 0; k < n; ++k) put(s, k, n, own, item);
+        while (big) {
+            const int src = __builtin_amdgcn_readfirstlane(__ffsll(big) - 1);
+            big &= big - 1;
+            PbItem g = s;
+            int* p = reinterpret_cast<int*>(&g);
+#pragma unroll
+            for (int i = 0; i < 11; ++i) p[i] = __builtin_amdgcn_readlane(p[i], src);
+            const int gn = __builtin_amdgcn_readlane(n, src), go = __builtin_amdgcn_readlane(own, src), gi = __builtin_amdgcn_readlane(item, src);
+            for (int k = lane; k < gn; k += 64) put(g, k, gn, go, gi);
+        }
+        big = __ballot(tasks > kMany);
+        if (__popcll(big) > kFewOf) big = 0;
+        if (!(big >> lane & 1))
+            for (int k = 0; k < tasks; ++k) a.plan[a.at.tasks + task + k] = code + step * k;
+        while (big) {
+            const int src = __builtin_amdgcn_readfirstlane(__ffsll(big) - 1);
+            big &= big - 1;
+            const int gn = __builtin_amdgcn_readlane(tasks, src), gt = __builtin_amdgcn_readlane(task, src);
+            const int gc = __builtin_amdgcn_readlane(code, src), gs = __builtin_amdgcn_readlane(step, src);
+            for (int k = lane; k < gn; k += 64) a.plan[a.at.tasks + gt + k] = gc + gs * k;
         }
         rec0 += sums[0];
         join0 += sums[1];
@@ -1068,8 +1151,9 @@ paged_items_f32_kernel(BatchArgs<T> a) {
     const PbWork w = pb_work(a);
     if (!w.any) return;
     const PbItem& s = w.s;
-    // 32 of the segment's queries: blocks of other y take the others
-    const int xb = 32 * blockIdx.y, nq = min(s.nq - xb, 32);
+    // 64 of the segment's queries, 32 where that leaves blocks too few: blocks of other y take
+    // the others (4 x 1024 new tokens 324 / 362 us, 3 of 1 to 257 25.8 / 19.0)
+    const int per = a.plan[1] >= a.at.slots ? 64 : 32, xb = per * blockIdx.y, nq = min(s.nq - xb, per);
     if (nq <= 0) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int lr = lane & 15, lq = lane >> 4;
@@ -1233,12 +1317,11 @@ paged_items_f32_kernel(BatchArgs<T> a) {
 }
 
 // ------------------------------------------------------------------ the join
-// Four queries of an own segment per task: their records are the chunks of the segment
-// itself and of the group's segments that hold them.  Where a query has few, a
-// wave does one, all its records in flight; else wave w takes records w, w + 4, .. of all
-// four, kPbJoin of each in flight, and the waves meet in LDS.  Bound by the records' bytes.
-constexpr int kPbJoin = 2;
-constexpr int kPbFew = 8;
+// The queries whose sums are in records, those of their own segment's chunks and of the
+// group's segment that holds them.  Of few records (kPbFew) a block's four waves take a
+// query each, all its records in flight; of more it takes one query: wave w records w,
+// w + 4, .., kPbJoin of them in flight, and the waves meet in LDS.  Bound by the records' bytes.
+constexpr int kPbJoin = 8;
 
 // (m, l, v) and a record's (e, y) as one
 template <int NV>
@@ -1257,8 +1340,8 @@ __global__ void __launch_bounds__(256)
 paged_batch_join_kernel(BatchArgs<T> a) {
     constexpr int HDP = HD < 16 ? 16 : HD;
     constexpr int NV = HDP > 128 ? 2 : 1, NL = HDP / 2 / NV;   // lanes of four sums
-    __shared__ float2 ml[4][4];
-    __shared__ __align__(16) float sums[4][4][2 * HDP];
+    __shared__ float2 ml[4];
+    __shared__ __align__(16) float sums[4][2 * HDP];
     const int kvh = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int at = min(lane, NL - 1);
     const bool kctx = a.k_out != nullptr;
@@ -1270,8 +1353,8 @@ paged_batch_join_kernel(BatchArgs<T> a) {
     const float* rml = a.rec + a.rec_ml + kvh * a.at.cap_recs * 2;
     for (int task = blockIdx.x; task < n_tasks; task += gridDim.x) {
         if (task != (int)blockIdx.x) next = a.plan[a.at.tasks + task];
-        const PbJoin t = joins[next / kPbParts];
-        const int y = 4 * (next % kPbParts), nx = min(4, t.nq - y);
+        const PbJoin t = joins[next / kPbQ];
+        const int y = next % kPbQ, nx = min(4, t.nq - y);
         const int base = t.base, x0 = t.x0 + y, own = t.own + y, own_step = t.nq, nc = t.common_n, n = nc + t.own_n;
         // the group's segments: 128 queries each but the last, all of the same chunks; query
         // `cut` of the four is the first of the next one
@@ -1314,56 +1397,47 @@ paged_batch_join_kernel(BatchArgs<T> a) {
             }
             continue;
         }
-        float m[4], l[4];
-        pg_f32x4 sum[4][NV];
+        float m = -INFINITY, l = 0.0f;
+        pg_f32x4 sum[NV];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            m[i] = -INFINITY;
-            l[i] = 0.0f;
-#pragma unroll
-            for (int v = 0; v < NV; ++v) sum[i][v] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int v = 0; v < NV; ++v) sum[v] = pg_f32x4{0.f, 0.f, 0.f, 0.f};
         for (int c0 = wave; c0 < n; c0 += 4 * kPbJoin) {
-            float2 e[4 * kPbJoin];
-            pg_f32x4 y[4 * kPbJoin][NV];
+            float2 e[kPbJoin];
+            pg_f32x4 z[kPbJoin][NV];
 #pragma unroll
-            for (int k = 0; k < 4 * kPbJoin; ++k) {                  // query k / kPbJoin, the wave's next record k % kPbJoin
-                const int64_t r = place(min(k / kPbJoin, nx - 1), min(c0 + 4 * (k % kPbJoin), n - 1));
+            for (int k = 0; k < kPbJoin; ++k) {
+                const int64_t r = place(0, min(c0 + 4 * k, n - 1));
                 e[k] = *reinterpret_cast<const float2*>(rml + 2 * r);
 #pragma unroll
-                for (int v = 0; v < NV; ++v)
-                    y[k][v] = *reinterpret_cast<const pg_f32x4*>(rec + r * 2 * HDP + 4 * (at + NL * v));
+                for (int v = 0; v < NV; ++v) z[k][v] = *reinterpret_cast<const pg_f32x4*>(rec + r * 2 * HDP + 4 * (at + NL * v));
             }
 #pragma unroll
-            for (int k = 0; k < 4 * kPbJoin; ++k)
-                if (c0 + 4 * (k % kPbJoin) < n) pb_add<NV>(m[k / kPbJoin], l[k / kPbJoin], sum[k / kPbJoin], e[k], y[k]);
+            for (int k = 0; k < kPbJoin; ++k)
+                if (c0 + 4 * k < n) pb_add<NV>(m, l, sum, e[k], z[k]);
         }
         __syncthreads();                             // the last task's sums are read
+        if (lane == 0) ml[wave] = make_float2(m, l);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (lane == 0) ml[i][wave] = make_float2(m[i], l[i]);
-#pragma unroll
-            for (int v = 0; v < NV; ++v)
-                if (lane < NL) *reinterpret_cast<pg_f32x4*>(&sums[i][wave][4 * (lane + NL * v)]) = sum[i][v];
-        }
+        for (int v = 0; v < NV; ++v)
+            if (lane < NL) *reinterpret_cast<pg_f32x4*>(&sums[wave][4 * (lane + NL * v)]) = sum[v];
         __syncthreads();
-        for (int k = threadIdx.x; k < nx * (HDP / 4) * 2; k += 256) {
-            const int i = k / (HDP / 2), d2 = 4 * (k - i * (HDP / 2));
-            float m = -INFINITY, l = 0.0f;
+        for (int k = threadIdx.x; k < HDP / 2; k += 256) {
+            const int d2 = 4 * k;
+            float most = -INFINITY, all = 0.0f;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) m = fmaxf(m, ml[i][v].x);
+            for (int v = 0; v < 4; ++v) most = fmaxf(most, ml[v].x);
             float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-                const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml[i][v].x - m);
-                l = fmaf(ml[i][v].y, f, l);
+                const float f = most == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml[v].x - most);
+                all = fmaf(ml[v].y, f, all);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) o[q] = fmaf(sums[i][v][d2 + q], f, o[q]);
+                for (int q = 0; q < 4; ++q) o[q] = fmaf(sums[v][d2 + q], f, o[q]);
             }
-            const float inv = 1.0f / l;
+            const float inv = 1.0f / all;
 #pragma unroll
             for (int q = 0; q < 4; ++q) o[q] *= inv;
-            out(i, d2, o);
+            out(0, d2, o);
         }
     }
 }
@@ -1528,13 +1602,17 @@ extern "C" int loom_paged_plan(const int32_t* table, int64_t table_ld, int64_t m
     a.cap = (int)(max_pages * page_size);
     a.n_pages = (int)n_pages;
     hipStream_t st = (hipStream_t)stream;
-    const dim3 blocks((unsigned)(1 + ceil_div(n_tokens, 1024)));
-    if (rows <= kPbFewRows) {
-        hipLaunchKernelGGL((paged_plan_kernel<true>), blocks, dim3(1024), 0, st, a);
+    // (about as many segments as threads: see pb_layout)
+    const int64_t entries = rows * max_pages, segs = n_tokens * a.G / kPbQ;
+    auto blocks = [&](int64_t nt) { return dim3((unsigned)(1 + ceil_div(n_tokens, nt))); };
+    if (rows <= 64 && entries <= 1024 && segs <= 64) {
+        hipLaunchKernelGGL((paged_plan_kernel<64, true>), blocks(64), dim3(64), 0, st, a);
+    } else if (rows <= 256 && entries <= 8192 && segs <= 256) {
+        hipLaunchKernelGGL((paged_plan_kernel<256, true>), blocks(256), dim3(256), 0, st, a);
     } else {
-        hipLaunchKernelGGL(paged_rows_kernel, dim3((unsigned)ceil_div(rows, 16)), dim3(1024), 0, st, a);
+        if (rows > 0) hipLaunchKernelGGL(paged_rows_kernel, dim3((unsigned)ceil_div(rows, 16)), dim3(1024), 0, st, a);
         if (int rc = launch_status("loom_paged_plan(rows)")) return rc;
-        hipLaunchKernelGGL((paged_plan_kernel<false>), blocks, dim3(1024), 0, st, a);
+        hipLaunchKernelGGL((paged_plan_kernel<1024, false>), blocks(1024), dim3(1024), 0, st, a);
     }
     return launch_status("loom_paged_plan(plan)");
 }
