@@ -46,11 +46,19 @@ class _BeamState:
 
     MAX_GRAPHS = 4
 
-    def __init__(self, eng: "LoomDecoder", beams: int, page_size: int, n_pages: Optional[int]):
+    def __init__(self, eng: "LoomDecoder", beams: int, page_size: int, n_pages: Optional[int], shared_reads: bool):
         c, dev = eng.cfg, eng.dev
-        self.beams, self.n_pages = beams, n_pages
+        self.beams, self.n_pages, self.shared_reads = beams, n_pages, shared_reads
         self.cache = PagedKVCache(c.L, eng.B, eng.max_len, c.KVH, c.HD, eng.dtype, dev, page_size, n_pages)
-        self.ws = self.cache.workspace(c.QH)
+        self.ws = None if shared_reads else self.cache.workspace(c.QH)
+        if shared_reads:                             # a step of one token per row: its plan and the layers' scratch
+            i32 = dict(dtype=torch.int32, device=dev)
+            self.new = torch.ones(eng.B, **i32)
+            self.starts, self.rows_of, self.positions, self.shared = (torch.empty(n, **i32) for n in (eng.B + 1, eng.B, eng.B, eng.B))
+            self.slots = torch.empty(eng.B, dtype=torch.int64, device=dev)
+            self.plan, self.plan_ws = (torch.empty(n, dtype=torch.uint8, device=dev) for n in (
+                eng.lib.loom_paged_plan_bytes(eng.B, eng.B, c.QH, c.KVH),
+                eng.lib.loom_paged_batch_workspace_bytes(eng.B, eng.B, c.QH, c.KVH, c.HD)))
         self.scores = torch.empty(eng.B // beams, beams, dtype=torch.float32, device=dev)
         self.finished = torch.empty(eng.B, dtype=torch.bool, device=dev)
         self.parent = torch.empty(eng.B, dtype=torch.int32, device=dev)
@@ -60,8 +68,8 @@ class _BeamState:
         self.eos_id, self.pad_id = -1, 0
         self._graphs: Dict[object, torch.cuda.CUDAGraph] = {}
 
-    def fits(self, beams: int, page_size: int, n_pages: Optional[int]) -> bool:
-        return (self.beams, self.cache.page_size, self.n_pages) == (beams, page_size, n_pages)
+    def fits(self, beams: int, page_size: int, n_pages: Optional[int], shared_reads: bool) -> bool:
+        return (self.beams, self.cache.page_size, self.n_pages, self.shared_reads) == (beams, page_size, n_pages, shared_reads)
 
     def begin(self, eng: "LoomDecoder", P: int, eos_id: int, pad_id: int) -> None:
         """The first beam of every prompt holds the P tokens of the dense cache and is
@@ -547,6 +555,13 @@ class LoomDecoder:
         length (the q, c and kctx buffers as the dense step leaves them)."""
         c, kc = self.cfg, bs.cache
         k, v = kc.k_pages[bi], kc.v_pages[bi]
+        if bs.shared_reads:                          # (every row brings a token, so flat places are rows)
+            self._call("loom_paged_batch_step", self.code, _P(self.qkv), self.qkv.stride(0), _P(k), _P(v), k.stride(0),
+                       k.stride(2), k.stride(1), kc.n_pages, kc.page_size, _P(kc.table), kc.table.stride(0),
+                       kc.table.shape[1], self.B, _P(bs.rows_of), _P(bs.positions), _P(bs.slots), _P(bs.plan),
+                       bs.plan.numel(), _P(self.cos), _P(self.sin), self.max_len, _P(self.q), _P(self.c), _P(self.kctx),
+                       c.N, _P(bs.plan_ws), bs.plan_ws.numel(), self.B, c.QH, c.KVH, c.HD, st)
+            return
         self._call("loom_paged_decode_step", self.code, _P(self.qkv), self.qkv.stride(0), _P(k), _P(v), k.stride(0),
                    k.stride(2), k.stride(1), kc.n_pages, kc.page_size, _P(kc.table), kc.table.stride(0),
                    kc.table.shape[1], _P(kc.lens), _P(self.cos), _P(self.sin), self.max_len, _P(self.q), _P(self.c),
@@ -662,12 +677,17 @@ class LoomDecoder:
         self._beam_choose(bs, [(self.trace, 1), (self.doc, 0), (self.pending, 0), (self.ca_k, 0), (self.ca_v, 0),
                                (self.ca_valid, 0), (self.tokens, 0)])
         bs.cache.update(parent=bs.parent, n_new=1, advance=1)
+        if bs.shared_reads:
+            c, kc = self.cfg, bs.cache
+            self._call("loom_paged_plan", _P(kc.table), kc.table.stride(0), kc.table.shape[1], kc.n_pages, kc.page_size,
+                       _P(kc.lens), _P(bs.new), self.B, self.B, c.QH, c.KVH, _P(bs.starts), _P(bs.rows_of), _P(bs.positions),
+                       _P(bs.slots), _P(bs.shared), _P(bs.plan), bs.plan.numel(), self._stream())
         self._launch_step(first=False, prompt_len=0, paged=bs)
 
     @torch.no_grad()
     def beam_search(self, prompt: torch.Tensor, n_new: int, beams: int, eos_id: Optional[int] = None, pad_id: int = 0,
                     chunked_prefill: bool = False, use_graph: bool = True, page_size: int = 64,
-                    n_pages: Optional[int] = None):
+                    n_pages: Optional[int] = None, shared_reads: bool = False):
         """The `beams` best continuations of `n_new` tokens of each prompt [S, P] by
         beam search over the sum of log-probabilities (infer's loop,
         loomformer.py:5290-5311, with a choice over beams in place of the argmax):
@@ -679,7 +699,10 @@ class LoomDecoder:
         beams' rows; its keys and values then go into pages (page_size tokens each)
         once per prompt, and the beams share them: a step forks the rows by their parents and copies only a
         partly filled last page.  n_pages: pages of the pool (default: enough for
-        beams that share nothing); running out raises.  One step is captured into
+        beams that share nothing); running out raises.  shared_reads: the attention
+        reads the pages that beams have in common once for all of them
+        (ops.paged_batch_step): faster for long prompts and many beams, other
+        roundings of the same sums.  One step is captured into
         a graph and replayed.  Afterwards the engine holds no sequence to continue
         (its dense cache ends with the prompt)."""
         S, P = prompt.shape
@@ -695,9 +718,9 @@ class LoomDecoder:
         total = P + n_new
         self._check_capacity(total - 1)
         bs = self._beams
-        if bs is None or not bs.fits(beams, page_size, n_pages):
+        if bs is None or not bs.fits(beams, page_size, n_pages, bool(shared_reads)):
             self._beams = None                       # frees the old pool first
-            bs = self._beams = _BeamState(self, beams, page_size, n_pages)
+            bs = self._beams = _BeamState(self, beams, page_size, n_pages, bool(shared_reads))
         rows = prompt.repeat_interleave(beams, 0)
         if chunked_prefill:
             self.prefill(rows)
