@@ -734,19 +734,15 @@ __device__ __forceinline__ bool pb_odd(const BatchArgs<T>& a, const PbItem& s) {
 }
 
 template <typename T>
-__device__ __noinline__ pg_f32x4 pb_poison(const T* pool, const uint8_t* odd, const int32_t* row, int64_t ps_page, int64_t ps_tok,
-                                           int lens, int log_ps, int n_pages, int first, int last, bool nan) {
-    pg_f32x4 c = {0.f, 0.f, 0.f, 0.f};
+__device__ __noinline__ float pb_poison(const T* pool, const uint8_t* odd, const int32_t* row, int64_t ps_page, int64_t ps_tok,
+                                        int lens, int log_ps, int n_pages, int first, int last, bool nan) {
+    float c = 0.0f;
     for (int i = first; i <= last; ++i) {
         if (odd[i] == 0) continue;
         const int t = lens + i, page = row[t >> log_ps];
         if ((unsigned)page >= (unsigned)n_pages) continue;
-        const T* p = pool + (int64_t)page * ps_page + (int64_t)(t & ((1 << log_ps) - 1)) * ps_tok;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float v = ld(p + e);
-            if (!(fabsf(v) < INFINITY)) c[e] += nan ? NAN : v;
-        }
+        const float v = ld(pool + (int64_t)page * ps_page + (int64_t)(t & ((1 << log_ps) - 1)) * ps_tok);
+        if (!(fabsf(v) < INFINITY)) c += nan ? NAN : v;
     }
     return c;
 }
@@ -763,49 +759,87 @@ __device__ __forceinline__ gqa_u4 pb_finite(gqa_u4 w) {
     return w;
 }
 
-// The end of an item, for 16 queries of each wave: the waves' (m, l, C, Kctx) from LDS
-// joined into records, or into the outputs where the queries have no other part.
-// part(w): the sums of wave w's queries as its lanes hold them, C then Kctx, four queries'
-// of one dimension side by side; ml[w][16]: (m, l).  QW waves stand side by side: wave w's
-// queries begin at first + (w % QW) apart, and waves w, w + QW, .. have the same.
-template <int HDP, bool KCTX, typename T, typename P>
-__device__ __forceinline__ void pb_finish(const BatchArgs<T>& a, const PbWork& w, int QW, int first, int apart, bool odd,
-                                          const float2 (*ml)[16], P part) {
+// The end of an item, for 16 queries of each of its four waves: their (m, l, C, Kctx) joined
+// into records, or into the outputs where the queries have no other part.  part(w): the sums of
+// wave w's queries as its lanes hold them, C then Kctx, four queries' of one dimension
+// side by side.  QW waves stand side by side: wave w's queries begin at first +
+// (w % QW) apart, and waves w, w + QW, .. have the same.  First a thread per query finds the
+// factors of its parts and where it goes, then every thread takes four queries' sums of one
+// dimension (4 tokens behind 333 8.3 -> 7.2 us for the kernel, 8 x 4 behind 2048 12.0 -> 11.0,
+// 2 x 16 behind 2048 16.7 -> 15.1, against factors and destinations found by every thread
+// in a loop that held the rare cases).
+struct PbEnd {
+    float2 ml[4][16];
+    __align__(16) float factor[4][64];
+    int64_t to[64];                                  // element of the outputs (< 0: none) or record
+    int last[64];                                    // the query's token in the row's new ones
+};
+
+template <int HDP, bool KCTX, int QW, typename T, typename P>
+__device__ __forceinline__ void pb_finish(const BatchArgs<T>& a, const PbWork& w, int first, int apart, bool odd, PbEnd& end, P part) {
     const PbItem& s = w.s;
-    constexpr int quads = HDP / 4, per = KCTX ? 2 * quads : quads;
-    const int KW = 4 / QW;
-    for (int k = threadIdx.x; k < QW * 16 * per; k += 256) {
-        const int y = k / per, e = k - y * per, which = e >= quads, d = 4 * (e - which * quads);
-        const int w0 = y >> 4, j = y & 15, x = first + w0 * apart + j;
-        if (x >= s.nq) continue;
-        float m = -INFINITY, l = 0.0f;
-        for (int g = 0; g < KW; ++g) m = fmaxf(m, ml[w0 + QW * g][j].x);
-        pg_f32x4 c = {0.f, 0.f, 0.f, 0.f};
-        for (int g = 0; g < KW; ++g) {
-            const float2 p = ml[w0 + QW * g][j];
-            const float f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(p.x - m);
-            // query j, dimension d: lane 16 (j / 4) + d % 16, element j % 4
-            const float* v = part(w0 + QW * g) + ((which * (HDP / 16) + (d >> 4)) * 64 + (j >> 2) * 16 + (d & 15)) * 4 + (j & 3);
-            l = fmaf(p.y, f, l);
+    constexpr int KW = 4 / QW, D = KCTX ? 2 * HDP : HDP;
+    const int tid = threadIdx.x;
+    __syncthreads();                                 // the parts are written
+    if (tid < 16 * QW) {
+        const int x = first + (tid >> 4) * apart + (tid & 15);
+        float m = -INFINITY, l = 0.0f, f[KW];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) c[i] = fmaf(v[4 * i], f, c[i]);
+        for (int g = 0; g < KW; ++g) m = fmaxf(m, end.ml[(tid >> 4) + QW * g][tid & 15].x);
+#pragma unroll
+        for (int g = 0; g < KW; ++g) {
+            const float2 p = end.ml[(tid >> 4) + QW * g][tid & 15];
+            f[g] = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(p.x - m);
+            l = fmaf(p.y, f[g], l);
         }
-        if (odd && !(HDP > a.HD && d >= a.HD))
-            c += pb_poison((which ? a.kp : a.vp) + w.kvh * a.ps_head + d, a.odd + s.base, a.table + (int64_t)s.row * a.table_ld, a.ps_page,
-                           a.ps_tok, s.lens, a.log_ps, a.n_pages, s.x0 / a.G + 1, (s.x0 + x) / a.G, which);
-        if (s.rec < 0) {
-            if (HDP > a.HD && d >= a.HD) continue;
-            const int h = w.kvh * a.G + (s.x0 + x) % a.G;
-            T* out = (which ? a.k_out : a.c_out) + (int64_t)pb_token(a, s, x) * a.out_ld + (int64_t)h * a.HD + d;
-            const float inv = 1.0f / l;
-            const float o[4] = {c[0] * inv, c[1] * inv, c[2] * inv, c[3] * inv};
-            store_e<T, 4>(out, o);
-        } else {
-            const int64_t r = w.kvh * a.at.cap_recs + s.rec + x;
-            *reinterpret_cast<pg_f32x4*>(a.rec + (r * 2 + which) * HDP + d) = c;
-            if (e == 0) *reinterpret_cast<float2*>(a.rec + a.rec_ml + 2 * r) = make_float2(m, l);
+        const float inv = s.rec < 0 ? 1.0f / l : 1.0f;
+#pragma unroll
+        for (int g = 0; g < KW; ++g) end.factor[g][tid] = f[g] * inv;
+        int64_t to = -1;
+        if (x < s.nq) {
+            const int i = (s.x0 + x) / a.G, h = w.kvh * a.G + s.x0 + x - i * a.G;
+            if (s.rec < 0) {
+                to = (int64_t)pb_token(a, s, x) * a.out_ld + (int64_t)h * a.HD;
+            } else {
+                to = w.kvh * a.at.cap_recs + s.rec + x;
+                *reinterpret_cast<float2*>(a.rec + a.rec_ml + 2 * to) = make_float2(m, l);
+            }
+            end.last[tid] = i;
         }
+        end.to[tid] = to;
     }
+    __syncthreads();
+    // the usual loop has neither the rare tokens nor the other destination in it: a block runs
+    // through this code once, and what it costs is fetching it
+    auto sums = [&](auto poison, auto out) {
+        const int lo = s.x0 / a.G + 1;
+#pragma unroll 1
+        for (int k = tid; k < 4 * QW * D; k += 256) {
+            const int four = k / D, dd = k - four * D, which = dd >= HDP, d = dd - which * HDP, w0 = four >> 2;
+            pg_f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int g = 0; g < KW; ++g) {
+                // queries 4 (four % 4) .. + 3, dimension d: lane 16 (four % 4) + d % 16
+                const pg_f32x4 v = reinterpret_cast<const pg_f32x4*>(part(w0 + QW * g))[(which * (HDP / 16) + (d >> 4)) * 64 + (four & 3) * 16 + (d & 15)];
+                c += v * *reinterpret_cast<const pg_f32x4*>(&end.factor[g][4 * four]);
+            }
+            if (HDP > a.HD && d >= a.HD && out) continue;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t to = end.to[4 * four + i];
+                if (to < 0) continue;
+                if (poison && d < a.HD)
+                    c[i] += pb_poison((which ? a.kp : a.vp) + w.kvh * a.ps_head + d, a.odd + s.base, a.table + (int64_t)s.row * a.table_ld,
+                                      a.ps_page, a.ps_tok, s.lens, a.log_ps, a.n_pages, lo, end.last[4 * four + i], which);
+                if (out) st((which ? a.k_out : a.c_out) + to + d, c[i]);
+                else a.rec[to * 2 * HDP + dd] = c[i];
+            }
+        }
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+    if (odd) s.rec < 0 ? sums(Yes{}, Yes{}) : sums(Yes{}, No{});
+    else s.rec < 0 ? sums(No{}, Yes{}) : sums(No{}, No{});
 }
 
 // ------------------------------------------------------------------ matrix-core form
@@ -868,7 +902,7 @@ paged_items_kernel(BatchArgs<T> a) {
     // a stage per array, so that a wait for one stage's loads never covers another's reads
     __shared__ __align__(16) gqa_u4 K0[R * CPR], V0[R * CPR], K1[R * CPR], V1[R * CPR];
     __shared__ __align__(16) gqa_u4 K2[NS == 3 ? R * CPR : 1], V2[NS == 3 ? R * CPR : 1];
-    __shared__ float2 ml[4][16];
+    __shared__ PbEnd end;
     using M = Mfma16<T>;
     const PbWork w = pb_work(a);
     if (!w.any) return;
@@ -1113,17 +1147,16 @@ paged_items_kernel(BatchArgs<T> a) {
         auto part = [&](int i) { return reinterpret_cast<float*>(i == 0 ? K0 : i == 1 ? V0 : i == 2 ? K1 : V1); };
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
-            __syncthreads();
+            __syncthreads();                         // the stages, or the last queries' sums, are read
             lh[n] = sum_16_32(lh[n]);
-            if (lq == 0) ml[wave][lr] = make_float2(mh[n], lh[n]);
+            if (lq == 0) end.ml[wave][lr] = make_float2(mh[n], lh[n]);
             pg_f32x4* mine = reinterpret_cast<pg_f32x4*>(part(wave)) + lane;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 mine[64 * dt] = accC[n][dt];
                 if constexpr (KCTX) mine[64 * (DT + dt)] = accK[n][dt];
             }
-            __syncthreads();
-            pb_finish<HD, KCTX>(a, w, QW, 16 * n, 16 * NQ, odd, ml, part);
+            pb_finish<HD, KCTX, QW>(a, w, 16 * n, 16 * NQ, odd, end, part);
         }
     };
     if (s.nq <= 16) body(I4{}, I1{});
@@ -1147,7 +1180,7 @@ paged_items_f32_kernel(BatchArgs<T> a) {
     constexpr int NP = (RT * PR + 255) / 256;        // pieces per thread and tensor
     constexpr int kTile = 2 * RT * PITCH, kRed = 4 * 16 * 2 * HDP;
     __shared__ __align__(16) float lds[kTile > kRed ? kTile : kRed];
-    __shared__ float2 ml[4][16];
+    __shared__ PbEnd end;
     const PbWork w = pb_work(a);
     if (!w.any) return;
     const PbItem& s = w.s;
@@ -1305,15 +1338,16 @@ paged_items_f32_kernel(BatchArgs<T> a) {
     lh = sum_16_32(lh);
     __syncthreads();
     auto part = [&](int i) { return lds + i * 16 * 2 * HDP; };
-    if (lq == 0) ml[wave][lr] = make_float2(mh, lh);
+    if (lq == 0) end.ml[wave][lr] = make_float2(mh, lh);
     pg_f32x4* mine = reinterpret_cast<pg_f32x4*>(part(wave)) + lane;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
         mine[64 * dt] = accC[dt];
         if constexpr (KCTX) mine[64 * (DT + dt)] = accK[dt];
     }
-    __syncthreads();
-    pb_finish<HDP, KCTX>(a, w, QW, xb, 16, odd, ml, part);
+    if (QW == 4) pb_finish<HDP, KCTX, 4>(a, w, xb, 16, odd, end, part);
+    else if (QW == 2) pb_finish<HDP, KCTX, 2>(a, w, xb, 16, odd, end, part);
+    else pb_finish<HDP, KCTX, 1>(a, w, xb, 16, odd, end, part);
 }
 
 // ------------------------------------------------------------------ the join
