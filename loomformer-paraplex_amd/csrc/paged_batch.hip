@@ -1145,6 +1145,27 @@ paged_items_kernel(BatchArgs<T> a) {
         // wave w's sums in the w-th of four stage arrays, whose size they have
         static_assert(16 * 2 * HD * sizeof(float) == sizeof(K0), "a wave's sums of 16 queries fill a stage");
         auto part = [&](int i) { return reinterpret_cast<float*>(i == 0 ? K0 : i == 1 ? V0 : i == 2 ? K1 : V1); };
+        // records of queries that one wave has alone go out of its registers as they are
+        if (KW == 1 && s.rec >= 0 && !odd) {
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                const int x = 16 * (NQ * wave + n);
+                const int64_t to = w.kvh * a.at.cap_recs + s.rec + x;
+                lh[n] = sum_16_32(lh[n]);
+                if (lq == 0 && x + lr < s.nq) *reinterpret_cast<float2*>(a.rec + a.rec_ml + 2 * (to + lr)) = make_float2(mh[n], lh[n]);
+                float* rec = a.rec + (to + 4 * lq) * 2 * HD + lr;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (x + 4 * lq + i >= s.nq) break;
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) {
+                        rec[i * 2 * HD + 16 * dt] = accC[n][dt][i];
+                        if constexpr (KCTX) rec[i * 2 * HD + HD + 16 * dt] = accK[n][dt][i];
+                    }
+                }
+            }
+            return;
+        }
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
             __syncthreads();                         // the stages, or the last queries' sums, are read
