@@ -27,7 +27,7 @@ constexpr int kPbMaxRows = 1024;
 constexpr int kPbQ = 128;           // queries (a token's heads of one kv head) of a block
 constexpr int kPbTile = 64;         // positions of a step of a block
 constexpr int kPbLeast = 1;         // an item has so many tiles at least
-constexpr float kPbRecord = 2.5e-4f;  // a query's record, in a block's time for a tile of its queries
+constexpr float kPbRecord = 4e-4f;  // a query's record, in a block's time for a tile of its queries
 constexpr int kPbFew = 8;           // records of a query that a wave of the join takes alone
 constexpr int kPbAlone = 64;        // rows with more queries fill a block by themselves and share nothing
 constexpr int kPbShare = 64;        // common positions from which reading them once pays
@@ -446,6 +446,9 @@ paged_plan_kernel(PlanArgs a) {
     // An item has at least the tiles that fill the device.  It leaves a record per query, which
     // is written and read at the copy's rate by all blocks together, while a tile is
     // one block's time: c tiles and work / c records take least where c^2 is their ratio.
+    // (kPbRecord 1.5e-4 / 2.5e-4 / 4e-4 / 1e-3, items and join, us: 64 rows behind 16384
+    // 71.1 / 70.5 / 62.5 / 76.2, 4 x 12 behind 1500 30.4 / 32.5 / 33.8 / 38.4, 2 x 16 behind 2048
+    // 21.0 / 20.5 / 19.1 / 19.4)
     const float ratio = kPbRecord * (float)a.KVH * 16.0f * ((float)tiles[2] * 1048576.0f + (float)tiles[3]);
     const int64_t fill = (all_tiles + a.at.slots - 1) / a.at.slots;
     const int chunk = max(max(kPbLeast, (int)sqrtf(ratio)), (int)min(fill, (int64_t)1 << 30));
