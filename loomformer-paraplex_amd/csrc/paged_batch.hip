@@ -120,7 +120,8 @@ __device__ __forceinline__ int pb_fresh(const PlanArgs& a, int r) {
 // start with the same page belong together; the lowest of them leads, found in a hash
 // table in LDS that every block fills from all rows' first entries.  A row's state: (the
 // leader or -1, whole pages in common with it, pages all there, 0).  Bound by the chain
-// first entries, hash, the two rows' entries, 256 of each in flight per wave.
+// first entries, hash, the two rows' entries, 256 of each in flight per wave (64 rows of up to
+// 17000 tokens 6.1 us, 256 rows of up to 6600 4.7).
 constexpr int kPbHash = 2048;
 
 struct PbHash {
@@ -308,7 +309,9 @@ __device__ __forceinline__ int4 pb_states(const PlanArgs& a, int m) {
 // Block 0 is one block because each stage needs the whole of the one before; it is
 // bound by their latency, a pass over the rows or the segments with a block scan each.
 // ALONE: of few table entries every block finds the states itself, and the launch before is
-// saved.  NT: at least as many threads as rows; a barrier of fewer waves is a shorter one.
+// saved.  NT: at least as many threads as rows; a barrier of fewer waves is a shorter one
+// (4 rows by one wave 6.3 us, by 16 with the launch before 9.2; 32 rows by four waves 12.1, 64
+// and 256 rows by 16 waves 9 to 11 behind the launch before).
 template <int NT, bool ALONE>
 __global__ void __launch_bounds__(NT)
 paged_plan_kernel(PlanArgs a) {
@@ -618,7 +621,8 @@ __device__ __forceinline__ void store_e(T* p, const float (&v)[E]) {
 // slot.  A thread takes E elements of a head and their partners half a head on, so that
 // each is loaded once.  Tokens behind the last give zeros, tokens of a row without room
 // or a page NaN; both are done here.  A copy with a little arithmetic: bound by the
-// bytes in and out, or, of few tokens, by one load after the other.
+// bytes in and out (5139 tokens of 48 heads of 128 25.4 us, 5.0 TB/s), or, of few tokens, by one
+// load after the other (32 tokens 4.7).
 template <typename T, int E>
 __global__ void __launch_bounds__(256)
 paged_append_kernel(BatchArgs<T> a) {
@@ -861,6 +865,12 @@ __device__ __forceinline__ void pb_finish(const BatchArgs<T>& a, const PbWork& w
 // the score registers, C = P V and Kctx = P K through the transposing LDS read.  A lane's
 // sum of weights is its own until the end, and the reference of the exponents is looked at
 // lane by lane: the lanes of a column meet only where it has to rise.
+//
+// Of long shared runs and of prompts bound by the matrix products and what feeds them: 5139
+// tokens of 32 heads of 128 in 295 us, 713 TFLOP/s (the 8192^3 product 1135); 62 rows behind
+// 16384 50.6 us, 498 TFLOP/s, of which the records' 25 MB written at once are some 8; 32 x 128 tokens
+// behind 1920 of 8 heads of 96 57.5 us, 651 TFLOP/s.  Of few rows by the chain item, page, first
+// tile, sums: 7.3 us (4 rows behind 333), 10.9 (8 x 4 behind 2048, 3.1 TB/s).
 template <int HD> constexpr int pb_stages() { return HD <= 96 ? 3 : 2; }
 
 // Where a row's 16-byte pieces lie in a stage: piece c of row r at c ^ swz(r), so that both
@@ -1195,6 +1205,8 @@ paged_items_kernel(BatchArgs<T> a) {
 // blocks; RT positions per step in one LDS buffer, the next ones in flight in registers.
 // The products' operands may take the dimensions in any order that both share: lane
 // group lq takes HD / 4 neighbouring ones of them, so that a lane's are 16-byte reads.
+// Three prompts to 257 tokens 15.5 us, 4 rows to 1300 10.3: the chain item, page, tile, sums, and
+// the fp32 rate behind long rows (4 x 1024 tokens behind 500 324 us, 59 TFLOP/s of 154).
 template <typename T, int HD, bool KCTX>
 __global__ void __launch_bounds__(256)
 paged_items_f32_kernel(BatchArgs<T> a) {
@@ -1378,7 +1390,9 @@ paged_items_f32_kernel(BatchArgs<T> a) {
 // The queries whose sums are in records, those of their own segment's chunks and of the
 // group's segment that holds them.  Of few records (kPbFew) a block's four waves take a
 // query each, all its records in flight; of more it takes one query: wave w records w,
-// w + 4, .., kPbJoin of them in flight, and the waves meet in LDS.  Bound by the records' bytes.
+// w + 4, .., kPbJoin of them in flight, and the waves meet in LDS.  Bound by the chain count,
+// task, records where those are few (32 rows behind 2048 4.6 us), by the records' bytes else (62
+// rows behind 16384, 32 heads of 128: 10.9 us).
 constexpr int kPbJoin = 8;
 
 // (m, l, v) and a record's (e, y) as one
@@ -1716,6 +1730,9 @@ extern "C" int loom_paged_batch_step(int dtype, const void* qkv, int64_t qkv_ld,
     LOOM_CHECK((((uintptr_t)q_out | (uintptr_t)c_out | (uintptr_t)kctx_out | (uintptr_t)cos_table | (uintptr_t)sin_table) % 16) == 0,
                "%s: the outputs and the rotary tables must be 16-byte aligned", who);
     LOOM_CHECK(n_pos >= 1, "%s: the rotary tables are empty", who);
+    // a launch's threads are counted in 32 bits (blocks of 256)
+    LOOM_CHECK((int64_t)pb_layout(rows, n_tokens, QH, KVH).cap_items * KVH < (int64_t)1 << 24,
+               "%s: %lld tokens of %lld query heads are too many for one call", who, (long long)n_tokens, (long long)QH);
     const int64_t pn = loom_paged_plan_bytes(rows, n_tokens, QH, KVH);
     LOOM_CHECK(plan_bytes >= pn && ((uintptr_t)plan % 64) == 0, "%s: a 64-byte aligned plan of %lld bytes is needed, got %lld", who,
                (long long)pn, (long long)plan_bytes);

@@ -569,3 +569,72 @@ def test_the_same_call_gives_the_same_bits():
     for r in runs[1:]:
         for a, b in zip(r, runs[0]):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_pages_past_2_to_the_32_elements(dt):
+    """The same pages at the end of a pool whose elements pass 2^32 bytes and 2^31 elements."""
+    from loom_amd import ops
+    g = torch.Generator().manual_seed(25)
+    lens, new, PS, HD, NP = [2100, 2090, 2048, 0], [1, 9, 1, 30], 1024, 128, 17000
+    kp, vp, table = _cache(g, lens, new, [([0, 1, 2], 2048)], 4, 1, PS, HD, dt, spare=1)
+    n, N = kp.shape[0], sum(new)
+    qkv = torch.randn(N, 6 * HD, generator=g).to(DEV, dt)
+    cos, sin = _tables(HD, 4 * PS)
+    big = [torch.empty(NP, 1, PS, HD, dtype=dt, device=DEV) for _ in range(2)]
+    for b, small in zip(big, (kp, vp)):
+        b[NP - n:] = small
+    far = torch.where(table >= 0, table + (NP - n), table).to(torch.int32)
+    want = ops.paged_batch_step(ops.paged_plan(kp, table, _i32(lens), _i32(new), N, 4), qkv, kp, vp, table, cos, sin)
+    plan = ops.paged_plan(big[0], far, _i32(lens), _i32(new), N, 4)
+    got = ops.paged_batch_step(plan, qkv, *big, far, cos, sin)
+    torch.cuda.synchronize()
+    assert not want[0].float().isnan().any()
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+    for b, small in zip(big, (kp, vp)):
+        assert torch.equal(_bits(b[NP - n:]), _bits(small))
+
+
+def test_a_plan_of_the_most_tokens():
+    """2^20 flat places, rows of up to half a million new tokens."""
+    from loom_amd import ops
+    PS, N, lens = 1024, 1 << 20, [5, -1, 70000, 0, 1]
+    new = [300000, 9, 0, 500000, N - 800000 - 11]
+    MP = 512
+    table = torch.arange(5 * MP, dtype=torch.int32).view(5, MP)
+    k = torch.empty(5 * MP, 2, PS, 8, dtype=BF, device=DEV)
+    plan = ops.paged_plan(k, table.to(DEV), _i32(lens), _i32(new), N, 8)
+    n = torch.tensor([m if at >= 0 else 0 for m, at in zip(new, lens)])
+    starts = torch.cat([torch.zeros(1, dtype=torch.int64), n.cumsum(0)])
+    rows = torch.repeat_interleave(torch.arange(5), n)
+    pos = torch.arange(int(n.sum())) - starts[rows] + torch.tensor(lens)[rows]
+    slots = table[rows, pos // PS].long() * PS + pos % PS
+    end = torch.full((11,), -1)
+    assert plan.starts.tolist() == starts.tolist()
+    assert torch.equal(plan.rows.cpu().long(), torch.cat([rows, end]))
+    assert torch.equal(plan.positions.cpu().long(), torch.cat([pos, end]))
+    assert torch.equal(plan.slots.cpu(), torch.cat([slots, end]))
+    assert plan.shared.tolist() == [0] * 5
+
+
+def test_a_plan_made_before_its_tables_changed_reads_and_writes_in_range():
+    """Table entries that are no pages any more: no place outside the pool is touched, and rows
+    that the change does not concern come out as before."""
+    from loom_amd import ops
+    g = torch.Generator().manual_seed(26)
+    lens, new = [300, 310, 200, 90], [1, 2, 1, 40]
+    for dt, HD in ((BF, 96), (FP, 16)):
+        kp, vp, table = _cache(g, lens, new, [([0, 1], 256)], 24, 2, 16, HD, dt)
+        cos, sin = _tables(HD, 24 * 16)
+        qkv = torch.randn(44, 12 * HD, generator=g).to(DEV, dt)
+        plan = ops.paged_plan(kp, table, _i32(lens), _i32(new), 44, 8)
+        want = ops.paged_batch_step(plan, qkv, kp, vp, table, cos, sin)
+        k1, v1 = kp.clone(), vp.clone()
+        table[2, 3:] = -1
+        table[3, 0] = 1 << 30
+        got = ops.paged_batch_step(plan, qkv, kp, vp, table, cos, sin)
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert torch.equal(a[:3], b[:3])
+        assert torch.equal(_bits(kp), _bits(k1)) and torch.equal(_bits(vp), _bits(v1))

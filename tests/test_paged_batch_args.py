@@ -54,6 +54,14 @@ def test_step_refuses():
         (dict(ws_bytes=16), "workspace"), (dict(ws=ctypes.c_void_p(260)), "workspace")])
 
 
+def test_step_refuses_more_blocks_than_a_launch_has():
+    n = 1 << 20
+    for QH, KVH in ((1024, 1), (1024, 2)):
+        width = (QH + 2 * KVH) * 96
+        _refuses("loom_paged_batch_step", dict(STEP, n_tokens=n, QH=QH, KVH=KVH, qkv_ld=width, out_ld=QH * 96, plan_bytes=1 << 40,
+                                               ws_bytes=1 << 50), [(dict(), "too many for one call")])
+
+
 def test_no_tokens_is_no_error():
     from loom_amd import _lib
     none = {k: None for k in ("qkv", "k", "v", "table", "rows_of", "positions", "slots", "plan", "cos", "sin", "q_out", "c", "kctx", "ws")}
