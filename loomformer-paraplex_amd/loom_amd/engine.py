@@ -46,7 +46,7 @@ class _BeamState:
 
     MAX_GRAPHS = 4
 
-    def __init__(self, eng: "LoomDecoder", beams: int, page_size: int, n_pages: Optional[int], shared_reads: bool):
+    def __init__(self, eng: "LoomDecoder", beams: int, page_size: int, n_pages: Optional[int], shared_reads: bool = False):
         c, dev = eng.cfg, eng.dev
         self.beams, self.n_pages, self.shared_reads = beams, n_pages, shared_reads
         self.cache = PagedKVCache(c.L, eng.B, eng.max_len, c.KVH, c.HD, eng.dtype, dev, page_size, n_pages)
@@ -68,7 +68,7 @@ class _BeamState:
         self.eos_id, self.pad_id = -1, 0
         self._graphs: Dict[object, torch.cuda.CUDAGraph] = {}
 
-    def fits(self, beams: int, page_size: int, n_pages: Optional[int], shared_reads: bool) -> bool:
+    def fits(self, beams: int, page_size: int, n_pages: Optional[int], shared_reads: bool = False) -> bool:
         return (self.beams, self.cache.page_size, self.n_pages, self.shared_reads) == (beams, page_size, n_pages, shared_reads)
 
     def begin(self, eng: "LoomDecoder", P: int, eos_id: int, pad_id: int) -> None:
