@@ -182,14 +182,14 @@ __device__ __forceinline__ int4 pb_row(const PlanArgs& a, const PbHash& hash, in
         int v[4], w[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const int c = c0 + 64 * u + lane;
-            v[u] = c < need ? row[c] : 0;
-            w[u] = c < whole && lead != r ? other[c] : v[u];
+            const int c = min(c0 + 64 * u + lane, need - 1);         // (a condition would wait for each load)
+            v[u] = row[c];
+            w[u] = other[c];
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             there &= !__any((unsigned)v[u] >= (unsigned)a.n_pages);
-            const unsigned long long differ = __ballot(v[u] != w[u]);
+            const unsigned long long differ = __ballot(c0 + 64 * u + lane < whole && v[u] != w[u]);
             if (differ) same = min(same, c0 + 64 * u + (int)__ffsll(differ) - 1);
         }
     }
@@ -282,7 +282,8 @@ __device__ __forceinline__ int4 pb_states(const PlanArgs& a, int m) {
     const int MP = a.cap >> a.log_ps, entries = a.R * MP;
     const float per = 1.0f / (float)MP;              // (entries are few: the quotient is off by one at most)
     for (int i0 = r; i0 < entries; i0 += 4 * NT) {
-        int v[4], w[4], row[4], col[4];
+        // (all of a round's entries are loaded, needed or not: a condition would wait for each)
+        int v[4], w[4], row[4], col[4], lead_row[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int i = min(i0 + u * NT, entries - 1);
@@ -290,14 +291,14 @@ __device__ __forceinline__ int4 pb_states(const PlanArgs& a, int m) {
             col[u] = i - row[u] * MP;
             if (col[u] < 0) --row[u], col[u] += MP;
             if (col[u] >= MP) ++row[u], col[u] -= MP;
-            const int l = page_of[row[u]];
-            v[u] = col[u] < need_of[row[u]] ? a.table[(int64_t)row[u] * a.table_ld + col[u]] : 0;
-            w[u] = col[u] < whole_of[row[u]] && l != row[u] ? a.table[(int64_t)max(l, 0) * a.table_ld + col[u]] : v[u];
+            lead_row[u] = max(page_of[row[u]], 0);
+            v[u] = a.table[(int64_t)row[u] * a.table_ld + col[u]];
+            w[u] = a.table[(int64_t)lead_row[u] * a.table_ld + col[u]];
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            if ((unsigned)v[u] >= (unsigned)a.n_pages) lacks[row[u]] = 1;
-            if (v[u] != w[u]) atomicMin(&same_of[row[u]], col[u]);
+            if (col[u] < need_of[row[u]] && (unsigned)v[u] >= (unsigned)a.n_pages) lacks[row[u]] = 1;
+            if (col[u] < whole_of[row[u]] && v[u] != w[u]) atomicMin(&same_of[row[u]], col[u]);
         }
     }
     __syncthreads();
