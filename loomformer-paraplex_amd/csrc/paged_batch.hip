@@ -121,7 +121,7 @@ __device__ __forceinline__ int pb_fresh(const PlanArgs& a, int r) {
 // table in LDS that every block fills from all rows' first entries.  A row's state: (the
 // leader or -1, whole pages in common with it, pages all there, 0).  Bound by the chain
 // first entries, hash, the two rows' entries, 256 of each in flight per wave (64 rows of up to
-// 17000 tokens 6.1 us, 256 rows of up to 6600 4.7).
+// 17000 tokens 4.7 us, 256 rows of up to 6600 4.3).
 constexpr int kPbHash = 2048;
 
 struct PbHash {
@@ -311,7 +311,7 @@ __device__ __forceinline__ int4 pb_states(const PlanArgs& a, int m) {
 // bound by their latency, a pass over the rows or the segments with a block scan each.
 // ALONE: of few table entries every block finds the states itself, and the launch before is
 // saved.  NT: at least as many threads as rows; a barrier of fewer waves is a shorter one
-// (4 rows by one wave 6.3 us, by 16 with the launch before 9.2; 32 rows by four waves 12.1, 64
+// (4 rows by one wave 6.1 us, by 16 with the launch before 9.2; 32 rows by four waves 10.8, 64
 // and 256 rows by 16 waves 9 to 11 behind the launch before).
 template <int NT, bool ALONE>
 __global__ void __launch_bounds__(NT)
@@ -871,7 +871,7 @@ __device__ __forceinline__ void pb_finish(const BatchArgs<T>& a, const PbWork& w
 // tokens of 32 heads of 128 in 295 us, 713 TFLOP/s (the 8192^3 product 1135); 62 rows behind
 // 16384 50.6 us, 498 TFLOP/s, of which the records' 25 MB written at once are some 8; 32 x 128 tokens
 // behind 1920 of 8 heads of 96 57.5 us, 651 TFLOP/s.  Of few rows by the chain item, page, first
-// tile, sums: 7.3 us (4 rows behind 333), 10.9 (8 x 4 behind 2048, 3.1 TB/s).
+// tile, sums: 7.3 us (4 rows behind 333), 10.9 (8 x 4 behind 2048, 1.6 TB/s).
 template <int HD> constexpr int pb_stages() { return HD <= 96 ? 3 : 2; }
 
 // Where a row's 16-byte pieces lie in a stage: piece c of row r at c ^ swz(r), so that both

@@ -262,6 +262,41 @@ def test_later_tokens_that_are_not_finite(dt, HD):
 
 
 @pytest.mark.parametrize("dt", [BF, HF, FP])
+@pytest.mark.parametrize("HD", [16, 64, 96, 128])
+@pytest.mark.parametrize("kctx", [True, False])
+def test_tokens_that_are_not_finite_where_rows_share_and_split(dt, HD, kctx):
+    """The same in rows whose sums come from several parts (a common one, chunks of a long row), of
+    1 to 64 queries that share and of 128 that do not: what is finite in 64 bits is right, the rest
+    is not finite."""
+    from loom_amd import ops
+    g = torch.Generator().manual_seed(27)
+    QH, KVH, PS = 8, 2, 16
+    lens, new = [640, 650, 645, 641, 2500, 700], [16, 8, 4, 1, 40, 1]
+    kp, vp, table = _cache(g, lens, new, [([0, 1, 2, 3], 640)], 170, KVH, PS, HD, dt)
+    N, qd = sum(new), QH * HD
+    qkv = torch.randn(N, (QH + 2 * KVH) * HD, generator=g).to(dt)
+    v0 = qd + KVH * HD
+    for t, at, value in ((5, v0 + 3, math.inf), (11, v0 + HD, math.nan), (17, v0 + 1, -math.inf), (26, qd + 2, math.nan),
+                         (45, v0 + 5, math.inf), (50, v0 + 5, -math.inf), (60, qd + HD, math.nan)):
+        qkv[t, at] = value
+    qkv = qkv.to(DEV)
+    cos, sin = _tables(HD, 2720)
+    plan = ops.paged_plan(kp, table, _i32(lens), _i32(new), N, QH)
+    assert plan.shared.tolist() == [640] * 4 + [0] * 2
+    c, kx, q = ops.paged_batch_step(plan, qkv, kp, vp, table, cos, sin, want_kctx=kctx)
+    torch.cuda.synchronize()
+    starts, _, _, _, ok = ref.maps(table.cpu(), torch.tensor(lens), torch.tensor(new), N, kp.shape[0], PS)
+    o = ref.batch_attention(q, kp, vp, table.cpu(), lens, starts, ok)
+    here = {k: torch.nan_to_num(v, nan=0.0, posinf=0.0, neginf=0.0) for k, v in o.items()}
+    for got, what in ((c, "c"), (kx, "kctx"))[:1 + kctx]:
+        want, y = o[what], got.cpu().double()
+        fine = want.isfinite()
+        assert 0 < int((~fine).sum()) < fine.numel() // 2
+        assert not y[~fine].isfinite().any()
+        _near(torch.where(fine, y, 0), torch.where(fine, want, 0), here[what + "_abs"], here, dt, HD, what)
+
+
+@pytest.mark.parametrize("dt", [BF, HF, FP])
 def test_rows_without_their_pages_or_their_places(dt):
     """A row that lacks a page (of the past or to come), whose tokens pass its table, or do not fit
     into the batch: NaN, and nothing written."""
