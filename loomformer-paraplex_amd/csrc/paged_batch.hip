@@ -869,9 +869,9 @@ __device__ __forceinline__ void pb_finish(const BatchArgs<T>& a, const PbWork& w
 //
 // Of long shared runs and of prompts bound by the matrix products and what feeds them: 5139
 // tokens of 32 heads of 128 in 295 us, 713 TFLOP/s (the 8192^3 product 1135); 62 rows behind
-// 16384 50.6 us, 498 TFLOP/s, of which the records' 25 MB written at once are some 8; 32 x 128 tokens
+// 16384 50.6 us, 498 TFLOP/s, of which the records' 40 MB written at once are some 8; 32 x 128 tokens
 // behind 1920 of 8 heads of 96 57.5 us, 651 TFLOP/s.  Of few rows by the chain item, page, first
-// tile, sums: 7.3 us (4 rows behind 333), 10.9 (8 x 4 behind 2048, 1.6 TB/s).
+// tile, sums: 7.3 us (4 rows behind 333), 10.9 (8 x 4 behind 2048, 1.4 TB/s).
 template <int HD> constexpr int pb_stages() { return HD <= 96 ? 3 : 2; }
 
 // Where a row's 16-byte pieces lie in a stage: piece c of row r at c ^ swz(r), so that both
