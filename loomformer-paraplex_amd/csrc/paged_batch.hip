@@ -83,7 +83,9 @@ static PbLayout pb_layout(int64_t R, int64_t N, int64_t QH, int64_t KVH) {
     p.cap_items = (int)(R + NG / 64 + R / 2 + some / kPbQ + 2) + p.slots;
     const int64_t split = kPbQ < NG ? kPbQ : NG;          // queries of a split segment
     p.cap_joins = (int)(p.slots + R + 1);
-    p.cap_tasks = (int)(p.slots * split + some + R + 1);
+    // a query is in one own segment, so in one task at most
+    const int64_t tasks = p.slots * split + some + R + 1;
+    p.cap_tasks = (int)(tasks < NG ? tasks : NG > 0 ? NG : 1);
     p.cap_toks = (int)some + 1;
     p.cap_recs = 2 * p.slots * split + 2 * some;
     p.rows = kPbHeader;
@@ -1206,7 +1208,7 @@ paged_items_kernel(BatchArgs<T> a) {
 // blocks; RT positions per step in one LDS buffer, the next ones in flight in registers.
 // The products' operands may take the dimensions in any order that both share: lane
 // group lq takes HD / 4 neighbouring ones of them, so that a lane's are 16-byte reads.
-// Three prompts to 257 tokens 15.5 us, 4 rows to 1300 10.3: the chain item, page, tile, sums, and
+// Three prompts to 257 tokens 13.8 us, 4 rows to 1300 9.4: the chain item, page, tile, sums, and
 // the fp32 rate behind long rows (4 x 1024 tokens behind 500 324 us, 59 TFLOP/s of 154).
 template <typename T, int HD, bool KCTX>
 __global__ void __launch_bounds__(256)
@@ -1392,8 +1394,8 @@ paged_items_f32_kernel(BatchArgs<T> a) {
 // group's segment that holds them.  Of few records (kPbFew) a block's four waves take a
 // query each, all its records in flight; of more it takes one query: wave w records w,
 // w + 4, .., kPbJoin of them in flight, and the waves meet in LDS.  Bound by the chain count,
-// task, records where those are few (32 rows behind 2048 4.6 us), by the records' bytes else (62
-// rows behind 16384, 32 heads of 128: 10.9 us).
+// task, records where those are few (32 rows behind 2048 4.0 us), by the records' bytes else (62
+// rows behind 16384, 32 heads of 128: 10.0 us).
 constexpr int kPbJoin = 8;
 
 // (m, l, v) and a record's (e, y) as one
@@ -1598,7 +1600,10 @@ static int batch_launch(const BatchCall& c, hipStream_t st) {
     if (c.HD >= 16) hipLaunchKernelGGL((paged_append_kernel<T, 8>), appends, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((paged_append_kernel<T, 4>), appends, dim3(256), 0, st, a);
     if (int rc = launch_status("loom_paged_batch_step(append)")) return rc;
-    const dim3 grid((unsigned)(a.at.cap_items * c.KVH));
+    // no more items than there are segments times a row's tiles (fp32, 3 rows
+    // of up to 257: 15.5 -> 13.8 us without the blocks that can have nothing)
+    const int64_t most = (int64_t)(a.at.cap_items - a.at.slots) * ceil_div((int64_t)a.cap, kPbTile);
+    const dim3 grid((unsigned)((most < a.at.cap_items ? most : a.at.cap_items) * c.KVH));
     bool done = false;
     if constexpr (sizeof(T) == 2) {
 #define LOOM_PB_M(HDV)                                                                              \
@@ -1623,7 +1628,8 @@ static int batch_launch(const BatchCall& c, hipStream_t st) {
     }
     LOOM_CHECK(done, "paged_batch_step: unsupported head_dim %lld (8, 16, 32, 64, 96, 128 or 256)", (long long)c.HD);
     if (int rc = launch_status("loom_paged_batch_step(items)")) return rc;
-    const int64_t joins = ceil_div(4096, c.KVH);
+    // (4096 blocks instead: 4.9 us for 4.4 of few joins, 7.9 for 7.4 of many)
+    const int64_t joins = ceil_div(1024, c.KVH);
     const dim3 jgrid((unsigned)(joins < a.at.cap_tasks ? joins : a.at.cap_tasks), (unsigned)c.KVH);
 #define LOOM_PB_J(HDV)                                                                              \
     if (c.HD == HDV) hipLaunchKernelGGL((paged_batch_join_kernel<T, HDV>), jgrid, dim3(256), 0, st, a);
