@@ -877,6 +877,8 @@ int loom_paged_plan(const int32_t* table, int64_t table_ld, int64_t max_pages, i
  * (or NULL), rows out_ld apart.  Pages that a new token is written to must be held
  * by its row alone (loom_paged_reserve).  Later tokens of the row and
  * whatever else lies in its pages have no influence, infinities and NaN included.
+ * An infinity of v is the readout of the tokens that see it (two of both signs:
+ * NaN; so too a weight that is zero in the type the product takes, for a token of an earlier step).
  * Padding gives zeros; tokens of a row without slots, and those whose position
  * lies past the rotary tables, give NaN and are not written.  A plan of other
  * sizes gives NaN.  workspace: loom_paged_batch_workspace_bytes, 16-byte aligned,

@@ -732,13 +732,29 @@ __device__ __forceinline__ int pb_sees(const BatchArgs<T>& a, const PbItem& s, i
 // Where a block has such a token (pb_odd), the products leave out what is not finite in
 // rows that not every query sees, and the item's end adds it to the sums of the
 // queries that do (pb_poison): an infinity of v is the sum's, one of k (whose score is NaN
-// or an infinity, and 0 times an infinity) is NaN.  Such tokens lie behind the first query's.
+// or an infinity, and 0 times an infinity) is NaN.  Such tokens lie behind the first query's
+// (pb_new), and only the item that holds a token's position adds it: in another one a query
+// that sees it may see nothing at all, and the join would take the infinity times zero.
+// What every query of the block sees, tokens of earlier steps among it, stays in the products: an
+// infinity of v there is the sum's where its weight is not zero in the type that the product
+// takes, and NaN where it is.
+struct PbNew {
+    int first, last;                // new tokens of the row, from 0
+};
+
+// New tokens whose positions the item holds and that some of the block's queries do not see
+template <typename T>
+__device__ __forceinline__ PbNew pb_new(const BatchArgs<T>& a, const PbItem& s) {
+    const int k0 = s.key0 + s.tile0 * kPbTile, kend = min(s.key1, s.key0 + s.tile1 * kPbTile);
+    return {max(s.x0 / a.G + 1, k0 - s.lens), min((s.x0 + s.nq - 1) / a.G, kend - 1 - s.lens)};
+}
+
 template <typename T>
 __device__ __forceinline__ bool pb_odd(const BatchArgs<T>& a, const PbItem& s) {
     bool odd = false;
     if (s.kind == kPbOwn) {
-        const int last = (s.x0 + s.nq - 1) / a.G;
-        for (int i = s.x0 / a.G + 1 + threadIdx.x; i <= last; i += 256) odd |= a.odd[s.base + i] != 0;
+        const PbNew n = pb_new(a, s);
+        for (int i = n.first + threadIdx.x; i <= n.last; i += 256) odd |= a.odd[s.base + i] != 0;
     }
     return odd;
 }
@@ -822,7 +838,7 @@ __device__ __forceinline__ void pb_finish(const BatchArgs<T>& a, const PbWork& w
     // the usual loop has neither the rare tokens nor the other destination in it: a block runs
     // through this code once, and what it costs is fetching it
     auto sums = [&](auto poison, auto out) {
-        const int lo = s.x0 / a.G + 1;
+        const PbNew mine = pb_new(a, s);
 #pragma unroll 1
         for (int k = tid; k < 4 * QW * D; k += 256) {
             const int four = k / D, dd = k - four * D, which = dd >= HDP, d = dd - which * HDP, w0 = four >> 2;
@@ -840,7 +856,7 @@ __device__ __forceinline__ void pb_finish(const BatchArgs<T>& a, const PbWork& w
                 if (to < 0) continue;
                 if (poison && d < a.HD)
                     c[i] += pb_poison((which ? a.kp : a.vp) + w.kvh * a.ps_head + d, a.odd + s.base, a.table + (int64_t)s.row * a.table_ld,
-                                      a.ps_page, a.ps_tok, s.lens, a.log_ps, a.n_pages, lo, end.last[4 * four + i], which);
+                                      a.ps_page, a.ps_tok, s.lens, a.log_ps, a.n_pages, mine.first, min(mine.last, end.last[4 * four + i]), which);
                 if (out) st((which ? a.k_out : a.c_out) + to + d, c[i]);
                 else a.rec[to * 2 * HDP + dd] = c[i];
             }
@@ -1258,6 +1274,7 @@ paged_items_f32_kernel(BatchArgs<T> a) {
     }
     const int sees = min(pb_sees(a, s, xq), kend);
     const int sees_first = __builtin_amdgcn_readfirstlane(min(pb_sees(a, s, min(x0, s.nq - 1)), kend));
+    const int seen_by_all = pb_sees(a, s, 0);        // positions that every query of the block sees
     const int sees_last = x0 >= s.nq ? 0 : __builtin_amdgcn_readfirstlane(min(pb_sees(a, s, min(x0 + 15, s.nq - 1)), kend));
     u32x4 kr[NP], vr[NP];
     auto load = [&](int t0) {                        // positions t0 .. t0 + RT - 1
@@ -1348,7 +1365,7 @@ paged_items_f32_kernel(BatchArgs<T> a) {
                 pv[r] = __builtin_amdgcn_exp2f(fmaf(sc[r], a.qscale, off));
                 lh += pv[r];
             }
-            const bool dirty = odd && mask;          // rows that not all columns see (pb_odd)
+            const bool dirty = odd && r0 + 16 > seen_by_all;     // rows that not all queries see (pb_odd)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int row = 16 * hf + 4 * lq + r;
@@ -1359,7 +1376,7 @@ paged_items_f32_kernel(BatchArgs<T> a) {
                     if constexpr (KCTX) k[dt] = tk[row * PITCH + lr + 16 * dt];
                 }
                 if (dirty) {
-                    const bool partly = t0 + row >= sees_first;
+                    const bool partly = t0 + row >= seen_by_all;
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt) {
                         if (partly && !(fabsf(v[dt]) < INFINITY)) v[dt] = 0.0f;
@@ -1398,12 +1415,18 @@ paged_items_f32_kernel(BatchArgs<T> a) {
 // rows behind 16384, 32 heads of 128: 10.0 us).
 constexpr int kPbJoin = 8;
 
+// What a part's sums weigh beside those of a part with the greater reference `most`.  Never
+// zero: an infinity that an item's end has put into a part stays one.  (2^-80 of a part's l, which is below
+// 2^40, is less than 2^-40 of the sum, whose l is at least 1: nothing of what is finite.)
+__device__ __forceinline__ float pb_weight(float m, float most) {
+    return most == -INFINITY ? 1.0f : fmaxf(__builtin_amdgcn_exp2f(m - most), 0x1p-80f);
+}
+
 // (m, l, v) and a record's (e, y) as one
 template <int NV>
 __device__ __forceinline__ void pb_add(float& m, float& l, pg_f32x4 (&v)[NV], float2 e, const pg_f32x4 (&y)[NV]) {
     const float most = fmaxf(m, e.x);
-    const float f = most == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - most);
-    const float g = most == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(e.x - most);
+    const float f = pb_weight(m, most), g = pb_weight(e.x, most);
     l = fmaf(l, f, e.y * g);
 #pragma unroll
     for (int k = 0; k < NV; ++k) v[k] = v[k] * f + y[k] * g;
@@ -1504,7 +1527,7 @@ paged_batch_join_kernel(BatchArgs<T> a) {
             float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-                const float f = most == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml[v].x - most);
+                const float f = pb_weight(ml[v].x, most);
                 all = fmaf(ml[v].y, f, all);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) o[q] = fmaf(sums[v][d2 + q], f, o[q]);
