@@ -869,6 +869,17 @@ int loom_paged_plan(const int32_t* table, int64_t table_ld, int64_t max_pages, i
                     int64_t KVH, int32_t* starts, int32_t* rows_of, int32_t* positions, int64_t* slots,
                     int32_t* shared, void* plan, int64_t plan_bytes, void* stream);
 
+/* loom_paged_plan that also says what became of the rows, for a caller that keeps
+ * lens: limit [rows] (or NULL) is set for every row that brings tokens, to INT32_MAX
+ * where they have slots and to 0 where they have none (such a row must not be
+ * taken to hold them), and other rows' entries stay; left_out [1] (or NULL) is
+ * increased by the number of rows whose tokens have none. */
+int loom_paged_plan_checked(const int32_t* table, int64_t table_ld, int64_t max_pages, int64_t n_pages, int64_t page_size,
+                            const int32_t* lens, const int32_t* new_tokens, int64_t rows, int64_t n_tokens, int64_t QH,
+                            int64_t KVH, int32_t* starts, int32_t* rows_of, int32_t* positions, int64_t* slots,
+                            int32_t* shared, void* plan, int64_t plan_bytes, int32_t* limit, int32_t* left_out,
+                            void* stream);
+
 /* A layer of a serving step (the attention of GroupedQueryCausalSelfAttention,
  * loomformer.py:3215-3332, over a paged cache and a ragged batch): qkv
  * [n_tokens, (QH + 2 KVH) HD] projection rows; q and k are roped at the token's

@@ -298,9 +298,9 @@ PyObject* paged_reserve(PyObject* const* x, Py_ssize_t n) {
 
 // ------------------------------------------------------------------ a ragged batch's step
 
-// (k_pages, table, lens, new, n_tokens, q_heads) -> starts, rows, positions, slots, shared, work, sizes
+// (k_pages, table, lens, new, n_tokens, q_heads, limit, left_out) -> starts, rows, positions, slots, shared, work, sizes
 PyObject* paged_plan(PyObject* const* x, Py_ssize_t n) {
-    const Args a("paged_plan", x, n, 6);
+    const Args a("paged_plan", x, n, 8);
     const at::Tensor& k = a.tensor(0, "k_pages");
     const int64_t d = k.dim();
     CHECK(d == 4 || d == 5, a.name, ": k_pages must be [pages, kv_heads, page_size, head_dim], or that of all layers");
@@ -309,6 +309,8 @@ PyObject* paged_plan(PyObject* const* x, Py_ssize_t n) {
     const at::Tensor &lens = i32(a, 2, "lens", t.rows, dev), &fresh = i32(a, 3, "new", t.rows, dev);
     const int64_t NP = k.size(d - 4), KVH = k.size(d - 3), PS = k.size(d - 2), N = a.integer(4), QH = a.integer(5), R = t.rows;
     CHECK(N >= 0 && N <= (1 << 20), a.name, ": n_tokens must be 0 to 2^20, got ", N);
+    int32_t* const limit = a.none(6) ? nullptr : (int32_t*)i32(a, 6, "limit", R, dev).data_ptr();
+    int32_t* const left_out = a.none(7) ? nullptr : (int32_t*)i32(a, 7, "left_out", 1, dev).data_ptr();
     OnDevice on(dev.index());
     const int64_t need = loom_paged_plan_bytes(R, N, QH, KVH);
     CHECK(need > 0, a.name, ": ", QH, " query heads over ", KVH, " kv heads, ", R, " rows (at most 1024)");
@@ -318,9 +320,10 @@ PyObject* paged_plan(PyObject* const* x, Py_ssize_t n) {
                      shared = at::empty({R}, opt.dtype(at::kInt)), work = bytes(need, dev);
     void* st = stream_of(dev.index());
     launch([&] {
-        return loom_paged_plan(t.p, t.ld, t.pages, NP, PS, (const int32_t*)lens.data_ptr(), (const int32_t*)fresh.data_ptr(),
-                               R, N, QH, KVH, (int32_t*)starts.data_ptr(), (int32_t*)rows.data_ptr(), (int32_t*)pos.data_ptr(),
-                               (int64_t*)slots.data_ptr(), (int32_t*)shared.data_ptr(), work.data_ptr(), need, st);
+        return loom_paged_plan_checked(t.p, t.ld, t.pages, NP, PS, (const int32_t*)lens.data_ptr(), (const int32_t*)fresh.data_ptr(),
+                                       R, N, QH, KVH, (int32_t*)starts.data_ptr(), (int32_t*)rows.data_ptr(),
+                                       (int32_t*)pos.data_ptr(), (int64_t*)slots.data_ptr(), (int32_t*)shared.data_ptr(),
+                                       work.data_ptr(), need, limit, left_out, st);
     });
     PyObject* l = list_of({&starts, &rows, &pos, &slots, &shared, &work, nullptr});
     PyObject* sizes = Py_BuildValue("(LLLLL)", (long long)NP, (long long)KVH, (long long)PS, (long long)t.pages, (long long)QH);

@@ -105,6 +105,7 @@ struct PlanArgs {
     int32_t *starts, *rows_of, *positions, *shared;
     int64_t* slots_of;
     int32_t* plan;
+    int32_t *limit, *left_out;      // (or NULL)
     PbLayout at;
     int R, N, QH, KVH, G, log_ps, cap, n_pages;
 };
@@ -354,6 +355,8 @@ paged_plan_kernel(PlanArgs a) {
     }
     if (r < a.R) a.starts[r] = start;
     if (r == 0) a.starts[a.R] = all1[0];
+    if (m > 0 && a.limit != nullptr) a.limit[r] = ok ? 0x7fffffff : 0;
+    if (m > 0 && !ok && a.left_out != nullptr) atomicAdd(a.left_out, 1);
 
     // groups: rows of one leader; what all of them have in common
     const int lead = ok && info.x >= 0 ? info.x : -1;
@@ -1675,6 +1678,15 @@ extern "C" int loom_paged_plan(const int32_t* table, int64_t table_ld, int64_t m
                                const int32_t* lens, const int32_t* new_tokens, int64_t rows, int64_t n_tokens, int64_t QH,
                                int64_t KVH, int32_t* starts, int32_t* rows_of, int32_t* positions, int64_t* slots,
                                int32_t* shared, void* plan, int64_t plan_bytes, void* stream) {
+    return loom_paged_plan_checked(table, table_ld, max_pages, n_pages, page_size, lens, new_tokens, rows, n_tokens, QH, KVH, starts,
+                                   rows_of, positions, slots, shared, plan, plan_bytes, nullptr, nullptr, stream);
+}
+
+extern "C" int loom_paged_plan_checked(const int32_t* table, int64_t table_ld, int64_t max_pages, int64_t n_pages,
+                                       int64_t page_size, const int32_t* lens, const int32_t* new_tokens, int64_t rows,
+                                       int64_t n_tokens, int64_t QH, int64_t KVH, int32_t* starts, int32_t* rows_of,
+                                       int32_t* positions, int64_t* slots, int32_t* shared, void* plan, int64_t plan_bytes,
+                                       int32_t* limit, int32_t* left_out, void* stream) {
     clear_error();
     const char* who = "paged_plan";
     if (int rc = batch_sizes(who, rows, n_tokens, QH, KVH, n_pages, page_size, max_pages, table_ld)) return rc;
@@ -1694,6 +1706,8 @@ extern "C" int loom_paged_plan(const int32_t* table, int64_t table_ld, int64_t m
     a.shared = shared;
     a.slots_of = slots;
     a.plan = (int32_t*)plan;
+    a.limit = limit;
+    a.left_out = left_out;
     a.at = pb_layout(rows, n_tokens, QH, KVH);
     a.R = (int)rows;
     a.N = (int)n_tokens;

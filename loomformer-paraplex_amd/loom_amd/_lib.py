@@ -132,6 +132,8 @@ SIGNATURES = {
     "loom_paged_reserve": [*_POOL, _P, c_int64, c_int64, _P, _P, _P, _P, _P, c_int64, c_int64, _P],
     "loom_paged_plan": [_P, c_int64, c_int64, c_int64, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int64, _P, _P, _P,
                         _P, _P, _P, c_int64, _P],
+    "loom_paged_plan_checked": [_P, c_int64, c_int64, c_int64, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int64, _P,
+                                _P, _P, _P, _P, _P, c_int64, _P, _P, _P],
     "loom_paged_batch_step": [c_int, _P, c_int64, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, _P, c_int64,
                               c_int64, c_int64, _P, _P, _P, _P, c_int64, _P, _P, c_int64, _P, _P, _P, c_int64, _P,
                               c_int64, c_int64, c_int64, c_int64, c_int64, _P],

@@ -634,7 +634,7 @@ class PagedPlan(NamedTuple):
 
 
 def paged_plan(k_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, new: torch.Tensor, n_tokens: int,
-               q_heads: int) -> PagedPlan:
+               q_heads: int, limit: Optional[torch.Tensor] = None, left_out: Optional[torch.Tensor] = None) -> PagedPlan:
     """Slot maps and work of a step in which row r brings new[r] tokens (int32 [rows];
     none, one, a prompt), from the tables and lengths on the device.  n_tokens: places of
     the flat batch, at least the sum of new.  k_pages: a layer's or all layers' pool
@@ -642,8 +642,10 @@ def paged_plan(k_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, n
     found, and paged_batch_step reads those once for all of them.  The plan holds
     for all layers, until table, lens or new change.  A row that lacks a page for
     one of its tokens (paged_reserve, paged_update), or whose tokens do not all fit into the
-    batch, has no slots."""
-    return PagedPlan(*(_host_module or _host()).paged_plan(k_pages, table, lens, new, n_tokens, q_heads))
+    batch, has no slots: it does not hold them after the step either, so its lens must stay.  limit
+    (int32 [rows]) says which: 2^31 - 1 for a row that brings tokens and has slots, 0 for one that has none,
+    untouched for the others.  left_out (int32 [1]) is increased by the rows that have none."""
+    return PagedPlan(*(_host_module or _host()).paged_plan(k_pages, table, lens, new, n_tokens, q_heads, limit, left_out))
 
 
 def paged_batch_step(plan: PagedPlan, qkv: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,

@@ -23,6 +23,7 @@ class PagedKVCache:
       lens  [rows] int32              tokens each row holds (-1: no sequence)
       refs  [n_pages] int32           table entries that hold each page
       status [1] int32                pages that could not be had (see check)
+      left_out [1] int32              rows whose tokens a plan had no place for (see check)
 
     A row's last tokens are dropped by lowering its entry of lens.  n_pages defaults to what rows that share nothing need, which never runs out.
     """
@@ -46,8 +47,11 @@ class PagedKVCache:
         self.table = torch.full((rows, max_pages), -1, **i32)
         self.lens = torch.full((rows,), -1, **i32)
         self.refs = torch.zeros(self.n_pages, **i32)
-        self.status = torch.zeros(1, **i32)
+        self._counts = torch.zeros(2, **i32)
+        self.status, self.left_out = self._counts[:1], self._counts[1:]
         self._used = torch.zeros(1, **i32)
+        # tokens that a row may advance by: none where the last plan had no place for those it brings
+        self._limit = torch.full((rows,), 2 ** 31 - 1, **i32)
 
     @property
     def rows(self) -> int:
@@ -58,7 +62,8 @@ class PagedKVCache:
         self.table.fill_(-1)
         self.lens.fill_(-1)
         self.refs.zero_()
-        self.status.zero_()
+        self._counts.zero_()
+        self._limit.fill_(2 ** 31 - 1)
 
     def start(self, rows: torch.Tensor) -> None:
         """Rows of a bool mask [rows] that hold no sequence begin one of no tokens."""
@@ -75,8 +80,9 @@ class PagedKVCache:
         ops.paged_reserve(self.k_pages, self.v_pages, self.table, self.lens, self.refs, self.status, new)
 
     def plan(self, new: torch.Tensor, n_tokens: int, q_heads: int) -> ops.PagedPlan:
-        """ops.paged_plan of a step in which each row brings new[r] tokens (reserved before)."""
-        return ops.paged_plan(self.k_pages, self.table, self.lens, new, n_tokens, q_heads)
+        """ops.paged_plan of a step in which each row brings new[r] tokens (reserved before).  A row that the
+        plan has no slots for is left out of the step: advance leaves it as it is, and check raises."""
+        return ops.paged_plan(self.k_pages, self.table, self.lens, new, n_tokens, q_heads, self._limit, self.left_out)
 
     def attend_batch(self, layer: int, plan: ops.PagedPlan, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                      want_kctx: bool = True) -> List[Optional[torch.Tensor]]:
@@ -84,8 +90,9 @@ class PagedKVCache:
         return ops.paged_batch_step(plan, qkv, self.k_pages[layer], self.v_pages[layer], self.table, cos, sin, want_kctx)
 
     def advance(self, new: torch.Tensor) -> None:
-        """Each row holds its new[r] tokens from now on (after the last layer of their step)."""
-        self.lens.add_(torch.where(self.lens >= 0, new.clamp(min=0), 0))
+        """Each row holds its new[r] tokens from now on (after the last layer of their step), but for rows
+        whose tokens had no slots in the cache's last plan for them, which nothing was written of."""
+        self.lens.add_(torch.where(self.lens >= 0, torch.minimum(new.clamp(min=0), self._limit), 0))
 
     def free(self, rows: torch.Tensor) -> None:
         """Rows of a bool mask [rows] let go of their pages and hold no sequence."""
@@ -109,11 +116,16 @@ class PagedKVCache:
         return int(self._used)
 
     def check(self) -> None:
-        """Raise if an update since the last reset found no page (a host sync)."""
-        n = int(self.status)
+        """Raise if an update or reservation since the last reset found no page, or a plan no places for a
+        row's tokens (a host sync)."""
+        n, rows = self._counts.tolist()
+        what = []
         if n:
-            raise RuntimeError(f"paged cache: {n} pages could not be had ({self.n_pages} pages of {self.page_size} tokens); "
-                               "rows without their page gave NaN")
+            what.append(f"{n} pages could not be had ({self.n_pages} pages of {self.page_size} tokens)")
+        if rows:
+            what.append(f"{rows} rows' tokens had no place in their step (pages, table or flat batch too small)")
+        if what:
+            raise RuntimeError(f"paged cache: {', '.join(what)}; such rows gave NaN")
 
     def workspace(self, q_heads: int) -> torch.Tensor:
         """Scratch for loom_paged_decode_step on this cache, for callers of the C entry

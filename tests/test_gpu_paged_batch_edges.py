@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import paged as ref
-from test_gpu_paged_batch import BF, DEV, FP, HF, _cache, _i32, _tables
+from test_gpu_paged_batch import BF, DEV, FP, HF, _cache, _i32, _near, _tables
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +48,145 @@ def test_infinities_of_values_keep_their_kind(dt, HD, scale, lens, new, share):
     for got, want in ((c.cpu(), o["c"]), (kx.cpu(), o["kctx"])):
         for kind in (torch.isnan, torch.isposinf, torch.isneginf):
             assert torch.equal(kind(got), kind(want)), kind.__name__
+
+
+# ------------------------------------------------------------------ rows that a step leaves out
+
+def _at_work(dt, rows, max_len, n_pages=None, L=1, KVH=2, HD=64, PS=16):
+    from loom_amd.paged import PagedKVCache
+    cache = PagedKVCache(L, rows, max_len, KVH, HD, dt, page_size=PS, n_pages=n_pages)
+    cache.k_pages.normal_()                               # what former holders of the pages left there
+    cache.v_pages.normal_()
+    cache.start(torch.ones(rows, dtype=torch.bool, device=DEV))
+    return cache
+
+
+def _step(cache, streams, new, places, QH, tables):
+    """reserve, plan, attend, advance; the outputs (c, kctx, q) of the tokens by row."""
+    lens, counts = cache.lens.tolist(), _i32(new)
+    cache.reserve(counts)
+    plan = cache.plan(counts, places, QH)
+    flat = torch.cat([streams[r, lens[r]:lens[r] + m] for r, m in enumerate(new)] + [streams[0, :places]])[:places].contiguous()
+    got = cache.attend_batch(0, plan, flat, *tables)
+    cache.advance(counts)
+    at = plan.starts.tolist()
+    return [[y[at[r]:at[r + 1]] for y in got] for r in range(len(new))]
+
+
+def _right(cache, r, got, first, dt):
+    """Outputs of row r's tokens from `first` on against the cache's own rows in 64 bits."""
+    c, kx, q = (y.cpu() for y in got)
+    T = first + q.shape[0]
+    o = ref.batch_attention(q, cache.k_pages[0], cache.v_pages[0], cache.table[r:r + 1].cpu(), [first], [0, q.shape[0]], [True])
+    _near(c, o["c"], o["c_abs"], o, dt, q.shape[2], "c")
+    _near(kx, o["kctx"], o["kctx_abs"], o, dt, q.shape[2], "kctx")
+    assert int(cache.lens[r]) >= T
+
+
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_a_row_that_does_not_fit_into_the_batch_does_not_advance(dt):
+    """A step whose last row finds no places, and the same row again in the next one: its lens stays, check
+    raises, and what it then reads is what was written."""
+    g = torch.Generator().manual_seed(41)
+    QH, KVH, HD = 8, 2, 64
+    streams = torch.randn(3, 60, (QH + 2 * KVH) * HD, generator=g).to(DEV, dt)
+    cache, tables = _at_work(dt, 3, 60), _tables(HD, 64)
+    out = _step(cache, streams, [4, 3, 0], 7, QH, tables)
+    cache.check()
+    out = _step(cache, streams, [2, 0, 20], 9, QH, tables)   # 22 tokens for 9 places
+    assert cache.lens.tolist() == [6, 3, 0]
+    _right(cache, 0, out[0], 4, dt)
+    with pytest.raises(RuntimeError, match="1 row.* no place"):
+        cache.check()
+    out = _step(cache, streams, [1, 1, 20], 30, QH, tables)
+    assert cache.lens.tolist() == [7, 4, 20]
+    _right(cache, 2, out[2], 0, dt)
+    out = _step(cache, streams, [1, 1, 1], 3, QH, tables)
+    assert cache.lens.tolist() == [8, 5, 21]
+    for r, first in ((0, 7), (1, 4), (2, 20)):
+        _right(cache, r, out[r], first, dt)
+    for r in range(3):                                    # the cache holds the rows' tokens and no others
+        n = int(cache.lens[r])
+        held = ref.rows_of(cache.v_pages[0].cpu(), cache.table[r].cpu(), n)
+        assert torch.equal(held, streams[r, :n].view(n, -1, HD)[:, QH + KVH:].transpose(0, 1).cpu().to(held.dtype))
+    cache.reset()
+    cache.check()
+
+
+def test_rows_without_pages_or_behind_the_table_do_not_advance():
+    g = torch.Generator().manual_seed(42)
+    QH, KVH, HD = 8, 2, 64
+    streams = torch.randn(2, 100, (QH + 2 * KVH) * HD, generator=g).to(DEV, BF)
+    tables = _tables(HD, 128)
+    cache = _at_work(BF, 2, 64, n_pages=4)
+    _step(cache, streams, [33, 40], 73, QH, tables)       # three pages each of four
+    assert cache.lens.tolist() == [33, 0]
+    with pytest.raises(RuntimeError, match="2 pages could not be had.*1 row"):
+        cache.check()
+    cache = _at_work(BF, 2, 64)
+    _step(cache, streams, [60, 3], 63, QH, tables)
+    _step(cache, streams, [5, 1], 6, QH, tables)          # 65 of 64
+    assert cache.lens.tolist() == [60, 4]
+    out = _step(cache, streams, [4, 1], 5, QH, tables)
+    assert cache.lens.tolist() == [64, 5]
+    _right(cache, 0, out[0], 60, BF)
+
+
+def test_two_plans_of_one_step_advance_their_own_rows():
+    """Prompts and single tokens planned apart, of which one prompt finds no places; and rows whose step
+    was planned by the operator itself."""
+    from loom_amd import ops
+    cache = _at_work(BF, 4, 64)
+    a, b = _i32([5, 0, 30, 0]), _i32([0, 2, 0, -1])
+    cache.reserve(_i32([5, 2, 30, 0]))
+    cache.plan(a, 20, 8)
+    cache.plan(b, 2, 8)
+    cache.advance(a)
+    cache.advance(b)
+    assert cache.lens.tolist() == [5, 2, 0, 0]
+    other, new = _at_work(BF, 4, 64), _i32([1, 2, 3, 0])
+    other.reserve(new)
+    ops.paged_plan(other.k_pages, other.table, other.lens, new, 6, 8)
+    other.advance(new)
+    assert other.lens.tolist() == [1, 2, 3, 0]
+    other.check()
+
+
+def test_a_captured_step_leaves_out_what_does_not_fit():
+    g = torch.Generator().manual_seed(43)
+    QH, KVH, HD = 8, 2, 64
+    streams = torch.randn(3, 200, (QH + 2 * KVH) * HD, generator=g).to(DEV, BF)
+    tables = _tables(HD, 208)
+    cache, new, flat = _at_work(BF, 3, 200), _i32([0, 0, 0]), torch.zeros(12, (QH + 2 * KVH) * HD, dtype=BF, device=DEV)
+
+    def step():
+        cache.reserve(new)
+        plan = cache.plan(new, 12, QH)
+        out = cache.attend_batch(0, plan, flat, *tables)
+        cache.advance(new)
+        return [plan.starts] + out
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    lens = [0, 0, 0]
+    for counts in ([4, 3, 5], [1, 1, 11], [1, 1, 10], [12, 1, 1], [13, 1, 1], [1, 1, 1], [2, 9, 2]):
+        rows = [streams[r, lens[r]:lens[r] + m] for r, m in enumerate(counts)]
+        flat.copy_(torch.cat(rows + [flat])[:12])
+        new.copy_(_i32(counts))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        at = outs[0].tolist()
+        for r, m in enumerate(counts):
+            if at[r] + m <= 12:
+                _right(cache, r, [y[at[r]:at[r] + m] for y in outs[1:]], lens[r], BF)
+                lens[r] += m
+        assert cache.lens.tolist() == lens, counts
+    with pytest.raises(RuntimeError, match="no place"):
+        cache.check()
