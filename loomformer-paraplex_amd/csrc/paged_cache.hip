@@ -181,7 +181,7 @@ paged_reserve_kernel(int32_t* __restrict__ table, int64_t ld, int MP, int32_t* _
     slot0[r] = held_pages(len, 0, log_ps);
     len_of[r] = len;
     __syncthreads();                                 // every parent's length is read
-    if (r < R) lens[r] = len;
+    if (r < R && n_each == nullptr) lens[r] = len;   // (a reservation per row leaves lens alone)
     if constexpr (FORK) {
         int er = r / MP, ec = r - er * MP;
         for (int i = r; i < R * MP; i += 1024) {

@@ -190,3 +190,18 @@ def test_a_captured_step_leaves_out_what_does_not_fit():
         assert cache.lens.tolist() == lens, counts
     with pytest.raises(RuntimeError, match="no place"):
         cache.check()
+
+
+def test_a_reservation_leaves_lens_as_they_are():
+    """Whatever stands there for rows that hold no sequence."""
+    from loom_amd import ops
+    g = torch.Generator().manual_seed(51)
+    k, v = (torch.randn(1, 20, 2, 16, 32, generator=g).to(DEV, BF) for _ in range(2))
+    held = [-2, 5, -1, -2 ** 31, 0, 100]
+    lens, refs, status = _i32(held), torch.zeros(20, dtype=torch.int32, device=DEV), _i32([0])
+    table = torch.full((6, 4), -1, dtype=torch.int32, device=DEV)
+    table[1, 0] = 3
+    refs[3] = 1
+    ops.paged_reserve(k, v, table, lens, refs, status, _i32([9, 30, 1, 2, 0, 1]))
+    assert lens.tolist() == held
+    assert table.tolist() == [[-1] * 4, [3, 0, 1, -1]] + [[-1] * 4] * 4 and int(status) == 1
