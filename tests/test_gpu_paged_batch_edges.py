@@ -1,12 +1,12 @@
 """A ragged batch's step at its edges, against plain implementations in 64 bits: which kind of value
-an infinity of a token gives."""
+an infinity of a token gives, rows that a step leaves out, what a reservation leaves alone, segments of 64 queries."""
 import math
 
 import pytest
 import torch
 
 from oracle import paged as ref
-from test_gpu_paged_batch import BF, DEV, FP, HF, _cache, _i32, _near, _tables
+from test_gpu_paged_batch import BF, DEV, FP, HF, _cache, _check, _i32, _near, _tables
 
 pytestmark = pytest.mark.gpu
 
@@ -205,3 +205,27 @@ def test_a_reservation_leaves_lens_as_they_are():
     ops.paged_reserve(k, v, table, lens, refs, status, _i32([9, 30, 1, 2, 0, 1]))
     assert lens.tolist() == held
     assert table.tolist() == [[-1] * 4, [3, 0, 1, -1]] + [[-1] * 4] * 4 and int(status) == 1
+
+
+# ------------------------------------------------------------------ segments of 64 queries
+
+@pytest.mark.parametrize("dt", [BF, HF, FP])
+@pytest.mark.parametrize("HD", [16, 64, 96, 128])
+@pytest.mark.parametrize("kind", ["alone", "beside rows that share", "G of 4"])
+def test_own_segments_of_64_queries(dt, HD, kind):
+    """Own segments are halved where halves fill the device and whole ones do not."""
+    slots_of = lambda KVH: 2 * torch.cuda.get_device_properties(0).multi_processor_count // KVH  # noqa: E731
+    QH, KVH = (64, 16) if kind == "G of 4" else (32, 32)
+    slots, G = slots_of(KVH), QH // KVH
+    # rows of more than 64 queries and up to 128, as many as take more than half the places
+    n = slots // 2 + 1
+    new = [(65 + (29 * i) % 64 + G - 1) // G for i in range(n)]
+    lens = [(83 * i) % 200 for i in range(n)]
+    share = []
+    if kind != "alone":                                   # single tokens behind one prompt, fewer than whole segments leave room for
+        more = slots - n - 1
+        share = [(range(n, n + more), 96)]
+        lens, new = lens + [96 + (7 * i) % 40 for i in range(more)], new + [1] * more
+    halves, wholes = (sum(-(-m * G // q) for m in new) for q in (64, 128))
+    assert wholes < slots <= halves
+    _check(dt, lens, new, QH, KVH, HD, 16, 24, 61, share=share, pad=2)
