@@ -858,7 +858,10 @@ int loom_paged_reserve(int dtype, void* k_pages, void* v_pages, int64_t layers, 
  *   slots [n_tokens]     int64: page * page_size + place in the page (-1: none)
  * shared [rows]: how many of the row's first tokens lie in pages that other rows of
  * the batch hold too and are read once for all of them (0: none), and `plan`, for
- * loom_paged_batch_step: the step's work cut into equal shares.  It holds for
+ * loom_paged_batch_step: the step's work cut into equal shares.  Rows share by their
+ * first page: of all rows that begin with the same one and bring at most 64 queries a kv
+ * head (tokens times QH / KVH), the whole pages that every one of them has in common, if
+ * they hold 64 tokens or more; one that parts early shortens it for all.  The plan holds for
  * the layers of one step, until table, lens or new_tokens change.  A row without a
  * page for each of its tokens, those to come included, with more than its
  * table takes, or whose tokens do not all fit into the batch, has no slots.
@@ -888,8 +891,8 @@ int loom_paged_plan_checked(const int32_t* table, int64_t table_ld, int64_t max_
  * (or NULL), rows out_ld apart.  Pages that a new token is written to must be held
  * by its row alone (loom_paged_reserve).  Later tokens of the row and
  * whatever else lies in its pages have no influence, infinities and NaN included.
- * An infinity of v is the readout of the tokens that see it (two of both signs:
- * NaN; so too a weight that is zero in the type the product takes, for a token of an earlier step).
+ * An infinity of v is the readout of the tokens that see it (NaN: two of both signs, or
+ * where its weight may have rounded to zero).
  * Padding gives zeros; tokens of a row without slots, and those whose position
  * lies past the rotary tables, give NaN and are not written.  A plan of other
  * sizes gives NaN.  workspace: loom_paged_batch_workspace_bytes, 16-byte aligned,

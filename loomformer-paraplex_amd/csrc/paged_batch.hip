@@ -10,6 +10,11 @@
 // partition is that of the work: the positions that rows share against all those
 // rows' queries at once, then each row's own.
 //
+// What rows share is one run of whole pages per first page: rows of up to kPbAlone queries that begin
+// with the same page are a group, and the run is the least that all its rows have in common.  A
+// row that parts early cuts it for the others (64 rows behind 16384 of which one parts after
+// 64: items 249 us, 52 without it).
+//
 // Which rows share what only the device knows, so a step is planned there, once for
 // all layers:
 //   rows     which rows begin with the same pages, and how many (paged_rows_kernel)
@@ -314,7 +319,7 @@ __device__ __forceinline__ int4 pb_states(const PlanArgs& a, int m) {
 // bound by their latency, a pass over the rows or the segments with a block scan each.
 // ALONE: of few table entries every block finds the states itself, and the launch before is
 // saved.  NT: at least as many threads as rows; a barrier of fewer waves is a shorter one
-// (4 rows by one wave 6.1 us, by 16 with the launch before 9.2; 32 rows by four waves 10.8, 64
+// (4 rows by one wave 6.2 us, by 16 with the launch before 9.2; 32 rows by four waves 11.1, 64
 // and 256 rows by 16 waves 9 to 11 behind the launch before).
 template <int NT, bool ALONE>
 __global__ void __launch_bounds__(NT)
@@ -455,9 +460,12 @@ paged_plan_kernel(PlanArgs a) {
     // An item has at least the tiles that fill the device.  It leaves a record per query, which
     // is written and read at the copy's rate by all blocks together, while a tile is
     // one block's time: c tiles and work / c records take least where c^2 is their ratio.
-    // (kPbRecord 1.5e-4 / 2.5e-4 / 4e-4 / 1e-3, items and join, us: 64 rows behind 16384
-    // 71.1 / 70.5 / 62.5 / 76.2, 4 x 12 behind 1500 30.4 / 32.5 / 33.8 / 38.4, 2 x 16 behind 2048
-    // 21.0 / 20.5 / 19.1 / 19.4)
+    // That is a rule of thumb: it does not know how many whole times the items fill the device, and
+    // `fill` counts a tile of few queries like one of 128, so times jump with c rather than
+    // follow a curve.  (kPbRecord 1.5e-4 / 2.5e-4 / 4e-4 / 1e-3, items and join, us: 64 rows behind
+    // 16384 71.1 / 70.5 / 62.5 / 76.2, with c 11 / 11 / 14 / 23, the first two what fills the device;
+    // 4 x 12 behind 1500 30.4 / 32.5 / 33.8 / 38.4, c 4 / 6 / 7 / 12; 2 x 16 behind 2048 21.0 / 20.5 /
+    // 19.1 / 19.4.  4e-4 is the best of them for two of the three and costs the third a tenth.)
     const float ratio = kPbRecord * (float)a.KVH * 16.0f * ((float)tiles[2] * 1048576.0f + (float)tiles[3]);
     const int64_t fill = (all_tiles + a.at.slots - 1) / a.at.slots;
     const int chunk = max(max(kPbLeast, (int)sqrtf(ratio)), (int)min(fill, (int64_t)1 << 30));
@@ -626,9 +634,11 @@ __device__ __forceinline__ void store_e(T* p, const float (&v)[E]) {
 // A block per token: q and k roped and rounded, q to q_out, k and v into the token's
 // slot.  A thread takes E elements of a head and their partners half a head on, so that
 // each is loaded once.  Tokens behind the last give zeros, tokens of a row without room
-// or a page NaN; both are done here.  A copy with a little arithmetic: bound by the
-// bytes in and out (5139 tokens of 48 heads of 128 25.4 us, 5.0 TB/s), or, of few tokens, by one
-// load after the other (32 tokens 4.7).
+// or a page NaN; both are done here.  A copy with a little arithmetic.  Of wide tokens bound by the
+// bytes in and out (5139 tokens of 48 heads of 128 25.4 us, 5.0 TB/s), of few tokens by one
+// load after the other (32 tokens 4.8).  Many narrow tokens are bound by neither: of 12 heads of 96 84
+// threads of a block have work, a piece each, and what counts is the blocks' number times
+// their latency (4096 tokens 11.1 us in bf16, 1.7 TB/s, and 11.7 in fp32).
 template <typename T, int E>
 __global__ void __launch_bounds__(256)
 paged_append_kernel(BatchArgs<T> a) {
@@ -889,10 +899,10 @@ __device__ __forceinline__ void pb_finish(const BatchArgs<T>& a, const PbWork& w
 // lane by lane: the lanes of a column meet only where it has to rise.
 //
 // Of long shared runs and of prompts bound by the matrix products and what feeds them: 5139
-// tokens of 32 heads of 128 in 295 us, 713 TFLOP/s (the 8192^3 product 1135); 62 rows behind
-// 16384 50.6 us, 498 TFLOP/s, of which the records' 40 MB written at once are some 8; 32 x 128 tokens
-// behind 1920 of 8 heads of 96 57.5 us, 651 TFLOP/s.  Of few rows by the chain item, page, first
-// tile, sums: 7.3 us (4 rows behind 333), 10.9 (8 x 4 behind 2048, 1.4 TB/s).
+// tokens of 32 heads of 128 in 284 us, 740 TFLOP/s (the 8192^3 product 1135), in half 323; without Kctx
+// 212; 62 rows behind 16384 51.8 us, 486 TFLOP/s, of which the records' 40 MB written at once are some 8
+// (without Kctx 41.5); 32 x 128 tokens behind 1920 of 8 heads of 96 58.2 us, 645 TFLOP/s.  Of few rows by the
+// chain item, page, first tile, sums: 7.2 us (4 rows behind 333), 11.1 (8 x 4 behind 2048, 1.4 TB/s).
 template <int HD> constexpr int pb_stages() { return HD <= 96 ? 3 : 2; }
 
 // Where a row's 16-byte pieces lie in a stage: piece c of row r at c ^ swz(r), so that both
@@ -1227,8 +1237,11 @@ paged_items_kernel(BatchArgs<T> a) {
 // blocks; RT positions per step in one LDS buffer, the next ones in flight in registers.
 // The products' operands may take the dimensions in any order that both share: lane
 // group lq takes HD / 4 neighbouring ones of them, so that a lane's are 16-byte reads.
-// Three prompts to 257 tokens 13.8 us, 4 rows to 1300 9.4: the chain item, page, tile, sums, and
-// the fp32 rate behind long rows (4 x 1024 tokens behind 500 324 us, 59 TFLOP/s of 154).
+// Three prompts to 257 tokens 14.1 us, 4 rows to 1300 9.5: the chain item, page, tile, sums.  Long prompts
+// by the operands of the products, of which each is one 4-byte LDS read that no second query block
+// shares (4 x 1024 tokens behind 500 322 us, 59 TFLOP/s of 154).  16-bit heads pay the fp32 products'
+// rate: 4 x 1024 tokens behind 500 with 8 heads of 256 662 us, 62 rows behind 16384 with 32 of
+// them 743 (of 128 on the 16-bit products 52), 32 x 128 tokens behind 1920 with 8 heads of 16 114.
 template <typename T, int HD, bool KCTX>
 __global__ void __launch_bounds__(256)
 paged_items_f32_kernel(BatchArgs<T> a) {
@@ -1243,7 +1256,7 @@ paged_items_f32_kernel(BatchArgs<T> a) {
     if (!w.any) return;
     const PbItem& s = w.s;
     // 64 of the segment's queries, 32 where that leaves blocks too few: blocks of other y take
-    // the others (4 x 1024 new tokens 324 / 362 us, 3 of 1 to 257 25.8 / 19.0)
+    // the others (when it was taken, 64 / 32 queries: 4 x 1024 new tokens 324 / 362 us, 3 of 1 to 257 25.8 / 19.0)
     const int per = a.plan[1] >= a.at.slots ? 64 : 32, xb = per * blockIdx.y, nq = min(s.nq - xb, per);
     if (nq <= 0) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -1415,7 +1428,8 @@ paged_items_f32_kernel(BatchArgs<T> a) {
 // query each, all its records in flight; of more it takes one query: wave w records w,
 // w + 4, .., kPbJoin of them in flight, and the waves meet in LDS.  Bound by the chain count,
 // task, records where those are few (32 rows behind 2048 4.0 us), by the records' bytes else (62
-// rows behind 16384, 32 heads of 128: 10.0 us).
+// rows behind 16384, 32 heads of 128: 10.3 us).  Without Kctx that half of a record is neither
+// written nor used, but it is read (10.5).
 constexpr int kPbJoin = 8;
 
 // What a part's sums weigh beside those of a part with the greater reference `most`.  Never

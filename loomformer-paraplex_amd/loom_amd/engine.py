@@ -703,9 +703,9 @@ class LoomDecoder:
         reads the pages that beams have in common once for all of them
         (ops.paged_batch_step); other roundings of the same sums.  Worth it where all
         rows together hold a million positions or more (us per token of the 10-block
-        model: 8 prompts of 32 beams behind 16384 tokens 5131 without it and 1794 with, 4 of 16
-        1495 and 1188, 1 of 16 behind 65536 1712 and 1171; but 2 of 16 behind 16384
-        901 and 935, 8 of 4 behind 2048 622 and 710).  One step is captured into a
+        model: 8 prompts of 32 beams behind 16384 tokens 5065 without it and 1745 with, 4 of 16
+        1492 and 1176, 1 of 16 behind 65536 1723 and 1146; but 2 of 16 behind 16384
+        902 and 915, 8 of 4 behind 2048 623 and 700).  One step is captured into a
         graph and replayed.  Afterwards the engine holds no sequence to continue
         (its dense cache ends with the prompt)."""
         S, P = prompt.shape

@@ -638,8 +638,10 @@ def paged_plan(k_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, n
     """Slot maps and work of a step in which row r brings new[r] tokens (int32 [rows];
     none, one, a prompt), from the tables and lengths on the device.  n_tokens: places of
     the flat batch, at least the sum of new.  k_pages: a layer's or all layers' pool
-    (its sizes alone count).  Rows whose first whole pages are the same are
-    found, and paged_batch_step reads those once for all of them.  The plan holds
+    (its sizes alone count).  Rows that begin with the same page and bring at most 64 queries a kv head
+    (new[r] * q_heads / kv_heads) are found, and paged_batch_step reads the whole pages that all of
+    them have in common once, if those hold 64 tokens or more; a row that parts from the others early
+    shortens it for all of them.  The plan holds
     for all layers, until table, lens or new change.  A row that lacks a page for
     one of its tokens (paged_reserve, paged_update), or whose tokens do not all fit into the
     batch, has no slots: it does not hold them after the step either, so its lens must stay.  limit
