@@ -91,7 +91,8 @@ class PagedKVCache:
 
     def advance(self, new: torch.Tensor) -> None:
         """Each row holds its new[r] tokens from now on (after the last layer of their step), but for rows
-        whose tokens had no slots in the cache's last plan for them, which nothing was written of."""
+        that this cache's last plan with tokens of theirs had no slots for, since nothing was written of them.
+        (What ops.paged_plan finds for a step that it plans itself is known to its own limit alone.)"""
         self.lens.add_(torch.where(self.lens >= 0, torch.minimum(new.clamp(min=0), self._limit), 0))
 
     def free(self, rows: torch.Tensor) -> None:
