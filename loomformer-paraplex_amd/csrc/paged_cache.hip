@@ -108,7 +108,8 @@ constexpr int kScanIds = 4;         // groups of four page ids per thread and ro
 // scan over refs: a free page's rank among the free ones names its row.
 // Bound by the latency of its stages, each a pass over the rows or over refs with a
 // block scan behind it: 256 rows, 67 places each, 8.8 us; 64 rows that get up to 128 pages each
-// 11.6, one row that gets 1024 38 (its thread walks its places).  One block and not a launch per stage, since each stage needs the whole of the one before.
+// 11.6, one row that gets 1024 38 (its thread walks its places).  One block and not a launch
+// per stage, since each stage needs the whole of the one before.
 // FORK: the block also forks the table, staged whole in LDS: a launch less, but
 // one CU's work.  All of a call in both forms (us, one launch / two): 92 entries
 // 8.0 / 9.9, 4384 10.6 / 11.1, 17152 20.5 / 17.2, 32512 19.6 / 13.7.
